@@ -25,6 +25,10 @@ use core::ffi::{c_char, c_int, c_void};
 
 pub const TYNX_CUDA_ABI_VERSION: c_int = 2;
 pub const TX_MAX_DIMS: usize = 8;
+pub const TX_ROTARY_PAIRS: usize = 128;
+pub const TX_DL_F32: c_int = 0;
+pub const TX_DL_I64: c_int = 1;
+pub const TX_DL_BOOL: c_int = 2;
 
 pub const TX_OK: c_int = 0;
 pub const TX_ERR_INVALID: c_int = 1;
@@ -153,6 +157,43 @@ pub struct tx_prefetch {
 
 #[repr(C)]
 #[derive(Clone, Copy)]
+pub struct tx_rotary {
+    pub dim: i32,
+    pub interleaved: i32,
+    pub factor: f32,
+    pub turns: [f64; TX_ROTARY_PAIRS],
+}
+
+#[repr(C)]
+#[derive(Clone, Copy)]
+pub struct tx_diff_attention {
+    pub batch: i64,
+    pub queries: i64,
+    pub keys: i64,
+    pub heads: i64,
+    pub kv_heads: i64,
+    pub dim: i64,
+    pub vdim: i64,
+    pub q: *const f32,
+    pub k: *const f32,
+    pub v: *const f32,
+    pub lam: *const f32,
+    pub key_lengths: *const i64,
+    pub scale: f32,
+    pub causal: i32,
+    pub query_start: i64,
+    pub out: *mut f32,
+    pub out2: *mut f32,
+    pub lse: *mut f32,
+    pub dout: *const f32,
+    pub dq: *mut f32,
+    pub dk: *mut f32,
+    pub dv: *mut f32,
+    pub dlam: *mut f32,
+}
+
+#[repr(C)]
+#[derive(Clone, Copy)]
 pub struct tx_gemm_desc {
     pub M: i64,
     pub N: i64,
@@ -236,6 +277,8 @@ extern "C" {
     pub fn tx_last_error(ctx: *mut tx_ctx, buf: *mut c_char, n: usize) -> c_int;
     pub fn tx_sync(ctx: *mut tx_ctx, timeout_ms: u64) -> c_int;
     pub fn tx_stream(ctx: *mut tx_ctx, out: *mut *mut c_void) -> c_int;
+    pub fn tx_dlpack_export(ctx: *mut tx_ctx, d_block: *mut c_void, d_data: *mut c_void, dtype: c_int, shape: *const i64, ndim: c_int, stream: *mut c_void, out: *mut *mut c_void) -> c_int;
+    pub fn tx_dlpack_release(managed: *mut c_void) -> c_int;
     pub fn tx_alloc(ctx: *mut tx_ctx, bytes: usize, d_out: *mut *mut c_void) -> c_int;
     pub fn tx_free(ctx: *mut tx_ctx, d_ptr: *mut c_void) -> c_int;
     pub fn tx_h2d(ctx: *mut tx_ctx, d_dst: *mut c_void, h_src: *const c_void, bytes: usize) -> c_int;
@@ -286,6 +329,11 @@ extern "C" {
     pub fn tx_avgpool2d_bwd(ctx: *mut tx_ctx, d_dy: *const f32, d_dx: *mut f32, planes: i64, H: i64, W: i64, geom: *const i64, count_include_pad: c_int, accumulate: c_int) -> c_int;
     pub fn tx_attention_fwd(ctx: *mut tx_ctx, d_q: *const f32, d_k: *const f32, d_v: *const f32, ld_in: i64, d_out: *mut f32, ld_out: i64, batch: i64, seq: i64, heads: i64, head_dim: i64, scale: f32, flags: c_int) -> c_int;
     pub fn tx_attention_bwd(ctx: *mut tx_ctx, d_q: *const f32, d_k: *const f32, d_v: *const f32, ld_in: i64, d_dout: *const f32, ld_dout: i64, d_dq: *mut f32, d_dk: *mut f32, d_dv: *mut f32, ld_grad: i64, batch: i64, seq: i64, heads: i64, head_dim: i64, scale: f32, flags: c_int) -> c_int;
+    pub fn tx_rotary_apply(ctx: *mut tx_ctx, d_x: *const f32, d_y: *mut f32, batch: i64, seq: i64, heads: i64, head_dim: i64, d_pos: *const i64, pos_stride: i64, rotary: *const tx_rotary, inverse: c_int) -> c_int;
+    pub fn tx_qk_norm_rotary_fwd(ctx: *mut tx_ctx, d_q: *const f32, d_k: *const f32, d_q_weight: *const f32, d_k_weight: *const f32, d_q_out: *mut f32, d_k_out: *mut f32, batch: i64, seq: i64, heads: i64, kv_heads: i64, head_dim: i64, d_pos: *const i64, pos_stride: i64, rotary: *const tx_rotary, eps: f32) -> c_int;
+    pub fn tx_qk_norm_rotary_bwd(ctx: *mut tx_ctx, d_q: *const f32, d_k: *const f32, d_q_weight: *const f32, d_k_weight: *const f32, d_dq_out: *const f32, d_dk_out: *const f32, d_dq: *mut f32, d_dk: *mut f32, d_dq_weight: *mut f32, d_dk_weight: *mut f32, batch: i64, seq: i64, heads: i64, kv_heads: i64, head_dim: i64, d_pos: *const i64, pos_stride: i64, rotary: *const tx_rotary, eps: f32) -> c_int;
+    pub fn tx_diff_attention_fwd(ctx: *mut tx_ctx, desc: *const tx_diff_attention) -> c_int;
+    pub fn tx_diff_attention_bwd(ctx: *mut tx_ctx, desc: *const tx_diff_attention) -> c_int;
     pub fn tx_ppo_loss_fwd(ctx: *mut tx_ctx, d_logits: *const f32, rows: i64, cols: i64, d_values: *const f32, d_actions: *const i64, d_old_log_prob: *const f32, d_advantages: *const f32, d_returns: *const f32, clip: f32, value_coef: f32, entropy_coef: f32, d_loss: *mut f32) -> c_int;
     pub fn tx_ppo_loss_bwd(ctx: *mut tx_ctx, d_logits: *const f32, rows: i64, cols: i64, d_values: *const f32, d_actions: *const i64, d_old_log_prob: *const f32, d_advantages: *const f32, d_returns: *const f32, clip: f32, value_coef: f32, entropy_coef: f32, d_dloss: *const f32, d_dlogits: *mut f32, d_dvalues: *mut f32, accumulate_logits: c_int, accumulate_values: c_int) -> c_int;
     pub fn tx_gather_rows(ctx: *mut tx_ctx, d_table: *const f32, rows: i64, width: i64, d_idx: *const i64, n_idx: i64, d_out: *mut f32) -> c_int;

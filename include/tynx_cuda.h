@@ -87,6 +87,20 @@ int tx_sync(tx_ctx *ctx, uint64_t timeout_ms);
 /* The compute stream as a cudaStream_t, for interop with other libraries. */
 int tx_stream(tx_ctx *ctx, void **out);
 
+/* Lend device memory to another library without a copy, as a DLManagedTensor
+ * of the DLPack protocol (*out): `d_data`, dense, of `shape` (ndim <=
+ * TX_MAX_DIMS) and TX_DL_* type, inside the block d_block that tx_alloc
+ * returned.  The given stream (a cudaStream_t of the borrower; NULL: the
+ * legacy default one) waits for the compute work issued so far.  The block is
+ * freed once tx_free was called and every loan has ended (the structure's
+ * deleter, callable from any thread); work issued after that waits for the
+ * borrower's stream before it reuses the memory.  Not allowed during a
+ * capture.  tx_dlpack_release calls the deleter of any such structure. */
+enum { TX_DL_F32 = 0, TX_DL_I64 = 1, TX_DL_BOOL = 2 };
+int tx_dlpack_export(tx_ctx *ctx, void *d_block, void *d_data, int dtype, const int64_t *shape, int ndim,
+                     void *stream, void **out);
+int tx_dlpack_release(void *managed);
+
 /* =========================================================================
  * Device memory (replaces Burn tensor storage behind DynTensor,
  * crates/tynx/src/tensor.rs:156-185).  Stream-ordered caching allocator.
@@ -369,6 +383,72 @@ int tx_attention_bwd(tx_ctx *ctx, const float *d_q, const float *d_k, const floa
                      const float *d_dout, int64_t ld_dout, float *d_dq, float *d_dk, float *d_dv,
                      int64_t ld_grad, int64_t batch, int64_t seq, int64_t heads, int64_t head_dim,
                      float scale, int flags);
+
+/* Rotary positions.  Of each head's head_dim elements the first `dim` (even)
+ * form dim / 2 pairs, (i, i + dim/2) or, interleaved, (2i, 2i + 1); pair i of
+ * a token at position p turns by p * turns[i] full turns, and both results are
+ * multiplied by `factor`; the other elements pass through.  x and y are
+ * [batch, seq, heads, head_dim], head_dim 1..256.  d_pos holds int64 positions
+ * (any value; angles are reduced in 64 bits): pos_stride 0 for one [seq] list,
+ * seq for [batch, seq]; NULL counts each sequence from 0.  `inverse` turns
+ * back (same factor): the gradient of the forward call.
+ * It has no counterpart in the reference, whose imported graphs carry learned
+ * position tables (Gather). */
+#define TX_ROTARY_PAIRS 128
+typedef struct tx_rotary {
+  int32_t dim, interleaved;
+  float factor;
+  double turns[TX_ROTARY_PAIRS];
+} tx_rotary;
+int tx_rotary_apply(tx_ctx *ctx, const float *d_x, float *d_y, int64_t batch, int64_t seq, int64_t heads,
+                    int64_t head_dim, const int64_t *d_pos, int64_t pos_stride, const tx_rotary *rotary,
+                    int inverse);
+/* Root-mean-square norm of each query and key head, x * rsqrt(mean(x^2) + eps)
+ * * weight[head_dim], and the rotation above, in one pass over q
+ * [batch, seq, heads, head_dim] and k [batch, seq, kv_heads, head_dim].  The
+ * backward takes the inputs again and writes the gradients of both inputs and
+ * both weights (sums in a fixed order). */
+int tx_qk_norm_rotary_fwd(tx_ctx *ctx, const float *d_q, const float *d_k, const float *d_q_weight,
+                          const float *d_k_weight, float *d_q_out, float *d_k_out, int64_t batch, int64_t seq,
+                          int64_t heads, int64_t kv_heads, int64_t head_dim, const int64_t *d_pos,
+                          int64_t pos_stride, const tx_rotary *rotary, float eps);
+int tx_qk_norm_rotary_bwd(tx_ctx *ctx, const float *d_q, const float *d_k, const float *d_q_weight,
+                          const float *d_k_weight, const float *d_dq_out, const float *d_dk_out, float *d_dq,
+                          float *d_dk, float *d_dq_weight, float *d_dk_weight, int64_t batch, int64_t seq,
+                          int64_t heads, int64_t kv_heads, int64_t head_dim, const int64_t *d_pos,
+                          int64_t pos_stride, const tx_rotary *rotary, float eps);
+
+/* Differential attention, the difference of two softmax maps per head:
+ *   out = softmax(scale q1 k1^T) v - lam[h] softmax(scale q2 k2^T) v
+ * over q [batch, queries, 2 * heads, dim] and k [batch, keys, 2 * kv_heads,
+ * dim] (the maps of head h at 2h and 2h + 1), v [batch, keys, kv_heads, vdim]
+ * and lam [heads]; heads / kv_heads (whole) query heads share each key head;
+ * dim 1..64, vdim 1..128.  Query i sees key j when j < key_lengths[b] (int64
+ * per sequence, NULL: all keys; a length outside [0, keys] raises the device
+ * error flag and counts as the nearest bound) and, with causal, j <= i +
+ * query_start.  Keys and values behind a sequence's length are not read.  A
+ * query that sees no key gives zeros and takes no gradient.
+ * The forward writes out [batch, queries, heads, vdim] and, for a backward,
+ * out2 (the second map's own output, same shape) and lse [batch, 2 * heads,
+ * queries] (log2 of each row's sum of exponentials; +inf where no key is
+ * seen); both NULL without one.  The backward reads out, out2, lse and dout
+ * and writes dq (unless NULL), dk and dv (unless both NULL) and dlam (unless
+ * NULL), sums in a fixed order.  fp32-class results in every math mode.
+ * The reference has softmax attention as composed nodes only
+ * (crates/tynx/src/interpreter/softmax.rs:9-17). */
+typedef struct tx_diff_attention {
+  int64_t batch, queries, keys, heads, kv_heads, dim, vdim;
+  const float *q, *k, *v, *lam;
+  const int64_t *key_lengths;
+  float scale;
+  int32_t causal;
+  int64_t query_start;
+  float *out, *out2, *lse;
+  const float *dout;
+  float *dq, *dk, *dv, *dlam;
+} tx_diff_attention;
+int tx_diff_attention_fwd(tx_ctx *ctx, const tx_diff_attention *desc);
+int tx_diff_attention_bwd(tx_ctx *ctx, const tx_diff_attention *desc);
 
 /* Clipped-surrogate PPO objective over [rows, cols] policy logits (cols <=
  * 64), per-row value estimates, int64 actions, behaviour log-probabilities,

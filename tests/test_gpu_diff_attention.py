@@ -1,0 +1,278 @@
+"""Differential attention against 64-bit numpy.
+
+Tolerances.  A product's operands carry at least 16 bits (a bf16 head and
+tail): each is within 2^-18 of its value and the product of the two tails is
+left out, 3 * 2^-18 of |a b| a product in all, E below.  So with c_ij = scale
+sum |q k| a score is within E c_ij, a weight within 2 E max_j c_ij of itself
+(numerator and sum), and an output within sum_j (a1 + |lam| a2) |v| times that
+and E for its own product.  The gradients' bounds follow the same way through
+dP (E sum |dO| |v|), D (the outputs' bound), dS and the last product.  Sums in
+fp32 add less than a tenth of this.  Those bounds are for the worst case at
+every element; over a whole tensor errors of this kind are independent, about
+1e-6 of its norm, and 1e-5 is allowed.
+"""
+
+import numpy as np
+import pytest
+
+pytestmark = pytest.mark.gpu
+
+E = 3 * 2.0**-18
+
+
+def reference(q, k, v, lam, dout, scale, causal, start, lengths):
+    """Values and elementwise error bounds of (out, dq, dk, dv, dlam)."""
+    B, T, H2, d = q.shape
+    S, Hk = k.shape[1], k.shape[2] // 2
+    H, dv = H2 // 2, v.shape[3]
+    q, k, v, lam, dout = (a.astype(np.float64) for a in (q, k, v, lam, dout))
+    val = [np.zeros((B, T, H, dv)), np.zeros_like(q), np.zeros_like(k), np.zeros_like(v), np.zeros(H)]
+    tol = [np.zeros_like(a) for a in val]
+    i, j = np.arange(T)[:, None], np.arange(S)[None, :]
+    for b in range(B):
+        n = S if lengths is None else int(lengths[b])
+        ok = (j < n) & ((j <= i + start) if causal else True)
+        ok = np.broadcast_to(ok, (T, S))[:, :n]
+        if n == 0:
+            continue
+        for h in range(H):
+            kv = h // (H // Hk)
+            vv, g = v[b, :n, kv], dout[b, :, h]
+            a, ea = [], []
+            for m in range(2):
+                qm, km = q[b, :, 2 * h + m], k[b, :n, 2 * kv + m]
+                s = np.where(ok, qm @ km.T * scale, -np.inf)
+                top = s.max(-1, keepdims=True)
+                p = np.where(ok, np.exp(s - np.where(np.isfinite(top), top, 0.0)), 0.0)
+                a.append(p / np.maximum(p.sum(-1, keepdims=True), 1e-300))
+                c = np.abs(qm) @ np.abs(km).T * abs(scale)
+                ea.append(2 * E * np.where(ok, c, 0.0).max(-1, keepdims=True) + 4e-7)  # relative error of the weights
+            w = a[0] - lam[h] * a[1]
+            ew = a[0] * ea[0] + abs(lam[h]) * a[1] * ea[1]
+            wabs = a[0] + abs(lam[h]) * a[1]
+            val[0][b, :, h] = w @ vv
+            tol[0][b, :, h] = (ew + E * wabs) @ np.abs(vv)
+            dp = g @ vv.T
+            edp = E * np.abs(g) @ np.abs(vv).T
+            val[3][b, :n, kv] += w.T @ g
+            tol[3][b, :n, kv] += (ew + E * wabs).T @ np.abs(g)
+            for m in range(2):
+                f = scale if m == 0 else -lam[h] * scale
+                D = (a[m] * dp).sum(-1, keepdims=True)
+                eD = ((a[m] * (ea[m] + E)) @ np.abs(vv) * np.abs(g)).sum(-1, keepdims=True)
+                ds = a[m] * (dp - D) * f
+                eds = abs(f) * a[m] * (edp + eD + (ea[m] + 4e-7) * np.abs(dp - D))
+                val[1][b, :, 2 * h + m] = ds @ k[b, :n, 2 * kv + m]
+                tol[1][b, :, 2 * h + m] = (eds + E * np.abs(ds)) @ np.abs(k[b, :n, 2 * kv + m])
+                val[2][b, :n, 2 * kv + m] += ds.T @ q[b, :, 2 * h + m]
+                tol[2][b, :n, 2 * kv + m] += (eds + E * np.abs(ds)).T @ np.abs(q[b, :, 2 * h + m])
+                if m == 1:
+                    val[4][h] -= D.sum()
+                    tol[4][h] += eD.sum() + 1e-5 * np.abs(D).sum()
+    return val, tol
+
+
+def check(got, val, tol):
+    for name, g, w, t in zip(("out", "dq", "dk", "dv", "dlam"), got, val, tol):
+        g = g.numpy().astype(np.float64)
+        assert g.shape == w.shape and np.isfinite(g).all(), name
+        off = np.abs(g - w)
+        assert np.all(off <= 1.1 * t + 1e-30), (name, float((off / (t + 1e-30)).max()))
+        norm = np.linalg.norm(w)
+        if norm > 1e-3:
+            assert np.linalg.norm(g - w) <= 1e-5 * norm, (name, np.linalg.norm(g - w) / norm)
+
+
+def call(q, k, v, lam, dout, **kw):
+    import tynx_b200 as tx
+
+    leaves = [tx.Tensor(a, requires_grad=True) for a in (q, k, v, lam)]
+    lengths = kw.pop("lengths")
+    out = tx.nn.functional.differential_attention(
+        *leaves, key_lengths=None if lengths is None else tx.Tensor(np.asarray(lengths, np.int64)), **kw)
+    out.backward(tx.Tensor(dout))
+    return [out.detach()] + [t.grad for t in leaves]
+
+
+def arrays(B, T, S, H, Hk, d, dv, seed):
+    rng = np.random.default_rng(seed)
+    n = lambda *s: rng.standard_normal(s).astype(np.float32)  # noqa: E731
+    return n(B, T, 2 * H, d), n(B, S, 2 * Hk, d), n(B, S, Hk, dv), rng.random(H).astype(np.float32), n(B, T, H, dv)
+
+
+CASES = [
+    # B, T, S, H, Hk, d, dv, causal, start, lengths
+    (1, 1, 1, 1, 1, 1, 1, False, 0, None),
+    (2, 1, 7, 2, 1, 8, 16, False, 0, None),
+    (2, 5, 5, 3, 3, 40, 72, True, 0, None),
+    (1, 64, 64, 2, 2, 64, 128, False, 0, None),
+    (1, 128, 128, 1, 1, 64, 128, True, 0, None),
+    (2, 129, 129, 2, 1, 64, 128, True, 0, [129, 65]),
+    (3, 33, 200, 4, 2, 32, 64, True, 167, [200, 0, 1]),
+    (2, 200, 31, 2, 2, 64, 64, True, -169, None),   # the first rows see nothing
+    (1, 70, 300, 6, 2, 63, 127, False, 0, [257]),
+    (4, 100, 100, 3, 1, 64, 128, True, 0, [0, 1, 63, 100]),
+    (1, 300, 513, 2, 2, 16, 32, True, 40, None),
+    (2, 3, 130, 8, 2, 64, 128, True, 127, [130, 64]),
+    (1, 257, 640, 1, 1, 64, 100, False, 0, None),
+]
+
+
+@pytest.mark.parametrize("case", CASES, ids=lambda c: "x".join(map(str, c[:7])))
+def test_values_and_gradients(case):
+    B, T, S, H, Hk, d, dv, causal, start, lengths = case
+    q, k, v, lam, dout = arrays(B, T, S, H, Hk, d, dv, T + S)
+    val, tol = reference(q, k, v, lam, dout, d ** -0.5, causal, start, lengths)
+    check(call(q, k, v, lam, dout, causal=causal, query_start=start, lengths=lengths), val, tol)
+
+
+@pytest.mark.parametrize("queries", [1, 3])
+@pytest.mark.parametrize("keys", [1, 63, 64, 65, 1000, 5000])
+def test_few_queries_against_many_keys(queries, keys):
+    import tynx_b200 as tx
+
+    q, k, v, lam, dout = arrays(3, queries, keys, 4, 2, 64, 128, keys)
+    lengths = [keys, max(0, keys - 7), keys // 2]
+    val, tol = reference(q, k, v, lam, dout, 0.125, False, 0, lengths)
+    with tx.no_grad():
+        out = tx.nn.functional.differential_attention(*(tx.Tensor(a) for a in (q, k, v, lam)),
+                                                      key_lengths=tx.Tensor(np.array(lengths)))
+    check([out], val[:1], tol[:1])
+
+
+def test_what_lies_behind_a_length_is_not_read():
+    q, k, v, lam, dout = arrays(2, 70, 150, 2, 1, 64, 128, 5)
+    lengths = [149, 70]
+    kw = dict(causal=False, query_start=0, lengths=lengths)
+    clean = call(q, k, v, lam, dout, **kw)
+    for b, n in enumerate(lengths):
+        k[b, n:] = np.nan
+        v[b, n:] = np.inf
+    for a, b in zip(clean, call(q, k, v, lam, dout, **kw)):
+        np.testing.assert_array_equal(a.numpy(), b.numpy())
+
+
+def test_queries_without_keys_give_zeros():
+    q, k, v, lam, dout = arrays(2, 6, 4, 2, 2, 16, 32, 6)
+    got = call(q, k, v, lam, dout, causal=True, query_start=None, lengths=None)  # the first two see nothing
+    np.testing.assert_array_equal(got[0].numpy()[:, :2], 0.0)
+    np.testing.assert_array_equal(got[1].numpy()[:, :2], 0.0)
+    got = call(q, k, v, lam, dout, causal=False, query_start=None, lengths=[0, 0])
+    for t in got:
+        np.testing.assert_array_equal(t.numpy(), 0.0)
+
+
+def test_no_keys_at_all():
+    q, k, v, lam, dout = arrays(2, 3, 0, 2, 2, 16, 32, 7)
+    for t in call(q, k, v, lam, dout, causal=False, query_start=None, lengths=None):
+        np.testing.assert_array_equal(t.numpy(), 0.0)
+
+
+def test_large_scores_stay_finite():
+    """Scores of several hundred: the running maximum keeps every exponential at most 1."""
+    q, k, v, lam, dout = arrays(1, 140, 300, 2, 2, 64, 128, 8)
+    q *= 40.0
+    got = call(q, k, v, lam, dout, causal=True, query_start=160, lengths=None)
+    val, tol = reference(q, k, v, lam, dout, 0.125, True, 160, None)
+    for g, w, t in zip(got, val, tol):
+        assert np.isfinite(g.numpy()).all()
+        assert np.all(np.abs(g.numpy() - w) <= 1.1 * t + 1e-30)
+
+
+def test_lengths_outside_the_keys_raise():
+    import tynx_b200 as tx
+
+    q, k, v, lam, _ = (tx.Tensor(a) for a in arrays(2, 3, 5, 2, 2, 16, 32, 9))
+    for bad in ([5, 6], [-1, 5]):
+        tx.nn.functional.differential_attention(q, k, v, lam, key_lengths=tx.Tensor(np.array(bad)))
+        with pytest.raises(IndexError):
+            tx.synchronize()
+    tx.synchronize()
+
+
+def test_gradient_agrees_with_differences():
+    import tynx_b200 as tx
+
+    data = list(arrays(1, 4, 5, 2, 1, 8, 6, 10))
+    dout = data.pop().astype(np.float64)
+    F = tx.nn.functional
+
+    def value(a):
+        with tx.no_grad():
+            return float((F.differential_attention(*(tx.Tensor(x) for x in a), causal=True).numpy() * dout).sum())
+
+    grads = call(*data, dout.astype(np.float32), causal=True, query_start=None, lengths=None)[1:]
+    rng = np.random.default_rng(11)
+    for i, g in enumerate(grads):
+        way = rng.standard_normal(data[i].shape).astype(np.float32)
+        h = 1e-2
+        plus, minus = ([a + (h * s * way if j == i else 0) for j, a in enumerate(data)] for s in (1, -1))
+        slope = (value(plus) - value(minus)) / (2 * h)
+        # third differences h^2 / 6, and 1e-6 of the value over 2 h
+        assert abs(slope - float((g.numpy() * way).sum())) <= 2e-3 * max(1.0, np.abs(g.numpy() * way).sum())
+
+
+def test_same_inputs_give_the_same_bits():
+    q, k, v, lam, dout = arrays(2, 150, 400, 4, 2, 64, 128, 12)
+    kw = dict(causal=True, query_start=250, lengths=[400, 333])
+    for a, b in zip(call(q, k, v, lam, dout, **kw), call(q, k, v, lam, dout, **kw)):
+        np.testing.assert_array_equal(a.numpy(), b.numpy())
+
+
+def test_layer_of_all_three_trains_and_replays():
+    """Projections, norms with rotation, differential attention and a loss, eager and as a
+    captured step replayed on other inputs, against each other and the 64-bit composition."""
+    import tynx_b200 as tx
+
+    F = tx.nn.functional
+    B, T, E_, H, Hk, d, dv = 2, 37, 48, 4, 2, 16, 32
+    rng = np.random.default_rng(13)
+    shapes = [(E_, 2 * H * d), (E_, 2 * Hk * d), (E_, Hk * dv)]
+    weights = [rng.standard_normal(s).astype(np.float32) / 7 for s in shapes] + \
+        [np.ones(d, np.float32), np.ones(d, np.float32), np.full(H, 0.5, np.float32)]
+    params = [tx.Tensor(w, requires_grad=True) for w in weights]
+    rotary = tx.nn.Rotary(d)
+    tx.set_math_mode("3xtf32")
+    try:
+        def step(x, y):
+            for p in params:
+                p.grad = None
+            q = (x @ params[0]).reshape(B, T, 2 * H, d)
+            k = (x @ params[1]).reshape(B, T, 2 * Hk, d)
+            v = (x @ params[2]).reshape(B, T, Hk, dv)
+            q, k = F.qk_norm_rotary(q, k, params[3], params[4], rotary)
+            out = F.differential_attention(q, k, v, params[5], causal=True)
+            loss = F.mse_loss(out, y)
+            loss.backward()
+            return [loss] + [p.grad for p in params]
+
+        compiled = tx.compile(step, fullgraph=True)
+        for seed in (0, 1, 2):
+            r = np.random.default_rng(seed)
+            x = tx.Tensor(r.standard_normal((B * T, E_)).astype(np.float32))
+            y = tx.Tensor(r.standard_normal((B, T, H, dv)).astype(np.float32))
+            replayed = [t.numpy() for t in compiled(x, y)]
+            eager = [t.numpy() for t in step(x, y)]
+            for a, b in zip(replayed, eager):
+                np.testing.assert_array_equal(a, b)
+        assert compiled.replay_count == 2
+        # the 64-bit composition of the last step
+        from tests.test_gpu_rotary import norm_reference, turned  # noqa: F401
+
+        x64, y64 = x.numpy().astype(np.float64), y.numpy().astype(np.float64)
+        q, k, v = (x64 @ w for w in weights[:3])
+        q, k, v = q.reshape(B, T, 2 * H, d), k.reshape(B, T, 2 * Hk, d), v.reshape(B, T, Hk, dv)
+        positions = np.broadcast_to(np.arange(T), (B, T))
+        qn, kn = (norm_reference(a, np.ones(d), rotary, positions, 1e-6, np.zeros_like(a))[0] for a in (q, k))
+        out = reference(qn, kn, v, weights[5], np.zeros((B, T, H, dv)), d ** -0.5, True, 0, None)[0][0]
+        dout = 2 * (out - y64) / out.size
+        val = reference(qn, kn, v, weights[5], dout, d ** -0.5, True, 0, None)[0]
+        dq = norm_reference(q, np.ones(d), rotary, positions, 1e-6, val[1])
+        dk = norm_reference(k, np.ones(d), rotary, positions, 1e-6, val[2])
+        want = [((out - y64) ** 2).mean().reshape(1), x64.T @ dq[1].reshape(B * T, -1), x64.T @ dk[1].reshape(B * T, -1),
+                x64.T @ val[3].reshape(B * T, -1), dq[2], dk[2], val[4]]
+        for name, a, b in zip(("loss", "wq", "wk", "wv", "qw", "kw", "lam"), eager, want):
+            # a chain of five stages of 1e-5 each
+            assert np.linalg.norm(a - b) <= 5e-5 * np.linalg.norm(b), (name, np.linalg.norm(a - b) / np.linalg.norm(b))
+    finally:
+        tx.set_math_mode("tf32")

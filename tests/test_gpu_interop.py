@@ -1,0 +1,95 @@
+"""Zero-copy exchange with torch in both directions."""
+
+import gc
+
+import numpy as np
+import pytest
+
+pytestmark = pytest.mark.gpu
+
+
+def test_both_directions_share_memory():
+    import torch
+
+    import tynx_b200 as tx
+
+    for array in (np.arange(12, dtype=np.float32).reshape(3, 4), np.arange(6), np.array([True, False]),
+                  np.zeros((2, 0, 3), np.float32)):
+        there = torch.from_dlpack(tx.Tensor(array))
+        np.testing.assert_array_equal(there.cpu().numpy(), array)
+        back = tx.from_dlpack(there)
+        assert back.shape == array.shape
+        np.testing.assert_array_equal(back.numpy(), array)
+    t = torch.zeros(5, device="cuda")
+    mine = tx.from_dlpack(t)
+    t += 2.0
+    torch.cuda.synchronize()
+    np.testing.assert_array_equal(mine.numpy(), 2.0)
+    assert torch.from_dlpack((mine * 3.0)).sum().item() == 30.0
+
+
+def test_order_of_the_streams():
+    """Results are handed over without a synchronisation on either side."""
+    import torch
+
+    import tynx_b200 as tx
+
+    a = torch.randn(2048, 2048, device="cuda")
+    for _ in range(20):
+        b = a @ a  # queued on torch's stream
+        mine = tx.from_dlpack(b)
+        c = torch.from_dlpack(mine + 1.0)
+        assert torch.equal(c, b + 1.0)
+
+
+def test_lent_memory_is_reused_only_after_the_borrower():
+    import torch
+
+    import tynx_b200 as tx
+
+    side = torch.cuda.Stream()
+    for i in range(10):
+        with torch.cuda.stream(side):
+            there = torch.from_dlpack(tx.ones(1 << 20) * float(i))
+            torch.cuda._sleep(2_000_000)  # the borrower reads late
+            copy = there.clone()
+            del there
+        gc.collect()
+        spoil = [tx.zeros(1 << 20) for _ in range(3)]
+        side.synchronize()
+        assert copy.min().item() == copy.max().item() == float(i)
+        del spoil
+
+
+def test_the_owner_may_go_first():
+    import torch
+
+    import tynx_b200 as tx
+
+    mine = tx.ones(1000)
+    there = torch.from_dlpack(mine)
+    view = torch.from_dlpack(mine.reshape(10, 100))
+    del mine
+    others = [tx.zeros(1000) for _ in range(4)]
+    tx.synchronize()
+    assert there.sum().item() == 1000.0 and view.sum().item() == 1000.0
+    del others
+
+
+def test_refusals():
+    import torch
+
+    import tynx_b200 as tx
+
+    with pytest.raises(ValueError, match="contiguous"):
+        tx.from_dlpack(torch.zeros(4, 6, device="cuda").t())
+    with pytest.raises(ValueError, match="float32, int64 or bool"):
+        tx.from_dlpack(torch.zeros(4, device="cuda", dtype=torch.float16))
+    with pytest.raises(ValueError, match="CUDA tensors"):
+        tx.from_dlpack(torch.zeros(4))
+    with pytest.raises(BufferError, match="detach"):
+        torch.from_dlpack(tx.ones(3).requires_grad_())
+    with pytest.raises(ValueError, match="owns its memory"):
+        tx.from_dlpack(torch.zeros(4, device="cuda")).__dlpack__()
+    tx.ones(3).__dlpack__()  # a capsule that nobody takes ends its loan
+    tx.synchronize()

@@ -23,11 +23,12 @@ int64 = "int64"
 bool = "bool"  # noqa: A001  (mirrors tynx.bool)
 
 _FROM = {
-    "._core": ("Device", "Prefetcher", "Tensor", "arange", "cat", "full", "full_like",
+    "._core": ("Device", "Prefetcher", "Tensor", "arange", "backward", "cat", "full", "full_like",
                "get_default_device", "is_grad_enabled", "matmul", "maximum", "minimum", "no_grad",
                "ones", "ones_like", "pinned", "rand", "randn", "set_math_mode", "synchronize",
                "tensor", "zeros", "zeros_like"),
     ".compiler": ("CompiledFunction", "compile"),
+    ".interop": ("from_dlpack",),
     ".imported": ("Buffer", "ImportedModel", "Parameter", "Session", "load"),
     ".checkpoint": ("save_checkpoint", "load_checkpoint"),
     ".onnx.ir": ("TrainabilityReport",),

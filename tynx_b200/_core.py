@@ -414,6 +414,15 @@ class Tensor:
             self.ctx.check(lib.tx_d2h(self.ctx.handle, out.ctypes.data, self.ptr, out.nbytes), "d2h")
         return out
 
+    def __dlpack__(self, *, stream=None, **unused):
+        """Lend this tensor to another library (``torch.from_dlpack(tensor)``)."""
+        from .interop import export
+
+        return export(self, stream)
+
+    def __dlpack_device__(self) -> tuple:
+        return (2, self.ctx.index)
+
     def tolist(self):
         return self.numpy().tolist()
 
@@ -1099,6 +1108,20 @@ def run_backward(roots: list, retain_graph: bool = False) -> None:
                 _accumulate(grads, (id(parent._fn), parent._out_index), g)
         if not retain_graph:
             fn.free()
+
+
+def backward(tensors: Sequence[Tensor], gradients: Sequence[Tensor], retain_graph: bool = False) -> None:
+    """One reverse sweep from several tensors with their gradients (the sweep of
+    :meth:`Tensor.backward`, for functions with more than one output)."""
+    tensors, gradients = list(tensors), list(gradients)
+    if len(tensors) != len(gradients):
+        raise ValueError(f"backward() got {len(tensors)} tensors and {len(gradients)} gradients")
+    for t, g in zip(tensors, gradients):
+        if not t.requires_grad:
+            raise ValueError("backward() called on a tensor that does not require gradients")
+        if g.shape != t.shape or g.dtype != "float32":
+            raise ValueError(f"backward() needs a float32 gradient of shape {t.shape}, got {g.dtype} {g.shape}")
+    run_backward(list(zip(tensors, gradients)), retain_graph=retain_graph)
 
 
 def _accumulate_leaf(t: Tensor, g: Tensor) -> None:

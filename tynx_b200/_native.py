@@ -33,6 +33,8 @@ TX_ERR_CAPTURE = 10
 
 TX_MATH = {"tf32": 0, "3xtf32": 1, "fp32": 2, "tf32trunc": 3}
 MAX_DIMS = 8
+ROTARY_PAIRS = 128
+DL_TYPES = {"float32": 0, "int64": 1, "bool": 2}
 
 ACT = {"none": 0, "relu": 1, "tanh": 2, "gelu": 3}
 TX_GEMM_A_TF32, TX_GEMM_B_TF32, TX_GEMM_ROUND_OUT, TX_GEMM_EXACT, TX_GEMM_A_SHARED = 1, 2, 4, 8, 16
@@ -100,6 +102,23 @@ class OptimCfg(C.Structure):
     ]
 
 
+class RotaryDesc(C.Structure):
+    _fields_ = [("dim", C.c_int32), ("interleaved", C.c_int32), ("factor", C.c_float),
+                ("turns", C.c_double * ROTARY_PAIRS)]
+
+
+class DiffAttentionDesc(C.Structure):
+    _fields_ = [
+        ("batch", C.c_int64), ("queries", C.c_int64), ("keys", C.c_int64), ("heads", C.c_int64),
+        ("kv_heads", C.c_int64), ("dim", C.c_int64), ("vdim", C.c_int64),
+        ("q", C.c_void_p), ("k", C.c_void_p), ("v", C.c_void_p), ("lam", C.c_void_p),
+        ("key_lengths", C.c_void_p), ("scale", C.c_float), ("causal", C.c_int32),
+        ("query_start", C.c_int64),
+        ("out", C.c_void_p), ("out2", C.c_void_p), ("lse", C.c_void_p), ("dout", C.c_void_p),
+        ("dq", C.c_void_p), ("dk", C.c_void_p), ("dv", C.c_void_p), ("dlam", C.c_void_p),
+    ]
+
+
 _vp = C.c_void_p
 _i64 = C.c_int64
 _i32 = C.c_int
@@ -118,6 +137,8 @@ SIGNATURES = {
     "tx_last_error": [_vp, C.c_char_p, C.c_size_t],
     "tx_sync": [_vp, C.c_uint64],
     "tx_stream": [_vp, C.POINTER(_vp)],
+    "tx_dlpack_export": [_vp, _vp, _vp, _i32, _p64, _i32, _vp, C.POINTER(_vp)],
+    "tx_dlpack_release": [_vp],
     "tx_alloc": [_vp, C.c_size_t, C.POINTER(_vp)],
     "tx_free": [_vp, _vp],
     "tx_h2d": [_vp, _vp, _vp, C.c_size_t],
@@ -167,6 +188,13 @@ SIGNATURES = {
     "tx_attention_fwd": [_vp, _vp, _vp, _vp, _i64, _vp, _i64, _i64, _i64, _i64, _i64, _f, _i32],
     "tx_attention_bwd": [_vp, _vp, _vp, _vp, _i64, _vp, _i64, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64,
                          _f, _i32],
+    "tx_rotary_apply": [_vp, _vp, _vp, _i64, _i64, _i64, _i64, _vp, _i64, C.POINTER(RotaryDesc), _i32],
+    "tx_qk_norm_rotary_fwd": [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _vp, _i64,
+                              C.POINTER(RotaryDesc), _f],
+    "tx_qk_norm_rotary_bwd": [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64,
+                              _i64, _vp, _i64, C.POINTER(RotaryDesc), _f],
+    "tx_diff_attention_fwd": [_vp, C.POINTER(DiffAttentionDesc)],
+    "tx_diff_attention_bwd": [_vp, C.POINTER(DiffAttentionDesc)],
     "tx_ppo_loss_fwd": [_vp, _vp, _i64, _i64, _vp, _vp, _vp, _vp, _vp, _f, _f, _f, _vp],
     "tx_ppo_loss_bwd": [_vp, _vp, _i64, _i64, _vp, _vp, _vp, _vp, _vp, _f, _f, _f, _vp, _vp, _vp, _i32,
                         _i32],

@@ -5,6 +5,7 @@
 #include <stdint.h>
 
 #include <map>
+#include <mutex>
 #include <string>
 #include <unordered_map>
 #include <unordered_set>
@@ -31,6 +32,13 @@ struct tx_allocator {
   tx_arena *arena = nullptr;  // non-null while capturing
   std::unordered_map<void *, tx_arena *> arena_owner;
   std::vector<void *> quarantine;  // eager blocks freed during a capture
+  // Blocks lent to other libraries (tx_dlpack_export): borrowers of each block
+  // beside its owner, and the loans that ended, with the stream of each, since
+  // the owner's thread last called.  Other threads touch `ended` only, under
+  // the lock.
+  std::unordered_map<void *, int> lent;
+  std::mutex lock;
+  std::vector<std::pair<void *, cudaStream_t>> ended;
 };
 
 struct tx_ctx {
@@ -45,6 +53,7 @@ struct tx_ctx {
   int *d_err = nullptr;  // device error flag [4]
   uint64_t *d_rng = nullptr;  // call counter of the dropout stream
   bool capturing = false;
+  cudaEvent_t order = nullptr;  // joins the compute stream with another library's
   // data parallel
   void *nccl = nullptr;
   int world = 1, rank = 0;
@@ -80,6 +89,20 @@ int tx_cuda_fail(tx_ctx *ctx, cudaError_t err, const char *what);
 // ---- allocation (stream ordered on ctx->stream) -----------------------------
 void *tx_alloc_raw(tx_ctx *ctx, size_t bytes);
 void tx_free_raw(tx_ctx *ctx, void *p);
+
+// Makes the context's device the calling thread's current one for a scope.
+struct DeviceScope {
+  int before = -1, mine;
+  explicit DeviceScope(const tx_ctx *c) : mine(c->device) {
+    if (cudaGetDevice(&before) != cudaSuccess) before = -1;
+    if (before != mine) cudaSetDevice(mine);
+  }
+  ~DeviceScope() {
+    if (before >= 0 && before != mine) cudaSetDevice(before);
+  }
+  DeviceScope(const DeviceScope &) = delete;
+  DeviceScope &operator=(const DeviceScope &) = delete;
+};
 
 // RAII scratch buffer from the context allocator.
 struct Scratch {

@@ -180,8 +180,11 @@ static void release_cached(tx_ctx *ctx) {
   ctx->alloc.cached = 0;
 }
 
+void tx_collect_loans(tx_ctx *ctx);  // dlpack.cpp
+
 void *tx_alloc_raw(tx_ctx *ctx, size_t bytes) {
   tx_allocator &A = ctx->alloc;
+  tx_collect_loans(ctx);
   if (A.arena) return arena_alloc(ctx, A.arena, bytes);
   size_t cls = size_class(bytes);
   auto it = A.free_blocks.find(cls);
@@ -216,6 +219,13 @@ void tx_free_raw(tx_ctx *ctx, void *p) {
   if (A.arena_owner.count(p)) return;  // arena memory lives as long as its exec
   auto it = A.live.find(p);
   if (it == A.live.end()) return;
+  if (!A.lent.empty()) {  // the last of the owner and the borrowers frees the block
+    auto b = A.lent.find(p);
+    if (b != A.lent.end()) {
+      if (--b->second == 0) A.lent.erase(b);
+      return;
+    }
+  }
   size_t cls = it->second;
   A.live.erase(it);
   A.in_use -= cls;
@@ -413,6 +423,7 @@ extern "C" int tx_ctx_destroy(tx_ctx *ctx) {
   for (void *p : ctx->alloc.quarantine) cudaFree(p);
   cudaFree(ctx->d_err);
   cudaFree(ctx->d_rng);
+  if (ctx->order) cudaEventDestroy(ctx->order);
   cudaStreamDestroy(ctx->stream);
   cudaStreamDestroy(ctx->comm);
   delete ctx;

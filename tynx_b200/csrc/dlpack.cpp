@@ -1,0 +1,113 @@
+// Zero-copy exchange of device tensors with other libraries in one process
+// (the DLPack in-memory structure), ordered on the streams of both sides.
+//
+// A lent block stays out of the allocator's free lists until its owner and
+// every borrower are done with it.  A loan may end on any thread (whichever
+// drops the borrowed tensor): that only notes it; the context's own thread
+// collects the note on its next allocation, makes the compute stream wait for
+// the borrower's stream, and frees the block in stream order.
+#include <new>
+
+#include "common.h"
+
+namespace {
+
+// The structure's layout is the protocol's (version without a header).
+struct DlDevice {
+  int32_t type, id;
+};
+struct DlType {
+  uint8_t code, bits;
+  uint16_t lanes;
+};
+struct DlTensor {
+  void *data;
+  DlDevice device;
+  int32_t ndim;
+  DlType dtype;
+  int64_t *shape, *strides;
+  uint64_t byte_offset;
+};
+struct DlManaged {
+  DlTensor t;
+  void *owner;
+  void (*deleter)(DlManaged *);
+};
+
+struct Loan {
+  DlManaged managed;
+  int64_t shape[TX_MAX_DIMS];
+  tx_ctx *ctx;
+  void *block;
+  cudaStream_t borrower;
+};
+
+void end_loan(DlManaged *m) {
+  Loan *loan = static_cast<Loan *>(m->owner);
+  {
+    std::lock_guard<std::mutex> hold(loan->ctx->alloc.lock);
+    loan->ctx->alloc.ended.push_back({loan->block, loan->borrower});
+  }
+  delete loan;
+}
+
+int join(tx_ctx *ctx, cudaStream_t first, cudaStream_t then) {
+  if (!ctx->order) TX_CUDA(ctx, cudaEventCreateWithFlags(&ctx->order, cudaEventDisableTiming));
+  TX_CUDA(ctx, cudaEventRecord(ctx->order, first));
+  TX_CUDA(ctx, cudaStreamWaitEvent(then, ctx->order, 0));
+  return TX_OK;
+}
+
+}  // namespace
+
+void tx_collect_loans(tx_ctx *ctx) {
+  if (ctx->capturing) return;  // a capture cannot wait for work outside it
+  std::vector<std::pair<void *, cudaStream_t>> ended;
+  {
+    std::lock_guard<std::mutex> hold(ctx->alloc.lock);
+    if (ctx->alloc.ended.empty()) return;
+    ended.swap(ctx->alloc.ended);
+  }
+  DeviceScope device(ctx);
+  for (size_t i = 0; i < ended.size(); ++i) {
+    bool joined = false;  // one wait for each borrowing stream
+    for (size_t j = 0; j < i && !joined; ++j) joined = ended[j].second == ended[i].second;
+    if (!joined) join(ctx, ended[i].second, ctx->stream);
+    tx_free_raw(ctx, ended[i].first);
+  }
+}
+
+extern "C" int tx_dlpack_export(tx_ctx *ctx, void *d_block, void *d_data, int dtype, const int64_t *shape, int ndim,
+                                void *stream, void **out) {
+  if (!ctx || !out) return TX_ERR_INVALID;
+  *out = nullptr;
+  if (ctx->capturing) return tx_fail(ctx, TX_ERR_CAPTURE, "a tensor cannot be exported during a capture");
+  if (dtype < TX_DL_F32 || dtype > TX_DL_BOOL || ndim < 0 || ndim > TX_MAX_DIMS || (ndim && !shape))
+    return tx_fail(ctx, TX_ERR_INVALID, "dlpack export: dtype or rank");
+  if (!ctx->alloc.live.count(d_block))
+    return tx_fail(ctx, TX_ERR_INVALID, "only a tensor that owns its memory can be exported; clone() it first");
+  DeviceScope device(ctx);
+  Loan *loan = new (std::nothrow) Loan();
+  if (!loan) return tx_fail(ctx, TX_ERR_OOM, "dlpack export");
+  if (int rc = join(ctx, ctx->stream, static_cast<cudaStream_t>(stream))) {
+    delete loan;
+    return rc;
+  }
+  static const DlType types[3] = {{2, 32, 1}, {0, 64, 1}, {6, 8, 1}};
+  for (int i = 0; i < ndim; ++i) loan->shape[i] = shape[i];
+  loan->managed.t = DlTensor{d_data, {2 /* CUDA */, ctx->device}, ndim, types[dtype], loan->shape, nullptr, 0};
+  loan->managed.owner = loan;
+  loan->managed.deleter = end_loan;
+  loan->ctx = ctx;
+  loan->block = d_block;
+  loan->borrower = static_cast<cudaStream_t>(stream);
+  ++ctx->alloc.lent[d_block];
+  *out = &loan->managed;
+  return TX_OK;
+}
+
+extern "C" int tx_dlpack_release(void *managed) {
+  DlManaged *m = static_cast<DlManaged *>(managed);
+  if (m && m->deleter) m->deleter(m);
+  return TX_OK;
+}

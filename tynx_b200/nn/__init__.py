@@ -1,5 +1,6 @@
 """Neural-network helpers for imported models (``tynx.nn`` subset on CUDA)."""
 
 from . import functional
+from .rotary import Rotary
 
-__all__ = ["functional"]
+__all__ = ["Rotary", "functional"]

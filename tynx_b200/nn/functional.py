@@ -1,4 +1,4 @@
-"""Loss functions on CUDA (``tynx.nn.functional``).
+"""Loss functions and layers on CUDA (``tynx.nn.functional``).
 
 ``cross_entropy`` keeps the reference's contract
 (``crates/tynx-python/python/tynx/nn/functional.py:133-145``: rank-2 float32 logits,
@@ -10,10 +10,13 @@ taped operations.  ``mse_loss`` follows ``loss.rs:10-23`` / ``functional.py:126-
 from __future__ import annotations
 
 import ctypes as C
+import math
+from typing import Optional
 
 from .. import _native as N
-from .._core import Fn, Tensor, _needs_grad, maximum
+from .._core import Fn, Tensor, _needs_grad, full, maximum
 from .._native import lib
+from .rotary import Rotary
 
 
 def cross_entropy(input: Tensor, target: Tensor, reduction: str = "mean") -> Tensor:
@@ -110,6 +113,182 @@ def ppo_loss(logits: Tensor, values: Tensor, actions: Tensor, old_log_prob: Tens
 
         loss._attach(Fn("ppo_loss", [logits, values], backward))
     return loss
+
+
+def _heads(name: str, what: str, t: Tensor, like: Tensor, heads: str = "heads") -> tuple:
+    if t.dtype != "float32" or t.ndim != 4:
+        raise ValueError(f"{name} {what} must be rank-4 float32 [batch, tokens, {heads}, head_dim], got "
+                         f"{t.dtype} {t.shape}")
+    _same_device(name, what, t, like)
+    return t.shape
+
+
+def _same_device(name: str, what: str, t: Tensor, like: Tensor) -> None:
+    if t.ctx is not like.ctx:
+        raise ValueError(f"{name} {what} is on {t.device}, the other tensors are on {like.device}")
+
+
+def _rotary_positions(name: str, rotary: Rotary, positions, like: Tensor) -> tuple:
+    """(pointer, sequence stride) of the positions of `like`'s tokens."""
+    batch, seq, _, dim = like.shape
+    if not isinstance(rotary, Rotary):
+        raise TypeError(f"{name} rotary must be a Rotary, got {type(rotary).__qualname__}")
+    if not 1 <= dim <= 2 * N.ROTARY_PAIRS:
+        raise NotImplementedError(f"{name} supports head dimensions 1..{2 * N.ROTARY_PAIRS}, got {dim}")
+    if rotary.dim > dim:
+        raise ValueError(f"{name}: the rotary dim {rotary.dim} exceeds the head dimension {dim}")
+    if positions is None:
+        return None, 0
+    if positions.dtype != "int64" or positions.shape not in ((seq,), (batch, seq)):
+        raise ValueError(f"{name} positions must be int64 [{seq}] or [{batch}, {seq}], got "
+                         f"{positions.dtype} {positions.shape}")
+    _same_device(name, "positions", positions, like)
+    return positions.ptr, seq if positions.ndim == 2 else 0
+
+
+def rotary_embedding(input: Tensor, rotary: Rotary, positions: Optional[Tensor] = None) -> Tensor:
+    """Rotate the pairs of every head of ``input [batch, tokens, heads, head_dim]``
+    by the tokens' positions (:class:`~tynx_b200.nn.Rotary`); elements behind
+    ``rotary.dim`` pass through.  ``positions`` is int64 [tokens] or
+    [batch, tokens]; None counts every sequence from 0."""
+    batch, seq, heads, dim = _heads("rotary_embedding", "input", input, input)
+    pos, stride = _rotary_positions("rotary_embedding", rotary, positions, input)
+    ctx, desc = input.ctx, rotary._desc
+    out = Tensor._empty(input.shape, "float32", ctx)
+    ctx.check(lib.tx_rotary_apply(ctx.handle, input.ptr, out.ptr, batch, seq, heads, dim, pos, stride, desc, 0),
+              "rotary_embedding")
+    if _needs_grad(input):
+        held = positions.detach() if positions is not None else None
+
+        def backward(g):
+            dx = Tensor._empty((batch, seq, heads, dim), "float32", ctx)
+            ctx.check(lib.tx_rotary_apply(ctx.handle, g[0].ptr, dx.ptr, batch, seq, heads, dim,
+                                          held.ptr if held is not None else None, stride, desc, 1),
+                      "rotary_embedding backward")
+            return [dx]
+
+        out._attach(Fn("rotary_embedding", [input], backward))
+    return out
+
+
+def qk_norm_rotary(q: Tensor, k: Tensor, q_weight: Tensor, k_weight: Tensor, rotary: Rotary,
+                   positions: Optional[Tensor] = None, eps: float = 1e-6) -> tuple:
+    """Root-mean-square norms of every query and key head, ``x / sqrt(mean(x^2) +
+    eps) * weight``, and the rotation of :func:`rotary_embedding`, as one kernel
+    over ``q [batch, tokens, heads, head_dim]`` and ``k [batch, tokens, kv_heads,
+    head_dim]``; the weights are [head_dim].  Returns both rotated tensors."""
+    name = "qk_norm_rotary"
+    batch, seq, heads, dim = _heads(name, "q", q, q)
+    _heads(name, "k", k, q, "kv_heads")
+    if k.shape[:2] != (batch, seq) or k.shape[3] != dim:
+        raise ValueError(f"{name} k must be [{batch}, {seq}, kv_heads, {dim}], got {k.shape}")
+    for what, w in (("q_weight", q_weight), ("k_weight", k_weight)):
+        if w.dtype != "float32" or w.shape != (dim,):
+            raise ValueError(f"{name} {what} must be a float32 Tensor of shape ({dim},), got {w.dtype} {w.shape}")
+        _same_device(name, what, w, q)
+    if not eps >= 0.0:
+        raise ValueError(f"{name} eps must not be negative, got {eps}")
+    pos, stride = _rotary_positions(name, rotary, positions, q)
+    kv_heads, ctx, desc = k.shape[2], q.ctx, rotary._desc
+    yq, yk = Tensor._empty(q.shape, "float32", ctx), Tensor._empty(k.shape, "float32", ctx)
+    ctx.check(lib.tx_qk_norm_rotary_fwd(ctx.handle, q.ptr, k.ptr, q_weight.ptr, k_weight.ptr, yq.ptr, yk.ptr, batch,
+                                        seq, heads, kv_heads, dim, pos, stride, desc, eps), name)
+    if _needs_grad(q, k, q_weight, k_weight):
+        sq, sk, swq, swk = (t.detach() for t in (q, k, q_weight, k_weight))
+        held = positions.detach() if positions is not None else None
+
+        def backward(g):
+            gq, gk = (t if t is not None else full(s.shape, 0.0, ctx=ctx) for t, s in zip(g, (sq, sk)))
+            dq, dk, dwq, dwk = (Tensor._empty(t.shape, "float32", ctx) for t in (sq, sk, swq, swk))
+            ctx.check(lib.tx_qk_norm_rotary_bwd(ctx.handle, sq.ptr, sk.ptr, swq.ptr, swk.ptr, gq.ptr, gk.ptr, dq.ptr,
+                                                dk.ptr, dwq.ptr, dwk.ptr, batch, seq, heads, kv_heads, dim,
+                                                held.ptr if held is not None else None, stride, desc, eps),
+                      "qk_norm_rotary backward")
+            return [dq, dk, dwq, dwk]
+
+        fn = Fn(name, [q, k, q_weight, k_weight], backward, n_out=2)
+        yq._attach(fn, 0)
+        yk._attach(fn, 1)
+    return yq, yk
+
+
+def differential_attention(q: Tensor, k: Tensor, v: Tensor, lam: Tensor, *, scale: Optional[float] = None,
+                           causal: bool = False, query_start: Optional[int] = None,
+                           key_lengths: Optional[Tensor] = None) -> Tensor:
+    """The difference of two attention maps a head with a learned weight,
+    ``softmax(scale q1 k1^T) v - lam softmax(scale q2 k2^T) v``.
+
+    ``q [batch, queries, 2 * heads, d]`` and ``k [batch, keys, 2 * kv_heads, d]``
+    hold the two maps of head h at 2h and 2h + 1 (the layout that
+    :func:`qk_norm_rotary` returns for twice the heads), ``v [batch, keys,
+    kv_heads, dv]``, ``lam [heads]``; ``heads`` is a multiple of ``kv_heads`` and
+    consecutive query heads share a key head; d <= 64, dv <= 128.  ``scale``
+    defaults to ``d ** -0.5``.
+
+    Query i sees key j if ``j < key_lengths[batch]`` (int64 [batch]; None: every
+    key) and, with ``causal``, ``j <= i + query_start`` (the position of the first
+    query among the keys; None: ``keys - queries``, so that the last query sees
+    every key).  Keys and values behind a sequence's length are never read, within
+    it they must be finite; a query that sees no key returns zeros.  A length
+    outside [0, keys] raises IndexError at the next synchronisation."""
+    name = "differential_attention"
+    batch, queries, maps, d = _heads(name, "q", q, q, "2 * heads")
+    _, keys, kv_maps, _ = _heads(name, "k", k, q, "2 * kv_heads")
+    _heads(name, "v", v, q, "kv_heads")
+    heads, kv_heads = maps // 2, kv_maps // 2
+    if maps % 2 or kv_maps % 2 or not heads or not kv_heads or heads % kv_heads:
+        raise ValueError(f"{name} needs two maps a head and a number of query heads that is a multiple of the key "
+                         f"heads', got {maps} and {kv_maps} maps")
+    if k.shape != (batch, keys, kv_maps, d):
+        raise ValueError(f"{name} k must be [{batch}, keys, 2 * kv_heads, {d}], got {k.shape}")
+    dv = v.shape[3]
+    if v.shape != (batch, keys, kv_heads, dv):
+        raise ValueError(f"{name} v must be [{batch}, {keys}, {kv_heads}, dv], got {v.shape}")
+    if not 1 <= d <= 64 or not 1 <= dv <= 128:
+        raise NotImplementedError(f"{name} supports head dimensions up to 64 and value dimensions up to 128, got "
+                                  f"{d} and {dv}")
+    if lam.dtype != "float32" or lam.shape != (heads,):
+        raise ValueError(f"{name} lam must be a float32 Tensor of shape ({heads},), got {lam.dtype} {lam.shape}")
+    _same_device(name, "lam", lam, q)
+    if key_lengths is not None:
+        if key_lengths.dtype != "int64" or key_lengths.shape != (batch,):
+            raise ValueError(f"{name} key_lengths must be int64 [{batch}], got {key_lengths.dtype} "
+                             f"{key_lengths.shape}")
+        _same_device(name, "key_lengths", key_lengths, q)
+    scale = d ** -0.5 if scale is None else float(scale)
+    if not math.isfinite(scale):
+        raise ValueError(f"{name} scale must be finite, got {scale}")
+    start = keys - queries if query_start is None else int(query_start)
+    ctx = q.ctx
+    out = Tensor._empty((batch, queries, heads, dv), "float32", ctx)
+    desc = N.DiffAttentionDesc(batch=batch, queries=queries, keys=keys, heads=heads, kv_heads=kv_heads, dim=d, vdim=dv,
+                               q=q.ptr, k=k.ptr, v=v.ptr, lam=lam.ptr,
+                               key_lengths=key_lengths.ptr if key_lengths is not None else None, scale=scale,
+                               causal=int(bool(causal)), query_start=start, out=out.ptr)
+    grad = _needs_grad(q, k, v, lam)
+    if grad:
+        out2 = Tensor._empty(out.shape, "float32", ctx)
+        lse = Tensor._empty((batch, maps, queries), "float32", ctx)
+        desc.out2, desc.lse = out2.ptr, lse.ptr
+    ctx.check(lib.tx_diff_attention_fwd(ctx.handle, desc), name)
+    if grad:
+        # detached views keep what the description points to alive until this node is freed
+        held = [t.detach() for t in (q, k, v, lam, out)] + [out2, lse, key_lengths]
+        want = [t.requires_grad for t in (q, k, v, lam)]
+
+        def backward(g):
+            dq = Tensor._empty(held[0].shape, "float32", ctx) if want[0] else None
+            dk = Tensor._empty(held[1].shape, "float32", ctx) if want[1] or want[2] else None
+            dv_ = Tensor._empty(held[2].shape, "float32", ctx) if want[1] or want[2] else None
+            dlam = Tensor._empty((heads,), "float32", ctx) if want[3] else None
+            desc.dout = g[0].ptr
+            for field, t in (("dq", dq), ("dk", dk), ("dv", dv_), ("dlam", dlam)):
+                setattr(desc, field, t.ptr if t is not None else None)
+            ctx.check(lib.tx_diff_attention_bwd(ctx.handle, desc), f"{name} backward")
+            return [dq, dk, dv_, dlam]
+
+        out._attach(Fn(name, [q, k, v, lam], backward))
+    return out
 
 
 def relu(input: Tensor) -> Tensor:
@@ -282,5 +461,6 @@ def dropout(input: Tensor, p: float = 0.5, training: bool = True, inplace: bool 
     return out
 
 
-__all__ = ["adaptive_avg_pool2d", "avg_pool2d", "binary_cross_entropy_with_logits", "cross_entropy", "dropout",
-           "embedding", "max_pool2d", "mse_loss", "ppo_loss", "relu"]
+__all__ = ["adaptive_avg_pool2d", "avg_pool2d", "binary_cross_entropy_with_logits", "cross_entropy",
+           "differential_attention", "dropout", "embedding", "max_pool2d", "mse_loss", "ppo_loss", "qk_norm_rotary",
+           "relu", "rotary_embedding"]
