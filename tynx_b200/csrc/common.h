@@ -15,7 +15,7 @@
 
 // Device-side error codes written into ctx->d_err[0] by kernels.  Kernels never
 // trap: they record the first problem, skip the offending access and return.
-enum { DEVERR_NONE = 0, DEVERR_INDEX = 1, DEVERR_TIMEOUT = 2, DEVERR_LABEL = 3 };
+enum { DEVERR_NONE = 0, DEVERR_INDEX = 1, DEVERR_TIMEOUT = 2, DEVERR_LABEL = 3, DEVERR_LAYOUT = 4 };
 
 struct tx_arena {
   std::vector<std::pair<char *, size_t>> chunks;

@@ -6,46 +6,119 @@
 // and A_m comes back from the saved log-sum-exp without a second softmax pass.
 // Statistics, sums and accumulators are fp32.
 #include <cmath>
+#include <mutex>
 
-#include "common.h"
+#include "diff_attn.cuh"
 
+namespace tx_diff {
 namespace {
 
-constexpr int kMaxDim = 64, kMaxVdim = 128;
-constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+PFN_cuTensorMapEncodeTiled_v12000 g_encode = nullptr;
+std::once_flag g_encode_once;
 
-struct Shape {
-  int64_t B, T, S;
-  int H, Hk, G, d, dv;  // G = H / Hk
-  const float *q, *k, *v, *lam;
-  const int64_t *len;
-  int causal;
-  int64_t start;
-  float scale;
-  int *err;
-
-  __device__ __forceinline__ int64_t length(int64_t b) const {
-    if (!len) return S;
-    const int64_t n = __ldg(len + b);
-    return n < 0 ? 0 : n > S ? S : n;
-  }
-  // keys that query t of sequence b (valid keys n) sees: [0, seen)
-  __device__ __forceinline__ int64_t seen(int64_t t, int64_t n) const {
-    if (!causal) return n;
-    const int64_t c = t + start + 1;
-    return c < 0 ? 0 : c < n ? c : n;
-  }
+// A block splits one tile of 128 rows of one head; blockIdx.z picks the tensor.
+struct SplitJob {
+  const float *src;
+  __half *dst;
+  float *f, *norm;  // norm: nullptr where it is not needed
+  int64_t N, tiles;  // rows and tiles of a head
+  int heads, w;
+  float factor;
+  int masked;  // rows behind the sequence's length become zeros
 };
-
-// A key length outside [0, S] raises the context's error flag.
-__device__ __forceinline__ void report_length(const Shape &s, int64_t b) {
-  if (!s.len) return;
-  const int64_t n = __ldg(s.len + b);
-  if (n < 0 || n > s.S)
-    if (atomicCAS(s.err, 0, DEVERR_INDEX) == 0) {
-      s.err[1] = (int)(n < -2147483647 ? -2147483647 : n > 2147483647 ? 2147483647 : n);
-      s.err[2] = (int)(s.S + 1);
+struct SplitJobs {
+  SplitJob j[4];
+};
+template <int W>
+__device__ __forceinline__ void split_tile(const Shape &s, const SplitJob &J, uint32_t *red) {
+  constexpr int PARTS = W / 8, ROWS = 256 / PARTS, UNITS = kRows / ROWS;  // 8 elements a thread and unit
+  const int64_t head = (int64_t)blockIdx.x / J.tiles, tile = (int64_t)blockIdx.x - head * J.tiles;
+  const int64_t b = head / J.heads, n0 = tile * kRows;
+  const int hh = (int)(head - b * J.heads), c = threadIdx.x % PARTS * 8, r0 = threadIdx.x / PARTS;
+  const int64_t n_end = J.masked ? s.length(b) : J.N;
+  const bool four = (J.w & 3) == 0 && ((uintptr_t)J.src & 15) == 0;
+  float x[UNITS][8];
+#pragma unroll
+  for (int u = 0; u < UNITS; ++u) {
+    const int64_t n = n0 + r0 + u * ROWS;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[u][i] = 0.f;
+    if (n < n_end) {
+      const float *src = J.src + ((b * J.N + n) * J.heads + hh) * J.w + c;
+      if (four) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+          if (c + 4 * i < J.w) {
+            const float4 v = __ldg(reinterpret_cast<const float4 *>(src) + i);
+            x[u][4 * i] = v.x, x[u][4 * i + 1] = v.y, x[u][4 * i + 2] = v.z, x[u][4 * i + 3] = v.w;
+          }
+      } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          if (c + i < J.w) x[u][i] = __ldg(src + i);
+      }
     }
+  }
+  // the tile's largest finite magnitude (and row norm)
+  uint32_t top = 0;
+  float norm = 0.f;
+#pragma unroll
+  for (int u = 0; u < UNITS; ++u) {
+    float ss = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      x[u][i] *= J.factor;
+      const uint32_t a = __float_as_uint(x[u][i]) & 0x7fffffffu;
+      if (a < 0x7f800000u && a > top) top = a;
+      ss += x[u][i] * x[u][i];
+    }
+    if (J.norm) {
+#pragma unroll
+      for (int o = PARTS / 2; o; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+      norm = fmaxf(norm, ss);
+    }
+  }
+  top = __reduce_max_sync(0xffffffffu, top);
+  const uint32_t nb = __reduce_max_sync(0xffffffffu, __float_as_uint(norm));
+  if ((threadIdx.x & 31) == 0) {
+    red[threadIdx.x >> 5] = top;
+    red[8 + (threadIdx.x >> 5)] = nb;
+  }
+  __syncthreads();
+  uint32_t most = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    top = red[i] > top ? red[i] : top;
+    most = red[8 + i] > most ? red[8 + i] : most;
+  }
+  int e = (int)(top >> 23) - 127 - 13;
+  e = e < -113 ? -113 : e > 114 ? 114 : e;
+  if (threadIdx.x == 0) {
+    J.f[blockIdx.x] = __uint_as_float((uint32_t)(127 + e) << 23);
+    if (J.norm) J.norm[blockIdx.x] = fminf(sqrtf(__uint_as_float(most)), 1e16f);
+  }
+  const float inv = __uint_as_float((uint32_t)(127 - e) << 23);
+#pragma unroll
+  for (int u = 0; u < UNITS; ++u) {
+    const int64_t n = n0 + r0 + u * ROWS;
+    if (n >= J.N) break;
+    uint32_t hi[4], lo[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) split2(x[u][2 * i] * inv, x[u][2 * i + 1] * inv, hi[i], lo[i]);
+    __half *dst = J.dst + (head * J.N + n) * (2 * W) + c;
+    *reinterpret_cast<uint4 *>(dst) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+    *reinterpret_cast<uint4 *>(dst + W) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+  }
+}
+__global__ void __launch_bounds__(256)
+    k_diff_split(const __grid_constant__ Shape s, const __grid_constant__ SplitJobs jobs, int vw) {
+  __shared__ uint32_t red[16];
+  const SplitJob &J = jobs.j[blockIdx.z];
+  if ((int64_t)blockIdx.x >= s.B * J.heads * J.tiles) return;
+  if (blockIdx.z >= 2 && vw == 128)
+    split_tile<128>(s, J, red);
+  else
+    split_tile<64>(s, J, red);
 }
 
 __device__ __forceinline__ float warp_max(float v) {
@@ -211,9 +284,10 @@ __global__ void __launch_bounds__(kMaxVdim)
 }
 
 // ---- backward ------------------------------------------------------------------------------
-// delta[0], delta[1]: D1 and D2 of each (b, h, t); a warp per row.
+// (lse1, lse2, D1, D2) of each (b, h, t); a warp per row.
 __global__ void __launch_bounds__(256)
-    k_diff_delta(const __grid_constant__ Shape s, const float *out, const float *out2, const float *dout, float *delta) {
+    k_diff_delta(const __grid_constant__ Shape s, const float *out, const float *out2, const float *lse,
+                 const float *dout, float4 *stats) {
   const int64_t row = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5), rows = s.B * s.T * s.H;
   const int lane = threadIdx.x & 31;
   if (row >= rows) return;
@@ -228,20 +302,18 @@ __global__ void __launch_bounds__(256)
   }
   d1 = warp_sum(d1);
   d2 = warp_sum(d2);
-  if (lane == 0) {
-    const int64_t i = (b * s.H + h) * s.T + t;
-    delta[i] = d1;
-    delta[rows + i] = d2;
-  }
+  if (lane == 0)
+    stats[(b * s.H + h) * s.T + t] = make_float4(lse[(b * 2 * s.H + 2 * h) * s.T + t],
+                                                 lse[(b * 2 * s.H + 2 * h + 1) * s.T + t], d1, d2);
 }
 
-__global__ void __launch_bounds__(256) k_diff_dlam(const __grid_constant__ Shape s, const float *delta2, float *dlam) {
+__global__ void __launch_bounds__(256) k_diff_dlam(const __grid_constant__ Shape s, const float4 *stats, float *dlam) {
   __shared__ float sums[8];
   const int h = blockIdx.x;
   float v = 0.f;
   for (int64_t i = threadIdx.x; i < s.B * s.T; i += 256) {
     const int64_t b = i / s.T, t = i - b * s.T;
-    v += delta2[(b * s.H + h) * s.T + t];
+    v += stats[(b * s.H + h) * s.T + t].w;
   }
   v = warp_sum(v);
   if ((threadIdx.x & 31) == 0) sums[threadIdx.x >> 5] = v;
@@ -252,85 +324,54 @@ __global__ void __launch_bounds__(256) k_diff_dlam(const __grid_constant__ Shape
   }
 }
 
-// both maps' weights and score gradients of one (query, key) pair
-struct Pair {
-  float w, ds1, ds2;
-};
-__device__ __forceinline__ Pair pair_grad(const Shape &s, const float *q, const float *k, const float *g, const float *v,
-                                          float lse1, float lse2, float d1, float d2, float lam) {
-  float s1 = 0.f, s2 = 0.f, dp = 0.f;
-  for (int c = 0; c < s.d; ++c) s1 += q[c] * k[c], s2 += q[s.d + c] * k[s.d + c];
-  for (int c = 0; c < s.dv; ++c) dp += g[c] * v[c];
-  const float f = s.scale * kLog2e;
-  const float a1 = exp2f(s1 * f - lse1), a2 = exp2f(s2 * f - lse2);
-  return {a1 - lam * a2, a1 * (dp - d1) * s.scale, -lam * a2 * (dp - d2) * s.scale};
-}
-
-__global__ void __launch_bounds__(128)
-    k_diff_dq(const __grid_constant__ Shape s, const float *lse, const float *delta, const float *dout, float *dq) {
-  __shared__ float g1[128], g2[128];
-  const int64_t bt = blockIdx.x, b = bt / s.T, t = bt - b * s.T;
-  const int h = blockIdx.y, hk = h / s.G, tid = threadIdx.x;
-  const int64_t rows = s.B * s.T * s.H, n = s.seen(t, s.length(b));
-  const float *q = s.q + (bt * 2 * s.H + 2 * h) * s.d, *g = dout + (bt * s.H + h) * s.dv;
-  const float lse1 = lse[(b * 2 * s.H + 2 * h) * s.T + t], lse2 = lse[(b * 2 * s.H + 2 * h + 1) * s.T + t];
-  const float d1 = delta[(b * s.H + h) * s.T + t], d2 = delta[rows + (b * s.H + h) * s.T + t], lam = s.lam[h];
-  float acc = 0.f;
-  for (int64_t j0 = 0; j0 < n; j0 += 128) {
-    const int64_t j = j0 + tid;
-    Pair p{0.f, 0.f, 0.f};
-    if (j < n)
-      p = pair_grad(s, q, s.k + ((b * s.S + j) * 2 * s.Hk + 2 * hk) * s.d, g, s.v + ((b * s.S + j) * s.Hk + hk) * s.dv,
-                    lse1, lse2, d1, d2, lam);
-    g1[tid] = p.ds1;
-    g2[tid] = p.ds2;
-    __syncthreads();
-    if (tid < 2 * s.d)
-      for (int i = 0; i < 128 && j0 + i < n; ++i)
-        acc += (tid < s.d ? g1 : g2)[i] * s.k[((b * s.S + j0 + i) * 2 * s.Hk + 2 * hk) * s.d + tid];
-    __syncthreads();
-  }
-  if (tid < 2 * s.d) dq[(bt * 2 * s.H + 2 * h) * s.d + tid] = acc;
-}
-
-__global__ void __launch_bounds__(128)
-    k_diff_dkv(const __grid_constant__ Shape s, const float *lse, const float *delta, const float *dout, float *dk,
-               float *dv) {
-  __shared__ float w[128], g1[128], g2[128];
-  const int64_t bj = blockIdx.x, b = bj / s.S, j = bj - b * s.S;
-  const int hk = blockIdx.y, tid = threadIdx.x;
-  const int64_t rows = s.B * s.T * s.H, n = s.length(b);
-  const float *k = s.k + (bj * 2 * s.Hk + 2 * hk) * s.d, *v = s.v + (bj * s.Hk + hk) * s.dv;
-  float ak = 0.f, av = 0.f;
-  int64_t t0 = 0;
-  if (s.causal && j - s.start > 0) t0 = j - s.start;
-  if (j < n)
-    for (int h = hk * s.G; h < (hk + 1) * s.G; ++h) {
-      const float lam = s.lam[h];
-      for (int64_t i0 = t0; i0 < s.T; i0 += 128) {
-        const int64_t t = i0 + tid, i = (b * s.H + h) * s.T + t;
-        Pair p{0.f, 0.f, 0.f};
-        if (t < s.T)
-          p = pair_grad(s, s.q + ((b * s.T + t) * 2 * s.H + 2 * h) * s.d, k, dout + ((b * s.T + t) * s.H + h) * s.dv, v,
-                        lse[(b * 2 * s.H + 2 * h) * s.T + t], lse[(b * 2 * s.H + 2 * h + 1) * s.T + t], delta[i],
-                        delta[rows + i], lam);
-        w[tid] = p.w;
-        g1[tid] = p.ds1;
-        g2[tid] = p.ds2;
-        __syncthreads();
-        for (int u = 0; u < 128 && i0 + u < s.T; ++u) {
-          const int64_t bt = b * s.T + i0 + u;
-          if (tid < 2 * s.d) ak += (tid < s.d ? g1 : g2)[u] * s.q[(bt * 2 * s.H + 2 * h) * s.d + tid];
-          if (tid < s.dv) av += w[u] * dout[(bt * s.H + h) * s.dv + tid];
-        }
-        __syncthreads();
-      }
-    }
-  if (tid < 2 * s.d) dk[(bj * 2 * s.Hk + 2 * hk) * s.d + tid] = ak;
-  if (tid < s.dv) dv[(bj * s.Hk + hk) * s.dv + tid] = av;
-}
-
 // ---- host ----------------------------------------------------------------------------------
+// The split operands of one call and their memory.
+struct Operands {
+  Split x;
+  Scratch data;
+  int64_t tq, tk, tv, tg;  // tiles
+  static int width(const Shape &s) { return s.dv <= 64 ? 64 : 128; }
+  static size_t total(const Shape &s, bool gradient) {
+    const int64_t w = width(s), qt = (s.T + kRows - 1) / kRows, kt = (s.S + kRows - 1) / kRows;
+    const int64_t halves = 2 * (s.B * 2 * s.H * s.T * 64 + s.B * 2 * s.Hk * s.S * 64 + s.B * s.Hk * s.S * w +
+                                (gradient ? s.B * s.H * s.T * w : 0));
+    return (size_t)halves * 2 + (size_t)(s.B * (2 * s.H * qt + 2 * s.Hk * kt + 2 * s.Hk * kt + 2 * s.H * qt)) * 4;
+  }
+  Operands(tx_ctx *ctx, const Shape &s, bool gradient) : data(ctx, total(s, gradient)) {
+    if (!data.ptr) return;
+    const int64_t w = width(s), qt = (s.T + kRows - 1) / kRows, kt = (s.S + kRows - 1) / kRows;
+    x.vw = (int)w;
+    x.qt = qt;
+    x.kt = kt;
+    tq = s.B * 2 * s.H * qt, tk = s.B * 2 * s.Hk * kt, tv = s.B * s.Hk * kt, tg = s.B * s.H * qt;
+    __half *p = data.as<__half>();
+    x.q = p, p += s.B * 2 * s.H * s.T * 128;
+    x.k = p, p += s.B * 2 * s.Hk * s.S * 128;
+    x.v = p, p += s.B * s.Hk * s.S * 2 * w;
+    x.g = p, p += gradient ? s.B * s.H * s.T * 2 * w : 0;
+    float *f = reinterpret_cast<float *>(p);
+    x.fq = f, f += tq;
+    x.fk = f, f += tk;
+    x.fv = f, f += tv;
+    x.nv = f, f += tv;
+    x.fg = f, f += tg;
+    x.ng = f;
+  }
+  int fill(tx_ctx *ctx, const Shape &s, const float *dout) {
+    if (!data.ptr) return TX_ERR_OOM;
+    auto w = [](const float *p) { return const_cast<float *>(p); };
+    SplitJobs jobs{};
+    jobs.j[0] = SplitJob{s.q, x.q, w(x.fq), nullptr, s.T, x.qt, 2 * s.H, s.d, s.scale * kLog2e, 0};
+    jobs.j[1] = SplitJob{s.k, x.k, w(x.fk), nullptr, s.S, x.kt, 2 * s.Hk, s.d, 1.0f, 1};
+    jobs.j[2] = SplitJob{s.v, x.v, w(x.fv), w(x.nv), s.S, x.kt, s.Hk, s.dv, 1.0f, 1};
+    jobs.j[3] = SplitJob{dout, x.g, w(x.fg), w(x.ng), s.T, x.qt, s.H, s.dv, 1.0f, 0};
+    const int64_t blocks = tq > tk ? tq : tk;
+    k_diff_split<<<dim3((unsigned)blocks, 1, dout ? 4u : 3u), 256, 0, ctx->stream>>>(s, jobs, x.vw);
+    TX_LAUNCHED(ctx, "k_diff_split");
+    return TX_OK;
+  }
+};
+
 int check_desc(tx_ctx *ctx, const tx_diff_attention *p, Shape &s) {
   if (!p) return tx_fail(ctx, TX_ERR_INVALID, "differential attention: no description");
   if (p->dim < 1 || p->dim > kMaxDim || p->vdim < 1 || p->vdim > kMaxVdim)
@@ -375,6 +416,28 @@ int launch_rows(tx_ctx *ctx, const Shape &s, float *out, float *out2, float *lse
 
 }  // namespace
 
+bool split_map(CUtensorMap *m, const __half *base, int w, int64_t rows, int64_t heads, int box) {
+  std::call_once(g_encode_once, [] {
+    void *fn = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &fn, cudaEnableDefault, &q) == cudaSuccess &&
+        q == cudaDriverEntryPointSuccess)
+      g_encode = (PFN_cuTensorMapEncodeTiled_v12000)fn;
+  });
+  if (!g_encode) return false;
+  cuuint64_t dims[3] = {(cuuint64_t)(2 * w), (cuuint64_t)rows, (cuuint64_t)heads};
+  cuuint64_t strides[2] = {(cuuint64_t)(4 * w), (cuuint64_t)(4 * w) * (cuuint64_t)rows};
+  cuuint32_t bx[3] = {64u, (cuuint32_t)box, 1u};
+  cuuint32_t es[3] = {1u, 1u, 1u};
+  return g_encode(m, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, (void *)base, dims, strides, bx, es,
+                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+}  // namespace tx_diff
+
+using namespace tx_diff;
+
 extern "C" int tx_diff_attention_fwd(tx_ctx *ctx, const tx_diff_attention *p) {
   if (!ctx) return TX_ERR_INVALID;
   Shape s;
@@ -388,7 +451,10 @@ extern "C" int tx_diff_attention_fwd(tx_ctx *ctx, const tx_diff_attention *p) {
   if (s.T * s.G <= 1) return launch_rows<1>(ctx, s, p->out, p->out2, p->lse);
   if (s.T * s.G <= 2) return launch_rows<2>(ctx, s, p->out, p->out2, p->lse);
   if (s.T * s.G <= 4) return launch_rows<4>(ctx, s, p->out, p->out2, p->lse);
-  return launch_rows<8>(ctx, s, p->out, p->out2, p->lse);
+  if (s.T * s.G <= 8 || s.S == 0) return launch_rows<8>(ctx, s, p->out, p->out2, p->lse);
+  Operands x(ctx, s, false);
+  TX_TRY(x.fill(ctx, s, nullptr));
+  return tc_forward(ctx, s, x.x, p->out, p->out2, p->lse);
 }
 
 extern "C" int tx_diff_attention_bwd(tx_ctx *ctx, const tx_diff_attention *p) {
@@ -401,25 +467,28 @@ extern "C" int tx_diff_attention_bwd(tx_ctx *ctx, const tx_diff_attention *p) {
   if (rows && (!p->q || !p->lam || !p->out || !p->out2 || !p->lse || !p->dout || (s.S && (!p->k || !p->v))))
     return tx_fail(ctx, TX_ERR_INVALID, "differential attention: null buffer");
   DeviceScope device(ctx);
-  Scratch delta(ctx, rows ? (size_t)rows * 8 : 8);
-  if (!delta.ptr) return TX_ERR_OOM;
+  Scratch stats(ctx, rows ? (size_t)rows * sizeof(float4) : 16);
+  if (!stats.ptr) return TX_ERR_OOM;
   if (rows) {
-    k_diff_delta<<<(unsigned)((rows + 7) / 8), 256, 0, ctx->stream>>>(s, p->out, p->out2, p->dout, delta.as<float>());
+    k_diff_delta<<<(unsigned)((rows + 7) / 8), 256, 0, ctx->stream>>>(s, p->out, p->out2, p->lse, p->dout,
+                                                                     stats.as<float4>());
     TX_LAUNCHED(ctx, "k_diff_delta");
   }
   if (p->dlam) {
-    k_diff_dlam<<<(unsigned)s.H, 256, 0, ctx->stream>>>(s, delta.as<float>() + rows, p->dlam);
+    k_diff_dlam<<<(unsigned)s.H, 256, 0, ctx->stream>>>(s, stats.as<float4>(), p->dlam);
     TX_LAUNCHED(ctx, "k_diff_dlam");
   }
-  if (p->dq && rows) {
-    k_diff_dq<<<dim3((unsigned)(s.B * s.T), (unsigned)s.H), 128, 0, ctx->stream>>>(s, p->lse, delta.as<float>(), p->dout,
-                                                                                  p->dq);
-    TX_LAUNCHED(ctx, "k_diff_dq");
+  if (!rows || !s.S) {  // nothing to multiply: no query or no key
+    if (p->dq) TX_CUDA(ctx, cudaMemsetAsync(p->dq, 0, (size_t)rows * 2 * s.d * 4, ctx->stream));
+    if (p->dk) {
+      const size_t keys = (size_t)(s.B * s.S * s.Hk);
+      TX_CUDA(ctx, cudaMemsetAsync(p->dk, 0, keys * 2 * s.d * 4, ctx->stream));
+      TX_CUDA(ctx, cudaMemsetAsync(p->dv, 0, keys * s.dv * 4, ctx->stream));
+    }
+    return TX_OK;
   }
-  if (p->dk && s.B * s.S) {
-    k_diff_dkv<<<dim3((unsigned)(s.B * s.S), (unsigned)s.Hk), 128, 0, ctx->stream>>>(s, p->lse, delta.as<float>(),
-                                                                                    p->dout, p->dk, p->dv);
-    TX_LAUNCHED(ctx, "k_diff_dkv");
-  }
-  return TX_OK;
+  if (!p->dq && !p->dk) return TX_OK;
+  Operands x(ctx, s, true);
+  TX_TRY(x.fill(ctx, s, p->dout));
+  return tc_backward(ctx, s, x.x, stats.as<float4>(), p->dq, p->dk, p->dv);
 }

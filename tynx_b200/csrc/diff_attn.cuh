@@ -1,0 +1,247 @@
+// Shared declarations of differential attention: the problem's shape, the
+// split operands of the tensor-core kernels, and their tcgen05 / TMA / mbarrier
+// wrappers.
+#pragma once
+#include <cuda.h>
+#include <cuda_fp16.h>
+#include <cudaTypedefs.h>
+
+#include "common.h"
+
+namespace tx_diff {
+
+constexpr int kMaxDim = 64, kMaxVdim = 128;
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+
+struct Shape {
+  int64_t B, T, S;
+  int H, Hk, G, d, dv;  // G = H / Hk
+  const float *q, *k, *v, *lam;
+  const int64_t *len;
+  int causal;
+  int64_t start;
+  float scale;
+  int *err;
+
+  __device__ __forceinline__ int64_t length(int64_t b) const {
+    if (!len) return S;
+    const int64_t n = __ldg(len + b);
+    return n < 0 ? 0 : n > S ? S : n;
+  }
+  // keys that query t of a sequence with n valid keys sees: [0, seen)
+  __device__ __forceinline__ int64_t seen(int64_t t, int64_t n) const {
+    if (!causal) return n;
+    const int64_t c = t + start + 1;
+    return c < 0 ? 0 : c < n ? c : n;
+  }
+};
+
+// A key length outside [0, S] raises the context's error flag.
+__device__ __forceinline__ void report_length(const Shape &s, int64_t b) {
+  if (!s.len) return;
+  const int64_t n = __ldg(s.len + b);
+  if (n < 0 || n > s.S)
+    if (atomicCAS(s.err, 0, DEVERR_INDEX) == 0) {
+      s.err[1] = (int)(n < -2147483647 ? -2147483647 : n > 2147483647 ? 2147483647 : n);
+      s.err[2] = (int)(s.S + 1);
+    }
+}
+
+// ---- split operands ------------------------------------------------------------------------
+// The tensor-core kernels multiply pairs of fp16: x = f (hi + lo) with f a
+// power of two for each tile of 128 rows that brings the tile's largest
+// element into [2^13, 2^14), hi = fp16(x / f), lo = fp16(x / f - hi), and
+// a b = hi hi + hi lo + lo hi.  That keeps 22 bits of every element down to 2^-17
+// of its tile's largest (below, 2^-39 of the largest), at the cost of three fp16
+// products: half the tensor time of three TF32 products of the same accuracy,
+// in the memory of the fp32 value.  (Pairs of bf16 need no f but keep 16 bits:
+// 6e-6 of an attention output's norm instead of 2e-7.)  A row is [W hi | W lo],
+// zero beyond its width, with W = 64 for queries and keys (queries carry scale *
+// log2 e, so scores come out in powers of two) and 64 or 128 for values.
+constexpr int kRows = 128;  // rows of a tile
+struct Split {
+  __half *q, *k, *v, *g;         // [b][map or head][row][2 W]; g: the output's gradient
+  const float *fq, *fk, *fv, *fg;  // f of each [b][map or head][tile]
+  const float *nv, *ng;          // the largest 2-norm of a tile's rows
+  int vw;                        // W of v and g
+  int64_t qt, kt;                // tiles of a head's queries and keys
+};
+// 3-D map {2 W, rows, heads} with boxes of 64 columns x `box` rows (128-byte swizzle)
+bool split_map(CUtensorMap *m, const __half *base, int w, int64_t rows, int64_t heads, int box);
+
+// stats: per (b, h, t) the log-sum-exp of both maps and D1, D2
+int tc_forward(tx_ctx *ctx, const Shape &s, const Split &x, float *out, float *out2, float *lse);
+int tc_backward(tx_ctx *ctx, const Shape &s, const Split &x, const float4 *stats, float *dq, float *dk, float *dv);
+
+// ---- device wrappers -------------------------------------------------------------------------
+constexpr uint64_t kWaitNs = 2000000000ull;  // 2 s
+
+__device__ __forceinline__ uint32_t su32(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
+__device__ __forceinline__ uint64_t gtime() {
+  uint64_t t;
+  asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
+  return t;
+}
+__device__ __forceinline__ void bar_init(uint64_t *b, uint32_t n) {
+  asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(su32(b)), "r"(n));
+}
+__device__ __forceinline__ void bar_expect(uint64_t *b, uint32_t bytes) {
+  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(su32(b)), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void bar_arrive(uint64_t *b) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(su32(b)) : "memory");
+}
+__device__ __forceinline__ bool bar_try(uint64_t *b, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(su32(b)), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
+// Bounded wait.  On expiry (or when another role gave up) false: the role
+// leaves its loop, so every role reaches the CTA's last barrier.
+__device__ __forceinline__ bool bar_wait(uint64_t *b, uint32_t parity, volatile int *abort_flag, int *err, int site) {
+  if (bar_try(b, parity)) return true;
+  const uint64_t t0 = gtime();
+  while (true) {
+    if (bar_try(b, parity)) return true;
+    if (*abort_flag) return false;
+    if (gtime() - t0 > kWaitNs) {
+      *abort_flag = 1;
+      if (atomicCAS(err, 0, DEVERR_TIMEOUT) == 0) err[1] = 200 + site;
+      return false;
+    }
+  }
+}
+// whatever the abort flag says: copies and MMAs in flight end before their memory is released
+__device__ __forceinline__ void bar_drain(uint64_t *b, uint32_t parity) {
+  const uint64_t t0 = gtime();
+  while (!bar_try(b, parity) && gtime() - t0 < kWaitNs) {
+  }
+}
+__device__ __forceinline__ void tma_3d(uint32_t dst, const CUtensorMap *map, uint64_t *b, int x, int y, int z) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(dst),
+      "l"(map), "r"(su32(b)), "r"(x), "r"(y), "r"(z)
+      : "memory");
+}
+// plain bulk copy: both addresses and the size multiples of 16 bytes
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void *src, uint32_t bytes, uint64_t *b) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
+               "l"(src), "r"(bytes), "r"(su32(b))
+               : "memory");
+}
+__device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void mma_commit(uint64_t *b) {
+  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(su32(b))
+               : "memory");
+}
+// D[tmem] (+)= A B^T, A in shared memory
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(acc)
+      : "memory");
+}
+// the same with A in TMEM (two fp16 a column)
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+      "r"(a), "l"(b), "r"(idesc), "r"(acc)
+      : "memory");
+}
+// shared-memory descriptor, 128-byte swizzle
+__device__ __forceinline__ uint64_t sdesc(uint32_t addr, uint32_t lbo, uint32_t sbo) {
+  return (uint64_t)((addr >> 4) & 0x3FFF) | (uint64_t)((lbo >> 4) & 0x3FFF) << 16 |
+         (uint64_t)((sbo >> 4) & 0x3FFF) << 32 | (uint64_t)1 << 46 | (uint64_t)2 << 61;
+}
+// 16-deep slice k of a [rows x 64] fp16 tile read along its columns (K-major)
+__device__ __forceinline__ uint64_t kdesc(uint32_t tile, int k) { return sdesc(tile + k * 32, 16, 1024); }
+// 16-deep slice k of [K rows x 64 columns] tiles read along their rows (MN-major);
+// `next` is the distance between the tiles of neighbouring 64-column blocks
+__device__ __forceinline__ uint64_t ndesc(uint32_t tile, int k, uint32_t next) {
+  return sdesc(tile + k * 2048, next, 1024);
+}
+// fp16 operands, fp32 accumulators, M = 128
+__device__ __forceinline__ constexpr uint32_t idesc(int n, bool b_mn) {
+  return (1u << 4) | ((b_mn ? 1u : 0u) << 16) | ((uint32_t)(n >> 3) << 17) |
+         ((uint32_t)(128 >> 4) << 24);
+}
+__device__ __forceinline__ void tld32_issue(uint32_t taddr, uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, "
+      "%12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, "
+      "%30, %31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
+        "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]),
+        "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]),
+        "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]),
+        "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(taddr));
+}
+__device__ __forceinline__ void tld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+// keeps every use of loaded registers behind the wait
+__device__ __forceinline__ void after_wait(uint32_t (&r)[32]) {
+  asm volatile(""
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]),
+                 "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]),
+                 "+r"(r[13]), "+r"(r[14]), "+r"(r[15]), "+r"(r[16]), "+r"(r[17]), "+r"(r[18]),
+                 "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]), "+r"(r[24]),
+                 "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]), "+r"(r[30]),
+                 "+r"(r[31]));
+}
+__device__ __forceinline__ void tst_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+// 2^x, good to 2^-22
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+// (a, b) as a pair of fp16 heads (a in the low half) and a pair of fp16 tails
+__device__ __forceinline__ void split2(float a, float b, uint32_t &hi, uint32_t &lo) {
+  const __half2 h = __floats2half2_rn(a, b);
+  const float2 f = __half22float2(h);
+  const __half2 l = __floats2half2_rn(a - f.x, b - f.y);
+  hi = *reinterpret_cast<const uint32_t *>(&h);
+  lo = *reinterpret_cast<const uint32_t *>(&l);
+}
+__device__ __forceinline__ void tld16_issue(uint32_t taddr, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, "
+      "%12, %13, %14, %15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
+        "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]),
+        "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr));
+}
+__device__ __forceinline__ void after_wait(uint32_t (&r)[16]) {
+  asm volatile(""
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]),
+                 "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]),
+                 "+r"(r[13]), "+r"(r[14]), "+r"(r[15]));
+}
+// 16 keys (rows) of an A operand: heads in columns 0 .. 7, tails in 8 .. 15
+__device__ __forceinline__ void tst_pairs(uint32_t taddr, const uint32_t (&hi)[8], const uint32_t (&lo)[8]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, "
+      "%13, %14, %15, %16};" ::"r"(taddr),
+      "r"(hi[0]), "r"(hi[1]), "r"(hi[2]), "r"(hi[3]), "r"(hi[4]), "r"(hi[5]), "r"(hi[6]), "r"(hi[7]),
+      "r"(lo[0]), "r"(lo[1]), "r"(lo[2]), "r"(lo[3]), "r"(lo[4]), "r"(lo[5]), "r"(lo[6]), "r"(lo[7])
+      : "memory");
+}
+// a factor of scores or gradients; neither infinite nor 0, so that nothing times it is NaN
+__device__ __forceinline__ float factor2(float a, float b) {
+  return fminf(fmaxf(a * b, 1.1754944e-38f), 1.7014118e38f);
+}
+
+}  // namespace tx_diff

@@ -1,0 +1,342 @@
+// Differential attention forward on tcgen05.
+//
+// A CTA owns 128 queries of one head and streams its keys in tiles of 128,
+// both maps side by side: one warpgroup keeps map 1's rows, the other map 2's
+// (running maximum, sum and output, a row a thread), and both maps multiply the
+// same value tile.  Per tile and map
+//   S = Q K^T               three fp16 products of 128 x 128 x 64   (768 cycles)
+//   P = 2^(S - maximum)     registers, split into fp16 pairs, back over S in TMEM
+//   O = P V                 three fp16 products of 128 x 128 x 128 (1536 cycles)
+// so while one map's warpgroup works on its softmax (128 exponentials a thread,
+// about 1400 issue slots a warp) the tensor core runs the other map's 2304
+// cycles: it is what bounds the kernel.  TMEM holds S1 | S2 | O1 | O2, all 512
+// columns; P lies over S (16 keys' heads and tails take the 16 columns of their
+// scores).  O is one tile's product and is added to the running output in
+// registers, rescaled there: the tensor core adds into its accumulator with
+// truncation, which over thousands of keys loses 1e-5 of the result, and over
+// the 24 products of one tile 1e-7.  Shared memory: Q of both maps (64 KB), one
+// key tile of both (64 KB, each map's half refilled as soon as its S is done),
+// and a ring of three half value tiles (96 KB).
+#include "diff_attn.cuh"
+
+namespace tx_diff {
+namespace {
+
+constexpr int kThreads = 384;  // producer, MMA, two spare warps, 2 x 4 softmax warps
+
+template <int DV>
+struct Cfg {
+  static constexpr int HALF = 128 * 64 * 2;           // [128 x 64] fp16
+  static constexpr int QK = 2 * HALF;                 // heads and tails of one map's tile
+  static constexpr int VBLK = 64 * 64 * 2;            // [64 keys x 64] fp16
+  static constexpr int VSLOT = 2 * (DV / 64) * VBLK;  // 64 keys: heads, tails
+  static constexpr int RING = 3;
+  static constexpr int SMEM = 4 * QK + RING * VSLOT + 1024 /*barriers*/ + 1024 /*align*/;
+  // at the end map 2's output passes through Q's and K's memory
+  static_assert(128 * DV * 4 <= 4 * QK, "output staging");
+};
+
+struct Out {
+  float *out, *out2, *lse;
+};
+
+// 16-byte chunk c of a staged output row: rows a warp touches together spread over the banks
+template <int DV>
+__device__ __forceinline__ float4 *staged(uint8_t *sm, int r, int c) {
+  return reinterpret_cast<float4 *>(sm) + r * (DV / 4) + (c ^ (r & 7));
+}
+
+__device__ __forceinline__ void store_row(float *dst, int c, const float *v, int dv, bool four) {
+  if (four) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (c + 4 * j < dv) *reinterpret_cast<float4 *>(dst + c + 4 * j) = make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 32; ++j)
+      if (c + j < dv) dst[c + j] = v[j];
+  }
+}
+
+template <int DV>
+__global__ void __launch_bounds__(kThreads, 1)
+    k_diff_fwd(const __grid_constant__ Shape s, const __grid_constant__ Split x, const __grid_constant__ CUtensorMap mq,
+               const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtensorMap mv, Out o) {
+  using C = Cfg<DV>;
+  extern __shared__ uint8_t raw[];
+  uint8_t *sm = (uint8_t *)(((uintptr_t)raw + 1023) & ~(uintptr_t)1023);
+  const uint32_t sq = su32(sm), sk = sq + 2 * C::QK, sv = sk + 2 * C::QK;
+  uint64_t *bars = reinterpret_cast<uint64_t *>(sm + 4 * C::QK + C::RING * C::VSLOT);
+  uint64_t *q_full = bars, *k_full = bars + 1, *k_empty = bars + 3, *v_full = bars + 5, *v_empty = bars + 8,
+           *s_full = bars + 11, *p_full = bars + 13, *o_full = bars + 15;
+  uint32_t *tmem_holder = reinterpret_cast<uint32_t *>(bars + 16);
+  volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_holder + 1);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+  // causal: the queries with most keys first
+  const int64_t heads = s.B * s.H;
+  const int64_t qt = x.qt - 1 - (int64_t)blockIdx.x / heads, bh = (int64_t)blockIdx.x % heads;
+  const int64_t b = bh / s.H;
+  const int h = (int)(bh - b * s.H), hk = h / s.G;
+  const int64_t t0 = qt * 128, tl = t0 + 127 < s.T ? t0 + 127 : s.T - 1;
+  const int64_t n = s.length(b);
+  const int tiles = (int)((s.seen(tl, n) + 127) / 128);
+
+  if (threadIdx.x == 0) {
+    bar_init(q_full, 1);
+    for (int m = 0; m < 2; ++m) {
+      bar_init(k_full + m, 1);
+      bar_init(k_empty + m, 1);
+      bar_init(s_full + m, 1);
+      bar_init(p_full + m, 128);
+    }
+    for (int i = 0; i < C::RING; ++i) {
+      bar_init(v_full + i, 1);
+      bar_init(v_empty + i, 1);
+    }
+    bar_init(o_full, 1);
+    *abort_flag = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    if (h == 0 && qt == 0) report_length(s, b);
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(su32(tmem_holder)),
+                 "r"(512));
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+  }
+  fence_before();
+  __syncthreads();
+  fence_after();
+  const uint32_t tmem = *tmem_holder;
+
+  if (warp < 4) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+    if (warp == 0 && lane == 0 && tiles) {
+      bar_expect(q_full, 2 * C::QK);
+      for (int m = 0; m < 2; ++m)
+        for (int p = 0; p < 2; ++p)
+          tma_3d(sq + m * C::QK + p * C::HALF, &mq, q_full, p * 64, (int)t0, (int)(b * 2 * s.H + 2 * h + m));
+      bool ok = true;
+      int loaded_k = 0, loaded_v = 0;
+      for (int i = 0; i < tiles && ok; ++i) {
+        for (int m = 0; m < 2 && ok; ++m) {
+          if (i) ok = bar_wait(k_empty + m, (i - 1) & 1, abort_flag, s.err, 1);
+          if (!ok) break;
+          bar_expect(k_full + m, C::QK);
+          for (int p = 0; p < 2; ++p)
+            tma_3d(sk + m * C::QK + p * C::HALF, &mk, k_full + m, p * 64, i * 128,
+                   (int)(b * 2 * s.Hk + 2 * hk + m));
+          ++loaded_k;
+        }
+        for (int hf = 0; hf < 2 && ok; ++hf) {
+          const int u = 2 * i + hf, slot = u % C::RING, use = u / C::RING;
+          if (use) ok = bar_wait(v_empty + slot, (use - 1) & 1, abort_flag, s.err, 2);
+          if (!ok) break;
+          bar_expect(v_full + slot, C::VSLOT);
+          for (int p = 0; p < 2 * (DV / 64); ++p)
+            tma_3d(sv + slot * C::VSLOT + p * C::VBLK, &mv, v_full + slot, p * 64, i * 128 + hf * 64,
+                   (int)(b * s.Hk + hk));
+          ++loaded_v;
+        }
+      }
+      // every copy has landed before the CTA's memory is released
+      bar_drain(q_full, 0);
+      for (int m = 0; m < 2; ++m) {
+        const int c = (loaded_k + 1 - m) / 2;  // loads of this map
+        if (c) bar_drain(k_full + m, (c - 1) & 1);
+      }
+      for (int u = loaded_v - 1; u >= 0 && u > loaded_v - 1 - C::RING; --u)
+        bar_drain(v_full + u % C::RING, (u / C::RING) & 1);
+    } else if (warp == 1 && lane == 0 && tiles) {
+      constexpr uint32_t id_s = idesc(128, false), id_o = idesc(DV, true);
+      bool ok = bar_wait(q_full, 0, abort_flag, s.err, 3);
+      for (int i = 0; i <= tiles && ok; ++i) {
+        for (int m = 0; m < 2 && ok; ++m) {
+          const uint32_t ts = tmem + m * 128, to = tmem + 256 + m * DV;
+          if (i) {  // O = P V of the tile before
+            ok = bar_wait(p_full + m, (i - 1) & 1, abort_flag, s.err, 4);
+            for (int hf = 0; hf < 2 && ok; ++hf) {
+              const int u = 2 * (i - 1) + hf, slot = u % C::RING;
+              ok = bar_wait(v_full + slot, (u / C::RING) & 1, abort_flag, s.err, 5);
+              if (!ok) break;
+              fence_after();
+              const uint32_t vh = sv + slot * C::VSLOT, vl = vh + (DV / 64) * C::VBLK;
+              // the small products first: truncation then takes from small sums
+#pragma unroll
+              for (int k = 0; k < 4; ++k) {
+                const uint32_t ph = ts + (hf * 4 + k) * 16;
+                mma_ts(to, ph, ndesc(vl, k, C::VBLK), id_o, (hf || k) ? 1u : 0u);
+                mma_ts(to, ph + 8, ndesc(vh, k, C::VBLK), id_o, 1u);
+              }
+#pragma unroll
+              for (int k = 0; k < 4; ++k) mma_ts(to, ts + (hf * 4 + k) * 16, ndesc(vh, k, C::VBLK), id_o, 1u);
+              if (m) mma_commit(v_empty + slot);
+            }
+          }
+          if (i < tiles && ok) {
+            ok = bar_wait(k_full + m, i & 1, abort_flag, s.err, 6);
+            if (!ok) break;
+            fence_after();
+            const uint32_t qh = sq + m * C::QK, ql = qh + C::HALF, kh = sk + m * C::QK, kl = kh + C::HALF;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              mma_ss(ts, kdesc(qh, k), kdesc(kl, k), id_s, k ? 1u : 0u);
+              mma_ss(ts, kdesc(ql, k), kdesc(kh, k), id_s, 1u);
+            }
+#pragma unroll
+            for (int k = 0; k < 4; ++k) mma_ss(ts, kdesc(qh, k), kdesc(kh, k), id_s, 1u);
+            mma_commit(k_empty + m);
+            mma_commit(s_full + m);  // and behind it the product O of the tile before
+          }
+        }
+      }
+      mma_commit(o_full);  // all products of this CTA
+      bar_drain(o_full, 0);
+    }
+  } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
+    const int m = (warp - 4) >> 2, quad = warp & 3, r = quad * 32 + lane;
+    const uint32_t lane_row = (uint32_t)(quad * 32) << 16;
+    const uint32_t ts = tmem + m * 128 + lane_row, to = tmem + 256 + m * DV + lane_row;
+    const int64_t t = t0 + r;
+    const int64_t seen = t < s.T ? s.seen(t, n) : s.seen(tl, n);
+    const float fq = __ldg(x.fq + (b * 2 * s.H + 2 * h + m) * x.qt + qt);
+    const float *fk = x.fk + (b * 2 * s.Hk + 2 * hk + m) * x.kt, *fv = x.fv + (b * s.Hk + hk) * x.kt;
+    // P carries 2^14 so that fp16 tails hold; O and the sum carry it alike
+    float top = -INFINITY, sum = 0.f, shrink = 1.f;
+    float acc[DV];
+#pragma unroll
+    for (int j = 0; j < DV; ++j) acc[j] = 0.f;
+    auto add_tile = [&](float f, float g) {  // acc = f acc + g O
+#pragma unroll
+      for (int c = 0; c < DV / 32; ++c) {
+        uint32_t y[32];
+        tld32_issue(to + 32 * c, y);
+        tld_wait();
+        after_wait(y);
+#pragma unroll
+        for (int j = 0; j < 32; ++j) acc[32 * c + j] = acc[32 * c + j] * f + __uint_as_float(y[j]) * g;
+      }
+    };
+    bool ok = true;
+    float gv = 0.f;
+    for (int i = 0; i < tiles; ++i) {
+      const float f = factor2(fq, __ldg(fk + i)), next_gv = __ldg(fv + i);
+      ok = __all_sync(0xffffffffu, bar_wait(s_full + m, i & 1, abort_flag, s.err, 7));
+      if (!ok) break;
+      fence_after();
+      if (i) add_tile(shrink, gv);
+      gv = next_gv;
+      const int64_t left = seen - (int64_t)i * 128;
+      const int lim = left < 0 ? 0 : left > 128 ? 128 : (int)left;
+      const bool whole = __all_sync(0xffffffffu, lim == 128);
+      float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        uint32_t y[32];
+        tld32_issue(ts + 32 * c, y);
+        tld_wait();
+        after_wait(y);
+        if (whole) {
+#pragma unroll
+          for (int j = 0; j < 32; ++j) mx[j & 3] = fmaxf(mx[j & 3], __uint_as_float(y[j]));
+        } else {
+#pragma unroll
+          for (int j = 0; j < 32; ++j)
+            if (32 * c + j < lim) mx[j & 3] = fmaxf(mx[j & 3], __uint_as_float(y[j]));
+        }
+      }
+      const float now = fmaxf(top, fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * f);
+      const float at = now == -INFINITY ? 0.f : now - 14.f;  // no key yet: all weights are 2^-inf
+      shrink = top == -INFINITY ? 0.f : ex2(top - now);
+      top = now;
+      float part[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int c = 0; c < 8; ++c) {
+        uint32_t y[16], hi[8], lo[8];
+        tld16_issue(ts + 16 * c, y);
+        tld_wait();
+        after_wait(y);
+        float p[16];
+#pragma unroll
+        for (int j = 0; j < 16; ++j) p[j] = ex2(fmaf(__uint_as_float(y[j]), f, -at));
+        if (!whole) {
+#pragma unroll
+          for (int j = 0; j < 16; ++j)
+            if (16 * c + j >= lim) p[j] = 0.f;
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          part[j & 3] += p[2 * j] + p[2 * j + 1];
+          split2(p[2 * j], p[2 * j + 1], hi[j], lo[j]);
+        }
+        tst_pairs(ts + 16 * c, hi, lo);
+      }
+      sum = sum * shrink + ((part[0] + part[1]) + (part[2] + part[3]));
+      tst_wait();
+      fence_before();
+      bar_arrive(p_full + m);
+    }
+    if (tiles) ok = __all_sync(0xffffffffu, ok && bar_wait(o_full, 0, abort_flag, s.err, 8));
+    fence_after();
+    if (tiles && ok) add_tile(shrink, gv);
+    const bool none = top == -INFINITY;
+    const float inv = none ? 0.f : 1.0f / sum;
+#pragma unroll
+    for (int j = 0; j < DV; ++j) acc[j] *= inv;
+    if (m == 1) {
+#pragma unroll
+      for (int c = 0; c < DV / 4; ++c)
+        *staged<DV>(sm, r, c) = make_float4(acc[4 * c], acc[4 * c + 1], acc[4 * c + 2], acc[4 * c + 3]);
+    }
+    asm volatile("bar.sync 1, 256;" ::: "memory");
+    const bool live = t < s.T && ok;
+    if (live && o.lse) o.lse[(b * 2 * s.H + 2 * h + m) * s.T + t] = none ? INFINITY : (top - 14.f) + log2f(sum);
+    const int64_t at = ((b * s.T + t) * s.H + h) * s.dv;
+    const bool four = (s.dv & 3) == 0 && ((uintptr_t)o.out & 15) == 0 && ((uintptr_t)o.out2 & 15) == 0;
+    if (m == 0) {
+      const float lam = __ldg(s.lam + h);
+#pragma unroll
+      for (int c = 0; c < DV / 4; ++c) {
+        const float4 y = *staged<DV>(sm, r, c);
+        acc[4 * c] -= lam * y.x;
+        acc[4 * c + 1] -= lam * y.y;
+        acc[4 * c + 2] -= lam * y.z;
+        acc[4 * c + 3] -= lam * y.w;
+      }
+    }
+    float *dst = m ? o.out2 : o.out;
+    if (live && dst) {
+#pragma unroll
+      for (int c = 0; c < DV; c += 32) store_row(dst + at, c, acc + c, s.dv, four);
+    }
+  }
+  fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512));
+  }
+}
+
+template <int DV>
+int launch(tx_ctx *ctx, const Shape &s, const Split &x, const Out &o) {
+  CUtensorMap mq, mk, mv;
+  if (!split_map(&mq, x.q, 64, s.T, s.B * 2 * s.H, 128) || !split_map(&mk, x.k, 64, s.S, s.B * 2 * s.Hk, 128) ||
+      !split_map(&mv, x.v, DV, s.S, s.B * s.Hk, 64))
+    return tx_fail(ctx, TX_ERR_UNSUPPORTED, "differential attention: tensor map");
+  TX_CUDA(ctx, cudaFuncSetAttribute(k_diff_fwd<DV>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<DV>::SMEM));
+  const int64_t blocks = x.qt * s.B * s.H;
+  k_diff_fwd<DV><<<(unsigned)blocks, kThreads, Cfg<DV>::SMEM, ctx->stream>>>(s, x, mq, mk, mv, o);
+  TX_LAUNCHED(ctx, "k_diff_fwd");
+  return TX_OK;
+}
+
+}  // namespace
+
+int tc_forward(tx_ctx *ctx, const Shape &s, const Split &x, float *out, float *out2, float *lse) {
+  const Out o{out, out2, lse};
+  return x.vw == 64 ? launch<64>(ctx, s, x, o) : launch<128>(ctx, s, x, o);
+}
+
+}  // namespace tx_diff
