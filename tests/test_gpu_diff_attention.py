@@ -8,10 +8,10 @@ sum |q k| a score is within E c_ij, a weight within 2 E max_j c_ij of itself
 and E for its own product.  The gradients' bounds follow the same way through
 dP (E sum |dO| |v|), D (the outputs' bound), dS and the last product.  Sums in
 fp32 add less than a tenth of this.  What is held in 16 bits has a floor besides:
-an fp16 tail is rounded to half of 2^-24, a weight carries 2^14 (2^13 / (1 +
-|lam|) at least in the backward), so it is within W = 2^-37 (1 + |lam|) however
-small it is, and a score gradient, scaled so that 2 max|dO| max|v| lies in
-[2^13, 2^14), within 2^-25 / 2^13 of that bound.  Those bounds are for the worst case at
+an fp16 head and tail are each rounded to half of 2^-24, 2^-24 in all, and a
+weight carries at least 2^8 (2^13 / (1 + |lam|) in the backward), so it is within
+2^-32 (1 + |lam|) however small it is; a score gradient, scaled so that 2 max|dO|
+max|v| lies in [2^13, 2^14), is within 2^-24 / 2^13 of that bound.  Those bounds are for the worst case at
 every element; over a whole tensor errors of this kind are independent, about
 1e-6 of its norm, and 1e-5 is allowed.
 """
@@ -51,7 +51,7 @@ def reference(q, k, v, lam, dout, scale, causal, start, lengths):
                 a.append(p / np.maximum(p.sum(-1, keepdims=True), 1e-300))
                 c = np.abs(qm) @ np.abs(km).T * abs(scale)
                 ea.append(2 * E * np.where(ok, c, 0.0).max(-1, keepdims=True) + 4e-7)  # relative error of the weights
-            floor = 2.0**-37 * (1 + abs(lam[h])) * ok
+            floor = 2.0**-32 * (1 + abs(lam[h])) * ok
             w = a[0] - lam[h] * a[1]
             ew = floor + a[0] * ea[0] + abs(lam[h]) * a[1] * ea[1]
             wabs = a[0] + abs(lam[h]) * a[1]
@@ -67,7 +67,7 @@ def reference(q, k, v, lam, dout, scale, causal, start, lengths):
                 eD = ((a[m] * (ea[m] + E)) @ np.abs(vv) * np.abs(g)).sum(-1, keepdims=True)
                 ds = a[m] * (dp - D) * f
                 bound = 2 * np.linalg.norm(dout[b, :, h], axis=-1).max() * np.linalg.norm(vv, axis=-1).max()
-                eds = abs(f) * 2.0**-38 * bound * ok + abs(f) * a[m] * (edp + eD + (ea[m] + 4e-7) * np.abs(dp - D))
+                eds = abs(f) * 2.0**-37 * bound * ok + abs(f) * a[m] * (edp + eD + (ea[m] + 4e-7) * np.abs(dp - D))
                 val[1][b, :, 2 * h + m] = ds @ k[b, :n, 2 * kv + m]
                 tol[1][b, :, 2 * h + m] = (eds + E * np.abs(ds)) @ np.abs(k[b, :n, 2 * kv + m])
                 val[2][b, :n, 2 * kv + m] += ds.T @ q[b, :, 2 * h + m]

@@ -16,6 +16,17 @@ namespace {
 PFN_cuTensorMapEncodeTiled_v12000 g_encode = nullptr;
 std::once_flag g_encode_once;
 
+__device__ __forceinline__ float warp_max(float v) {
+#pragma unroll
+  for (int o = 16; o; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
+  return v;
+}
+__device__ __forceinline__ float warp_sum(float v) {
+#pragma unroll
+  for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+
 // A block splits one tile of 128 rows of one head; blockIdx.z picks the tensor.
 struct SplitJob {
   const float *src;
@@ -28,9 +39,13 @@ struct SplitJob {
 };
 struct SplitJobs {
   SplitJob j[4];
+  // with the output's gradient (job 3) its rows' D1 = dO . (out + lam out2) and D2 = dO . out2 go to
+  // stats, beside lse, and each tile's sum of D2 to sums
+  const float *out, *out2, *lse;
+  float *stats, *sums;
 };
-template <int W>
-__device__ __forceinline__ void split_tile(const Shape &s, const SplitJob &J, uint32_t *red) {
+template <int W, bool STATS>
+__device__ __forceinline__ void split_tile(const Shape &s, const SplitJobs &jobs, const SplitJob &J, uint32_t *red) {
   constexpr int PARTS = W / 8, ROWS = 256 / PARTS, UNITS = kRows / ROWS;  // 8 elements a thread and unit
   const int64_t head = (int64_t)blockIdx.x / J.tiles, tile = (int64_t)blockIdx.x - head * J.tiles;
   const int64_t b = head / J.heads, n0 = tile * kRows;
@@ -58,6 +73,52 @@ __device__ __forceinline__ void split_tile(const Shape &s, const SplitJob &J, ui
           if (c + i < J.w) x[u][i] = __ldg(src + i);
       }
     }
+  }
+  if (STATS) {
+    const float lam = __ldg(s.lam + hh);
+    const int64_t steps = (J.N + 63) / 64;
+    float total = 0.f;
+#pragma unroll
+    for (int u = 0; u < UNITS; ++u) {
+      const int64_t n = n0 + r0 + u * ROWS, at = ((b * J.N + n) * J.heads + hh) * J.w + c;
+      float d1 = 0.f, d2 = 0.f;
+      if (n < J.N) {
+        auto add = [&](float g, float y, float y2) {
+          d1 += g * (y + lam * y2);
+          d2 += g * y2;
+        };
+        if (four && ((uintptr_t)jobs.out & 15) == 0 && ((uintptr_t)jobs.out2 & 15) == 0) {
+#pragma unroll
+          for (int i = 0; i < 2; ++i)
+            if (c + 4 * i < J.w) {
+              const float4 y = __ldg(reinterpret_cast<const float4 *>(jobs.out + at) + i);
+              const float4 z = __ldg(reinterpret_cast<const float4 *>(jobs.out2 + at) + i);
+              add(x[u][4 * i], y.x, z.x), add(x[u][4 * i + 1], y.y, z.y);
+              add(x[u][4 * i + 2], y.z, z.z), add(x[u][4 * i + 3], y.w, z.w);
+            }
+        } else {
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            if (c + i < J.w) add(x[u][i], __ldg(jobs.out + at + i), __ldg(jobs.out2 + at + i));
+        }
+      }
+#pragma unroll
+      for (int o = PARTS / 2; o; o >>= 1) {
+        d1 += __shfl_xor_sync(0xffffffffu, d1, o);
+        d2 += __shfl_xor_sync(0xffffffffu, d2, o);
+      }
+      if (c == 0 && n / 64 < steps) {  // rows behind the last up to a step's end too
+        float *to = jobs.stats + (head * steps + n / 64) * 256 + n % 64;
+        const bool live = n < J.N;
+        to[0] = live ? __ldg(jobs.lse + (b * 2 * s.H + 2 * hh) * J.N + n) : INFINITY;
+        to[64] = live ? __ldg(jobs.lse + (b * 2 * s.H + 2 * hh + 1) * J.N + n) : INFINITY;
+        to[128] = d1;
+        to[192] = d2;
+        total += d2;
+      }
+    }
+    total = warp_sum(total);
+    if ((threadIdx.x & 31) == 0) red[16 + (threadIdx.x >> 5)] = __float_as_uint(total);
   }
   // the tile's largest finite magnitude (and row norm)
   uint32_t top = 0;
@@ -96,6 +157,11 @@ __device__ __forceinline__ void split_tile(const Shape &s, const SplitJob &J, ui
   if (threadIdx.x == 0) {
     J.f[blockIdx.x] = __uint_as_float((uint32_t)(127 + e) << 23);
     if (J.norm) J.norm[blockIdx.x] = fminf(sqrtf(__uint_as_float(most)), 1e16f);
+    if (STATS) {
+      float total = 0.f;
+      for (int i = 0; i < 8; ++i) total += __uint_as_float(red[16 + i]);
+      jobs.sums[blockIdx.x] = total;
+    }
   }
   const float inv = __uint_as_float((uint32_t)(127 - e) << 23);
 #pragma unroll
@@ -112,24 +178,19 @@ __device__ __forceinline__ void split_tile(const Shape &s, const SplitJob &J, ui
 }
 __global__ void __launch_bounds__(256)
     k_diff_split(const __grid_constant__ Shape s, const __grid_constant__ SplitJobs jobs, int vw) {
-  __shared__ uint32_t red[16];
+  __shared__ uint32_t red[24];
   const SplitJob &J = jobs.j[blockIdx.z];
   if ((int64_t)blockIdx.x >= s.B * J.heads * J.tiles) return;
-  if (blockIdx.z >= 2 && vw == 128)
-    split_tile<128>(s, J, red);
-  else
-    split_tile<64>(s, J, red);
-}
-
-__device__ __forceinline__ float warp_max(float v) {
-#pragma unroll
-  for (int o = 16; o; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
-  return v;
-}
-__device__ __forceinline__ float warp_sum(float v) {
-#pragma unroll
-  for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  return v;
+  if (blockIdx.z == 3) {
+    if (vw == 128)
+      split_tile<128, true>(s, jobs, J, red);
+    else
+      split_tile<64, true>(s, jobs, J, red);
+  } else if (blockIdx.z == 2 && vw == 128) {
+    split_tile<128, false>(s, jobs, J, red);
+  } else {
+    split_tile<64, false>(s, jobs, J, red);
+  }
 }
 
 // ---- few query rows against many keys ----------------------------------------------------
@@ -283,43 +344,21 @@ __global__ void __launch_bounds__(kMaxVdim)
   }
 }
 
-// ---- backward ------------------------------------------------------------------------------
-// (lse1, lse2, D1, D2) of each (b, h, t); a warp per row.
-__global__ void __launch_bounds__(256)
-    k_diff_delta(const __grid_constant__ Shape s, const float *out, const float *out2, const float *lse,
-                 const float *dout, float4 *stats) {
-  const int64_t row = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5), rows = s.B * s.T * s.H;
-  const int lane = threadIdx.x & 31;
-  if (row >= rows) return;
-  const int h = (int)(row % s.H);
-  const int64_t bt = row / s.H, b = bt / s.T, t = bt - b * s.T;
-  const float lam = __ldg(s.lam + h);
-  float d1 = 0.f, d2 = 0.f;
-  for (int c = lane; c < s.dv; c += 32) {
-    const float g = dout[row * s.dv + c], o2 = out2[row * s.dv + c];
-    d1 += g * (out[row * s.dv + c] + lam * o2);
-    d2 += g * o2;
-  }
-  d1 = warp_sum(d1);
-  d2 = warp_sum(d2);
-  if (lane == 0)
-    stats[(b * s.H + h) * s.T + t] = make_float4(lse[(b * 2 * s.H + 2 * h) * s.T + t],
-                                                 lse[(b * 2 * s.H + 2 * h + 1) * s.T + t], d1, d2);
-}
-
-__global__ void __launch_bounds__(256) k_diff_dlam(const __grid_constant__ Shape s, const float4 *stats, float *dlam) {
-  __shared__ float sums[8];
+// dlam = -sum of D2, from the tiles' sums
+__global__ void __launch_bounds__(256) k_diff_dlam(const __grid_constant__ Shape s, const float *sums, int64_t tiles,
+                                                   float *dlam) {
+  __shared__ float part[8];
   const int h = blockIdx.x;
   float v = 0.f;
-  for (int64_t i = threadIdx.x; i < s.B * s.T; i += 256) {
-    const int64_t b = i / s.T, t = i - b * s.T;
-    v += stats[(b * s.H + h) * s.T + t].w;
+  for (int64_t i = threadIdx.x; i < s.B * tiles; i += 256) {
+    const int64_t b = i / tiles;
+    v += sums[(b * s.H + h) * tiles + (i - b * tiles)];
   }
   v = warp_sum(v);
-  if ((threadIdx.x & 31) == 0) sums[threadIdx.x >> 5] = v;
+  if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = v;
   __syncthreads();
   if (threadIdx.x == 0) {
-    for (int i = 1; i < 8; ++i) v += sums[i];
+    for (int i = 1; i < 8; ++i) v += part[i];
     dlam[h] = -v;
   }
 }
@@ -329,7 +368,7 @@ __global__ void __launch_bounds__(256) k_diff_dlam(const __grid_constant__ Shape
 struct Operands {
   Split x;
   Scratch data;
-  int64_t tq, tk, tv, tg;  // tiles
+  int64_t tq = 0, tk = 0, tv = 0, tg = 0;  // tiles
   static int width(const Shape &s) { return s.dv <= 64 ? 64 : 128; }
   static size_t total(const Shape &s, bool gradient) {
     const int64_t w = width(s), qt = (s.T + kRows - 1) / kRows, kt = (s.S + kRows - 1) / kRows;
@@ -357,14 +396,17 @@ struct Operands {
     x.fg = f, f += tg;
     x.ng = f;
   }
-  int fill(tx_ctx *ctx, const Shape &s, const float *dout) {
+  // p: the backward's description, or null
+  int fill(tx_ctx *ctx, const Shape &s, const tx_diff_attention *p, float *stats, float *sums) {
     if (!data.ptr) return TX_ERR_OOM;
+    const float *dout = p ? p->dout : nullptr;
     auto w = [](const float *p) { return const_cast<float *>(p); };
     SplitJobs jobs{};
     jobs.j[0] = SplitJob{s.q, x.q, w(x.fq), nullptr, s.T, x.qt, 2 * s.H, s.d, s.scale * kLog2e, 0};
     jobs.j[1] = SplitJob{s.k, x.k, w(x.fk), nullptr, s.S, x.kt, 2 * s.Hk, s.d, 1.0f, 1};
     jobs.j[2] = SplitJob{s.v, x.v, w(x.fv), w(x.nv), s.S, x.kt, s.Hk, s.dv, 1.0f, 1};
     jobs.j[3] = SplitJob{dout, x.g, w(x.fg), w(x.ng), s.T, x.qt, s.H, s.dv, 1.0f, 0};
+    if (p) jobs.out = p->out, jobs.out2 = p->out2, jobs.lse = p->lse, jobs.stats = stats, jobs.sums = sums;
     const int64_t blocks = tq > tk ? tq : tk;
     k_diff_split<<<dim3((unsigned)blocks, 1, dout ? 4u : 3u), 256, 0, ctx->stream>>>(s, jobs, x.vw);
     TX_LAUNCHED(ctx, "k_diff_split");
@@ -390,6 +432,13 @@ int check_desc(tx_ctx *ctx, const tx_diff_attention *p, Shape &s) {
   return TX_OK;
 }
 
+int join(tx_ctx *ctx, const Shape &s, const Parts &parts, float *out, float *out2, float *lse) {
+  k_diff_join<<<(unsigned)(s.B * s.T * s.H), kMaxVdim, 0, ctx->stream>>>(s, parts.splits, parts.o, parts.ml, out, out2,
+                                                                       lse);
+  TX_LAUNCHED(ctx, "k_diff_join");
+  return TX_OK;
+}
+
 template <int RP>
 int launch_rows(tx_ctx *ctx, const Shape &s, float *out, float *out2, float *lse) {
   const int64_t items = s.T * s.G, chunks = (items + RP - 1) / RP;
@@ -408,15 +457,12 @@ int launch_rows(tx_ctx *ctx, const Shape &s, float *out, float *out2, float *lse
   k_diff_rows<RP><<<dim3((unsigned)splits, (unsigned)(s.B * s.Hk), (unsigned)chunks), kRowThreads, smem, ctx->stream>>>(
       s, (int)splits, per, po.as<float>(), pm.as<float2>());
   TX_LAUNCHED(ctx, "k_diff_rows");
-  k_diff_join<<<(unsigned)(s.B * s.Hk * items), kMaxVdim, 0, ctx->stream>>>(s, (int)splits, po.as<float>(),
-                                                                           pm.as<float2>(), out, out2, lse);
-  TX_LAUNCHED(ctx, "k_diff_join");
-  return TX_OK;
+  return join(ctx, s, Parts{po.as<float>(), pm.as<float2>(), (int)splits}, out, out2, lse);
 }
 
 }  // namespace
 
-bool split_map(CUtensorMap *m, const __half *base, int w, int64_t rows, int64_t heads, int box) {
+bool split_map(CUtensorMap *m, const __half *base, int w, int64_t rows, int64_t heads) {
   std::call_once(g_encode_once, [] {
     void *fn = nullptr;
     cudaDriverEntryPointQueryResult q;
@@ -427,7 +473,7 @@ bool split_map(CUtensorMap *m, const __half *base, int w, int64_t rows, int64_t 
   if (!g_encode) return false;
   cuuint64_t dims[3] = {(cuuint64_t)(2 * w), (cuuint64_t)rows, (cuuint64_t)heads};
   cuuint64_t strides[2] = {(cuuint64_t)(4 * w), (cuuint64_t)(4 * w) * (cuuint64_t)rows};
-  cuuint32_t bx[3] = {64u, (cuuint32_t)box, 1u};
+  cuuint32_t bx[3] = {64u, 64u, 1u};
   cuuint32_t es[3] = {1u, 1u, 1u};
   return g_encode(m, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, (void *)base, dims, strides, bx, es,
                   CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
@@ -453,8 +499,15 @@ extern "C" int tx_diff_attention_fwd(tx_ctx *ctx, const tx_diff_attention *p) {
   if (s.T * s.G <= 4) return launch_rows<4>(ctx, s, p->out, p->out2, p->lse);
   if (s.T * s.G <= 8 || s.S == 0) return launch_rows<8>(ctx, s, p->out, p->out2, p->lse);
   Operands x(ctx, s, false);
-  TX_TRY(x.fill(ctx, s, nullptr));
-  return tc_forward(ctx, s, x.x, p->out, p->out2, p->lse);
+  TX_TRY(x.fill(ctx, s, nullptr, nullptr, nullptr));
+  const int splits = tc_forward_splits(ctx, s);
+  if (splits == 1) return tc_forward(ctx, s, x.x, p->out, p->out2, p->lse, Parts{nullptr, nullptr, 1});
+  const int64_t rows = s.B * s.H * s.T * 2;
+  Scratch po(ctx, (size_t)(rows * splits * s.dv) * 4), pm(ctx, (size_t)(rows * splits) * 8);
+  if (!po.ptr || !pm.ptr) return TX_ERR_OOM;
+  const Parts parts{po.as<float>(), pm.as<float2>(), splits};
+  TX_TRY(tc_forward(ctx, s, x.x, p->out, p->out2, p->lse, parts));
+  return join(ctx, s, parts, p->out, p->out2, p->lse);
 }
 
 extern "C" int tx_diff_attention_bwd(tx_ctx *ctx, const tx_diff_attention *p) {
@@ -467,17 +520,6 @@ extern "C" int tx_diff_attention_bwd(tx_ctx *ctx, const tx_diff_attention *p) {
   if (rows && (!p->q || !p->lam || !p->out || !p->out2 || !p->lse || !p->dout || (s.S && (!p->k || !p->v))))
     return tx_fail(ctx, TX_ERR_INVALID, "differential attention: null buffer");
   DeviceScope device(ctx);
-  Scratch stats(ctx, rows ? (size_t)rows * sizeof(float4) : 16);
-  if (!stats.ptr) return TX_ERR_OOM;
-  if (rows) {
-    k_diff_delta<<<(unsigned)((rows + 7) / 8), 256, 0, ctx->stream>>>(s, p->out, p->out2, p->lse, p->dout,
-                                                                     stats.as<float4>());
-    TX_LAUNCHED(ctx, "k_diff_delta");
-  }
-  if (p->dlam) {
-    k_diff_dlam<<<(unsigned)s.H, 256, 0, ctx->stream>>>(s, stats.as<float4>(), p->dlam);
-    TX_LAUNCHED(ctx, "k_diff_dlam");
-  }
   if (!rows || !s.S) {  // nothing to multiply: no query or no key
     if (p->dq) TX_CUDA(ctx, cudaMemsetAsync(p->dq, 0, (size_t)rows * 2 * s.d * 4, ctx->stream));
     if (p->dk) {
@@ -485,10 +527,18 @@ extern "C" int tx_diff_attention_bwd(tx_ctx *ctx, const tx_diff_attention *p) {
       TX_CUDA(ctx, cudaMemsetAsync(p->dk, 0, keys * 2 * s.d * 4, ctx->stream));
       TX_CUDA(ctx, cudaMemsetAsync(p->dv, 0, keys * s.dv * 4, ctx->stream));
     }
+    if (p->dlam) TX_CUDA(ctx, cudaMemsetAsync(p->dlam, 0, (size_t)s.H * 4, ctx->stream));
     return TX_OK;
   }
-  if (!p->dq && !p->dk) return TX_OK;
+  Scratch stats(ctx, (size_t)(s.B * s.H * ((s.T + 63) / 64)) * 256 * 4);
   Operands x(ctx, s, true);
-  TX_TRY(x.fill(ctx, s, p->dout));
-  return tc_backward(ctx, s, x.x, stats.as<float4>(), p->dq, p->dk, p->dv);
+  Scratch sums(ctx, (size_t)x.tg * 4);
+  if (!stats.ptr || !sums.ptr) return TX_ERR_OOM;
+  TX_TRY(x.fill(ctx, s, p, stats.as<float>(), sums.as<float>()));
+  if (p->dlam) {
+    k_diff_dlam<<<(unsigned)s.H, 256, 0, ctx->stream>>>(s, sums.as<float>(), x.x.qt, p->dlam);
+    TX_LAUNCHED(ctx, "k_diff_dlam");
+  }
+  if (!p->dq && !p->dk) return TX_OK;
+  return tc_backward(ctx, s, x.x, stats.as<float>(), p->dq, p->dk, p->dv);
 }

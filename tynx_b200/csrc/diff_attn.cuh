@@ -66,12 +66,24 @@ struct Split {
   int vw;                        // W of v and g
   int64_t qt, kt;                // tiles of a head's queries and keys
 };
-// 3-D map {2 W, rows, heads} with boxes of 64 columns x `box` rows (128-byte swizzle)
-bool split_map(CUtensorMap *m, const __half *base, int w, int64_t rows, int64_t heads, int box);
+// 3-D map {2 W, rows, heads} with boxes of 64 columns x 64 rows (128-byte swizzle)
+bool split_map(CUtensorMap *m, const __half *base, int w, int64_t rows, int64_t heads);
 
-// stats: per (b, h, t) the log-sum-exp of both maps and D1, D2
-int tc_forward(tx_ctx *ctx, const Shape &s, const Split &x, float *out, float *out2, float *lse);
-int tc_backward(tx_ctx *ctx, const Shape &s, const Split &x, const float4 *stats, float *dq, float *dk, float *dv);
+// Partial results of ranges of keys, joined afterwards: part_ml[(at * 2 + map) *
+// splits + split] holds the reference and the sum of the range's exponentials
+// (reference -inf: no key), part_o the same times dv the unnormalised output; at
+// counts (b, key head, query, head of its group).
+struct Parts {
+  float *o;
+  float2 *ml;
+  int splits;
+};
+// how many ranges of keys the tensor-core forward should take
+int tc_forward_splits(tx_ctx *ctx, const Shape &s);
+// out, out2 and lse, or with parts.splits > 1 the partial results
+int tc_forward(tx_ctx *ctx, const Shape &s, const Split &x, float *out, float *out2, float *lse, const Parts &parts);
+// stats [b][h][ceil(T / 64)][4][64]: the log-sum-exp of both maps (+inf behind the last query), D1, D2
+int tc_backward(tx_ctx *ctx, const Shape &s, const Split &x, const float *stats, float *dq, float *dk, float *dv);
 
 // ---- device wrappers -------------------------------------------------------------------------
 constexpr uint64_t kWaitNs = 2000000000ull;  // 2 s
@@ -207,7 +219,54 @@ __device__ __forceinline__ float ex2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-// (a, b) as a pair of fp16 heads (a in the low half) and a pair of fp16 tails
+// two fp32 values in a register pair, and arithmetic on both at once
+__device__ __forceinline__ uint64_t two(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t two(uint32_t a, uint32_t b) { return two(__uint_as_float(a), __uint_as_float(b)); }
+__device__ __forceinline__ void untwo(uint64_t r, float &a, float &b) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(r));
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t sub2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("sub.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+// a pair of fp32 as fp16 heads (the first in the low half) and tails.  The head
+// is cut off, not rounded: it needs no conversion back, and the tail keeps the
+// cut part to 2^-21 of the value (an operand that meets rounded pairs, so the
+// cut's sign does not add up).
+__device__ __forceinline__ void cut2(uint64_t v, uint32_t &hi, uint32_t &lo) {
+  float a, b, ra, rb;
+  untwo(v, a, b);
+  const float ha = __uint_as_float(__float_as_uint(a) & 0xffffe000u), hb = __uint_as_float(__float_as_uint(b) & 0xffffe000u);
+  untwo(sub2(v, two(ha, hb)), ra, rb);
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(hi) : "f"(hb), "f"(ha));
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(lo) : "f"(rb), "f"(ra));
+}
+// the same with a rounded head: within 2^-22 of the value
 __device__ __forceinline__ void split2(float a, float b, uint32_t &hi, uint32_t &lo) {
   const __half2 h = __floats2half2_rn(a, b);
   const float2 f = __half22float2(h);

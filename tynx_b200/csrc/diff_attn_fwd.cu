@@ -32,29 +32,29 @@ struct Cfg {
   static constexpr int VSLOT = 2 * (DV / 64) * VBLK;  // 64 keys: heads, tails
   static constexpr int RING = 3;
   static constexpr int SMEM = 4 * QK + RING * VSLOT + 1024 /*barriers*/ + 1024 /*align*/;
-  // at the end map 2's output passes through Q's and K's memory
-  static_assert(128 * DV * 4 <= 4 * QK, "output staging");
+  // at the end both maps' outputs pass through Q's and K's memory
+  static_assert(2 * 128 * DV * 4 <= 4 * QK, "output staging");
 };
 
 struct Out {
   float *out, *out2, *lse;
+  Parts parts;
+  int per;  // tiles of a range of keys
 };
 
-// 16-byte chunk c of a staged output row: rows a warp touches together spread over the banks
+// 16-byte chunk c of a staged output row: rows a warp writes together spread over the banks
 template <int DV>
-__device__ __forceinline__ float4 *staged(uint8_t *sm, int r, int c) {
-  return reinterpret_cast<float4 *>(sm) + r * (DV / 4) + (c ^ (r & 7));
+__device__ __forceinline__ float4 *staged(uint8_t *sm, int m, int r, int c) {
+  return reinterpret_cast<float4 *>(sm) + m * (128 * DV / 4) + r * (DV / 4) + (c ^ (r & 7));
 }
-
-__device__ __forceinline__ void store_row(float *dst, int c, const float *v, int dv, bool four) {
+__device__ __forceinline__ void store4(float *dst, int c, float4 v, int dv, bool four) {
   if (four) {
-#pragma unroll
-    for (int j = 0; j < 8; ++j)
-      if (c + 4 * j < dv) *reinterpret_cast<float4 *>(dst + c + 4 * j) = make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+    if (c < dv) *reinterpret_cast<float4 *>(dst + c) = v;
   } else {
-#pragma unroll
-    for (int j = 0; j < 32; ++j)
-      if (c + j < dv) dst[c + j] = v[j];
+    if (c < dv) dst[c] = v.x;
+    if (c + 1 < dv) dst[c + 1] = v.y;
+    if (c + 2 < dv) dst[c + 2] = v.z;
+    if (c + 3 < dv) dst[c + 3] = v.w;
   }
 }
 
@@ -75,12 +75,14 @@ __global__ void __launch_bounds__(kThreads, 1)
 
   // causal: the queries with most keys first
   const int64_t heads = s.B * s.H;
+  const int split = blockIdx.y;
   const int64_t qt = x.qt - 1 - (int64_t)blockIdx.x / heads, bh = (int64_t)blockIdx.x % heads;
   const int64_t b = bh / s.H;
   const int h = (int)(bh - b * s.H), hk = h / s.G;
   const int64_t t0 = qt * 128, tl = t0 + 127 < s.T ? t0 + 127 : s.T - 1;
   const int64_t n = s.length(b);
-  const int tiles = (int)((s.seen(tl, n) + 127) / 128);
+  const int tile0 = split * o.per, all = (int)((s.seen(tl, n) + 127) / 128);  // this range's tiles
+  const int tiles = all <= tile0 ? 0 : all - tile0 < o.per ? all - tile0 : o.per;
 
   if (threadIdx.x == 0) {
     bar_init(q_full, 1);
@@ -97,7 +99,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     bar_init(o_full, 1);
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-    if (h == 0 && qt == 0) report_length(s, b);
+    if (h == 0 && qt == 0 && split == 0) report_length(s, b);
   }
   if (warp == 1) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(su32(tmem_holder)),
@@ -114,8 +116,9 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (warp == 0 && lane == 0 && tiles) {
       bar_expect(q_full, 2 * C::QK);
       for (int m = 0; m < 2; ++m)
-        for (int p = 0; p < 2; ++p)
-          tma_3d(sq + m * C::QK + p * C::HALF, &mq, q_full, p * 64, (int)t0, (int)(b * 2 * s.H + 2 * h + m));
+        for (int p = 0; p < 4; ++p)  // (head or tail, 64-row half)
+          tma_3d(sq + m * C::QK + p * C::VBLK, &mq, q_full, (p >> 1) * 64, (int)t0 + (p & 1) * 64,
+                 (int)(b * 2 * s.H + 2 * h + m));
       bool ok = true;
       int loaded_k = 0, loaded_v = 0;
       for (int i = 0; i < tiles && ok; ++i) {
@@ -123,8 +126,8 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (i) ok = bar_wait(k_empty + m, (i - 1) & 1, abort_flag, s.err, 1);
           if (!ok) break;
           bar_expect(k_full + m, C::QK);
-          for (int p = 0; p < 2; ++p)
-            tma_3d(sk + m * C::QK + p * C::HALF, &mk, k_full + m, p * 64, i * 128,
+          for (int p = 0; p < 4; ++p)
+            tma_3d(sk + m * C::QK + p * C::VBLK, &mk, k_full + m, (p >> 1) * 64, (tile0 + i) * 128 + (p & 1) * 64,
                    (int)(b * 2 * s.Hk + 2 * hk + m));
           ++loaded_k;
         }
@@ -134,7 +137,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (!ok) break;
           bar_expect(v_full + slot, C::VSLOT);
           for (int p = 0; p < 2 * (DV / 64); ++p)
-            tma_3d(sv + slot * C::VSLOT + p * C::VBLK, &mv, v_full + slot, p * 64, i * 128 + hf * 64,
+            tma_3d(sv + slot * C::VSLOT + p * C::VBLK, &mv, v_full + slot, p * 64, (tile0 + i) * 128 + hf * 64,
                    (int)(b * s.Hk + hk));
           ++loaded_v;
         }
@@ -199,23 +202,75 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t lane_row = (uint32_t)(quad * 32) << 16;
     const uint32_t ts = tmem + m * 128 + lane_row, to = tmem + 256 + m * DV + lane_row;
     const int64_t t = t0 + r;
-    const int64_t seen = t < s.T ? s.seen(t, n) : s.seen(tl, n);
+    const int64_t seen = (t < s.T ? s.seen(t, n) : s.seen(tl, n)) - (int64_t)tile0 * 128;
     const float fq = __ldg(x.fq + (b * 2 * s.H + 2 * h + m) * x.qt + qt);
-    const float *fk = x.fk + (b * 2 * s.Hk + 2 * hk + m) * x.kt, *fv = x.fv + (b * s.Hk + hk) * x.kt;
-    // P carries 2^14 so that fp16 tails hold; O and the sum carry it alike
-    float top = -INFINITY, sum = 0.f, shrink = 1.f;
-    float acc[DV];
+    const float *fk = x.fk + (b * 2 * s.Hk + 2 * hk + m) * x.kt + tile0, *fv = x.fv + (b * s.Hk + hk) * x.kt + tile0;
+    // P = 2^(S - ref): the reference is kCarry below the row's maximum when it is set, so that fp16
+    // tails hold, and follows only when the maximum has outgrown it by kSlack more (fp16 ends at 2^16)
+    constexpr float kCarry = 8.f, kSlack = 6.f;
+    float ref = -INFINITY, top = -INFINITY;  // top: the maximum that ref was set by
+    uint64_t sum2[2] = {two(0.f, 0.f), two(0.f, 0.f)};
+    uint64_t acc[DV / 2];
 #pragma unroll
-    for (int j = 0; j < DV; ++j) acc[j] = 0.f;
-    auto add_tile = [&](float f, float g) {  // acc = f acc + g O
+    for (int j = 0; j < DV / 2; ++j) acc[j] = two(0.f, 0.f);
+    auto add_tile = [&](float g) {  // acc += g O
+      const uint64_t g2 = two(g, g);
+      uint32_t y[2][16];
+      tld16_issue(to, y[0]);
 #pragma unroll
-      for (int c = 0; c < DV / 32; ++c) {
-        uint32_t y[32];
-        tld32_issue(to + 32 * c, y);
+      for (int c = 0; c < DV / 16; ++c) {
         tld_wait();
-        after_wait(y);
+        after_wait(y[c & 1]);
+        if (c + 1 < DV / 16) tld16_issue(to + 16 * (c + 1), y[(c + 1) & 1]);
 #pragma unroll
-        for (int j = 0; j < 32; ++j) acc[32 * c + j] = acc[32 * c + j] * f + __uint_as_float(y[j]) * g;
+        for (int j = 0; j < 8; ++j) acc[8 * c + j] = fma2(two(y[c & 1][2 * j], y[c & 1][2 * j + 1]), g2, acc[8 * c + j]);
+      }
+    };
+    // columns from lim on are masked out of a tile's last chunk(s)
+    auto tile_max = [&](int lim, bool whole) {
+      float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+      uint32_t y[2][16];
+      tld16_issue(ts, y[0]);
+#pragma unroll
+      for (int c = 0; c < 8; ++c) {
+        tld_wait();
+        after_wait(y[c & 1]);
+        if (c < 7) tld16_issue(ts + 16 * (c + 1), y[(c + 1) & 1]);
+        if (!whole) {
+#pragma unroll
+          for (int j = 0; j < 16; ++j)
+            if (16 * c + j >= lim) y[c & 1][j] = 0xff800000u;  // -inf
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          mx[j & 3] = max3(mx[j & 3], __uint_as_float(y[c & 1][2 * j]), __uint_as_float(y[c & 1][2 * j + 1]));
+      }
+      return fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+    };
+    auto tile_exp = [&](int lim, bool whole, float f, float at) {
+      const uint64_t f2 = two(f, f), at2 = two(-at, -at);
+      uint32_t y[2][16];
+      tld16_issue(ts, y[0]);
+#pragma unroll
+      for (int c = 0; c < 8; ++c) {
+        tld_wait();
+        after_wait(y[c & 1]);
+        if (c < 7) tld16_issue(ts + 16 * (c + 1), y[(c + 1) & 1]);
+        if (!whole) {
+#pragma unroll
+          for (int j = 0; j < 16; ++j)
+            if (16 * c + j >= lim) y[c & 1][j] = 0xff800000u;
+        }
+        uint32_t hi[8], lo[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          float a, d;
+          untwo(fma2(two(y[c & 1][2 * j], y[c & 1][2 * j + 1]), f2, at2), a, d);
+          const uint64_t p = two(ex2(a), ex2(d));
+          sum2[j & 1] = add2(sum2[j & 1], p);
+          cut2(p, hi[j], lo[j]);
+        }
+        tst_pairs(ts + 16 * c, hi, lo);
       }
     };
     bool ok = true;
@@ -225,90 +280,77 @@ __global__ void __launch_bounds__(kThreads, 1)
       ok = __all_sync(0xffffffffu, bar_wait(s_full + m, i & 1, abort_flag, s.err, 7));
       if (!ok) break;
       fence_after();
-      if (i) add_tile(shrink, gv);
-      gv = next_gv;
       const int64_t left = seen - (int64_t)i * 128;
       const int lim = left < 0 ? 0 : left > 128 ? 128 : (int)left;
       const bool whole = __all_sync(0xffffffffu, lim == 128);
-      float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+      const float mx = tile_max(lim, whole) * f;
+      if (i) add_tile(gv);
+      gv = next_gv;
+      if (__any_sync(0xffffffffu, mx > top + kSlack || (top == -INFINITY && mx > top))) {
+        const float now = fmaxf(top, mx);
+        const float shrink = top == -INFINITY ? 0.f : ex2(top - now);
+        const uint64_t s2 = two(shrink, shrink);
+        top = now;
+        ref = now - kCarry;
+        sum2[0] = mul2(sum2[0], s2);
+        sum2[1] = mul2(sum2[1], s2);
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        uint32_t y[32];
-        tld32_issue(ts + 32 * c, y);
-        tld_wait();
-        after_wait(y);
-        if (whole) {
-#pragma unroll
-          for (int j = 0; j < 32; ++j) mx[j & 3] = fmaxf(mx[j & 3], __uint_as_float(y[j]));
-        } else {
-#pragma unroll
-          for (int j = 0; j < 32; ++j)
-            if (32 * c + j < lim) mx[j & 3] = fmaxf(mx[j & 3], __uint_as_float(y[j]));
-        }
+        for (int j = 0; j < DV / 2; ++j) acc[j] = mul2(acc[j], s2);
       }
-      const float now = fmaxf(top, fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * f);
-      const float at = now == -INFINITY ? 0.f : now - 14.f;  // no key yet: all weights are 2^-inf
-      shrink = top == -INFINITY ? 0.f : ex2(top - now);
-      top = now;
-      float part[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int c = 0; c < 8; ++c) {
-        uint32_t y[16], hi[8], lo[8];
-        tld16_issue(ts + 16 * c, y);
-        tld_wait();
-        after_wait(y);
-        float p[16];
-#pragma unroll
-        for (int j = 0; j < 16; ++j) p[j] = ex2(fmaf(__uint_as_float(y[j]), f, -at));
-        if (!whole) {
-#pragma unroll
-          for (int j = 0; j < 16; ++j)
-            if (16 * c + j >= lim) p[j] = 0.f;
-        }
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          part[j & 3] += p[2 * j] + p[2 * j + 1];
-          split2(p[2 * j], p[2 * j + 1], hi[j], lo[j]);
-        }
-        tst_pairs(ts + 16 * c, hi, lo);
-      }
-      sum = sum * shrink + ((part[0] + part[1]) + (part[2] + part[3]));
+      const float at = top == -INFINITY ? 0.f : ref;  // no key yet: all weights are 2^-inf
+      if (whole)
+        tile_exp(128, true, f, at);
+      else
+        tile_exp(lim, false, f, at);
       tst_wait();
       fence_before();
       bar_arrive(p_full + m);
     }
     if (tiles) ok = __all_sync(0xffffffffu, ok && bar_wait(o_full, 0, abort_flag, s.err, 8));
     fence_after();
-    if (tiles && ok) add_tile(shrink, gv);
-    const bool none = top == -INFINITY;
-    const float inv = none ? 0.f : 1.0f / sum;
+    if (tiles && ok) add_tile(gv);
+    float s0, s1, s2, s3;
+    untwo(sum2[0], s0, s1);
+    untwo(sum2[1], s2, s3);
+    const float sum = (s0 + s1) + (s2 + s3);
+    const bool none = top == -INFINITY, live = t < s.T && ok;
+    const bool parts = o.parts.splits > 1;
+    const float inv = parts ? 1.f : none ? 0.f : 1.0f / sum;
+    const int64_t n_items = s.T * s.G;
+    const int64_t at0 = (b * s.Hk + hk) * n_items + (h - hk * s.G);  // + t * G
+    if (live && parts)
+      o.parts.ml[((at0 + t * s.G) * 2 + m) * o.parts.splits + split] = make_float2(none ? -INFINITY : ref, sum);
+    if (live && !parts && o.lse) o.lse[(b * 2 * s.H + 2 * h + m) * s.T + t] = none ? INFINITY : ref + log2f(sum);
 #pragma unroll
-    for (int j = 0; j < DV; ++j) acc[j] *= inv;
-    if (m == 1) {
-#pragma unroll
-      for (int c = 0; c < DV / 4; ++c)
-        *staged<DV>(sm, r, c) = make_float4(acc[4 * c], acc[4 * c + 1], acc[4 * c + 2], acc[4 * c + 3]);
+    for (int c = 0; c < DV / 4; ++c) {
+      float4 v;
+      untwo(acc[2 * c], v.x, v.y);
+      untwo(acc[2 * c + 1], v.z, v.w);
+      *staged<DV>(sm, m, r, c) = make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv);
     }
     asm volatile("bar.sync 1, 256;" ::: "memory");
-    const bool live = t < s.T && ok;
-    if (live && o.lse) o.lse[(b * 2 * s.H + 2 * h + m) * s.T + t] = none ? INFINITY : (top - 14.f) + log2f(sum);
-    const int64_t at = ((b * s.T + t) * s.H + h) * s.dv;
-    const bool four = (s.dv & 3) == 0 && ((uintptr_t)o.out & 15) == 0 && ((uintptr_t)o.out2 & 15) == 0;
-    if (m == 0) {
+    // rows of the tile, whole lines at a time
+    if (ok) {
+      constexpr int LINES = 128 / DV;  // rows a warp stores at once
       const float lam = __ldg(s.lam + h);
-#pragma unroll
-      for (int c = 0; c < DV / 4; ++c) {
-        const float4 y = *staged<DV>(sm, r, c);
-        acc[4 * c] -= lam * y.x;
-        acc[4 * c + 1] -= lam * y.y;
-        acc[4 * c + 2] -= lam * y.z;
-        acc[4 * c + 3] -= lam * y.w;
+      const int c = lane % (DV / 4), sub = lane / (DV / 4);
+      for (int k = (warp - 4) * LINES + sub; k < 128; k += 8 * LINES) {
+        const int64_t tt = t0 + k;
+        if (tt >= s.T) break;
+        float4 a = *staged<DV>(sm, 0, k, c), d = *staged<DV>(sm, 1, k, c);
+        if (parts) {
+          float *dst = o.parts.o + ((at0 + tt * s.G) * 2 * o.parts.splits + split) * s.dv;
+          const bool four = (s.dv & 3) == 0;
+          store4(dst, 4 * c, a, s.dv, four);
+          store4(dst + (int64_t)o.parts.splits * s.dv, 4 * c, d, s.dv, four);
+        } else {
+          const int64_t at = ((b * s.T + tt) * s.H + h) * s.dv;
+          const bool four = (s.dv & 3) == 0 && ((uintptr_t)o.out & 15) == 0 && ((uintptr_t)o.out2 & 15) == 0;
+          a = make_float4(a.x - lam * d.x, a.y - lam * d.y, a.z - lam * d.z, a.w - lam * d.w);
+          store4(o.out + at, 4 * c, a, s.dv, four);
+          if (o.out2) store4(o.out2 + at, 4 * c, d, s.dv, four);
+        }
       }
-    }
-    float *dst = m ? o.out2 : o.out;
-    if (live && dst) {
-#pragma unroll
-      for (int c = 0; c < DV; c += 32) store_row(dst + at, c, acc + c, s.dv, four);
     }
   }
   fence_before();
@@ -322,20 +364,30 @@ __global__ void __launch_bounds__(kThreads, 1)
 template <int DV>
 int launch(tx_ctx *ctx, const Shape &s, const Split &x, const Out &o) {
   CUtensorMap mq, mk, mv;
-  if (!split_map(&mq, x.q, 64, s.T, s.B * 2 * s.H, 128) || !split_map(&mk, x.k, 64, s.S, s.B * 2 * s.Hk, 128) ||
-      !split_map(&mv, x.v, DV, s.S, s.B * s.Hk, 64))
+  if (!split_map(&mq, x.q, 64, s.T, s.B * 2 * s.H) || !split_map(&mk, x.k, 64, s.S, s.B * 2 * s.Hk) ||
+      !split_map(&mv, x.v, DV, s.S, s.B * s.Hk))
     return tx_fail(ctx, TX_ERR_UNSUPPORTED, "differential attention: tensor map");
   TX_CUDA(ctx, cudaFuncSetAttribute(k_diff_fwd<DV>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<DV>::SMEM));
   const int64_t blocks = x.qt * s.B * s.H;
-  k_diff_fwd<DV><<<(unsigned)blocks, kThreads, Cfg<DV>::SMEM, ctx->stream>>>(s, x, mq, mk, mv, o);
+  k_diff_fwd<DV><<<dim3((unsigned)blocks, (unsigned)o.parts.splits), kThreads, Cfg<DV>::SMEM, ctx->stream>>>(s, x, mq, mk,
+                                                                                                        mv, o);
   TX_LAUNCHED(ctx, "k_diff_fwd");
   return TX_OK;
 }
 
 }  // namespace
 
-int tc_forward(tx_ctx *ctx, const Shape &s, const Split &x, float *out, float *out2, float *lse) {
-  const Out o{out, out2, lse};
+int tc_forward_splits(tx_ctx *ctx, const Shape &s) {
+  // too few blocks of queries for the SMs: the keys are shared out too, two tiles at least a block
+  const int64_t blocks = (s.T + kRows - 1) / kRows * s.B * s.H, tiles = (s.S + kRows - 1) / kRows;
+  int64_t splits = ctx->num_sms / (blocks ? blocks : 1);
+  if (splits > (tiles + 1) / 2) splits = (tiles + 1) / 2;
+  return splits < 1 ? 1 : (int)splits;
+}
+
+int tc_forward(tx_ctx *ctx, const Shape &s, const Split &x, float *out, float *out2, float *lse, const Parts &parts) {
+  const int64_t tiles = (s.S + kRows - 1) / kRows;
+  const Out o{out, out2, lse, parts, (int)((tiles + parts.splits - 1) / parts.splits)};
   return x.vw == 64 ? launch<64>(ctx, s, x, o) : launch<128>(ctx, s, x, o);
 }
 
