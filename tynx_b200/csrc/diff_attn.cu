@@ -44,9 +44,10 @@ struct SplitJobs {
   const float *out, *out2, *lse;
   float *stats, *sums;
 };
+constexpr int kSplitThreads = 512, kSplitWarps = kSplitThreads / 32;
 template <int W, bool STATS>
 __device__ __forceinline__ void split_tile(const Shape &s, const SplitJobs &jobs, const SplitJob &J, uint32_t *red) {
-  constexpr int PARTS = W / 8, ROWS = 256 / PARTS, UNITS = kRows / ROWS;  // 8 elements a thread and unit
+  constexpr int PARTS = W / 8, ROWS = kSplitThreads / PARTS, UNITS = kRows / ROWS;  // 8 elements a thread and unit
   const int64_t head = (int64_t)blockIdx.x / J.tiles, tile = (int64_t)blockIdx.x - head * J.tiles;
   const int64_t b = head / J.heads, n0 = tile * kRows;
   const int hh = (int)(head - b * J.heads), c = threadIdx.x % PARTS * 8, r0 = threadIdx.x / PARTS;
@@ -118,7 +119,7 @@ __device__ __forceinline__ void split_tile(const Shape &s, const SplitJobs &jobs
       }
     }
     total = warp_sum(total);
-    if ((threadIdx.x & 31) == 0) red[16 + (threadIdx.x >> 5)] = __float_as_uint(total);
+    if ((threadIdx.x & 31) == 0) red[2 * kSplitWarps + (threadIdx.x >> 5)] = __float_as_uint(total);
   }
   // the tile's largest finite magnitude (and row norm)
   uint32_t top = 0;
@@ -143,14 +144,14 @@ __device__ __forceinline__ void split_tile(const Shape &s, const SplitJobs &jobs
   const uint32_t nb = __reduce_max_sync(0xffffffffu, __float_as_uint(norm));
   if ((threadIdx.x & 31) == 0) {
     red[threadIdx.x >> 5] = top;
-    red[8 + (threadIdx.x >> 5)] = nb;
+    red[kSplitWarps + (threadIdx.x >> 5)] = nb;
   }
   __syncthreads();
   uint32_t most = 0;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
+  for (int i = 0; i < kSplitWarps; ++i) {
     top = red[i] > top ? red[i] : top;
-    most = red[8 + i] > most ? red[8 + i] : most;
+    most = red[kSplitWarps + i] > most ? red[kSplitWarps + i] : most;
   }
   int e = (int)(top >> 23) - 127 - 13;
   e = e < -113 ? -113 : e > 114 ? 114 : e;
@@ -159,7 +160,7 @@ __device__ __forceinline__ void split_tile(const Shape &s, const SplitJobs &jobs
     if (J.norm) J.norm[blockIdx.x] = fminf(sqrtf(__uint_as_float(most)), 1e16f);
     if (STATS) {
       float total = 0.f;
-      for (int i = 0; i < 8; ++i) total += __uint_as_float(red[16 + i]);
+      for (int i = 0; i < kSplitWarps; ++i) total += __uint_as_float(red[2 * kSplitWarps + i]);
       jobs.sums[blockIdx.x] = total;
     }
   }
@@ -176,21 +177,19 @@ __device__ __forceinline__ void split_tile(const Shape &s, const SplitJobs &jobs
     *reinterpret_cast<uint4 *>(dst + W) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
   }
 }
-__global__ void __launch_bounds__(256)
-    k_diff_split(const __grid_constant__ Shape s, const __grid_constant__ SplitJobs jobs, int vw) {
-  __shared__ uint32_t red[24];
-  const SplitJob &J = jobs.j[blockIdx.z];
+// W: the values' width (queries and keys have 64); GRAD: the output's gradient alone
+template <int W, bool GRAD>
+__global__ void __launch_bounds__(kSplitThreads, 2)
+    k_diff_split(const __grid_constant__ Shape s, const __grid_constant__ SplitJobs jobs) {
+  __shared__ uint32_t red[3 * kSplitWarps];
+  const SplitJob &J = jobs.j[GRAD ? 3 : blockIdx.z];
   if ((int64_t)blockIdx.x >= s.B * J.heads * J.tiles) return;
-  if (blockIdx.z == 3) {
-    if (vw == 128)
-      split_tile<128, true>(s, jobs, J, red);
-    else
-      split_tile<64, true>(s, jobs, J, red);
-  } else if (blockIdx.z == 2 && vw == 128) {
-    split_tile<128, false>(s, jobs, J, red);
-  } else {
+  if (GRAD)
+    split_tile<W, true>(s, jobs, J, red);
+  else if (blockIdx.z < 2)
     split_tile<64, false>(s, jobs, J, red);
-  }
+  else
+    split_tile<W, false>(s, jobs, J, red);
 }
 
 // ---- few query rows against many keys ----------------------------------------------------
@@ -408,8 +407,18 @@ struct Operands {
     jobs.j[3] = SplitJob{dout, x.g, w(x.fg), w(x.ng), s.T, x.qt, s.H, s.dv, 1.0f, 0};
     if (p) jobs.out = p->out, jobs.out2 = p->out2, jobs.lse = p->lse, jobs.stats = stats, jobs.sums = sums;
     const int64_t blocks = tq > tk ? tq : tk;
-    k_diff_split<<<dim3((unsigned)blocks, 1, dout ? 4u : 3u), 256, 0, ctx->stream>>>(s, jobs, x.vw);
+    const dim3 grid((unsigned)blocks, 1, 3);
+    if (x.vw == 64)
+      k_diff_split<64, false><<<grid, kSplitThreads, 0, ctx->stream>>>(s, jobs);
+    else
+      k_diff_split<128, false><<<grid, kSplitThreads, 0, ctx->stream>>>(s, jobs);
     TX_LAUNCHED(ctx, "k_diff_split");
+    if (!p) return TX_OK;
+    if (x.vw == 64)
+      k_diff_split<64, true><<<(unsigned)tg, kSplitThreads, 0, ctx->stream>>>(s, jobs);
+    else
+      k_diff_split<128, true><<<(unsigned)tg, kSplitThreads, 0, ctx->stream>>>(s, jobs);
+    TX_LAUNCHED(ctx, "k_diff_split (gradient)");
     return TX_OK;
   }
 };

@@ -326,8 +326,7 @@ __device__ __forceinline__ void body(const Shape &s, const Split &x, const CUten
       const bool whole = __all_sync(0xffffffffu, lo_c == 0 && hi_c == 32);
       const uint32_t ts = tmem + lane_row + st * 192 + 32 * half;
       const float *col = stat + st * (4 * kStep) + 32 * half;
-      auto elementwise = [&](bool all) {
-#pragma unroll
+#pragma unroll 1  // rolled: the warps run it at different places, and unrolled they wait for instructions
         for (int c = 0; c < 2; ++c) {
           uint32_t y0[16], y1[16], yp[16];
           tld16_issue(ts + 16 * c, y0);
@@ -356,7 +355,7 @@ __device__ __forceinline__ void body(const Shape &s, const Split &x, const CUten
               untwo(sub2(mul2(two(y0[e0], y0[e1]), f02), st2(0)), a, d);
               untwo(sub2(mul2(two(y1[e0], y1[e1]), f12), st2(1)), a1, d1);
               a = ex2(a), d = ex2(d), a1 = ex2(a1), d1 = ex2(d1);
-              if (!all) {
+              if (!whole) {
                 if (16 * c + e0 < lo_c || 16 * c + e0 >= hi_c) a = a1 = 0.f;
                 if (16 * c + e1 < lo_c || 16 * c + e1 >= hi_c) d = d1 = 0.f;
               }
@@ -373,11 +372,6 @@ __device__ __forceinline__ void body(const Shape &s, const Split &x, const CUten
           tst_pairs(ts + 16 * c, h0, l0);
           if (MODE != kModeV) tst_pairs(ts + 64 + 16 * c, h1, l1);
         }
-      };
-      if (whole)
-        elementwise(true);
-      else
-        elementwise(false);
       if (i) {  // ran under this step's scores
         ok = __all_sync(0xffffffffu, bar_wait(a_full, (i - 1) & 1, abort_flag, s.err, 19));
         if (!ok) break;

@@ -226,51 +226,63 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int j = 0; j < 8; ++j) acc[8 * c + j] = fma2(two(y[c & 1][2 * j], y[c & 1][2 * j + 1]), g2, acc[8 * c + j]);
       }
     };
-    // columns from lim on are masked out of a tile's last chunk(s)
+    // The loops over a tile's columns stay rolled: two warps a scheduler run them at different places,
+    // and unrolled they wait for instructions more than for anything else.
+    auto mask = [&](uint32_t (&y)[16], int left) {  // columns from `left` on are not seen
+#pragma unroll
+      for (int j = 0; j < 16; ++j)
+        if (j >= left) y[j] = 0xff800000u;  // -inf
+    };
     auto tile_max = [&](int lim, bool whole) {
-      float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-      uint32_t y[2][16];
-      tld16_issue(ts, y[0]);
-#pragma unroll
-      for (int c = 0; c < 8; ++c) {
-        tld_wait();
-        after_wait(y[c & 1]);
-        if (c < 7) tld16_issue(ts + 16 * (c + 1), y[(c + 1) & 1]);
-        if (!whole) {
-#pragma unroll
-          for (int j = 0; j < 16; ++j)
-            if (16 * c + j >= lim) y[c & 1][j] = 0xff800000u;  // -inf
-        }
+      float mx[2] = {-INFINITY, -INFINITY};
+      auto part = [&](uint32_t (&y)[16], int c) {
+        if (!whole) mask(y, lim - 16 * c);
 #pragma unroll
         for (int j = 0; j < 8; ++j)
-          mx[j & 3] = max3(mx[j & 3], __uint_as_float(y[c & 1][2 * j]), __uint_as_float(y[c & 1][2 * j + 1]));
+          mx[j & 1] = max3(mx[j & 1], __uint_as_float(y[2 * j]), __uint_as_float(y[2 * j + 1]));
+      };
+      uint32_t y0[16], y1[16];
+      tld16_issue(ts, y0);
+#pragma unroll 1
+      for (int c = 0; c < 8; c += 2) {
+        tld_wait();
+        after_wait(y0);
+        tld16_issue(ts + 16 * c + 16, y1);
+        part(y0, c);
+        tld_wait();
+        after_wait(y1);
+        if (c < 6) tld16_issue(ts + 16 * c + 32, y0);
+        part(y1, c + 1);
       }
-      return fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+      return fmaxf(mx[0], mx[1]);
     };
     auto tile_exp = [&](int lim, bool whole, float f, float at) {
       const uint64_t f2 = two(f, f), at2 = two(-at, -at);
-      uint32_t y[2][16];
-      tld16_issue(ts, y[0]);
-#pragma unroll
-      for (int c = 0; c < 8; ++c) {
-        tld_wait();
-        after_wait(y[c & 1]);
-        if (c < 7) tld16_issue(ts + 16 * (c + 1), y[(c + 1) & 1]);
-        if (!whole) {
-#pragma unroll
-          for (int j = 0; j < 16; ++j)
-            if (16 * c + j >= lim) y[c & 1][j] = 0xff800000u;
-        }
+      auto part = [&](uint32_t (&y)[16], int c) {
+        if (!whole) mask(y, lim - 16 * c);
         uint32_t hi[8], lo[8];
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
           float a, d;
-          untwo(fma2(two(y[c & 1][2 * j], y[c & 1][2 * j + 1]), f2, at2), a, d);
+          untwo(fma2(two(y[2 * j], y[2 * j + 1]), f2, at2), a, d);
           const uint64_t p = two(ex2(a), ex2(d));
           sum2[j & 1] = add2(sum2[j & 1], p);
           cut2(p, hi[j], lo[j]);
         }
         tst_pairs(ts + 16 * c, hi, lo);
+      };
+      uint32_t y0[16], y1[16];
+      tld16_issue(ts, y0);
+#pragma unroll 1
+      for (int c = 0; c < 8; c += 2) {
+        tld_wait();
+        after_wait(y0);
+        tld16_issue(ts + 16 * c + 16, y1);
+        part(y0, c);
+        tld_wait();
+        after_wait(y1);
+        if (c < 6) tld16_issue(ts + 16 * c + 32, y0);
+        part(y1, c + 1);
       }
     };
     bool ok = true;
@@ -298,10 +310,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int j = 0; j < DV / 2; ++j) acc[j] = mul2(acc[j], s2);
       }
       const float at = top == -INFINITY ? 0.f : ref;  // no key yet: all weights are 2^-inf
-      if (whole)
-        tile_exp(128, true, f, at);
-      else
-        tile_exp(lim, false, f, at);
+      tile_exp(lim, whole, f, at);
       tst_wait();
       fence_before();
       bar_arrive(p_full + m);
