@@ -129,6 +129,10 @@ __device__ __forceinline__ bool bar_wait(uint64_t *b, uint32_t parity, volatile 
     }
   }
 }
+// the same for a whole warp: one answer
+__device__ __forceinline__ bool mma_wait(uint64_t *b, uint32_t parity, volatile int *abort_flag, int *err, int site) {
+  return __all_sync(0xffffffffu, bar_wait(b, parity, abort_flag, err, site));
+}
 // whatever the abort flag says: copies and MMAs in flight end before their memory is released
 __device__ __forceinline__ void bar_drain(uint64_t *b, uint32_t parity) {
   const uint64_t t0 = gtime();
@@ -150,39 +154,59 @@ __device__ __forceinline__ void bulk_load(uint32_t dst, const void *src, uint32_
 }
 __device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
-__device__ __forceinline__ void mma_commit(uint64_t *b) {
-  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(su32(b))
-               : "memory");
-}
-// D[tmem] (+)= A B^T, A in shared memory
-__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+// The MMA warp runs its loop with all lanes, and these instructions under the
+// predicate of one: the descriptors then stay in uniform registers (issued from
+// a branch of one lane an instruction took 80 to 100 cycles, not the tensor
+// core's 64).
+__device__ __forceinline__ uint32_t elect_one() {
+  uint32_t one;
   asm volatile(
       "{\n\t.reg .pred p;\n\t"
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(one));
+  return one;
+}
+__device__ __forceinline__ void mma_commit(uint64_t *b, uint32_t one) {
+  asm volatile(
+      "{\n\t.reg .pred q;\n\t"
+      "setp.ne.b32 q, %1, 0;\n\t"
+      "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(su32(b)),
+      "r"(one)
+      : "memory");
+}
+// Shared-memory descriptors, 128-byte swizzle, 8-row groups 1024 bytes apart: the low word carries the
+// address and the distance of 64-column blocks, the high word is one constant.
+constexpr uint32_t kDescHigh = (1024u >> 4) | (1u << 14) | (2u << 29);
+// 16-deep slice k of a [rows x 64] fp16 tile read along its columns (K-major)
+__device__ __forceinline__ uint32_t kdesc(uint32_t tile, int k) { return ((tile + k * 32) >> 4) | (1u << 16); }
+// 16-deep slice k of [K rows x 64 columns] tiles read along their rows (MN-major);
+// `next` is the distance between the tiles of neighbouring 64-column blocks
+__device__ __forceinline__ uint32_t ndesc(uint32_t tile, int k, uint32_t next) {
+  return ((tile + k * 2048) >> 4) | ((next >> 4) << 16);
+}
+// D[tmem] (+)= A B^T, A in shared memory
+__device__ __forceinline__ void mma_ss(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t acc, uint32_t one) {
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t.reg .b64 da, db;\n\t"
       "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
-      "l"(a), "l"(b), "r"(idesc), "r"(acc)
+      "setp.ne.b32 q, %5, 0;\n\t"
+      "mov.b64 da, {%1, %6};\n\t"
+      "mov.b64 db, {%2, %6};\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %3, p;\n\t}" ::"r"(d),
+      "r"(a), "r"(b), "r"(idesc), "r"(acc), "r"(one), "r"(kDescHigh)
       : "memory");
 }
 // the same with A in TMEM (two fp16 a column)
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t acc, uint32_t one) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\t"
+      "{\n\t.reg .pred p, q;\n\t.reg .b64 db;\n\t"
       "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
-      "r"(a), "l"(b), "r"(idesc), "r"(acc)
+      "setp.ne.b32 q, %5, 0;\n\t"
+      "mov.b64 db, {%2, %6};\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], db, %3, p;\n\t}" ::"r"(d),
+      "r"(a), "r"(b), "r"(idesc), "r"(acc), "r"(one), "r"(kDescHigh)
       : "memory");
-}
-// shared-memory descriptor, 128-byte swizzle
-__device__ __forceinline__ uint64_t sdesc(uint32_t addr, uint32_t lbo, uint32_t sbo) {
-  return (uint64_t)((addr >> 4) & 0x3FFF) | (uint64_t)((lbo >> 4) & 0x3FFF) << 16 |
-         (uint64_t)((sbo >> 4) & 0x3FFF) << 32 | (uint64_t)1 << 46 | (uint64_t)2 << 61;
-}
-// 16-deep slice k of a [rows x 64] fp16 tile read along its columns (K-major)
-__device__ __forceinline__ uint64_t kdesc(uint32_t tile, int k) { return sdesc(tile + k * 32, 16, 1024); }
-// 16-deep slice k of [K rows x 64 columns] tiles read along their rows (MN-major);
-// `next` is the distance between the tiles of neighbouring 64-column blocks
-__device__ __forceinline__ uint64_t ndesc(uint32_t tile, int k, uint32_t next) {
-  return sdesc(tile + k * 2048, next, 1024);
 }
 // fp16 operands, fp32 accumulators, M = 128
 __device__ __forceinline__ constexpr uint32_t idesc(int n, bool b_mn) {

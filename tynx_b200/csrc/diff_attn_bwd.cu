@@ -27,7 +27,7 @@
 namespace tx_diff {
 namespace {
 
-constexpr int kThreads = 384, kStep = 64;
+constexpr int kThreads = 640, kStep = 64;  // producer, MMA, two spare warps, 16 elementwise warps
 enum { kModeK = 0, kModeQ = 1, kModeV = 2 };
 
 template <int DV>
@@ -48,8 +48,29 @@ struct Cfg {
 struct Grads {
   const float *stats;  // [b][h][ceil(T / 64)][4][64]
   float *dq, *dk, *dv;
-  unsigned k_blocks, q_blocks;
+  // blocks of one tile level: K, Q and V; in turn level by level, or kind after kind
+  unsigned nk, nq, levels, by_level, kt, qt;
 };
+// the block's kind and its index within it
+__device__ __forceinline__ int block_kind(const Grads &o, unsigned i, unsigned &block) {
+  if (o.by_level) {
+    const unsigned per = 2 * o.nk + o.nq;
+    unsigned level = i / per, at = i - level * per;
+    if (level >= o.levels) {  // the side with more tiles goes on alone
+      const unsigned rest = i - o.levels * per, each = o.kt > o.levels ? 2 * o.nk : o.nq;
+      level = o.levels + rest / each;
+      at = rest % each + (o.kt > o.levels ? 0 : o.nk);
+      if (o.kt > o.levels && at >= o.nk) at += o.nq;
+    }
+    const int kind = at < o.nk ? kModeK : at < o.nk + o.nq ? kModeQ : kModeV;
+    const unsigned before = kind == kModeK ? 0 : kind == kModeQ ? o.nk : o.nk + o.nq;
+    block = level * (kind == kModeQ ? o.nq : o.nk) + (at - before);
+    return kind;
+  }
+  const unsigned k = o.nk * o.kt, q = o.nq * o.qt;
+  block = i < k ? i : i < k + q ? i - k : i - k - q;
+  return i < k ? kModeK : i < k + q ? kModeQ : kModeV;
+}
 
 template <int DV, int MODE>
 __device__ __forceinline__ void body(const Shape &s, const Split &x, const CUtensorMap &mq, const CUtensorMap &mk,
@@ -68,7 +89,7 @@ __device__ __forceinline__ void body(const Shape &s, const Split &x, const CUten
   uint32_t *tmem_holder = reinterpret_cast<uint32_t *>(bars + 16);
   volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_holder + 1);
   uint32_t *vmax = tmem_holder + 2;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
 
   // keys: the first tiles are seen by most queries; queries: the last tiles see most keys
   const int heads = KEYS ? s.Hk : s.H;
@@ -88,7 +109,7 @@ __device__ __forceinline__ void body(const Shape &s, const Split &x, const CUten
     const int64_t last = r0 + 127 < s.T ? r0 + 127 : s.T - 1;
     per_head = (int)((s.seen(last, n) + kStep - 1) / kStep);
   }
-  const int steps = KEYS ? per_head * s.G : per_head;
+  const int steps = __shfl_sync(0xffffffffu, KEYS ? per_head * s.G : per_head, 0);
 
   if (threadIdx.x == 0) {
     bar_init(r_full, 1);
@@ -96,7 +117,7 @@ __device__ __forceinline__ void body(const Shape &s, const Split &x, const CUten
       bar_init(x_full + i, 1);
       bar_init(x_empty + i, 1);
       bar_init(s_full + i, 1);
-      bar_init(p_full + i, 256);
+      bar_init(p_full + i, 512);
     }
     bar_init(v_full, 1);
     bar_init(v_empty, 1);
@@ -127,7 +148,7 @@ __device__ __forceinline__ void body(const Shape &s, const Split &x, const CUten
   auto step_of = [&](int i) { return KEYS ? first + i % per_head : i; };
 
   if (warp < 4) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
     if (warp == 0 && lane == 0 && steps) {
       bar_expect(r_full, 2 * C::RQ + (MODE == kModeV ? 0 : C::RV));
       for (int p = 0; p < 8; ++p)  // (map, head or tail, 64-row half)
@@ -168,27 +189,28 @@ __device__ __forceinline__ void body(const Shape &s, const Split &x, const CUten
       bar_drain(r_full, 0);
       for (int i = lx - 1; i >= 0 && i > lx - 3; --i) bar_drain(x_full + (i & 1), (i >> 1) & 1);
       if (lv) bar_drain(v_full, (lv - 1) & 1);
-    } else if (warp == 1 && lane == 0 && steps) {
+    } else if (warp == 1 && steps) {
+      const uint32_t one = elect_one();
       constexpr uint32_t id_s = idesc(kStep, false), id_a = idesc(64, true), id_v = idesc(DV, true);
-      bool ok = bar_wait(r_full, 0, abort_flag, s.err, 13);
+      bool ok = mma_wait(r_full, 0, abort_flag, s.err, 13);
       auto scores = [&](int i) {  // S_1, S_2 and dP of step i
         const uint32_t ts = tmem + (i & 1) * 192;
         const int st = i & 1;
-        ok = ok && bar_wait(x_full + st, (i >> 1) & 1, abort_flag, s.err, 14);
+        ok = ok && mma_wait(x_full + st, (i >> 1) & 1, abort_flag, s.err, 14);
         if (!ok) return;
         fence_after();
         for (int m = 0; m < 2; ++m) {
           const uint32_t rh_ = srq + m * C::RQ, rl = rh_ + C::RQ / 2, xh = sxq + st * 2 * C::XQ + m * C::XQ, xl = xh + C::XBLK;
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
-            mma_ss(ts + m * 64, kdesc(rh_, k), kdesc(xl, k), id_s, k ? 1u : 0u);
-            mma_ss(ts + m * 64, kdesc(rl, k), kdesc(xh, k), id_s, 1u);
+            mma_ss(ts + m * 64, kdesc(rh_, k), kdesc(xl, k), id_s, k ? 1u : 0u, one);
+            mma_ss(ts + m * 64, kdesc(rl, k), kdesc(xh, k), id_s, 1u, one);
           }
 #pragma unroll
-          for (int k = 0; k < 4; ++k) mma_ss(ts + m * 64, kdesc(rh_, k), kdesc(xh, k), id_s, 1u);
+          for (int k = 0; k < 4; ++k) mma_ss(ts + m * 64, kdesc(rh_, k), kdesc(xh, k), id_s, 1u, one);
         }
         if (MODE != kModeV) {
-          ok = bar_wait(v_full, i & 1, abort_flag, s.err, 15);
+          ok = mma_wait(v_full, i & 1, abort_flag, s.err, 15);
           if (!ok) return;
           fence_after();
 #pragma unroll
@@ -197,62 +219,62 @@ __device__ __forceinline__ void body(const Shape &s, const Split &x, const CUten
                            xl = xh + (DV / 64) * C::XBLK;
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
-              mma_ss(ts + 128, kdesc(rh_, k), kdesc(xl, k), id_s, (c || k) ? 1u : 0u);
-              mma_ss(ts + 128, kdesc(rl, k), kdesc(xh, k), id_s, 1u);
+              mma_ss(ts + 128, kdesc(rh_, k), kdesc(xl, k), id_s, (c || k) ? 1u : 0u, one);
+              mma_ss(ts + 128, kdesc(rl, k), kdesc(xh, k), id_s, 1u, one);
             }
           }
 #pragma unroll
           for (int c = 0; c < DV / 64; ++c)
 #pragma unroll
             for (int k = 0; k < 4; ++k)
-              mma_ss(ts + 128, kdesc(srv + c * 16384, k), kdesc(sxv + c * C::XBLK, k), id_s, 1u);
-          mma_commit(v_empty);
+              mma_ss(ts + 128, kdesc(srv + c * 16384, k), kdesc(sxv + c * C::XBLK, k), id_s, 1u, one);
+          mma_commit(v_empty, one);
         }
-        mma_commit(s_full + st);
+        mma_commit(s_full + st, one);
       };
       scores(0);
       for (int i = 0; i < steps && ok; ++i) {
         if (i + 1 < steps) scores(i + 1);
         const uint32_t ts = tmem + (i & 1) * 192;
         const int st = i & 1;
-        ok = ok && bar_wait(p_full + st, (i >> 1) & 1, abort_flag, s.err, 16);
+        ok = ok && mma_wait(p_full + st, (i >> 1) & 1, abort_flag, s.err, 16);
         if (!ok) break;
         fence_after();
         if (MODE == kModeV) {
           const uint32_t xh = xv_at(i), xl = xh + (DV / 64) * C::XBLK, ta = tmem + ACC;
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
-            mma_ts(ta, ts + k * 16, ndesc(xl, k, C::XBLK), id_v, k ? 1u : 0u);
-            mma_ts(ta, ts + k * 16 + 8, ndesc(xh, k, C::XBLK), id_v, 1u);
+            mma_ts(ta, ts + k * 16, ndesc(xl, k, C::XBLK), id_v, k ? 1u : 0u, one);
+            mma_ts(ta, ts + k * 16 + 8, ndesc(xh, k, C::XBLK), id_v, 1u, one);
           }
 #pragma unroll
-          for (int k = 0; k < 4; ++k) mma_ts(ta, ts + k * 16, ndesc(xh, k, C::XBLK), id_v, 1u);
+          for (int k = 0; k < 4; ++k) mma_ts(ta, ts + k * 16, ndesc(xh, k, C::XBLK), id_v, 1u, one);
         } else {
           for (int m = 0; m < 2; ++m) {
             const uint32_t xh = sxq + st * 2 * C::XQ + m * C::XQ, xl = xh + C::XBLK, ta = tmem + ACC + m * 64;
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
-              mma_ts(ta, ts + m * 64 + k * 16, ndesc(xl, k, C::XBLK), id_a, k ? 1u : 0u);
-              mma_ts(ta, ts + m * 64 + k * 16 + 8, ndesc(xh, k, C::XBLK), id_a, 1u);
+              mma_ts(ta, ts + m * 64 + k * 16, ndesc(xl, k, C::XBLK), id_a, k ? 1u : 0u, one);
+              mma_ts(ta, ts + m * 64 + k * 16 + 8, ndesc(xh, k, C::XBLK), id_a, 1u, one);
             }
 #pragma unroll
-            for (int k = 0; k < 4; ++k) mma_ts(ta, ts + m * 64 + k * 16, ndesc(xh, k, C::XBLK), id_a, 1u);
+            for (int k = 0; k < 4; ++k) mma_ts(ta, ts + m * 64 + k * 16, ndesc(xh, k, C::XBLK), id_a, 1u, one);
           }
         }
-        mma_commit(x_empty + st);
-        mma_commit(a_full);
+        mma_commit(x_empty + st, one);
+        mma_commit(a_full, one);
       }
-      mma_commit(all_done);
+      mma_commit(all_done, one);
       bar_drain(all_done, 0);
     }
   } else {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
-    // warpgroup `half` takes streamed rows 32 half .. of every step, and of the
-    // results map `half`'s (K, Q) or its half of the columns (V)
-    const int half = (warp - 4) >> 2, quad = warp & 3, r = quad * 32 + lane;
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 104;");
+    // warpgroup `part` takes streamed rows 16 part .. of every step, and of the results half of map
+    // part / 2's columns (K, Q) or a quarter of the columns (V)
+    const int part = (warp - 4) >> 2, half = part >> 1, quad = warp & 3, r = quad * 32 + lane;
     const uint32_t lane_row = (uint32_t)(quad * 32) << 16;
     const int64_t row = r0 + r;
-    constexpr int AC = MODE == kModeV ? DV / 2 : 64;  // columns of the result a thread sums
+    constexpr int AC = MODE == kModeV ? DV / 4 : 32;  // columns of the result a thread sums
     uint64_t acc[AC / 2];
 #pragma unroll
     for (int j = 0; j < AC / 2; ++j) acc[j] = two(0.f, 0.f);
@@ -273,13 +295,13 @@ __device__ __forceinline__ void body(const Shape &s, const Split &x, const CUten
     auto add_products = [&]() {
       const uint64_t g2 = two(ga, ga);
 #pragma unroll
-      for (int c = 0; c < AC / 32; ++c) {
-        uint32_t y[32];
-        tld32_issue(tmem + lane_row + ACC + half * AC + 32 * c, y);
+      for (int c = 0; c < AC / 16; ++c) {
+        uint32_t y[16];
+        tld16_issue(tmem + lane_row + ACC + part * AC + 16 * c, y);
         tld_wait();
         after_wait(y);
 #pragma unroll
-        for (int j = 0; j < 16; ++j) acc[16 * c + j] = fma2(two(y[2 * j], y[2 * j + 1]), g2, acc[16 * c + j]);
+        for (int j = 0; j < 8; ++j) acc[8 * c + j] = fma2(two(y[2 * j], y[2 * j + 1]), g2, acc[8 * c + j]);
       }
     };
     for (int i = 0; i < steps; ++i) {
@@ -311,67 +333,66 @@ __device__ __forceinline__ void body(const Shape &s, const Split &x, const CUten
       if (KEYS) ok = ok && __all_sync(0xffffffffu, bar_wait(x_full + st, (i >> 1) & 1, abort_flag, s.err, 18));
       if (!ok) break;
       fence_after();
-      // columns of this half's 32 that are seen: [lo_c, hi_c); queries behind the last have lse = +inf
-      int lo_c = 0, hi_c = 32;
+      // columns of these 16 that are seen: [lo_c, hi_c); queries behind the last have lse = +inf
+      int lo_c = 0, hi_c = 16;
       if (KEYS) {
         if (s.causal) {
-          const int64_t from = row - s.start - x0 - 32 * half;  // the first query that sees this key
-          lo_c = from < 0 ? 0 : from > 32 ? 32 : (int)from;
+          const int64_t from = row - s.start - x0 - 16 * part;  // the first query that sees this key
+          lo_c = from < 0 ? 0 : from > 16 ? 16 : (int)from;
         }
         if (row >= n) hi_c = 0;
       } else {
-        const int64_t end = seen - x0 - 32 * half;
-        hi_c = end < 0 ? 0 : end > 32 ? 32 : (int)end;
+        const int64_t end = seen - x0 - 16 * part;
+        hi_c = end < 0 ? 0 : end > 16 ? 16 : (int)end;
       }
-      const bool whole = __all_sync(0xffffffffu, lo_c == 0 && hi_c == 32);
-      const uint32_t ts = tmem + lane_row + st * 192 + 32 * half;
-      const float *col = stat + st * (4 * kStep) + 32 * half;
-#pragma unroll 1  // rolled: the warps run it at different places, and unrolled they wait for instructions
-        for (int c = 0; c < 2; ++c) {
-          uint32_t y0[16], y1[16], yp[16];
-          tld16_issue(ts + 16 * c, y0);
-          tld16_issue(ts + 64 + 16 * c, y1);
-          if (MODE != kModeV) tld16_issue(ts + 128 + 16 * c, yp);
-          tld_wait();
-          after_wait(y0);
-          after_wait(y1);
-          if (MODE != kModeV) after_wait(yp);
-          uint32_t h0[8], l0[8], h1[8], l1[8];
+      const bool whole = __all_sync(0xffffffffu, lo_c == 0 && hi_c == 16);
+      const uint32_t ts = tmem + lane_row + st * 192 + 16 * part;
+      const float *col = stat + st * (4 * kStep) + 16 * part;
+      {
+        uint32_t y0[16], y1[16], yp[16];
+        tld16_issue(ts, y0);
+        tld16_issue(ts + 64, y1);
+        if (MODE != kModeV) tld16_issue(ts + 128, yp);
+        tld_wait();
+        after_wait(y0);
+        after_wait(y1);
+        if (MODE != kModeV) after_wait(yp);
+        uint32_t h0[8], l0[8], h1[8], l1[8];
 #pragma unroll
-          for (int j4 = 0; j4 < 4; ++j4) {  // four columns
-            float q[4][4];
-            if (KEYS) {
+        for (int j4 = 0; j4 < 4; ++j4) {  // four columns
+          float q[4][4];
+          if (KEYS) {
 #pragma unroll
-              for (int k = 0; k < (MODE == kModeV ? 2 : 4); ++k) {
-                const float4 v = *reinterpret_cast<const float4 *>(col + k * kStep + 16 * c + 4 * j4);
-                q[k][0] = v.x, q[k][1] = v.y, q[k][2] = v.z, q[k][3] = v.w;
-              }
-            }
-#pragma unroll
-            for (int u = 0; u < 2; ++u) {
-              const int j = 2 * j4 + u, e0 = 2 * j, e1 = e0 + 1;
-              auto st2 = [&](int k) { return KEYS ? two(q[k][2 * u], q[k][2 * u + 1]) : two(mine[k], mine[k]); };
-              float a, d, a1, d1;
-              untwo(sub2(mul2(two(y0[e0], y0[e1]), f02), st2(0)), a, d);
-              untwo(sub2(mul2(two(y1[e0], y1[e1]), f12), st2(1)), a1, d1);
-              a = ex2(a), d = ex2(d), a1 = ex2(a1), d1 = ex2(d1);
-              if (!whole) {
-                if (16 * c + e0 < lo_c || 16 * c + e0 >= hi_c) a = a1 = 0.f;
-                if (16 * c + e1 < lo_c || 16 * c + e1 >= hi_c) d = d1 = 0.f;
-              }
-              const uint64_t p0 = two(a, d), p1 = two(a1, d1);
-              if (MODE == kModeV) {
-                cut2(fma2(p1, lw2, mul2(p0, sw2)), h0[j], l0[j]);
-              } else {
-                const uint64_t dp = two(yp[e0], yp[e1]);
-                cut2(mul2(p0, fma2(dp, fp2, mul2(st2(2), nb2))), h0[j], l0[j]);
-                cut2(mul2(p1, fma2(dp, fp2, mul2(st2(3), nb2))), h1[j], l1[j]);
-              }
+            for (int k = 0; k < (MODE == kModeV ? 2 : 4); ++k) {
+              const float4 v = *reinterpret_cast<const float4 *>(col + k * kStep + 4 * j4);
+              q[k][0] = v.x, q[k][1] = v.y, q[k][2] = v.z, q[k][3] = v.w;
             }
           }
-          tst_pairs(ts + 16 * c, h0, l0);
-          if (MODE != kModeV) tst_pairs(ts + 64 + 16 * c, h1, l1);
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            const int j = 2 * j4 + u, e0 = 2 * j, e1 = e0 + 1;
+            auto st2 = [&](int k) { return KEYS ? two(q[k][2 * u], q[k][2 * u + 1]) : two(mine[k], mine[k]); };
+            float a, d, a1, d1;
+            untwo(sub2(mul2(two(y0[e0], y0[e1]), f02), st2(0)), a, d);
+            untwo(sub2(mul2(two(y1[e0], y1[e1]), f12), st2(1)), a1, d1);
+            a = ex2(a), d = ex2(d), a1 = ex2(a1), d1 = ex2(d1);
+            if (!whole) {
+              if (e0 < lo_c || e0 >= hi_c) a = a1 = 0.f;
+              if (e1 < lo_c || e1 >= hi_c) d = d1 = 0.f;
+            }
+            const uint64_t p0 = two(a, d), p1 = two(a1, d1);
+            if (MODE == kModeV) {
+              cut2(fma2(p1, lw2, mul2(p0, sw2)), h0[j], l0[j]);
+            } else {
+              const uint64_t dp = two(yp[e0], yp[e1]);
+              cut2(mul2(p0, fma2(dp, fp2, mul2(st2(2), nb2))), h0[j], l0[j]);
+              cut2(mul2(p1, fma2(dp, fp2, mul2(st2(3), nb2))), h1[j], l1[j]);
+            }
+          }
         }
+        tst_pairs(ts, h0, l0);
+        if (MODE != kModeV) tst_pairs(ts + 64, h1, l1);
+      }
       if (i) {  // ran under this step's scores
         ok = __all_sync(0xffffffffu, bar_wait(a_full, (i - 1) & 1, abort_flag, s.err, 19));
         if (!ok) break;
@@ -389,16 +410,16 @@ __device__ __forceinline__ void body(const Shape &s, const Split &x, const CUten
       if (ok) add_products();
     }
     // through shared memory, so that a warp stores whole rows
-    constexpr int W = 2 * AC, CH = W / 4;  // columns of the block's result: both maps, or V's
+    constexpr int W = 4 * AC, CH = W / 4;  // columns of the block's result: both maps, or V's
     float4 *stage = reinterpret_cast<float4 *>(sm);
 #pragma unroll
     for (int c = 0; c < AC / 4; ++c) {
       float4 v;
       untwo(acc[2 * c], v.x, v.y);
       untwo(acc[2 * c + 1], v.z, v.w);
-      stage[r * CH + ((half * (AC / 4) + c) ^ (r & 7))] = v;
+      stage[r * CH + ((part * (AC / 4) + c) ^ (r & 7))] = v;
     }
-    asm volatile("bar.sync 1, 256;" ::: "memory");
+    asm volatile("bar.sync 1, 512;" ::: "memory");
     const int64_t rows = KEYS ? s.S : s.T;
     if (ok) {
       const int w = MODE == kModeV ? s.dv : s.d;  // a result row: one of w, or two maps' of w
@@ -406,7 +427,7 @@ __device__ __forceinline__ void body(const Shape &s, const Split &x, const CUten
       const bool four = (w & 3) == 0 && ((uintptr_t)dst & 15) == 0;
       const int c = lane % CH, sub = lane / CH;
       const int m = MODE == kModeV ? 0 : c / 16, e = 4 * (MODE == kModeV ? c : c % 16);
-      for (int k = (warp - 4) * (32 / CH) + sub; k < 128; k += 8 * (32 / CH)) {
+      for (int k = (warp - 4) * (32 / CH) + sub; k < 128; k += 16 * (32 / CH)) {
         if (r0 + k >= rows) break;
         const float4 v = stage[k * CH + (c ^ (k & 7))];
         float *p = dst + ((b * rows + r0 + k) * heads + rh) * (MODE == kModeV ? w : 2 * w) + m * w + e;
@@ -439,12 +460,14 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (threadIdx.x == 0) atomicCAS(s.err, 0, DEVERR_LAYOUT);
     return;
   }
-  if (blockIdx.x < o.k_blocks)
-    body<DV, kModeK>(s, x, mq, mk, mv, mg, o, sm, blockIdx.x);
-  else if (blockIdx.x < o.k_blocks + o.q_blocks)
-    body<DV, kModeQ>(s, x, mq, mk, mv, mg, o, sm, blockIdx.x - o.k_blocks);
+  unsigned block;
+  const int kind = block_kind(o, blockIdx.x, block);
+  if (kind == kModeK)
+    body<DV, kModeK>(s, x, mq, mk, mv, mg, o, sm, block);
+  else if (kind == kModeQ)
+    body<DV, kModeQ>(s, x, mq, mk, mv, mg, o, sm, block);
   else
-    body<DV, kModeV>(s, x, mq, mk, mv, mg, o, sm, blockIdx.x - o.k_blocks - o.q_blocks);
+    body<DV, kModeV>(s, x, mq, mk, mv, mg, o, sm, block);
 }
 
 template <int DV>
@@ -453,10 +476,14 @@ int launch(tx_ctx *ctx, const Shape &s, const Split &x, const float *stats, floa
   if (!split_map(&mq, x.q, 64, s.T, s.B * 2 * s.H) || !split_map(&mk, x.k, 64, s.S, s.B * 2 * s.Hk) ||
       !split_map(&mv, x.v, DV, s.S, s.B * s.Hk) || !split_map(&mg, x.g, DV, s.T, s.B * s.H))
     return tx_fail(ctx, TX_ERR_UNSUPPORTED, "differential attention: tensor map");
-  const unsigned kb = dk ? (unsigned)(x.kt * s.B * s.Hk) : 0, qb = dq ? (unsigned)(x.qt * s.B * s.H) : 0;
-  const Grads o{stats, dq, dk, dv, kb, qb};
+  const unsigned nk = dk ? (unsigned)(s.B * s.Hk) : 0, nq = dq ? (unsigned)(s.B * s.H) : 0;
+  // Blocks start in order, so the longest come first.  Causal tiles get shorter from level to level:
+  // the kinds take turns, and the last blocks are the shortest of each.  Otherwise K and Q blocks are
+  // alike and V blocks half as long, so V comes last.
+  const unsigned kt = (unsigned)x.kt, qt = (unsigned)x.qt;
+  const Grads o{stats, dq, dk, dv, nk, nq, kt < qt ? kt : qt, (unsigned)(s.causal && nk && nq), kt, qt};
   TX_CUDA(ctx, cudaFuncSetAttribute(k_diff_bwd<DV>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<DV>::SMEM));
-  k_diff_bwd<DV><<<2 * kb + qb, kThreads, Cfg<DV>::SMEM, ctx->stream>>>(s, x, mq, mk, mv, mg, o);
+  k_diff_bwd<DV><<<2 * nk * kt + nq * qt, kThreads, Cfg<DV>::SMEM, ctx->stream>>>(s, x, mq, mk, mv, mg, o);
   TX_LAUNCHED(ctx, "k_diff_bwd");
   return TX_OK;
 }

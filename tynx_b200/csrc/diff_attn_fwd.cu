@@ -1,15 +1,16 @@
 // Differential attention forward on tcgen05.
 //
 // A CTA owns 128 queries of one head and streams its keys in tiles of 128,
-// both maps side by side: one warpgroup keeps map 1's rows, the other map 2's
-// (running maximum, sum and output, a row a thread), and both maps multiply the
-// same value tile.  Per tile and map
+// both maps side by side: eight warps keep map 1's rows (running maximum, sum
+// and output; two threads a row, half of the keys and of the output columns
+// each), eight map 2's, and both maps multiply the same value tile.  Per tile and map
 //   S = Q K^T               three fp16 products of 128 x 128 x 64   (768 cycles)
 //   P = 2^(S - maximum)     registers, split into fp16 pairs, back over S in TMEM
 //   O = P V                 three fp16 products of 128 x 128 x 128 (1536 cycles)
-// so while one map's warpgroup works on its softmax (128 exponentials a thread,
-// about 1400 issue slots a warp) the tensor core runs the other map's 2304
-// cycles: it is what bounds the kernel.  TMEM holds S1 | S2 | O1 | O2, all 512
+// so while one map's warps work on their softmax (about 450 instructions a
+// warp, two warps a scheduler; with one warp of all 128 columns the chain of
+// dependent instructions took 5400 cycles a tile) the tensor core runs the
+// other map's 2304 cycles: it is what bounds the kernel.  TMEM holds S1 | S2 | O1 | O2, all 512
 // columns; P lies over S (16 keys' heads and tails take the 16 columns of their
 // scores).  O is one tile's product and is added to the running output in
 // registers, rescaled there: the tensor core adds into its accumulator with
@@ -22,7 +23,7 @@
 namespace tx_diff {
 namespace {
 
-constexpr int kThreads = 384;  // producer, MMA, two spare warps, 2 x 4 softmax warps
+constexpr int kThreads = 640;  // producer, MMA, two spare warps, 2 x 8 softmax warps
 
 template <int DV>
 struct Cfg {
@@ -31,7 +32,8 @@ struct Cfg {
   static constexpr int VBLK = 64 * 64 * 2;            // [64 keys x 64] fp16
   static constexpr int VSLOT = 2 * (DV / 64) * VBLK;  // 64 keys: heads, tails
   static constexpr int RING = 3;
-  static constexpr int SMEM = 4 * QK + RING * VSLOT + 1024 /*barriers*/ + 1024 /*align*/;
+  static constexpr int SMEM = 4 * QK + RING * VSLOT + 512 /*barriers*/ + 2048 /*row exchange*/;
+  static_assert(SMEM <= 232448, "shared memory of an SM");
   // at the end both maps' outputs pass through Q's and K's memory
   static_assert(2 * 128 * DV * 4 <= 4 * QK, "output staging");
 };
@@ -63,15 +65,20 @@ __global__ void __launch_bounds__(kThreads, 1)
     k_diff_fwd(const __grid_constant__ Shape s, const __grid_constant__ Split x, const __grid_constant__ CUtensorMap mq,
                const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtensorMap mv, Out o) {
   using C = Cfg<DV>;
-  extern __shared__ uint8_t raw[];
-  uint8_t *sm = (uint8_t *)(((uintptr_t)raw + 1023) & ~(uintptr_t)1023);
+  extern __shared__ __align__(1024) uint8_t sm[];
+  if (su32(sm) & 1023) {  // the swizzled tiles need it
+    if (threadIdx.x == 0) atomicCAS(s.err, 0, DEVERR_LAYOUT);
+    return;
+  }
   const uint32_t sq = su32(sm), sk = sq + 2 * C::QK, sv = sk + 2 * C::QK;
   uint64_t *bars = reinterpret_cast<uint64_t *>(sm + 4 * C::QK + C::RING * C::VSLOT);
   uint64_t *q_full = bars, *k_full = bars + 1, *k_empty = bars + 3, *v_full = bars + 5, *v_empty = bars + 8,
-           *s_full = bars + 11, *p_full = bars + 13, *o_full = bars + 15;
-  uint32_t *tmem_holder = reinterpret_cast<uint32_t *>(bars + 16);
+           *s_full = bars + 11, *p_full = bars + 13, *o_full = bars + 15;  // o_full: of each map's tile
+  uint64_t *all_done = bars + 17;
+  uint32_t *tmem_holder = reinterpret_cast<uint32_t *>(bars + 18);
   volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_holder + 1);
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  float *swap = reinterpret_cast<float *>(bars + 64);  // [map][half][row]
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
 
   // causal: the queries with most keys first
   const int64_t heads = s.B * s.H;
@@ -82,7 +89,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int64_t t0 = qt * 128, tl = t0 + 127 < s.T ? t0 + 127 : s.T - 1;
   const int64_t n = s.length(b);
   const int tile0 = split * o.per, all = (int)((s.seen(tl, n) + 127) / 128);  // this range's tiles
-  const int tiles = all <= tile0 ? 0 : all - tile0 < o.per ? all - tile0 : o.per;
+  const int tiles = __shfl_sync(0xffffffffu, all <= tile0 ? 0 : all - tile0 < o.per ? all - tile0 : o.per, 0);
 
   if (threadIdx.x == 0) {
     bar_init(q_full, 1);
@@ -90,13 +97,14 @@ __global__ void __launch_bounds__(kThreads, 1)
       bar_init(k_full + m, 1);
       bar_init(k_empty + m, 1);
       bar_init(s_full + m, 1);
-      bar_init(p_full + m, 128);
+      bar_init(p_full + m, 256);
+      bar_init(o_full + m, 1);
     }
     for (int i = 0; i < C::RING; ++i) {
       bar_init(v_full + i, 1);
       bar_init(v_empty + i, 1);
     }
-    bar_init(o_full, 1);
+    bar_init(all_done, 1);
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     if (h == 0 && qt == 0 && split == 0) report_length(s, b);
@@ -112,7 +120,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   const uint32_t tmem = *tmem_holder;
 
   if (warp < 4) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
     if (warp == 0 && lane == 0 && tiles) {
       bar_expect(q_full, 2 * C::QK);
       for (int m = 0; m < 2; ++m)
@@ -150,17 +158,18 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       for (int u = loaded_v - 1; u >= 0 && u > loaded_v - 1 - C::RING; --u)
         bar_drain(v_full + u % C::RING, (u / C::RING) & 1);
-    } else if (warp == 1 && lane == 0 && tiles) {
+    } else if (warp == 1 && tiles) {
+      const uint32_t one = elect_one();
       constexpr uint32_t id_s = idesc(128, false), id_o = idesc(DV, true);
-      bool ok = bar_wait(q_full, 0, abort_flag, s.err, 3);
+      bool ok = mma_wait(q_full, 0, abort_flag, s.err, 3);
       for (int i = 0; i <= tiles && ok; ++i) {
         for (int m = 0; m < 2 && ok; ++m) {
           const uint32_t ts = tmem + m * 128, to = tmem + 256 + m * DV;
           if (i) {  // O = P V of the tile before
-            ok = bar_wait(p_full + m, (i - 1) & 1, abort_flag, s.err, 4);
+            ok = mma_wait(p_full + m, (i - 1) & 1, abort_flag, s.err, 4);
             for (int hf = 0; hf < 2 && ok; ++hf) {
               const int u = 2 * (i - 1) + hf, slot = u % C::RING;
-              ok = bar_wait(v_full + slot, (u / C::RING) & 1, abort_flag, s.err, 5);
+              ok = mma_wait(v_full + slot, (u / C::RING) & 1, abort_flag, s.err, 5);
               if (!ok) break;
               fence_after();
               const uint32_t vh = sv + slot * C::VSLOT, vl = vh + (DV / 64) * C::VBLK;
@@ -168,135 +177,112 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
               for (int k = 0; k < 4; ++k) {
                 const uint32_t ph = ts + (hf * 4 + k) * 16;
-                mma_ts(to, ph, ndesc(vl, k, C::VBLK), id_o, (hf || k) ? 1u : 0u);
-                mma_ts(to, ph + 8, ndesc(vh, k, C::VBLK), id_o, 1u);
+                mma_ts(to, ph, ndesc(vl, k, C::VBLK), id_o, (hf || k) ? 1u : 0u, one);
+                mma_ts(to, ph + 8, ndesc(vh, k, C::VBLK), id_o, 1u, one);
               }
 #pragma unroll
-              for (int k = 0; k < 4; ++k) mma_ts(to, ts + (hf * 4 + k) * 16, ndesc(vh, k, C::VBLK), id_o, 1u);
-              if (m) mma_commit(v_empty + slot);
+              for (int k = 0; k < 4; ++k) mma_ts(to, ts + (hf * 4 + k) * 16, ndesc(vh, k, C::VBLK), id_o, 1u, one);
+              if (m) mma_commit(v_empty + slot, one);
             }
+            mma_commit(o_full + m, one);
           }
           if (i < tiles && ok) {
-            ok = bar_wait(k_full + m, i & 1, abort_flag, s.err, 6);
+            ok = mma_wait(k_full + m, i & 1, abort_flag, s.err, 6);
             if (!ok) break;
             fence_after();
             const uint32_t qh = sq + m * C::QK, ql = qh + C::HALF, kh = sk + m * C::QK, kl = kh + C::HALF;
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
-              mma_ss(ts, kdesc(qh, k), kdesc(kl, k), id_s, k ? 1u : 0u);
-              mma_ss(ts, kdesc(ql, k), kdesc(kh, k), id_s, 1u);
+              mma_ss(ts, kdesc(qh, k), kdesc(kl, k), id_s, k ? 1u : 0u, one);
+              mma_ss(ts, kdesc(ql, k), kdesc(kh, k), id_s, 1u, one);
             }
 #pragma unroll
-            for (int k = 0; k < 4; ++k) mma_ss(ts, kdesc(qh, k), kdesc(kh, k), id_s, 1u);
-            mma_commit(k_empty + m);
-            mma_commit(s_full + m);  // and behind it the product O of the tile before
+            for (int k = 0; k < 4; ++k) mma_ss(ts, kdesc(qh, k), kdesc(kh, k), id_s, 1u, one);
+            mma_commit(k_empty + m, one);
+            mma_commit(s_full + m, one);
           }
         }
       }
-      mma_commit(o_full);  // all products of this CTA
-      bar_drain(o_full, 0);
+      mma_commit(all_done, one);  // all products of this CTA
+      bar_drain(all_done, 0);
     }
   } else {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
-    const int m = (warp - 4) >> 2, quad = warp & 3, r = quad * 32 + lane;
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 104;");
+    const int m = (warp - 4) >> 3, half = ((warp - 4) >> 2) & 1, quad = warp & 3, r = quad * 32 + lane;
+    constexpr int DH = DV / 2;  // output columns of this thread
     const uint32_t lane_row = (uint32_t)(quad * 32) << 16;
-    const uint32_t ts = tmem + m * 128 + lane_row, to = tmem + 256 + m * DV + lane_row;
+    const uint32_t ts = tmem + m * 128 + 64 * half + lane_row, to = tmem + 256 + m * DV + half * DH + lane_row;
     const int64_t t = t0 + r;
-    const int64_t seen = (t < s.T ? s.seen(t, n) : s.seen(tl, n)) - (int64_t)tile0 * 128;
+    const int64_t seen = (t < s.T ? s.seen(t, n) : s.seen(tl, n)) - (int64_t)tile0 * 128 - 64 * half;
     const float fq = __ldg(x.fq + (b * 2 * s.H + 2 * h + m) * x.qt + qt);
     const float *fk = x.fk + (b * 2 * s.Hk + 2 * hk + m) * x.kt + tile0, *fv = x.fv + (b * s.Hk + hk) * x.kt + tile0;
+    float *mine = swap + (2 * m + half) * 128 + r, *other = swap + (2 * m + (half ^ 1)) * 128 + r;
+    auto pair_sync = [&]() { asm volatile("bar.sync %0, 64;" ::"r"(1 + 4 * m + quad) : "memory"); };
     // P = 2^(S - ref): the reference is kCarry below the row's maximum when it is set, so that fp16
     // tails hold, and follows only when the maximum has outgrown it by kSlack more (fp16 ends at 2^16)
     constexpr float kCarry = 8.f, kSlack = 6.f;
+    constexpr uint32_t kGone = 0x7fc0dead;  // in a maximum's place: this warp gave up (no product has these bits)
     float ref = -INFINITY, top = -INFINITY;  // top: the maximum that ref was set by
     uint64_t sum2[2] = {two(0.f, 0.f), two(0.f, 0.f)};
-    uint64_t acc[DV / 2];
+    uint64_t acc[DH / 2];
 #pragma unroll
-    for (int j = 0; j < DV / 2; ++j) acc[j] = two(0.f, 0.f);
+    for (int j = 0; j < DH / 2; ++j) acc[j] = two(0.f, 0.f);
     auto add_tile = [&](float g) {  // acc += g O
       const uint64_t g2 = two(g, g);
-      uint32_t y[2][16];
-      tld16_issue(to, y[0]);
 #pragma unroll
-      for (int c = 0; c < DV / 16; ++c) {
+      for (int c = 0; c < DH / 16; ++c) {
+        uint32_t y[16];
+        tld16_issue(to + 16 * c, y);
         tld_wait();
-        after_wait(y[c & 1]);
-        if (c + 1 < DV / 16) tld16_issue(to + 16 * (c + 1), y[(c + 1) & 1]);
+        after_wait(y);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) acc[8 * c + j] = fma2(two(y[c & 1][2 * j], y[c & 1][2 * j + 1]), g2, acc[8 * c + j]);
+        for (int j = 0; j < 8; ++j) acc[8 * c + j] = fma2(two(y[2 * j], y[2 * j + 1]), g2, acc[8 * c + j]);
       }
     };
-    // The loops over a tile's columns stay rolled: two warps a scheduler run them at different places,
-    // and unrolled they wait for instructions more than for anything else.
+    // The loops over a tile's columns stay rolled: the warps of a scheduler run them at different
+    // places, and unrolled they wait for instructions more than for anything else.
     auto mask = [&](uint32_t (&y)[16], int left) {  // columns from `left` on are not seen
 #pragma unroll
       for (int j = 0; j < 16; ++j)
         if (j >= left) y[j] = 0xff800000u;  // -inf
     };
-    auto tile_max = [&](int lim, bool whole) {
-      float mx[2] = {-INFINITY, -INFINITY};
-      auto part = [&](uint32_t (&y)[16], int c) {
-        if (!whole) mask(y, lim - 16 * c);
-#pragma unroll
-        for (int j = 0; j < 8; ++j)
-          mx[j & 1] = max3(mx[j & 1], __uint_as_float(y[2 * j]), __uint_as_float(y[2 * j + 1]));
-      };
-      uint32_t y0[16], y1[16];
-      tld16_issue(ts, y0);
-#pragma unroll 1
-      for (int c = 0; c < 8; c += 2) {
-        tld_wait();
-        after_wait(y0);
-        tld16_issue(ts + 16 * c + 16, y1);
-        part(y0, c);
-        tld_wait();
-        after_wait(y1);
-        if (c < 6) tld16_issue(ts + 16 * c + 32, y0);
-        part(y1, c + 1);
-      }
-      return fmaxf(mx[0], mx[1]);
-    };
-    auto tile_exp = [&](int lim, bool whole, float f, float at) {
-      const uint64_t f2 = two(f, f), at2 = two(-at, -at);
-      auto part = [&](uint32_t (&y)[16], int c) {
-        if (!whole) mask(y, lim - 16 * c);
-        uint32_t hi[8], lo[8];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          float a, d;
-          untwo(fma2(two(y[2 * j], y[2 * j + 1]), f2, at2), a, d);
-          const uint64_t p = two(ex2(a), ex2(d));
-          sum2[j & 1] = add2(sum2[j & 1], p);
-          cut2(p, hi[j], lo[j]);
-        }
-        tst_pairs(ts + 16 * c, hi, lo);
-      };
-      uint32_t y0[16], y1[16];
-      tld16_issue(ts, y0);
-#pragma unroll 1
-      for (int c = 0; c < 8; c += 2) {
-        tld_wait();
-        after_wait(y0);
-        tld16_issue(ts + 16 * c + 16, y1);
-        part(y0, c);
-        tld_wait();
-        after_wait(y1);
-        if (c < 6) tld16_issue(ts + 16 * c + 32, y0);
-        part(y1, c + 1);
-      }
-    };
     bool ok = true;
     float gv = 0.f;
     for (int i = 0; i < tiles; ++i) {
       const float f = factor2(fq, __ldg(fk + i)), next_gv = __ldg(fv + i);
-      ok = __all_sync(0xffffffffu, bar_wait(s_full + m, i & 1, abort_flag, s.err, 7));
-      if (!ok) break;
-      fence_after();
+      if (i) {  // the last tile's product, while the tensor core works on this tile's scores
+        ok = __all_sync(0xffffffffu, bar_wait(o_full + m, (i - 1) & 1, abort_flag, s.err, 8));
+        fence_after();
+        if (ok) add_tile(gv);
+      }
+      ok = ok && __all_sync(0xffffffffu, bar_wait(s_full + m, i & 1, abort_flag, s.err, 7));
       const int64_t left = seen - (int64_t)i * 128;
-      const int lim = left < 0 ? 0 : left > 128 ? 128 : (int)left;
-      const bool whole = __all_sync(0xffffffffu, lim == 128);
-      const float mx = tile_max(lim, whole) * f;
-      if (i) add_tile(gv);
+      const int lim = left < 0 ? 0 : left > 64 ? 64 : (int)left;
+      const bool whole = __all_sync(0xffffffffu, lim == 64);
+      float mx = -INFINITY;
+      fence_after();
+      if (ok) {
+        float mx2[2] = {-INFINITY, -INFINITY};
+#pragma unroll 1
+        for (int c = 0; c < 4; ++c) {
+          uint32_t y[16];
+          tld16_issue(ts + 16 * c, y);
+          tld_wait();
+          after_wait(y);
+          if (!whole) mask(y, lim - 16 * c);
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            mx2[j & 1] = max3(mx2[j & 1], __uint_as_float(y[2 * j]), __uint_as_float(y[2 * j + 1]));
+        }
+        mx = fmaxf(mx2[0], mx2[1]) * f;
+      }
+      // a pair leaves the loop together, or one of them would wait for the other without a limit
+      *mine = ok ? mx : __uint_as_float(kGone);
+      pair_sync();
+      const float theirs = *other;
+      ok = ok && !__any_sync(0xffffffffu, __float_as_uint(theirs) == kGone);
+      if (!ok) break;
+      mx = fmaxf(mx, theirs);
       gv = next_gv;
       if (__any_sync(0xffffffffu, mx > top + kSlack || (top == -INFINITY && mx > top))) {
         const float now = fmaxf(top, mx);
@@ -307,43 +293,67 @@ __global__ void __launch_bounds__(kThreads, 1)
         sum2[0] = mul2(sum2[0], s2);
         sum2[1] = mul2(sum2[1], s2);
 #pragma unroll
-        for (int j = 0; j < DV / 2; ++j) acc[j] = mul2(acc[j], s2);
+        for (int j = 0; j < DH / 2; ++j) acc[j] = mul2(acc[j], s2);
       }
       const float at = top == -INFINITY ? 0.f : ref;  // no key yet: all weights are 2^-inf
-      tile_exp(lim, whole, f, at);
+      const uint64_t f2 = two(f, f), at2 = two(-at, -at);
+#pragma unroll 1
+      for (int c = 0; c < 4; ++c) {
+        uint32_t y[16], hi[8], lo[8];
+        tld16_issue(ts + 16 * c, y);
+        tld_wait();
+        after_wait(y);
+        if (!whole) mask(y, lim - 16 * c);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          float a, d;
+          untwo(fma2(two(y[2 * j], y[2 * j + 1]), f2, at2), a, d);
+          const uint64_t p = two(ex2(a), ex2(d));
+          sum2[j & 1] = add2(sum2[j & 1], p);
+          cut2(p, hi[j], lo[j]);
+        }
+        tst_pairs(ts + 16 * c, hi, lo);
+      }
       tst_wait();
       fence_before();
       bar_arrive(p_full + m);
     }
-    if (tiles) ok = __all_sync(0xffffffffu, ok && bar_wait(o_full, 0, abort_flag, s.err, 8));
+    if (tiles) ok = __all_sync(0xffffffffu, ok && bar_wait(o_full + m, (tiles - 1) & 1, abort_flag, s.err, 9));
     fence_after();
     if (tiles && ok) add_tile(gv);
+    // the staging below takes Q's and K's memory: no product reads it any more
+    if (tiles) ok = __all_sync(0xffffffffu, ok && bar_wait(all_done, 0, abort_flag, s.err, 10));
     float s0, s1, s2, s3;
     untwo(sum2[0], s0, s1);
     untwo(sum2[1], s2, s3);
-    const float sum = (s0 + s1) + (s2 + s3);
+    const float part = (s0 + s1) + (s2 + s3);
+    pair_sync();  // both have read the last maxima
+    *mine = part;
+    pair_sync();
+    const float sum = half ? *other + part : part + *other;
     const bool none = top == -INFINITY, live = t < s.T && ok;
     const bool parts = o.parts.splits > 1;
     const float inv = parts ? 1.f : none ? 0.f : 1.0f / sum;
     const int64_t n_items = s.T * s.G;
     const int64_t at0 = (b * s.Hk + hk) * n_items + (h - hk * s.G);  // + t * G
-    if (live && parts)
+    if (live && parts && half == 0)
       o.parts.ml[((at0 + t * s.G) * 2 + m) * o.parts.splits + split] = make_float2(none ? -INFINITY : ref, sum);
-    if (live && !parts && o.lse) o.lse[(b * 2 * s.H + 2 * h + m) * s.T + t] = none ? INFINITY : ref + log2f(sum);
+    if (live && !parts && o.lse && half == 0)
+      o.lse[(b * 2 * s.H + 2 * h + m) * s.T + t] = none ? INFINITY : ref + log2f(sum);
 #pragma unroll
-    for (int c = 0; c < DV / 4; ++c) {
+    for (int c = 0; c < DH / 4; ++c) {
       float4 v;
       untwo(acc[2 * c], v.x, v.y);
       untwo(acc[2 * c + 1], v.z, v.w);
-      *staged<DV>(sm, m, r, c) = make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv);
+      *staged<DV>(sm, m, r, half * (DH / 4) + c) = make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv);
     }
-    asm volatile("bar.sync 1, 256;" ::: "memory");
+    asm volatile("bar.sync 9, 512;" ::: "memory");
     // rows of the tile, whole lines at a time
     if (ok) {
       constexpr int LINES = 128 / DV;  // rows a warp stores at once
       const float lam = __ldg(s.lam + h);
       const int c = lane % (DV / 4), sub = lane / (DV / 4);
-      for (int k = (warp - 4) * LINES + sub; k < 128; k += 8 * LINES) {
+      for (int k = (warp - 4) * LINES + sub; k < 128; k += 16 * LINES) {
         const int64_t tt = t0 + k;
         if (tt >= s.T) break;
         float4 a = *staged<DV>(sm, 0, k, c), d = *staged<DV>(sm, 1, k, c);
