@@ -193,148 +193,237 @@ __global__ void __launch_bounds__(kSplitThreads, 2)
 }
 
 // ---- few query rows against many keys ----------------------------------------------------
-// A block takes RP queries (token, head of the group) of one key head, both maps, and a range
-// of keys, in tiles of 64: a thread works out a key's dots with all its map's rows, a warp the
-// running maximum and sum of a row, a thread one column of all the rows' outputs.
-constexpr int kTile = 64, kRowThreads = 128, kKeyLd = 132;
+// Bound by reading the keys and values once: about 1 us for each 6 MB.  A block takes RP
+// queries (token, head of the group) of one key head, both maps, and a range of keys; its warps
+// take four keys at a time in turn and meet only at the end.  A lane holds four of a key's 64
+// elements (half a warp a map) and four of a value's 128.  The 4 RP dot products of a map are
+// added over its 16 lanes by halving: each exchange passes on the half that the partner keeps, so
+// the sum costs about one shuffle a product and leaves one (key, query) score a lane, where its
+// exponential is taken.  The weights go through 32 RP bytes of shared memory back to all lanes.
+// The running maximum is followed only when it has grown by 2^16 (fp32 sums lose nothing below).
+constexpr int kRowWarps = 8, kRowThreads = 32 * kRowWarps, kGroup = 4;
 
 template <int RP>
-__global__ void __launch_bounds__(kRowThreads)
-    k_diff_rows(const __grid_constant__ Shape s, int splits, int64_t keys_per_split, float *part_o, float2 *part_ml) {
-  extern __shared__ float4 smem4[];
-  float *ks = reinterpret_cast<float *>(smem4);       // [64][132]: map 0, map 1
-  float *vs = ks + kTile * kKeyLd;                    // [64][128]
-  float *qs = vs + kTile * kMaxVdim;                  // [2 RP][64]
-  float *ps = qs + 2 * RP * kMaxDim;                  // [64][2 RP]
-  float *al = ps + kTile * 2 * RP;                    // [2 RP]
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+struct RowSmem {
+  float p[kRowWarps][kGroup][2 * RP];  // weights; then the factors of a new maximum
+  float2 ml[kRowWarps][2 * RP];
+  float acc[kRowWarps][2 * RP][kMaxVdim];
+};
+
+__device__ __forceinline__ float4 load4(const float *p, int have, bool four) {
+  float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (four) {
+    if (have > 0) v = __ldg(reinterpret_cast<const float4 *>(p));
+  } else {
+    if (have > 0) v.x = __ldg(p);
+    if (have > 1) v.y = __ldg(p + 1);
+    if (have > 2) v.z = __ldg(p + 2);
+    if (have > 3) v.w = __ldg(p + 3);
+  }
+  return v;
+}
+
+template <int RP>
+__global__ void __launch_bounds__(kRowThreads, 2)
+    k_diff_rows(const __grid_constant__ Shape s, const Parts parts, int64_t keys_per_split) {
+  extern __shared__ __align__(16) uint8_t raw[];
+  RowSmem<RP> &sh = *reinterpret_cast<RowSmem<RP> *>(raw);
+  constexpr int NV = kGroup * RP;                // scores of a map's group, v = query * 4 + key
+  constexpr int HELD = NV > 16 ? NV / 16 : 1;    // of them in a lane at the end
+  constexpr int COPY = NV < 16 ? 16 / NV : 1;    // lanes that hold the same one
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, m = lane >> 4, l16 = lane & 15;
   const int64_t b = blockIdx.y / s.Hk;
   const int hk = (int)(blockIdx.y - b * s.Hk);
   const int64_t n_items = s.T * s.G, item0 = (int64_t)blockIdx.z * RP;
   const int64_t n = s.length(b);
-  if (tid == 0 && hk == 0 && blockIdx.x == 0 && blockIdx.z == 0) report_length(s, b);
+  if (threadIdx.x == 0 && hk == 0 && blockIdx.x == 0 && blockIdx.z == 0) report_length(s, b);
   const int64_t last = item0 + RP <= n_items ? item0 + RP - 1 : n_items - 1;
   const int64_t k0 = (int64_t)blockIdx.x * keys_per_split;
   int64_t k1 = s.seen(last / s.G, n);
   if (k1 > k0 + keys_per_split) k1 = k0 + keys_per_split;
 
-  for (int i = tid; i < 2 * RP * kMaxDim; i += kRowThreads) {
-    const int c = i % kMaxDim, row = i / kMaxDim, m = row % 2;
-    const int64_t item = item0 + row / 2;
-    float x = 0.f;
-    if (item < n_items && c < s.d) {
-      const int64_t t = item / s.G;
-      const int h = hk * s.G + (int)(item - t * s.G);
-      x = s.q[((b * s.T + t) * (2 * s.H) + 2 * h + m) * s.d + c] * (s.scale * kLog2e);
-    }
-    qs[i] = x;
+  // this lane's elements of its map's queries, and the query whose scores it holds
+  float4 q[RP];
+  const int have_d = s.d - 4 * l16, have_v = s.dv - 4 * lane;
+#pragma unroll
+  for (int r = 0; r < RP; ++r) {
+    const int64_t item = item0 + r < n_items ? item0 + r : last;
+    const int64_t t = item / s.G;
+    const int h = hk * s.G + (int)(item - t * s.G);
+    q[r] = load4(s.q + ((b * s.T + t) * (2 * s.H) + 2 * h + m) * s.d + 4 * l16, have_d, false);
+    const float f = s.scale * kLog2e;
+    q[r] = make_float4(q[r].x * f, q[r].y * f, q[r].z * f, q[r].w * f);
   }
-  float acc[2 * RP], mx[(2 * RP + 3) / 4], sum[(2 * RP + 3) / 4];
-#pragma unroll
-  for (int r = 0; r < 2 * RP; ++r) acc[r] = 0.f;
-#pragma unroll
-  for (int i = 0; i < (2 * RP + 3) / 4; ++i) mx[i] = -INFINITY, sum[i] = 0.f;
+  const int mine = (NV > 16 ? l16 * HELD : l16 / COPY) / kGroup;  // query
+  const int64_t my_item = item0 + mine < n_items ? item0 + mine : last;
+  const int64_t seen = s.seen(my_item / s.G, n);
+  const bool four_d = (s.d & 3) == 0 && ((uintptr_t)s.k & 15) == 0, four_v = (s.dv & 3) == 0 && ((uintptr_t)s.v & 15) == 0;
 
-  for (int64_t j0 = k0; j0 < k1; j0 += kTile) {
-    __syncthreads();
-    for (int i = tid; i < kTile * 2 * kMaxDim; i += kRowThreads) {
-      const int c = i % kMaxDim, m = (i / kMaxDim) % 2, j = i / (2 * kMaxDim);
-      ks[j * kKeyLd + m * kMaxDim + c] =
-          (j0 + j < k1 && c < s.d) ? s.k[((b * s.S + j0 + j) * (2 * s.Hk) + 2 * hk + m) * s.d + c] : 0.f;
-    }
-    for (int i = tid; i < kTile * kMaxVdim; i += kRowThreads) {
-      const int c = i % kMaxVdim, j = i / kMaxVdim;
-      vs[i] = (j0 + j < k1 && c < s.dv) ? s.v[((b * s.S + j0 + j) * s.Hk + hk) * s.dv + c] : 0.f;
-    }
-    __syncthreads();
-    {
-      const int j = tid & 63, m = tid >> 6;
-      float dot[RP];
+  float4 acc[2 * RP];
 #pragma unroll
-      for (int r = 0; r < RP; ++r) dot[r] = 0.f;
-      for (int c = 0; c < kMaxDim; c += 4) {
-        const float4 kk = *reinterpret_cast<const float4 *>(ks + j * kKeyLd + m * kMaxDim + c);
+  for (int r = 0; r < 2 * RP; ++r) acc[r] = make_float4(0.f, 0.f, 0.f, 0.f);
+  float ref = -INFINITY, sum = 0.f;
+  const int64_t k_stride = (int64_t)2 * s.Hk * s.d, v_stride = (int64_t)s.Hk * s.dv;
+  const float *kp = s.k + (b * s.S) * k_stride + (2 * hk + m) * s.d + 4 * l16;
+  const float *vp = s.v + (b * s.S) * v_stride + hk * s.dv + 4 * lane;
+  float4 kk[kGroup], vv[kGroup];
+  auto fetch = [&](const float *p, int64_t stride, int64_t j0, int have, bool four, float4 (&x)[kGroup]) {
 #pragma unroll
-        for (int r = 0; r < RP; ++r) {
-          const float4 qq = *reinterpret_cast<const float4 *>(qs + (2 * r + m) * kMaxDim + c);
-          dot[r] += kk.x * qq.x + kk.y * qq.y + kk.z * qq.z + kk.w * qq.w;
-        }
-      }
+    for (int g = 0; g < kGroup; ++g) x[g] = load4(p + (j0 + g) * stride, j0 + g < k1 ? have : 0, four);
+  };
+  int64_t j0 = k0 + kGroup * warp;
+  if (j0 < k1) fetch(kp, k_stride, j0, have_d, four_d, kk);
+  for (; j0 < k1; j0 += kGroup * kRowWarps) {  // uniform in a warp
+    fetch(vp, v_stride, j0, have_v, four_v, vv);
+    float v[NV];
 #pragma unroll
-      for (int r = 0; r < RP; ++r) {
-        const int64_t item = item0 + r;
-        const bool ok = item < n_items && j0 + j < k1 && j0 + j < s.seen(item / s.G, n);
-        ps[j * 2 * RP + 2 * r + m] = ok ? dot[r] : -INFINITY;
-      }
-    }
-    __syncthreads();
+    for (int r = 0; r < RP; ++r)
 #pragma unroll
-    for (int i = 0; i < (2 * RP + 3) / 4; ++i) {
-      const int r = i * 4 + warp;
-      if (r < 2 * RP) {
-        const float a = ps[lane * 2 * RP + r], c = ps[(lane + 32) * 2 * RP + r];
-        const float m = fmaxf(mx[i], warp_max(fmaxf(a, c)));
-        const float at = m == -INFINITY ? 0.f : m;  // no key yet: all weights are exp2(-inf) = 0
-        const float pa = exp2f(a - at), pc = exp2f(c - at), f = exp2f(mx[i] - at);
-        ps[lane * 2 * RP + r] = pa;
-        ps[(lane + 32) * 2 * RP + r] = pc;
-        sum[i] = sum[i] * f + warp_sum(pa + pc);
-        mx[i] = m;
-        if (lane == 0) al[r] = f;
+      for (int g = 0; g < kGroup; ++g)
+        v[r * kGroup + g] = kk[g].x * q[r].x + kk[g].y * q[r].y + kk[g].z * q[r].z + kk[g].w * q[r].w;
+    if (j0 + kGroup * kRowWarps < k1) fetch(kp, k_stride, j0 + kGroup * kRowWarps, have_d, four_d, kk);
+    int left = NV;
+#pragma unroll
+    for (int o = 8; o; o >>= 1) {
+      if (left > 1) {  // pass on the half that the partner keeps
+        const bool up = l16 & o;
+        left >>= 1;
+#pragma unroll
+        for (int i = 0; i < NV / 2; ++i)
+          if (i < left) {
+            const float keep = up ? v[i + left] : v[i], give = up ? v[i] : v[i + left];
+            v[i] = keep + __shfl_xor_sync(0xffffffffu, give, o);
+          }
+      } else {
+        v[0] += __shfl_xor_sync(0xffffffffu, v[0], o);
       }
     }
-    __syncthreads();
+    // v[0 .. HELD): scores of query `mine`, key(s) of this lane
+    const int key0 = NV > 16 ? (l16 * HELD) % kGroup : (l16 / COPY) % kGroup;
+    float top = -INFINITY;
 #pragma unroll
-    for (int r = 0; r < 2 * RP; ++r) acc[r] *= al[r];
-    for (int j = 0; j < kTile; ++j) {
-      const float x = vs[j * kMaxVdim + tid];
-#pragma unroll
-      for (int r = 0; r < 2 * RP; ++r) acc[r] += ps[j * 2 * RP + r] * x;
+    for (int i = 0; i < HELD; ++i) {
+      if (j0 + key0 + i >= k1 || j0 + key0 + i >= seen) v[i] = -INFINITY;
+      top = fmaxf(top, v[i]);
     }
+#pragma unroll
+    for (int o = COPY; o < COPY * kGroup / HELD; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    if (__any_sync(0xffffffffu, top > ref + 16.f || (ref == -INFINITY && top > ref))) {
+      const float now = fmaxf(ref, top), f = ref == -INFINITY ? 0.f : ex2(ref - now);
+      sum *= f;
+      ref = now;
+      if (l16 % (16 / RP) == 0) sh.p[warp][0][m * RP + mine] = f;
+      __syncwarp();
+#pragma unroll
+      for (int r = 0; r < 2 * RP; ++r) {
+        const float g = sh.p[warp][0][r];
+        acc[r] = make_float4(acc[r].x * g, acc[r].y * g, acc[r].z * g, acc[r].w * g);
+      }
+      __syncwarp();
+    }
+    const float at = ref == -INFINITY ? 0.f : ref;  // no key yet: all weights are 2^-inf
+#pragma unroll
+    for (int i = 0; i < HELD; ++i) {
+      const float p = ex2(v[i] - at);
+      sum += p;
+      if (l16 % COPY == 0) sh.p[warp][key0 + i][m * RP + mine] = p;
+    }
+    __syncwarp();
+#pragma unroll
+    for (int g = 0; g < kGroup; ++g) {
+      float p[2 * RP];
+      if (RP >= 2) {
+#pragma unroll
+        for (int r = 0; r < 2 * RP; r += 4)
+          *reinterpret_cast<float4 *>(p + r) = *reinterpret_cast<const float4 *>(&sh.p[warp][g][r]);
+      } else {
+        p[0] = sh.p[warp][g][0], p[1] = sh.p[warp][g][1];
+      }
+#pragma unroll
+      for (int r = 0; r < 2 * RP; ++r)
+        acc[r] = make_float4(acc[r].x + p[r] * vv[g].x, acc[r].y + p[r] * vv[g].y, acc[r].z + p[r] * vv[g].z,
+                             acc[r].w + p[r] * vv[g].w);
+    }
+    __syncwarp();
   }
-  // partial rows: [b][hk][item][map] x [split]
 #pragma unroll
-  for (int i = 0; i < (2 * RP + 3) / 4; ++i) {
-    const int r = i * 4 + warp;
-    const int64_t item = item0 + r / 2;
-    if (r < 2 * RP && lane == 0 && item < n_items)
-      part_ml[(((b * s.Hk + hk) * n_items + item) * 2 + (r & 1)) * splits + blockIdx.x] = make_float2(mx[i], sum[i]);
-  }
+  for (int o = COPY; o < COPY * kGroup / HELD; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  if (l16 % (16 / RP) == 0) sh.ml[warp][m * RP + mine] = make_float2(ref, sum);
 #pragma unroll
-  for (int r = 0; r < 2 * RP; ++r) {
-    const int64_t item = item0 + r / 2;
-    if (item < n_items && tid < s.dv)
-      part_o[((((b * s.Hk + hk) * n_items + item) * 2 + (r & 1)) * splits + blockIdx.x) * s.dv + tid] = acc[r];
+  for (int r = 0; r < 2 * RP; ++r) *reinterpret_cast<float4 *>(&sh.acc[warp][r][4 * lane]) = acc[r];
+  __syncthreads();
+  // the warps' shares, in their order
+  for (int i = threadIdx.x; i < 2 * RP * kMaxVdim; i += kRowThreads) {
+    const int row = i / kMaxVdim, c = i % kMaxVdim, mm = row / RP;
+    const int64_t item = item0 + row % RP;
+    if (item >= n_items) continue;
+    float top = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < kRowWarps; ++w) top = fmaxf(top, sh.ml[w][row].x);
+    const float at = top == -INFINITY ? 0.f : top;
+    float x = 0.f, l = 0.f;
+#pragma unroll
+    for (int w = 0; w < kRowWarps; ++w) {
+      const float2 ml = sh.ml[w][row];
+      const float f = ex2(ml.x - at);
+      l += ml.y * f;
+      x += sh.acc[w][row][c] * f;
+    }
+    const int64_t to = (((b * s.Hk + hk) * n_items + item) * 2 + mm) * parts.splits + blockIdx.x;
+    if (c == 0) parts.ml[to] = make_float2(top, l);
+    if (c < s.dv) parts.o[to * s.dv + c] = x;
   }
 }
 
-// out, out2 and lse from the splits' partial rows: a block per query and head.
+// out, out2 and lse from the ranges' partial rows: a block per query and head, a warp per quarter of
+// the ranges.
+constexpr int kJoinMost = 512;  // ranges at most
 __global__ void __launch_bounds__(kMaxVdim)
-    k_diff_join(const __grid_constant__ Shape s, int splits, const float *part_o, const float2 *part_ml, float *out,
-                float *out2, float *lse) {
+    k_diff_join(const __grid_constant__ Shape s, const Parts parts, float *out, float *out2, float *lse) {
+  __shared__ float w[2][kJoinMost];
+  __shared__ float tops[2][4], sums[2][4];
   const int64_t n_items = s.T * s.G;
   const int64_t at = blockIdx.x;  // (b, hk, item)
   const int64_t item = at % n_items, bh = at / n_items;
   const int64_t b = bh / s.Hk, t = item / s.G;
   const int hk = (int)(bh - b * s.Hk), h = hk * s.G + (int)(item - t * s.G);
-  const int c = threadIdx.x;
+  const int c = threadIdx.x, warp = c >> 5, splits = parts.splits;
+  float top[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+  for (int m = 0; m < 2; ++m) {
+    for (int i = c; i < splits; i += kMaxVdim) top[m] = fmaxf(top[m], __ldg(&parts.ml[(at * 2 + m) * splits + i].x));
+    top[m] = warp_max(top[m]);
+    if ((c & 31) == 0) tops[m][warp] = top[m];
+  }
+  __syncthreads();
+  float part[2] = {0.f, 0.f};
+#pragma unroll
+  for (int m = 0; m < 2; ++m) {
+    top[m] = fmaxf(fmaxf(tops[m][0], tops[m][1]), fmaxf(tops[m][2], tops[m][3]));
+    const float ref = top[m] == -INFINITY ? 0.f : top[m];
+    for (int i = c; i < splits; i += kMaxVdim) {
+      const float2 ml = __ldg(&parts.ml[(at * 2 + m) * splits + i]);
+      const float f = ex2(ml.x - ref);
+      w[m][i] = f;
+      part[m] += ml.y * f;
+    }
+    part[m] = warp_sum(part[m]);
+    if ((c & 31) == 0) sums[m][warp] = part[m];
+  }
+  __syncthreads();
   float o[2];
 #pragma unroll
   for (int m = 0; m < 2; ++m) {
-    const float2 *ml = part_ml + (at * 2 + m) * splits;
-    float top = -INFINITY;
-    for (int i = 0; i < splits; ++i) top = fmaxf(top, ml[i].x);
-    const float ref = top == -INFINITY ? 0.f : top;
-    float sum = 0.f, x = 0.f;
-    for (int i = 0; i < splits; ++i) {
-      const float2 p = ml[i];
-      const float w = exp2f(p.x - ref);
-      sum += p.y * w;
-      if (c < s.dv && w != 0.f) x += part_o[((at * 2 + m) * splits + i) * s.dv + c] * w;
+    const float sum = (sums[m][0] + sums[m][1]) + (sums[m][2] + sums[m][3]);
+    const bool none = top[m] == -INFINITY;
+    float x = 0.f;
+    if (c < s.dv && !none) {
+      const float *p = parts.o + (at * 2 + m) * splits * s.dv + c;
+#pragma unroll 8
+      for (int i = 0; i < splits; ++i) x += __ldg(p + (int64_t)i * s.dv) * w[m][i];
     }
-    const bool none = top == -INFINITY;
     o[m] = none ? 0.f : x / sum;
-    if (lse && c == 0) lse[(b * 2 * s.H + 2 * h + m) * s.T + t] = none ? INFINITY : ref + log2f(sum);
+    if (lse && c == 0) lse[(b * 2 * s.H + 2 * h + m) * s.T + t] = none ? INFINITY : top[m] + log2f(sum);
   }
   if (c < s.dv) {
     const int64_t i = ((b * s.T + t) * s.H + h) * s.dv + c;
@@ -442,31 +531,40 @@ int check_desc(tx_ctx *ctx, const tx_diff_attention *p, Shape &s) {
 }
 
 int join(tx_ctx *ctx, const Shape &s, const Parts &parts, float *out, float *out2, float *lse) {
-  k_diff_join<<<(unsigned)(s.B * s.T * s.H), kMaxVdim, 0, ctx->stream>>>(s, parts.splits, parts.o, parts.ml, out, out2,
-                                                                       lse);
+  k_diff_join<<<(unsigned)(s.B * s.T * s.H), kMaxVdim, 0, ctx->stream>>>(s, parts, out, out2, lse);
   TX_LAUNCHED(ctx, "k_diff_join");
   return TX_OK;
 }
 
+// Partial results' memory.
+struct PartMemory {
+  Scratch o, ml;
+  Parts parts;
+  PartMemory(tx_ctx *ctx, const Shape &s, int splits)
+      : o(ctx, (size_t)(s.B * s.H * s.T * 2 * splits * s.dv) * 4), ml(ctx, (size_t)(s.B * s.H * s.T * 2 * splits) * 8) {
+    parts = Parts{o.as<float>(), ml.as<float2>(), splits};
+  }
+  bool ok() const { return o.ptr && ml.ptr; }
+};
+
 template <int RP>
 int launch_rows(tx_ctx *ctx, const Shape &s, float *out, float *out2, float *lse) {
-  const int64_t items = s.T * s.G, chunks = (items + RP - 1) / RP;
-  if (chunks > 65535) return tx_fail(ctx, TX_ERR_SHAPE, "differential attention: too many queries");
-  const int64_t blocks = chunks * s.B * s.Hk;
-  int64_t splits = (2 * ctx->num_sms + blocks - 1) / blocks, tiles = (s.S + kTile - 1) / kTile;
-  if (splits > tiles) splits = tiles;
+  const int64_t chunks = (s.T * s.G + RP - 1) / RP, blocks = chunks * s.B * s.Hk;
+  // two blocks an SM, each with four rounds of its warps at least
+  constexpr int64_t round = kGroup * kRowWarps;
+  int64_t splits = 2 * ctx->num_sms / blocks, most = (s.S + 4 * round - 1) / (4 * round);
+  if (splits > most) splits = most;
+  if (splits > kJoinMost) splits = kJoinMost;
   if (splits < 1) splits = 1;
-  int64_t per = ((tiles + splits - 1) / splits) * kTile;
-  if (per < kTile) per = kTile;
-  const int64_t rows = s.B * s.Hk * items * 2;
-  Scratch po(ctx, (size_t)(rows * splits * s.dv) * 4), pm(ctx, (size_t)(rows * splits) * 8);
-  if (!po.ptr || !pm.ptr) return TX_ERR_OOM;
-  const int smem = (kTile * kKeyLd + kTile * kMaxVdim + 2 * RP * kMaxDim + kTile * 2 * RP + 2 * RP) * 4;
+  const int64_t per = ((s.S + splits - 1) / splits + round - 1) / round * round;
+  PartMemory mem(ctx, s, (int)splits);
+  if (!mem.ok()) return TX_ERR_OOM;
+  const int smem = (int)sizeof(RowSmem<RP>);
   TX_CUDA(ctx, cudaFuncSetAttribute(k_diff_rows<RP>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
   k_diff_rows<RP><<<dim3((unsigned)splits, (unsigned)(s.B * s.Hk), (unsigned)chunks), kRowThreads, smem, ctx->stream>>>(
-      s, (int)splits, per, po.as<float>(), pm.as<float2>());
+      s, mem.parts, per);
   TX_LAUNCHED(ctx, "k_diff_rows");
-  return join(ctx, s, Parts{po.as<float>(), pm.as<float2>(), (int)splits}, out, out2, lse);
+  return join(ctx, s, mem.parts, out, out2, lse);
 }
 
 }  // namespace
@@ -503,20 +601,25 @@ extern "C" int tx_diff_attention_fwd(tx_ctx *ctx, const tx_diff_attention *p) {
   if (!p->q || !p->lam || !p->out || (s.S && (!p->k || !p->v)))
     return tx_fail(ctx, TX_ERR_INVALID, "differential attention: null buffer");
   DeviceScope device(ctx);
+  if (s.S == 0) {
+    const size_t rows = (size_t)(s.B * s.T * s.H);
+    TX_CUDA(ctx, cudaMemsetAsync(p->out, 0, rows * s.dv * 4, ctx->stream));
+    if (!p->out2) return TX_OK;
+    TX_CUDA(ctx, cudaMemsetAsync(p->out2, 0, rows * s.dv * 4, ctx->stream));
+    return tx_fill_f32(ctx, p->lse, (int64_t)(2 * rows), INFINITY);
+  }
   if (s.T * s.G <= 1) return launch_rows<1>(ctx, s, p->out, p->out2, p->lse);
   if (s.T * s.G <= 2) return launch_rows<2>(ctx, s, p->out, p->out2, p->lse);
   if (s.T * s.G <= 4) return launch_rows<4>(ctx, s, p->out, p->out2, p->lse);
-  if (s.T * s.G <= 8 || s.S == 0) return launch_rows<8>(ctx, s, p->out, p->out2, p->lse);
+  if (s.T * s.G <= 8) return launch_rows<8>(ctx, s, p->out, p->out2, p->lse);
   Operands x(ctx, s, false);
   TX_TRY(x.fill(ctx, s, nullptr, nullptr, nullptr));
   const int splits = tc_forward_splits(ctx, s);
   if (splits == 1) return tc_forward(ctx, s, x.x, p->out, p->out2, p->lse, Parts{nullptr, nullptr, 1});
-  const int64_t rows = s.B * s.H * s.T * 2;
-  Scratch po(ctx, (size_t)(rows * splits * s.dv) * 4), pm(ctx, (size_t)(rows * splits) * 8);
-  if (!po.ptr || !pm.ptr) return TX_ERR_OOM;
-  const Parts parts{po.as<float>(), pm.as<float2>(), splits};
-  TX_TRY(tc_forward(ctx, s, x.x, p->out, p->out2, p->lse, parts));
-  return join(ctx, s, parts, p->out, p->out2, p->lse);
+  PartMemory mem(ctx, s, splits);
+  if (!mem.ok()) return TX_ERR_OOM;
+  TX_TRY(tc_forward(ctx, s, x.x, p->out, p->out2, p->lse, mem.parts));
+  return join(ctx, s, mem.parts, p->out, p->out2, p->lse);
 }
 
 extern "C" int tx_diff_attention_bwd(tx_ctx *ctx, const tx_diff_attention *p) {
