@@ -199,31 +199,37 @@ __global__ void __launch_bounds__(kSplitThreads, 2)
 // elements (half a warp a map) and four of a value's 128.  The 4 RP dot products of a map are
 // added over its 16 lanes by halving: each exchange passes on the half that the partner keeps, so
 // the sum costs about one shuffle a product and leaves one (key, query) score a lane, where its
-// exponential is taken.  The weights go through 32 RP bytes of shared memory back to all lanes.
+// exponential is taken.  The weights go through shared memory back to all lanes.
 // The running maximum is followed only when it has grown by 2^16 (fp32 sums lose nothing below).
 constexpr int kRowWarps = 8, kRowThreads = 32 * kRowWarps, kGroup = 4;
 
 template <int RP>
 struct RowSmem {
-  float p[kRowWarps][kGroup][2 * RP];  // weights; then the factors of a new maximum
+  float2 p[kRowWarps][kGroup][2 * RP];  // weights, each twice (a pair's factor); then factors of a new maximum
   float2 ml[kRowWarps][2 * RP];
   float acc[kRowWarps][2 * RP][kMaxVdim];
 };
 
-__device__ __forceinline__ float4 load4(const float *p, int have, bool four) {
-  float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-  if (four) {
-    if (have > 0) v = __ldg(reinterpret_cast<const float4 *>(p));
+// four elements of which `have` exist, as two pairs; VEC: all or none, 16-byte aligned
+template <bool VEC>
+__device__ __forceinline__ void load4(const float *p, int have, uint64_t (&x)[2]) {
+  x[0] = x[1] = two(0.f, 0.f);
+  if (VEC) {
+    if (have > 0) {
+      const ulonglong2 v = __ldg(reinterpret_cast<const ulonglong2 *>(p));
+      x[0] = v.x, x[1] = v.y;
+    }
   } else {
-    if (have > 0) v.x = __ldg(p);
-    if (have > 1) v.y = __ldg(p + 1);
-    if (have > 2) v.z = __ldg(p + 2);
-    if (have > 3) v.w = __ldg(p + 3);
+    float v[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (have > i) v[i] = __ldg(p + i);
+    x[0] = two(v[0], v[1]), x[1] = two(v[2], v[3]);
   }
-  return v;
 }
 
-template <int RP>
+// VEC: key and value rows can be read four elements at a time
+template <int RP, bool VEC>
 __global__ void __launch_bounds__(kRowThreads, 2)
     k_diff_rows(const __grid_constant__ Shape s, const Parts parts, int64_t keys_per_split) {
   extern __shared__ __align__(16) uint8_t raw[];
@@ -239,49 +245,55 @@ __global__ void __launch_bounds__(kRowThreads, 2)
   if (threadIdx.x == 0 && hk == 0 && blockIdx.x == 0 && blockIdx.z == 0) report_length(s, b);
   const int64_t last = item0 + RP <= n_items ? item0 + RP - 1 : n_items - 1;
   const int64_t k0 = (int64_t)blockIdx.x * keys_per_split;
-  int64_t k1 = s.seen(last / s.G, n);
-  if (k1 > k0 + keys_per_split) k1 = k0 + keys_per_split;
+  const int64_t end = s.seen(last / s.G, n) - k0;
+  const int keys = end < 0 ? 0 : end > keys_per_split ? (int)keys_per_split : (int)end;  // of this block
 
   // this lane's elements of its map's queries, and the query whose scores it holds
-  float4 q[RP];
+  uint64_t q[RP][2];
   const int have_d = s.d - 4 * l16, have_v = s.dv - 4 * lane;
 #pragma unroll
   for (int r = 0; r < RP; ++r) {
     const int64_t item = item0 + r < n_items ? item0 + r : last;
     const int64_t t = item / s.G;
     const int h = hk * s.G + (int)(item - t * s.G);
-    q[r] = load4(s.q + ((b * s.T + t) * (2 * s.H) + 2 * h + m) * s.d + 4 * l16, have_d, false);
+    load4<false>(s.q + ((b * s.T + t) * (2 * s.H) + 2 * h + m) * s.d + 4 * l16, have_d, q[r]);
     const float f = s.scale * kLog2e;
-    q[r] = make_float4(q[r].x * f, q[r].y * f, q[r].z * f, q[r].w * f);
+    q[r][0] = mul2(q[r][0], two(f, f)), q[r][1] = mul2(q[r][1], two(f, f));
   }
   const int mine = (NV > 16 ? l16 * HELD : l16 / COPY) / kGroup;  // query
+  const int key0 = NV > 16 ? (l16 * HELD) % kGroup : (l16 / COPY) % kGroup;
   const int64_t my_item = item0 + mine < n_items ? item0 + mine : last;
-  const int64_t seen = s.seen(my_item / s.G, n);
-  const bool four_d = (s.d & 3) == 0 && ((uintptr_t)s.k & 15) == 0, four_v = (s.dv & 3) == 0 && ((uintptr_t)s.v & 15) == 0;
+  const int64_t my_end = s.seen(my_item / s.G, n) - k0;
+  const int seen = my_end < 0 ? 0 : my_end > keys ? keys : (int)my_end;
 
-  float4 acc[2 * RP];
+  uint64_t acc[2 * RP][2];
 #pragma unroll
-  for (int r = 0; r < 2 * RP; ++r) acc[r] = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int r = 0; r < 2 * RP; ++r) acc[r][0] = acc[r][1] = two(0.f, 0.f);
   float ref = -INFINITY, sum = 0.f;
   const int64_t k_stride = (int64_t)2 * s.Hk * s.d, v_stride = (int64_t)s.Hk * s.dv;
-  const float *kp = s.k + (b * s.S) * k_stride + (2 * hk + m) * s.d + 4 * l16;
-  const float *vp = s.v + (b * s.S) * v_stride + hk * s.dv + 4 * lane;
-  float4 kk[kGroup], vv[kGroup];
-  auto fetch = [&](const float *p, int64_t stride, int64_t j0, int have, bool four, float4 (&x)[kGroup]) {
+  int j0 = kGroup * warp;
+  const float *kp = s.k + (b * s.S + k0 + j0) * k_stride + (2 * hk + m) * s.d + 4 * l16;
+  const float *vp = s.v + (b * s.S + k0 + j0) * v_stride + hk * s.dv + 4 * lane;
+  uint64_t kk[kGroup][2], vv[kGroup][2];
 #pragma unroll
-    for (int g = 0; g < kGroup; ++g) x[g] = load4(p + (j0 + g) * stride, j0 + g < k1 ? have : 0, four);
-  };
-  int64_t j0 = k0 + kGroup * warp;
-  if (j0 < k1) fetch(kp, k_stride, j0, have_d, four_d, kk);
-  for (; j0 < k1; j0 += kGroup * kRowWarps) {  // uniform in a warp
-    fetch(vp, v_stride, j0, have_v, four_v, vv);
+  for (int g = 0; g < kGroup; ++g) load4<VEC>(kp + g * k_stride, j0 + g < keys ? have_d : 0, kk[g]);
+  for (; j0 < keys; j0 += kGroup * kRowWarps) {  // uniform in a warp
+#pragma unroll
+    for (int g = 0; g < kGroup; ++g) load4<VEC>(vp + g * v_stride, j0 + g < keys ? have_v : 0, vv[g]);
+    vp += kGroup * kRowWarps * v_stride;
     float v[NV];
 #pragma unroll
     for (int r = 0; r < RP; ++r)
 #pragma unroll
-      for (int g = 0; g < kGroup; ++g)
-        v[r * kGroup + g] = kk[g].x * q[r].x + kk[g].y * q[r].y + kk[g].z * q[r].z + kk[g].w * q[r].w;
-    if (j0 + kGroup * kRowWarps < k1) fetch(kp, k_stride, j0 + kGroup * kRowWarps, have_d, four_d, kk);
+      for (int g = 0; g < kGroup; ++g) {
+        float x, y;
+        untwo(fma2(kk[g][0], q[r][0], mul2(kk[g][1], q[r][1])), x, y);
+        v[r * kGroup + g] = x + y;
+      }
+    kp += kGroup * kRowWarps * k_stride;
+#pragma unroll
+    for (int g = 0; g < kGroup; ++g)
+      load4<VEC>(kp + g * k_stride, j0 + kGroup * kRowWarps + g < keys ? have_d : 0, kk[g]);
     int left = NV;
 #pragma unroll
     for (int o = 8; o; o >>= 1) {
@@ -298,12 +310,11 @@ __global__ void __launch_bounds__(kRowThreads, 2)
         v[0] += __shfl_xor_sync(0xffffffffu, v[0], o);
       }
     }
-    // v[0 .. HELD): scores of query `mine`, key(s) of this lane
-    const int key0 = NV > 16 ? (l16 * HELD) % kGroup : (l16 / COPY) % kGroup;
+    // v[0 .. HELD): scores of query `mine`, key(s) key0 ..
     float top = -INFINITY;
 #pragma unroll
     for (int i = 0; i < HELD; ++i) {
-      if (j0 + key0 + i >= k1 || j0 + key0 + i >= seen) v[i] = -INFINITY;
+      if (j0 + key0 + i >= seen) v[i] = -INFINITY;
       top = fmaxf(top, v[i]);
     }
 #pragma unroll
@@ -312,12 +323,12 @@ __global__ void __launch_bounds__(kRowThreads, 2)
       const float now = fmaxf(ref, top), f = ref == -INFINITY ? 0.f : ex2(ref - now);
       sum *= f;
       ref = now;
-      if (l16 % (16 / RP) == 0) sh.p[warp][0][m * RP + mine] = f;
+      if (l16 % (16 / RP) == 0) sh.p[warp][0][m * RP + mine] = make_float2(f, f);
       __syncwarp();
 #pragma unroll
       for (int r = 0; r < 2 * RP; ++r) {
-        const float g = sh.p[warp][0][r];
-        acc[r] = make_float4(acc[r].x * g, acc[r].y * g, acc[r].z * g, acc[r].w * g);
+        const uint64_t g = *reinterpret_cast<const uint64_t *>(&sh.p[warp][0][r]);
+        acc[r][0] = mul2(acc[r][0], g), acc[r][1] = mul2(acc[r][1], g);
       }
       __syncwarp();
     }
@@ -326,31 +337,25 @@ __global__ void __launch_bounds__(kRowThreads, 2)
     for (int i = 0; i < HELD; ++i) {
       const float p = ex2(v[i] - at);
       sum += p;
-      if (l16 % COPY == 0) sh.p[warp][key0 + i][m * RP + mine] = p;
+      if (l16 % COPY == 0) sh.p[warp][key0 + i][m * RP + mine] = make_float2(p, p);
     }
     __syncwarp();
 #pragma unroll
-    for (int g = 0; g < kGroup; ++g) {
-      float p[2 * RP];
-      if (RP >= 2) {
+    for (int g = 0; g < kGroup; ++g)
 #pragma unroll
-        for (int r = 0; r < 2 * RP; r += 4)
-          *reinterpret_cast<float4 *>(p + r) = *reinterpret_cast<const float4 *>(&sh.p[warp][g][r]);
-      } else {
-        p[0] = sh.p[warp][g][0], p[1] = sh.p[warp][g][1];
+      for (int r = 0; r < 2 * RP; r += 2) {
+        const ulonglong2 p = *reinterpret_cast<const ulonglong2 *>(&sh.p[warp][g][r]);
+        acc[r][0] = fma2(vv[g][0], p.x, acc[r][0]), acc[r][1] = fma2(vv[g][1], p.x, acc[r][1]);
+        acc[r + 1][0] = fma2(vv[g][0], p.y, acc[r + 1][0]), acc[r + 1][1] = fma2(vv[g][1], p.y, acc[r + 1][1]);
       }
-#pragma unroll
-      for (int r = 0; r < 2 * RP; ++r)
-        acc[r] = make_float4(acc[r].x + p[r] * vv[g].x, acc[r].y + p[r] * vv[g].y, acc[r].z + p[r] * vv[g].z,
-                             acc[r].w + p[r] * vv[g].w);
-    }
     __syncwarp();
   }
 #pragma unroll
   for (int o = COPY; o < COPY * kGroup / HELD; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
   if (l16 % (16 / RP) == 0) sh.ml[warp][m * RP + mine] = make_float2(ref, sum);
 #pragma unroll
-  for (int r = 0; r < 2 * RP; ++r) *reinterpret_cast<float4 *>(&sh.acc[warp][r][4 * lane]) = acc[r];
+  for (int r = 0; r < 2 * RP; ++r)
+    *reinterpret_cast<ulonglong2 *>(&sh.acc[warp][r][4 * lane]) = make_ulonglong2(acc[r][0], acc[r][1]);
   __syncthreads();
   // the warps' shares, in their order
   for (int i = threadIdx.x; i < 2 * RP * kMaxVdim; i += kRowThreads) {
@@ -375,61 +380,60 @@ __global__ void __launch_bounds__(kRowThreads, 2)
   }
 }
 
-// out, out2 and lse from the ranges' partial rows: a block per query and head, a warp per quarter of
-// the ranges.
+// out, out2 and lse from the ranges' partial rows: a block per query and head, 128 threads a map and a
+// column each.  Latency alone: the ranges' references are read once, the columns' loads do not depend
+// on one another.
 constexpr int kJoinMost = 512;  // ranges at most
-__global__ void __launch_bounds__(kMaxVdim)
+__global__ void __launch_bounds__(2 * kMaxVdim)
     k_diff_join(const __grid_constant__ Shape s, const Parts parts, float *out, float *out2, float *lse) {
   __shared__ float w[2][kJoinMost];
-  __shared__ float tops[2][4], sums[2][4];
+  __shared__ float tops[8], sums[8], second[kMaxVdim];
   const int64_t n_items = s.T * s.G;
   const int64_t at = blockIdx.x;  // (b, hk, item)
   const int64_t item = at % n_items, bh = at / n_items;
   const int64_t b = bh / s.Hk, t = item / s.G;
   const int hk = (int)(bh - b * s.Hk), h = hk * s.G + (int)(item - t * s.G);
-  const int c = threadIdx.x, warp = c >> 5, splits = parts.splits;
-  float top[2] = {-INFINITY, -INFINITY};
+  const int m = threadIdx.x >> 7, c = threadIdx.x & 127, warp = threadIdx.x >> 5, splits = parts.splits;
+  const float2 *ml = parts.ml + (at * 2 + m) * splits;
+  float2 mine[kJoinMost / kMaxVdim];
+  float top = -INFINITY;
 #pragma unroll
-  for (int m = 0; m < 2; ++m) {
-    for (int i = c; i < splits; i += kMaxVdim) top[m] = fmaxf(top[m], __ldg(&parts.ml[(at * 2 + m) * splits + i].x));
-    top[m] = warp_max(top[m]);
-    if ((c & 31) == 0) tops[m][warp] = top[m];
+  for (int i = 0; i < kJoinMost / kMaxVdim; ++i) {
+    mine[i] = c + i * kMaxVdim < splits ? __ldg(ml + c + i * kMaxVdim) : make_float2(-INFINITY, 0.f);
+    top = fmaxf(top, mine[i].x);
+  }
+  top = warp_max(top);
+  if ((threadIdx.x & 31) == 0) tops[warp] = top;
+  __syncthreads();
+  top = fmaxf(fmaxf(tops[4 * m], tops[4 * m + 1]), fmaxf(tops[4 * m + 2], tops[4 * m + 3]));
+  const bool none = top == -INFINITY;
+  const float ref = none ? 0.f : top;
+  float sum = 0.f;
+#pragma unroll
+  for (int i = 0; i < kJoinMost / kMaxVdim; ++i) {
+    const float f = ex2(mine[i].x - ref);
+    if (c + i * kMaxVdim < splits) w[m][c + i * kMaxVdim] = f;
+    sum += mine[i].y * f;
+  }
+  sum = warp_sum(sum);
+  if ((threadIdx.x & 31) == 0) sums[warp] = sum;
+  __syncthreads();
+  sum = (sums[4 * m] + sums[4 * m + 1]) + (sums[4 * m + 2] + sums[4 * m + 3]);
+  float x = 0.f;
+  if (c < s.dv && !none) {
+    const float *p = parts.o + (at * 2 + m) * splits * s.dv + c;
+#pragma unroll 16
+    for (int i = 0; i < splits; ++i) x += __ldg(p + (int64_t)i * s.dv) * w[m][i];
+    x /= sum;
+  }
+  if (lse && c == 0) lse[(b * 2 * s.H + 2 * h + m) * s.T + t] = none ? INFINITY : top + log2f(sum);
+  const int64_t i = ((b * s.T + t) * s.H + h) * s.dv + c;
+  if (m) {
+    second[c] = x;
+    if (out2 && c < s.dv) out2[i] = x;
   }
   __syncthreads();
-  float part[2] = {0.f, 0.f};
-#pragma unroll
-  for (int m = 0; m < 2; ++m) {
-    top[m] = fmaxf(fmaxf(tops[m][0], tops[m][1]), fmaxf(tops[m][2], tops[m][3]));
-    const float ref = top[m] == -INFINITY ? 0.f : top[m];
-    for (int i = c; i < splits; i += kMaxVdim) {
-      const float2 ml = __ldg(&parts.ml[(at * 2 + m) * splits + i]);
-      const float f = ex2(ml.x - ref);
-      w[m][i] = f;
-      part[m] += ml.y * f;
-    }
-    part[m] = warp_sum(part[m]);
-    if ((c & 31) == 0) sums[m][warp] = part[m];
-  }
-  __syncthreads();
-  float o[2];
-#pragma unroll
-  for (int m = 0; m < 2; ++m) {
-    const float sum = (sums[m][0] + sums[m][1]) + (sums[m][2] + sums[m][3]);
-    const bool none = top[m] == -INFINITY;
-    float x = 0.f;
-    if (c < s.dv && !none) {
-      const float *p = parts.o + (at * 2 + m) * splits * s.dv + c;
-#pragma unroll 8
-      for (int i = 0; i < splits; ++i) x += __ldg(p + (int64_t)i * s.dv) * w[m][i];
-    }
-    o[m] = none ? 0.f : x / sum;
-    if (lse && c == 0) lse[(b * 2 * s.H + 2 * h + m) * s.T + t] = none ? INFINITY : top[m] + log2f(sum);
-  }
-  if (c < s.dv) {
-    const int64_t i = ((b * s.T + t) * s.H + h) * s.dv + c;
-    out[i] = o[0] - __ldg(s.lam + h) * o[1];
-    if (out2) out2[i] = o[1];
-  }
+  if (!m && c < s.dv) out[i] = x - __ldg(s.lam + h) * second[c];
 }
 
 // dlam = -sum of D2, from the tiles' sums
@@ -531,7 +535,7 @@ int check_desc(tx_ctx *ctx, const tx_diff_attention *p, Shape &s) {
 }
 
 int join(tx_ctx *ctx, const Shape &s, const Parts &parts, float *out, float *out2, float *lse) {
-  k_diff_join<<<(unsigned)(s.B * s.T * s.H), kMaxVdim, 0, ctx->stream>>>(s, parts, out, out2, lse);
+  k_diff_join<<<(unsigned)(s.B * s.T * s.H), 2 * kMaxVdim, 0, ctx->stream>>>(s, parts, out, out2, lse);
   TX_LAUNCHED(ctx, "k_diff_join");
   return TX_OK;
 }
@@ -560,8 +564,10 @@ int launch_rows(tx_ctx *ctx, const Shape &s, float *out, float *out2, float *lse
   PartMemory mem(ctx, s, (int)splits);
   if (!mem.ok()) return TX_ERR_OOM;
   const int smem = (int)sizeof(RowSmem<RP>);
-  TX_CUDA(ctx, cudaFuncSetAttribute(k_diff_rows<RP>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-  k_diff_rows<RP><<<dim3((unsigned)splits, (unsigned)(s.B * s.Hk), (unsigned)chunks), kRowThreads, smem, ctx->stream>>>(
+  const bool vec = (s.d & 3) == 0 && (s.dv & 3) == 0 && ((uintptr_t)s.k & 15) == 0 && ((uintptr_t)s.v & 15) == 0;
+  auto kernel = vec ? k_diff_rows<RP, true> : k_diff_rows<RP, false>;
+  TX_CUDA(ctx, cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+  kernel<<<dim3((unsigned)splits, (unsigned)(s.B * s.Hk), (unsigned)chunks), kRowThreads, smem, ctx->stream>>>(
       s, mem.parts, per);
   TX_LAUNCHED(ctx, "k_diff_rows");
   return join(ctx, s, mem.parts, out, out2, lse);
