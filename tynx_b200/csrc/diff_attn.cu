@@ -201,11 +201,14 @@ __global__ void __launch_bounds__(kSplitThreads, 2)
 // the sum costs about one shuffle a product and leaves one (key, query) score a lane, where its
 // exponential is taken.  The weights go through shared memory back to all lanes.
 // The running maximum is followed only when it has grown by 2^16 (fp32 sums lose nothing below).
-constexpr int kRowWarps = 8, kRowThreads = 32 * kRowWarps, kGroup = 4;
+constexpr int kRowWarps = 8, kRowThreads = 32 * kRowWarps;
+// keys of a group: a lane holds 4 RP products before they are added, 2 RP for eight queries
+template <int RP>
+constexpr int kGroupOf = RP == 8 ? 2 : 4;
 
 template <int RP>
 struct RowSmem {
-  float2 p[kRowWarps][kGroup][2 * RP];  // weights, each twice (a pair's factor); then factors of a new maximum
+  float2 p[kRowWarps][kGroupOf<RP>][2 * RP];  // weights, each twice (a pair's factor); then factors of a new maximum
   float2 ml[kRowWarps][2 * RP];
   float acc[kRowWarps][2 * RP][kMaxVdim];
 };
@@ -234,16 +237,16 @@ __global__ void __launch_bounds__(kRowThreads, 2)
     k_diff_rows(const __grid_constant__ Shape s, const Parts parts, int64_t keys_per_split) {
   extern __shared__ __align__(16) uint8_t raw[];
   RowSmem<RP> &sh = *reinterpret_cast<RowSmem<RP> *>(raw);
-  constexpr int NV = kGroup * RP;                // scores of a map's group, v = query * 4 + key
-  constexpr int HELD = NV > 16 ? NV / 16 : 1;    // of them in a lane at the end
-  constexpr int COPY = NV < 16 ? 16 / NV : 1;    // lanes that hold the same one
+  constexpr int kGroup = kGroupOf<RP>;
+  constexpr int NV = kGroup * RP;                // scores of a map's group, v = query * kGroup + key
+  static_assert(NV <= 16, "one score a lane at the end");
+  constexpr int COPY = 16 / NV;                  // lanes that hold the same one
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, m = lane >> 4, l16 = lane & 15;
-  const int64_t b = blockIdx.y / s.Hk;
-  const int hk = (int)(blockIdx.y - b * s.Hk);
-  const int64_t n_items = s.T * s.G, item0 = (int64_t)blockIdx.z * RP;
+  const int b = blockIdx.y / s.Hk, hk = blockIdx.y - b * s.Hk;
+  const int n_items = (int)(s.T * s.G), item0 = blockIdx.z * RP;  // at most eight: launch_rows
   const int64_t n = s.length(b);
   if (threadIdx.x == 0 && hk == 0 && blockIdx.x == 0 && blockIdx.z == 0) report_length(s, b);
-  const int64_t last = item0 + RP <= n_items ? item0 + RP - 1 : n_items - 1;
+  const int last = item0 + RP <= n_items ? item0 + RP - 1 : n_items - 1;
   const int64_t k0 = (int64_t)blockIdx.x * keys_per_split;
   const int64_t end = s.seen(last / s.G, n) - k0;
   const int keys = end < 0 ? 0 : end > keys_per_split ? (int)keys_per_split : (int)end;  // of this block
@@ -253,16 +256,13 @@ __global__ void __launch_bounds__(kRowThreads, 2)
   const int have_d = s.d - 4 * l16, have_v = s.dv - 4 * lane;
 #pragma unroll
   for (int r = 0; r < RP; ++r) {
-    const int64_t item = item0 + r < n_items ? item0 + r : last;
-    const int64_t t = item / s.G;
-    const int h = hk * s.G + (int)(item - t * s.G);
+    const int item = item0 + r < n_items ? item0 + r : last, t = item / s.G, h = hk * s.G + item - t * s.G;
     load4<false>(s.q + ((b * s.T + t) * (2 * s.H) + 2 * h + m) * s.d + 4 * l16, have_d, q[r]);
     const float f = s.scale * kLog2e;
     q[r][0] = mul2(q[r][0], two(f, f)), q[r][1] = mul2(q[r][1], two(f, f));
   }
-  const int mine = (NV > 16 ? l16 * HELD : l16 / COPY) / kGroup;  // query
-  const int key0 = NV > 16 ? (l16 * HELD) % kGroup : (l16 / COPY) % kGroup;
-  const int64_t my_item = item0 + mine < n_items ? item0 + mine : last;
+  const int mine = l16 / COPY / kGroup, key = l16 / COPY % kGroup;
+  const int my_item = item0 + mine < n_items ? item0 + mine : last;
   const int64_t my_end = s.seen(my_item / s.G, n) - k0;
   const int seen = my_end < 0 ? 0 : my_end > keys ? keys : (int)my_end;
 
@@ -310,15 +310,11 @@ __global__ void __launch_bounds__(kRowThreads, 2)
         v[0] += __shfl_xor_sync(0xffffffffu, v[0], o);
       }
     }
-    // v[0 .. HELD): scores of query `mine`, key(s) key0 ..
-    float top = -INFINITY;
+    // v[0]: the score of query `mine` and key `key`
+    if (j0 + key >= seen) v[0] = -INFINITY;
+    float top = v[0];
 #pragma unroll
-    for (int i = 0; i < HELD; ++i) {
-      if (j0 + key0 + i >= seen) v[i] = -INFINITY;
-      top = fmaxf(top, v[i]);
-    }
-#pragma unroll
-    for (int o = COPY; o < COPY * kGroup / HELD; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    for (int o = COPY; o < COPY * kGroup; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
     if (__any_sync(0xffffffffu, top > ref + 16.f || (ref == -INFINITY && top > ref))) {
       const float now = fmaxf(ref, top), f = ref == -INFINITY ? 0.f : ex2(ref - now);
       sum *= f;
@@ -333,12 +329,9 @@ __global__ void __launch_bounds__(kRowThreads, 2)
       __syncwarp();
     }
     const float at = ref == -INFINITY ? 0.f : ref;  // no key yet: all weights are 2^-inf
-#pragma unroll
-    for (int i = 0; i < HELD; ++i) {
-      const float p = ex2(v[i] - at);
-      sum += p;
-      if (l16 % COPY == 0) sh.p[warp][key0 + i][m * RP + mine] = make_float2(p, p);
-    }
+    const float w = ex2(v[0] - at);
+    sum += w;
+    if (l16 % COPY == 0) sh.p[warp][key][m * RP + mine] = make_float2(w, w);
     __syncwarp();
 #pragma unroll
     for (int g = 0; g < kGroup; ++g)
@@ -351,7 +344,7 @@ __global__ void __launch_bounds__(kRowThreads, 2)
     __syncwarp();
   }
 #pragma unroll
-  for (int o = COPY; o < COPY * kGroup / HELD; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  for (int o = COPY; o < COPY * kGroup; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
   if (l16 % (16 / RP) == 0) sh.ml[warp][m * RP + mine] = make_float2(ref, sum);
 #pragma unroll
   for (int r = 0; r < 2 * RP; ++r)
@@ -360,7 +353,7 @@ __global__ void __launch_bounds__(kRowThreads, 2)
   // the warps' shares, in their order
   for (int i = threadIdx.x; i < 2 * RP * kMaxVdim; i += kRowThreads) {
     const int row = i / kMaxVdim, c = i % kMaxVdim, mm = row / RP;
-    const int64_t item = item0 + row % RP;
+    const int item = item0 + row % RP;
     if (item >= n_items) continue;
     float top = -INFINITY;
 #pragma unroll
@@ -374,7 +367,7 @@ __global__ void __launch_bounds__(kRowThreads, 2)
       l += ml.y * f;
       x += sh.acc[w][row][c] * f;
     }
-    const int64_t to = (((b * s.Hk + hk) * n_items + item) * 2 + mm) * parts.splits + blockIdx.x;
+    const int64_t to = (((int64_t)blockIdx.y * n_items + item) * 2 + mm) * parts.splits + blockIdx.x;
     if (c == 0) parts.ml[to] = make_float2(top, l);
     if (c < s.dv) parts.o[to * s.dv + c] = x;
   }
@@ -555,7 +548,7 @@ template <int RP>
 int launch_rows(tx_ctx *ctx, const Shape &s, float *out, float *out2, float *lse) {
   const int64_t chunks = (s.T * s.G + RP - 1) / RP, blocks = chunks * s.B * s.Hk;
   // two blocks an SM, each with four rounds of its warps at least
-  constexpr int64_t round = kGroup * kRowWarps;
+  constexpr int64_t round = kGroupOf<RP> * kRowWarps;
   int64_t splits = 2 * ctx->num_sms / blocks, most = (s.S + 4 * round - 1) / (4 * round);
   if (splits > most) splits = most;
   if (splits > kJoinMost) splits = kJoinMost;
