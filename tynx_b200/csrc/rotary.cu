@@ -19,8 +19,8 @@
 // of one a pair and head), and walks the (token, head) rows with 8 elements a
 // lane, so a row of 128 takes half a warp and both elements of every pair sit
 // in one lane: the rotation needs no exchange, the norm a shuffle sum over the
-// row's lanes.  Rows whose elements cannot be taken four at a time (dim or
-// head_dim no multiple of 8, unaligned) run the same code with a warp a row
+// row's lanes.  Rows whose elements cannot be taken four at a time
+// (head_dim, or in halves also dim, no multiple of 8, unaligned) run the same code with a warp a row
 // and single-element accesses.
 #include "common.h"
 
@@ -39,13 +39,18 @@ struct RowShape {
   int half;  // rotating pairs
 };
 
-// VEC: the lane holds pairs 4 u .. 4 u + 3 of unit u (two float4: elements
-// 4 u and half + 4 u, or interleaved 8 u and 8 u + 4; behind the rotating
-// part 8 consecutive elements).  Otherwise pairs lane + 32 i one by one.
+// VEC: the lane holds two float4 of unit u: pairs 4 u .. 4 u + 3 as elements 4 u
+// and half + 4 u (behind the rotating part 8 consecutive elements); interleaved,
+// elements 4 u and dim / 2 + 4 u, two pairs each, so that a warp's accesses are
+// whole lines either way.  Otherwise pairs lane + 32 i one by one.
 template <bool VEC, bool INTER>
 struct Lane {
-  static __device__ __forceinline__ int pair(int lane, int i) { return VEC ? 4 * lane + i : lane + 32 * i; }
-  // element of pair p's lo and hi
+  static __device__ __forceinline__ int pair(const RowShape s, int lane, int i) {
+    if (!VEC) return lane + 32 * i;
+    if (INTER) return (i < 2 ? 0 : s.dim >> 2) + 2 * lane + (i & 1);
+    return 4 * lane + i;
+  }
+  // elements of pair p's lo and hi
   static __device__ __forceinline__ void place(const RowShape s, int p, int &a, int &b) {
     if (INTER || p >= s.half) {
       a = 2 * p;
@@ -55,19 +60,24 @@ struct Lane {
       b = p + s.half;
     }
   }
+  // VEC: first elements of the two float4
+  static __device__ __forceinline__ void place4(const RowShape s, int lane, int &a, int &b) {
+    a = 4 * lane;
+    if (INTER) {
+      b = a + (s.dim >> 1);
+    } else if (a >= s.half) {
+      a *= 2;
+      b = a + 4;
+    } else {
+      b = a + s.half;
+    }
+  }
   static __device__ __forceinline__ void load(const float *row, const RowShape s, int lane, Eight &e) {
     if (VEC) {
       int a, b;
-      const int p = 4 * lane;
-      if (INTER || p >= s.half) {
-        a = 2 * p;
-        b = a + 4;
-      } else {
-        a = p;
-        b = p + s.half;
-      }
+      place4(s, lane, a, b);
       float4 x = make_float4(0.f, 0.f, 0.f, 0.f), y = x;
-      if (2 * p < s.dim) {
+      if (8 * lane < s.dim) {
         x = __ldg(reinterpret_cast<const float4 *>(row + a));
         y = __ldg(reinterpret_cast<const float4 *>(row + b));
       }
@@ -80,7 +90,7 @@ struct Lane {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         int a, b;
-        place(s, pair(lane, i), a, b);
+        place(s, pair(s, lane, i), a, b);
         e.lo[i] = a < s.dim ? __ldg(row + a) : 0.f;
         e.hi[i] = b < s.dim ? __ldg(row + b) : 0.f;
       }
@@ -89,15 +99,8 @@ struct Lane {
   static __device__ __forceinline__ void store(float *row, const RowShape s, int lane, const Eight &e) {
     if (VEC) {
       int a, b;
-      const int p = 4 * lane;
-      if (2 * p >= s.dim) return;
-      if (INTER || p >= s.half) {
-        a = 2 * p;
-        b = a + 4;
-      } else {
-        a = p;
-        b = p + s.half;
-      }
+      place4(s, lane, a, b);
+      if (8 * lane >= s.dim) return;
       float4 x, y;
       if (INTER) {
         x = make_float4(e.lo[0], e.hi[0], e.lo[1], e.hi[1]);
@@ -112,7 +115,7 @@ struct Lane {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         int a, b;
-        place(s, pair(lane, i), a, b);
+        place(s, pair(s, lane, i), a, b);
         if (a < s.dim) row[a] = e.lo[i];
         if (b < s.dim) row[b] = e.hi[i];
       }
@@ -137,11 +140,11 @@ __device__ __forceinline__ void fill_angles(float2 *cs, const tx_rotary &rot, co
 }
 
 template <bool VEC, bool INTER, bool BACK>
-__device__ __forceinline__ void turn(Eight &e, const float2 *cs, int half, int lane) {
+__device__ __forceinline__ void turn(Eight &e, const float2 *cs, const RowShape s, int lane) {
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const int p = Lane<VEC, INTER>::pair(lane, i);
-    if (p < half) {
+    const int p = Lane<VEC, INTER>::pair(s, lane, i);
+    if (p < s.half) {
       const float2 a = cs[p];
       const float s = BACK ? -a.y : a.y, lo = e.lo[i], hi = e.hi[i];
       e.lo[i] = lo * a.x - hi * s;
@@ -170,11 +173,11 @@ struct Args {
 // NORM: rows are normalised (q and k in turn), else rotated only (x[0]).
 // BACK (without NORM): the gradient's rotation.
 template <bool VEC, bool INTER, int LANES, bool NORM, bool BACK>
-__global__ void __launch_bounds__(kThreads, VEC ? 4 : 2)
+__global__ void __launch_bounds__(kThreads, VEC ? (NORM ? 3 : 4) : 2)
     k_rotary(const __grid_constant__ Args A, const __grid_constant__ tx_rotary rot) {
   using L = Lane<VEC, INTER>;
   __shared__ float2 cs[kAngles];
-  constexpr int SLOTS = kThreads / LANES, UN = VEC ? 4 : 2;
+  constexpr int SLOTS = kThreads / LANES, UN = 2;
   const int lane = threadIdx.x % LANES, slot = threadIdx.x / LANES;
   const RowShape s{A.dim, rot.dim >> 1};
   const int64_t t0 = (int64_t)blockIdx.x * A.group;
@@ -184,48 +187,57 @@ __global__ void __launch_bounds__(kThreads, VEC ? 4 : 2)
     L::load(A.w[0], s, lane, w[0]);
     L::load(A.w[1], s, lane, w[1]);
   }
+  // rows of q, then of k, UN a time; the next ones come while these are worked on, the first ones
+  // while the angles are
+  const int rows0 = nt * A.heads[0], rows = rows0 + (NORM ? nt * A.heads[1] : 0);
+  Eight e[UN], next[UN];
+  auto row_of = [&](float *const *base, int r) {
+    return NORM && r >= rows0 ? base[1] + (t0 * A.heads[1] + r - rows0) * s.dim : base[0] + (t0 * A.heads[0] + r) * s.dim;
+  };
+  auto fetch = [&](int r0) {
+#pragma unroll
+    for (int u = 0; u < UN; ++u)
+      if (r0 + u * SLOTS < rows) L::load(row_of(const_cast<float *const *>(A.x), r0 + u * SLOTS), s, lane, next[u]);
+  };
+  fetch(slot);
   fill_angles(cs, rot, A.pos, A.pos_stride, t0, nt, A.seq);
   __syncthreads();
   const float inv = 1.0f / (float)A.dim;
+  for (int r0 = slot; r0 < rows + slot; r0 += SLOTS * UN) {  // uniform within a warp: shuffles below
 #pragma unroll
-  for (int which = 0; which < (NORM ? 2 : 1); ++which) {
-    const int H = A.heads[which], rows = nt * H;
-    const int64_t base = t0 * H;
-    for (int r0 = slot; r0 < rows + slot; r0 += SLOTS * UN) {  // uniform within a warp: shuffles below
-      Eight e[UN];
+    for (int u = 0; u < UN; ++u) e[u] = next[u];
+    fetch(r0 + SLOTS * UN);
 #pragma unroll
-      for (int u = 0; u < UN; ++u) {
-        const int r = r0 + u * SLOTS;
-        if (r < rows) L::load(A.x[which] + (base + r) * s.dim, s, lane, e[u]);
-      }
-#pragma unroll
-      for (int u = 0; u < UN; ++u) {
-        const int r = r0 + u * SLOTS;
-        if (NORM) {
-          float ss = 0.f;
-          if (r < rows) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) ss += e[u].lo[i] * e[u].lo[i] + e[u].hi[i] * e[u].hi[i];
-          }
-          const float n = rsqrtf(row_sum<LANES>(ss) * inv + A.eps);
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            e[u].lo[i] *= n * w[which].lo[i];
-            e[u].hi[i] *= n * w[which].hi[i];
-          }
-        }
+    for (int u = 0; u < UN; ++u) {
+      const int r = r0 + u * SLOTS;
+      const bool second = NORM && r >= rows0;
+      if (NORM) {
+        float ss = 0.f;
         if (r < rows) {
-          turn<VEC, INTER, BACK>(e[u], cs + (r / H) * s.half, s.half, lane);
-          L::store(A.y[which] + (base + r) * s.dim, s, lane, e[u]);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) ss += e[u].lo[i] * e[u].lo[i] + e[u].hi[i] * e[u].hi[i];
         }
+        const float n = rsqrtf(row_sum<LANES>(ss) * inv + A.eps);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          e[u].lo[i] *= n * (second ? w[NORM].lo[i] : w[0].lo[i]);
+          e[u].hi[i] *= n * (second ? w[NORM].hi[i] : w[0].hi[i]);
+        }
+      }
+      if (r < rows) {
+        const int token = second ? (r - rows0) / A.heads[1] : r / A.heads[0];
+        turn<VEC, INTER, BACK>(e[u], cs + token * s.half, s, lane);
+        L::store(row_of(A.y, r), s, lane, e[u]);
       }
     }
   }
 }
 
+constexpr int kBackBlocks = 3;  // resident blocks an SM
+
 // The norm's backward: dx, and this block's share of both weight gradients.
 template <bool VEC, bool INTER, int LANES>
-__global__ void __launch_bounds__(kThreads, 2)
+__global__ void __launch_bounds__(kThreads, kBackBlocks)
     k_qk_norm_bwd(const __grid_constant__ Args A, const __grid_constant__ tx_rotary rot) {
   using L = Lane<VEC, INTER>;
   __shared__ float2 cs[kAngles];
@@ -264,7 +276,7 @@ __global__ void __launch_bounds__(kThreads, 2)
 #pragma unroll
         for (int u = 0; u < UN; ++u) {
           const int r = r0 + u * SLOTS;
-          if (r < rows) turn<VEC, INTER, true>(g[u], cs + (r / H) * s.half, s.half, lane);
+          if (r < rows) turn<VEC, INTER, true>(g[u], cs + (r / H) * s.half, s, lane);
           float ss = 0.f, dot = 0.f;
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
@@ -310,31 +322,36 @@ __global__ void __launch_bounds__(kThreads, 2)
 }
 
 // dw[which][c] = sum over the blocks' shares, 32 columns a block.
-__global__ void __launch_bounds__(256) k_qk_norm_dw(const float *part, int blocks, int dim, float *dqw, float *dkw) {
-  __shared__ float sums[8][33];
-  const int which = blockIdx.y, c = blockIdx.x * 32 + (threadIdx.x & 31), part_row = threadIdx.x >> 5;
+__global__ void __launch_bounds__(1024) k_qk_norm_dw(const float *part, int blocks, int dim, float *dqw, float *dkw) {
+  __shared__ float sums[32][33];
+  const int which = blockIdx.y, c = blockIdx.x * 32 + (threadIdx.x & 31), row = threadIdx.x >> 5;
   float v = 0.f;
-  if (c < dim)
-    for (int b = part_row; b < blocks; b += 8) v += part[((int64_t)b * 2 + which) * 256 + c];
-  sums[part_row][threadIdx.x & 31] = v;
-  __syncthreads();
-  if (part_row == 0 && c < dim) {
-#pragma unroll
-    for (int i = 1; i < 8; ++i) v += sums[i][threadIdx.x & 31];
-    (which ? dkw : dqw)[c] = v;
+  if (c < dim) {
+#pragma unroll 4
+    for (int b = row; b < blocks; b += 32) v += part[((int64_t)b * 2 + which) * 256 + c];
   }
+  sums[row][threadIdx.x & 31] = v;
+  __syncthreads();
+  v = sums[threadIdx.x & 31][row];  // a warp a column
+#pragma unroll
+  for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  if ((threadIdx.x & 31) == 0 && blockIdx.x * 32 + row < dim) (which ? dkw : dqw)[blockIdx.x * 32 + row] = v;
 }
 
 bool four(const void *p) { return ((uintptr_t)p & 15) == 0; }
 
-// tokens a block takes: about four rows a slot, within the angle table
-int group_of(int lanes, int heads, int half, int64_t tokens, int sms) {
+// Tokens a block takes at a time, within the angle table.  Long inputs: with the norm, eight rows a
+// slot, so that weights, angles and the block's start are shared by more (4 x 4096 tokens of 20 heads of
+// 128: forward 61.5 us, backward 92 us; with four 65 and 104), without it four (8 x 2048 tokens of 16
+// heads of 64: 21.9 us, with eight 23.6).  Short ones four, so that all SMs have blocks.
+int group_of(int lanes, int heads, int half, int64_t tokens, int sms, bool norm) {
   const int slots = kThreads / lanes;
-  int64_t g = (4 * slots + heads - 1) / heads;
+  int64_t g = 8 * slots / heads;
+  if (!norm || tokens < 6 * sms * g) g = 4 * slots / heads;
   const int64_t share = (tokens + sms - 1) / sms;  // few tokens: one wave of smaller blocks
   if (g > share) g = share;
   if (half && g > kAngles / half) g = kAngles / half;
-  return g < 1 ? 1 : (int)g;
+  return g < 1 ? 1 : (int)g;  // half <= 128: the table holds one token's angles at least
 }
 
 int check_rotary(tx_ctx *ctx, int64_t batch, int64_t seq, int64_t heads, int64_t kv_heads, int64_t head_dim,
@@ -353,20 +370,21 @@ int check_rotary(tx_ctx *ctx, int64_t batch, int64_t seq, int64_t heads, int64_t
 template <bool VEC, bool INTER, int LANES>
 int launch_rows(tx_ctx *ctx, Args &A, const tx_rotary &rot, int mode, float *dqw, float *dkw) {
   const int heads = A.heads[0] + A.heads[1];
-  A.group = group_of(LANES, heads, rot.dim >> 1, A.tokens, ctx->num_sms);
+  A.group = group_of(LANES, heads, rot.dim >> 1, A.tokens, ctx->num_sms, mode >= 2);
   const int64_t groups = (A.tokens + A.group - 1) / A.group;
   if (mode == 0) k_rotary<VEC, INTER, LANES, false, false><<<(unsigned)groups, kThreads, 0, ctx->stream>>>(A, rot);
   if (mode == 1) k_rotary<VEC, INTER, LANES, false, true><<<(unsigned)groups, kThreads, 0, ctx->stream>>>(A, rot);
   if (mode == 2) k_rotary<VEC, INTER, LANES, true, false><<<(unsigned)groups, kThreads, 0, ctx->stream>>>(A, rot);
   if (mode == 3) {
-    // two resident blocks an SM; the blocks' shares are summed in their order
-    const unsigned blocks = (unsigned)(groups < 2 * ctx->num_sms ? groups : 2 * ctx->num_sms);
+    // one wave; the blocks' shares are summed in their order
+    const int64_t wave = (int64_t)kBackBlocks * ctx->num_sms;
+    const unsigned blocks = (unsigned)(groups < wave ? groups : wave);
     Scratch part(ctx, (size_t)blocks * 512 * sizeof(float));
     if (!part.ptr) return TX_ERR_OOM;
     A.part = part.as<float>();
     k_qk_norm_bwd<VEC, INTER, LANES><<<blocks, kThreads, 0, ctx->stream>>>(A, rot);
     TX_LAUNCHED(ctx, "k_qk_norm_bwd");
-    k_qk_norm_dw<<<dim3((unsigned)((A.dim + 31) / 32), 2), 256, 0, ctx->stream>>>(part.as<float>(), (int)blocks, A.dim,
+    k_qk_norm_dw<<<dim3((unsigned)((A.dim + 31) / 32), 2), 1024, 0, ctx->stream>>>(part.as<float>(), (int)blocks, A.dim,
                                                                                dqw, dkw);
   }
   TX_LAUNCHED(ctx, "k_rotary");
@@ -382,7 +400,7 @@ int launch_layout(tx_ctx *ctx, Args &A, const tx_rotary &rot, int mode, bool vec
 }
 
 int launch(tx_ctx *ctx, Args &A, const tx_rotary &rot, int mode, float *dqw = nullptr, float *dkw = nullptr) {
-  bool vec = A.dim % 8 == 0 && rot.dim % 8 == 0;
+  bool vec = A.dim % 8 == 0 && (rot.interleaved || rot.dim % 8 == 0);
   for (int i = 0; i < 2; ++i) vec = vec && four(A.x[i]) && four(A.y[i]) && four(A.w[i]) && four(A.dy[i]);
   return rot.interleaved ? launch_layout<true>(ctx, A, rot, mode, vec, dqw, dkw)
                          : launch_layout<false>(ctx, A, rot, mode, vec, dqw, dkw);
