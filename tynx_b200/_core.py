@@ -108,15 +108,18 @@ class Context:
         self.index = index
         self.owner = threading.get_ident()
         self.capturing = False
+        self._out = C.c_void_p()  # result of an allocation
+        self._out_ref = C.byref(self._out)
 
     def check(self, code: int, what: str = "") -> None:
         if code != N.TX_OK:
             N.raise_for(code, self.handle, what)
 
     def alloc(self, nbytes: int) -> int:
-        out = C.c_void_p()
-        self.check(lib.tx_alloc(self.handle, max(int(nbytes), 1), C.byref(out)), "alloc")
-        return out.value
+        code = lib.tx_alloc(self.handle, nbytes or 1, self._out_ref)
+        if code:
+            N.raise_for(code, self.handle, "alloc")
+        return self._out.value
 
     def free(self, ptr: int) -> None:
         lib.tx_free(self.handle, ptr)
@@ -219,7 +222,7 @@ class Storage:
 def _shape_tuple(shape) -> tuple:
     if isinstance(shape, int):
         return (shape,)
-    return tuple(int(s) for s in shape)
+    return tuple(map(int, shape))
 
 
 def _numel(shape) -> int:
@@ -295,6 +298,9 @@ def _needs_grad(*tensors) -> bool:
     return is_grad_enabled() and any(isinstance(t, Tensor) and t.requires_grad for t in tensors)
 
 
+_export = None  # interop.export, once it is needed
+
+
 class Tensor:
     """A dense device tensor (float32, int64 or bool) with an optional tape node."""
 
@@ -346,6 +352,14 @@ class Tensor:
         shape = _shape_tuple(shape)
         t = object.__new__(cls)
         t._init(Storage(ctx, _numel(shape) * _DTYPES[dtype][1]), 0, shape, dtype)
+        return t
+
+    def detach(self) -> "Tensor":
+        t = object.__new__(Tensor)
+        t._storage, t._offset, t.shape, t.dtype = self._storage, self._offset, self.shape, self.dtype
+        t.requires_grad = False
+        t._grad = t._fn = None
+        t._out_index = 0
         return t
 
     @classmethod
@@ -416,9 +430,10 @@ class Tensor:
 
     def __dlpack__(self, *, stream=None, **unused):
         """Lend this tensor to another library (``torch.from_dlpack(tensor)``)."""
-        from .interop import export
-
-        return export(self, stream)
+        global _export
+        if _export is None:
+            from .interop import export as _export
+        return _export(self, stream)
 
     def __dlpack_device__(self) -> tuple:
         return (2, self.ctx.index)
@@ -433,9 +448,6 @@ class Tensor:
 
     def __float__(self) -> float:
         return float(self.item())
-
-    def detach(self) -> "Tensor":
-        return Tensor._view(self._storage, self._offset, self.shape, self.dtype)
 
     def clone(self) -> "Tensor":
         out = Tensor._empty(self.shape, self.dtype, self.ctx)

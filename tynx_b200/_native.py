@@ -14,6 +14,7 @@ there is none.
 from __future__ import annotations
 
 import ctypes as C
+import importlib.util
 import os
 from pathlib import Path
 
@@ -234,12 +235,28 @@ SIGNATURES = {
 }
 
 
+def _share_nccl() -> None:
+    """Load the NCCL of the Python environment, where there is one, before the
+    engine would load the system's: a process holds one ``libnccl.so.2``, and
+    PyTorch, imported later for ``from_dlpack``, does not load with an older one."""
+    spec = importlib.util.find_spec("nvidia")
+    for place in (spec.submodule_search_locations or ()) if spec else ():
+        library = Path(place) / "nccl" / "lib" / "libnccl.so.2"
+        if library.exists():
+            try:
+                C.CDLL(str(library))
+            except OSError:  # the system's it is
+                pass
+            return
+
+
 def _load() -> C.CDLL:
     if not _LIB_PATH.exists():
         raise ImportError(
             f"{_LIB_PATH} is missing: build it with `python -m tynx_b200.build` "
             "(the CUDA engine has no CPU fallback)"
         )
+    _share_nccl()
     lib = C.CDLL(str(_LIB_PATH), mode=os.RTLD_NOW | os.RTLD_GLOBAL)
     for name, argtypes in SIGNATURES.items():
         fn = getattr(lib, name)

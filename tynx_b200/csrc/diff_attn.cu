@@ -16,17 +16,6 @@ namespace {
 PFN_cuTensorMapEncodeTiled_v12000 g_encode = nullptr;
 std::once_flag g_encode_once;
 
-__device__ __forceinline__ float warp_max(float v) {
-#pragma unroll
-  for (int o = 16; o; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
-  return v;
-}
-__device__ __forceinline__ float warp_sum(float v) {
-#pragma unroll
-  for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  return v;
-}
-
 // A block splits one tile of 128 rows of one head; blockIdx.z picks the tensor.
 struct SplitJob {
   const float *src;
@@ -177,14 +166,14 @@ __device__ __forceinline__ void split_tile(const Shape &s, const SplitJobs &jobs
     *reinterpret_cast<uint4 *>(dst + W) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
   }
 }
-// W: the values' width (queries and keys have 64); GRAD: the output's gradient alone
-template <int W, bool GRAD>
+// W: the values' width (queries and keys have 64)
+template <int W>
 __global__ void __launch_bounds__(kSplitThreads, 2)
     k_diff_split(const __grid_constant__ Shape s, const __grid_constant__ SplitJobs jobs) {
   __shared__ uint32_t red[3 * kSplitWarps];
-  const SplitJob &J = jobs.j[GRAD ? 3 : blockIdx.z];
+  const SplitJob &J = jobs.j[blockIdx.z];
   if ((int64_t)blockIdx.x >= s.B * J.heads * J.tiles) return;
-  if (GRAD)
+  if (blockIdx.z == 3)
     split_tile<W, true>(s, jobs, J, red);
   else if (blockIdx.z < 2)
     split_tile<64, false>(s, jobs, J, red);
@@ -373,79 +362,87 @@ __global__ void __launch_bounds__(kRowThreads, 2)
   }
 }
 
-// out, out2 and lse from the ranges' partial rows: a block per query and head, 128 threads a map and a
-// column each.  Latency alone: the ranges' references are read once, the columns' loads do not depend
-// on one another.
-constexpr int kJoinMost = 512;  // ranges at most
-__global__ void __launch_bounds__(2 * kMaxVdim)
+// out, out2 and lse from the ranges' partial rows: a warp per query, head and map, four columns a
+// lane.  Latency alone: 32 ranges' references at a time, one a lane, then loads that do not depend on
+// one another.
+constexpr int kJoinRows = 4;  // a block at most
+__global__ void __launch_bounds__(64 * kJoinRows)
     k_diff_join(const __grid_constant__ Shape s, const Parts parts, float *out, float *out2, float *lse) {
-  __shared__ float w[2][kJoinMost];
-  __shared__ float tops[8], sums[8], second[kMaxVdim];
-  const int64_t n_items = s.T * s.G;
-  const int64_t at = blockIdx.x;  // (b, hk, item)
-  const int64_t item = at % n_items, bh = at / n_items;
-  const int64_t b = bh / s.Hk, t = item / s.G;
-  const int hk = (int)(bh - b * s.Hk), h = hk * s.G + (int)(item - t * s.G);
-  const int m = threadIdx.x >> 7, c = threadIdx.x & 127, warp = threadIdx.x >> 5, splits = parts.splits;
-  const float2 *ml = parts.ml + (at * 2 + m) * splits;
-  float2 mine[kJoinMost / kMaxVdim];
-  float top = -INFINITY;
-#pragma unroll
-  for (int i = 0; i < kJoinMost / kMaxVdim; ++i) {
-    mine[i] = c + i * kMaxVdim < splits ? __ldg(ml + c + i * kMaxVdim) : make_float2(-INFINITY, 0.f);
-    top = fmaxf(top, mine[i].x);
-  }
+  __shared__ float4 second[kJoinRows][32];
+  const int lane = threadIdx.x & 31, m = (threadIdx.x >> 5) & 1, row = threadIdx.x >> 6, splits = parts.splits;
+  const int64_t n_items = s.T * s.G, rows = s.B * s.Hk * n_items;
+  const int64_t at = (int64_t)blockIdx.x * (blockDim.x >> 6) + row;  // (b, hk, item)
+  const bool live = at < rows;
+  const float2 *ml = parts.ml + (live ? at * 2 + m : 0) * splits;
+  // the first 32 ranges' references stay in registers
+  const float2 mine = lane < splits ? __ldg(ml + lane) : make_float2(-INFINITY, 0.f);
+  float top = mine.x;
+  for (int i = lane + 32; i < splits; i += 32) top = fmaxf(top, __ldg(ml + i).x);
   top = warp_max(top);
-  if ((threadIdx.x & 31) == 0) tops[warp] = top;
-  __syncthreads();
-  top = fmaxf(fmaxf(tops[4 * m], tops[4 * m + 1]), fmaxf(tops[4 * m + 2], tops[4 * m + 3]));
   const bool none = top == -INFINITY;
   const float ref = none ? 0.f : top;
+  const int c = 4 * lane;
+  const bool four = (s.dv & 3) == 0;  // the partial rows are aligned
+  const float *p = parts.o + (live ? at * 2 + m : 0) * splits * s.dv + c;
   float sum = 0.f;
+  float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int i0 = 0; i0 < splits; i0 += 32) {
+    const float2 v = i0 == 0 ? mine : i0 + lane < splits ? __ldg(ml + i0 + lane) : make_float2(-INFINITY, 0.f);
+    const float w = ex2(v.x - ref);
+    sum += v.y * w;
+    const int n = splits - i0 < 32 ? splits - i0 : 32;
+    for (int j = 0; j < n; j += 12) {  // loads of twelve ranges in flight
+      float4 y[12];
 #pragma unroll
-  for (int i = 0; i < kJoinMost / kMaxVdim; ++i) {
-    const float f = ex2(mine[i].x - ref);
-    if (c + i * kMaxVdim < splits) w[m][c + i * kMaxVdim] = f;
-    sum += mine[i].y * f;
+      for (int i = 0; i < 12; ++i) {
+        y[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (j + i < n) {
+          const float *q = p + (int64_t)(i0 + j + i) * s.dv;
+          if (four) {
+            if (c < s.dv) y[i] = __ldg(reinterpret_cast<const float4 *>(q));
+          } else {
+            if (c < s.dv) y[i].x = __ldg(q);
+            if (c + 1 < s.dv) y[i].y = __ldg(q + 1);
+            if (c + 2 < s.dv) y[i].z = __ldg(q + 2);
+            if (c + 3 < s.dv) y[i].w = __ldg(q + 3);
+          }
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < 12; ++i) {
+        const float f = __shfl_sync(0xffffffffu, w, (j + i) & 31);
+        if (j + i < n) x = make_float4(x.x + y[i].x * f, x.y + y[i].y * f, x.z + y[i].z * f, x.w + y[i].w * f);
+      }
+    }
   }
   sum = warp_sum(sum);
-  if ((threadIdx.x & 31) == 0) sums[warp] = sum;
+  const float inv = none ? 0.f : 1.f / sum;
+  x = make_float4(x.x * inv, x.y * inv, x.z * inv, x.w * inv);
+  if (m) second[row][lane] = x;
   __syncthreads();
-  sum = (sums[4 * m] + sums[4 * m + 1]) + (sums[4 * m + 2] + sums[4 * m + 3]);
-  float x = 0.f;
-  if (c < s.dv && !none) {
-    const float *p = parts.o + (at * 2 + m) * splits * s.dv + c;
-#pragma unroll 16
-    for (int i = 0; i < splits; ++i) x += __ldg(p + (int64_t)i * s.dv) * w[m][i];
-    x /= sum;
+  if (!live) return;
+  const int64_t bh = at / n_items, item = at - bh * n_items;
+  const int64_t b = bh / s.Hk, t = item / s.G;
+  const int hk = (int)(bh - b * s.Hk), h = hk * s.G + (int)(item - t * s.G);
+  if (lse && lane == 0) lse[(b * 2 * s.H + 2 * h + m) * s.T + t] = none ? INFINITY : top + log2f(sum);
+  float *dst = m ? out2 : out;
+  if (!dst) return;
+  if (!m) {
+    const float lam = __ldg(s.lam + h);
+    const float4 y = second[row][lane];
+    x = make_float4(x.x - lam * y.x, x.y - lam * y.y, x.z - lam * y.z, x.w - lam * y.w);
   }
-  if (lse && c == 0) lse[(b * 2 * s.H + 2 * h + m) * s.T + t] = none ? INFINITY : top + log2f(sum);
-  const int64_t i = ((b * s.T + t) * s.H + h) * s.dv + c;
-  if (m) {
-    second[c] = x;
-    if (out2 && c < s.dv) out2[i] = x;
-  }
-  __syncthreads();
-  if (!m && c < s.dv) out[i] = x - __ldg(s.lam + h) * second[c];
+  dst += ((b * s.T + t) * s.H + h) * s.dv + c;
+  if (c < s.dv) dst[0] = x.x;
+  if (c + 1 < s.dv) dst[1] = x.y;
+  if (c + 2 < s.dv) dst[2] = x.z;
+  if (c + 3 < s.dv) dst[3] = x.w;
 }
 
-// dlam = -sum of D2, from the tiles' sums
-__global__ void __launch_bounds__(256) k_diff_dlam(const __grid_constant__ Shape s, const float *sums, int64_t tiles,
-                                                   float *dlam) {
-  __shared__ float part[8];
-  const int h = blockIdx.x;
-  float v = 0.f;
-  for (int64_t i = threadIdx.x; i < s.B * tiles; i += 256) {
-    const int64_t b = i / tiles;
-    v += sums[(b * s.H + h) * tiles + (i - b * tiles)];
-  }
-  v = warp_sum(v);
-  if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = v;
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    for (int i = 1; i < 8; ++i) v += part[i];
-    dlam[h] = -v;
-  }
+// dlam where it is the only gradient wanted (otherwise the backward's blocks sum it)
+__global__ void __launch_bounds__(32) k_diff_dlam(const __grid_constant__ Shape s, const float *sums, int64_t tiles,
+                                                  float *dlam) {
+  sum_dlam(s, sums, tiles, dlam, blockIdx.x);
 }
 
 // ---- host ----------------------------------------------------------------------------------
@@ -493,18 +490,12 @@ struct Operands {
     jobs.j[3] = SplitJob{dout, x.g, w(x.fg), w(x.ng), s.T, x.qt, s.H, s.dv, 1.0f, 0};
     if (p) jobs.out = p->out, jobs.out2 = p->out2, jobs.lse = p->lse, jobs.stats = stats, jobs.sums = sums;
     const int64_t blocks = tq > tk ? tq : tk;
-    const dim3 grid((unsigned)blocks, 1, 3);
+    const dim3 grid((unsigned)blocks, 1, p ? 4 : 3);
     if (x.vw == 64)
-      k_diff_split<64, false><<<grid, kSplitThreads, 0, ctx->stream>>>(s, jobs);
+      k_diff_split<64><<<grid, kSplitThreads, 0, ctx->stream>>>(s, jobs);
     else
-      k_diff_split<128, false><<<grid, kSplitThreads, 0, ctx->stream>>>(s, jobs);
+      k_diff_split<128><<<grid, kSplitThreads, 0, ctx->stream>>>(s, jobs);
     TX_LAUNCHED(ctx, "k_diff_split");
-    if (!p) return TX_OK;
-    if (x.vw == 64)
-      k_diff_split<64, true><<<(unsigned)tg, kSplitThreads, 0, ctx->stream>>>(s, jobs);
-    else
-      k_diff_split<128, true><<<(unsigned)tg, kSplitThreads, 0, ctx->stream>>>(s, jobs);
-    TX_LAUNCHED(ctx, "k_diff_split (gradient)");
     return TX_OK;
   }
 };
@@ -528,7 +519,9 @@ int check_desc(tx_ctx *ctx, const tx_diff_attention *p, Shape &s) {
 }
 
 int join(tx_ctx *ctx, const Shape &s, const Parts &parts, float *out, float *out2, float *lse) {
-  k_diff_join<<<(unsigned)(s.B * s.T * s.H), 2 * kMaxVdim, 0, ctx->stream>>>(s, parts, out, out2, lse);
+  const int64_t rows = s.B * s.T * s.H;
+  const int each = rows < 8 * ctx->num_sms ? 1 : kJoinRows;  // few rows: an SM each
+  k_diff_join<<<(unsigned)((rows + each - 1) / each), 64 * each, 0, ctx->stream>>>(s, parts, out, out2, lse);
   TX_LAUNCHED(ctx, "k_diff_join");
   return TX_OK;
 }
@@ -551,7 +544,6 @@ int launch_rows(tx_ctx *ctx, const Shape &s, float *out, float *out2, float *lse
   constexpr int64_t round = kGroupOf<RP> * kRowWarps;
   int64_t splits = 2 * ctx->num_sms / blocks, most = (s.S + 4 * round - 1) / (4 * round);
   if (splits > most) splits = most;
-  if (splits > kJoinMost) splits = kJoinMost;
   if (splits < 1) splits = 1;
   const int64_t per = ((s.S + splits - 1) / splits + round - 1) / round * round;
   PartMemory mem(ctx, s, (int)splits);
@@ -559,7 +551,8 @@ int launch_rows(tx_ctx *ctx, const Shape &s, float *out, float *out2, float *lse
   const int smem = (int)sizeof(RowSmem<RP>);
   const bool vec = (s.d & 3) == 0 && (s.dv & 3) == 0 && ((uintptr_t)s.k & 15) == 0 && ((uintptr_t)s.v & 15) == 0;
   auto kernel = vec ? k_diff_rows<RP, true> : k_diff_rows<RP, false>;
-  TX_CUDA(ctx, cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+  static SmemGrant granted[2];
+  TX_TRY(granted[vec].take(ctx, (const void *)kernel, smem));
   kernel<<<dim3((unsigned)splits, (unsigned)(s.B * s.Hk), (unsigned)chunks), kRowThreads, smem, ctx->stream>>>(
       s, mem.parts, per);
   TX_LAUNCHED(ctx, "k_diff_rows");
@@ -646,10 +639,10 @@ extern "C" int tx_diff_attention_bwd(tx_ctx *ctx, const tx_diff_attention *p) {
   Scratch sums(ctx, (size_t)x.tg * 4);
   if (!stats.ptr || !sums.ptr) return TX_ERR_OOM;
   TX_TRY(x.fill(ctx, s, p, stats.as<float>(), sums.as<float>()));
+  if (p->dq || p->dk) return tc_backward(ctx, s, x.x, stats.as<float>(), sums.as<float>(), p->dq, p->dk, p->dv, p->dlam);
   if (p->dlam) {
-    k_diff_dlam<<<(unsigned)s.H, 256, 0, ctx->stream>>>(s, sums.as<float>(), x.x.qt, p->dlam);
+    k_diff_dlam<<<(unsigned)s.H, 32, 0, ctx->stream>>>(s, sums.as<float>(), x.x.qt, p->dlam);
     TX_LAUNCHED(ctx, "k_diff_dlam");
   }
-  if (!p->dq && !p->dk) return TX_OK;
-  return tc_backward(ctx, s, x.x, stats.as<float>(), p->dq, p->dk, p->dv);
+  return TX_OK;
 }

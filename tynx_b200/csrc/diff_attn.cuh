@@ -36,6 +36,41 @@ struct Shape {
   }
 };
 
+__device__ __forceinline__ float warp_max(float v) {
+#pragma unroll
+  for (int o = 16; o; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
+  return v;
+}
+__device__ __forceinline__ float warp_sum(float v) {
+#pragma unroll
+  for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+
+// dlam[h] = -sum of D2 over the tiles' sums [b][h][tiles], in a fixed order, by one warp
+__device__ __forceinline__ void sum_dlam(const Shape &s, const float *sums, int64_t tiles, float *dlam, int h) {
+  const int lane = threadIdx.x & 31;
+  float v = 0.f;
+  for (int64_t i = lane; i < s.B * tiles; i += 32) {
+    const int64_t b = i / tiles;
+    v += __ldg(sums + (b * s.H + h) * tiles + (i - b * tiles));
+  }
+  v = warp_sum(v);
+  if (lane == 0) dlam[h] = -v;
+}
+
+// Grants a kernel its dynamic shared memory once a device.
+struct SmemGrant {
+  uint64_t devices = 0;
+  int take(tx_ctx *ctx, const void *kernel, int bytes) {
+    const uint64_t bit = ctx->device < 64 ? uint64_t(1) << ctx->device : 0;
+    if (devices & bit) return TX_OK;
+    TX_CUDA(ctx, cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+    devices |= bit;
+    return TX_OK;
+  }
+};
+
 // A key length outside [0, S] raises the context's error flag.
 __device__ __forceinline__ void report_length(const Shape &s, int64_t b) {
   if (!s.len) return;
@@ -83,7 +118,9 @@ int tc_forward_splits(tx_ctx *ctx, const Shape &s);
 // out, out2 and lse, or with parts.splits > 1 the partial results
 int tc_forward(tx_ctx *ctx, const Shape &s, const Split &x, float *out, float *out2, float *lse, const Parts &parts);
 // stats [b][h][ceil(T / 64)][4][64]: the log-sum-exp of both maps (+inf behind the last query), D1, D2
-int tc_backward(tx_ctx *ctx, const Shape &s, const Split &x, const float *stats, float *dq, float *dk, float *dv);
+// sums [b][h][tiles of queries]: the tiles' sums of D2; dq, dk and dv, dlam are optional
+int tc_backward(tx_ctx *ctx, const Shape &s, const Split &x, const float *stats, const float *sums, float *dq,
+                float *dk, float *dv, float *dlam);
 
 // ---- device wrappers -------------------------------------------------------------------------
 constexpr uint64_t kWaitNs = 2000000000ull;  // 2 s

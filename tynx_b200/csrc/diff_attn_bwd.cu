@@ -46,8 +46,8 @@ struct Cfg {
 };
 
 struct Grads {
-  const float *stats;  // [b][h][ceil(T / 64)][4][64]
-  float *dq, *dk, *dv;
+  const float *stats, *sums;  // [b][h][ceil(T / 64)][4][64], [b][h][qt]
+  float *dq, *dk, *dv, *dlam;
   // blocks of one tile level: K, Q and V; in turn level by level, or kind after kind
   unsigned nk, nq, levels, by_level, kt, qt;
 };
@@ -266,6 +266,8 @@ __device__ __forceinline__ void body(const Shape &s, const Split &x, const CUten
       }
       mma_commit(all_done, one);
       bar_drain(all_done, 0);
+    } else if (warp == 2 && o.dlam) {
+      for (int h = blockIdx.x; h < s.H; h += gridDim.x) sum_dlam(s, o.sums, x.qt, o.dlam, h);
     }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 104;");
@@ -471,7 +473,8 @@ __global__ void __launch_bounds__(kThreads, 1)
 }
 
 template <int DV>
-int launch(tx_ctx *ctx, const Shape &s, const Split &x, const float *stats, float *dq, float *dk, float *dv) {
+int launch(tx_ctx *ctx, const Shape &s, const Split &x, const float *stats, const float *sums, float *dq, float *dk,
+           float *dv, float *dlam) {
   CUtensorMap mq, mk, mv, mg;
   if (!split_map(&mq, x.q, 64, s.T, s.B * 2 * s.H) || !split_map(&mk, x.k, 64, s.S, s.B * 2 * s.Hk) ||
       !split_map(&mv, x.v, DV, s.S, s.B * s.Hk) || !split_map(&mg, x.g, DV, s.T, s.B * s.H))
@@ -481,8 +484,9 @@ int launch(tx_ctx *ctx, const Shape &s, const Split &x, const float *stats, floa
   // the kinds take turns, and the last blocks are the shortest of each.  Otherwise K and Q blocks are
   // alike and V blocks half as long, so V comes last.
   const unsigned kt = (unsigned)x.kt, qt = (unsigned)x.qt;
-  const Grads o{stats, dq, dk, dv, nk, nq, kt < qt ? kt : qt, (unsigned)(s.causal && nk && nq), kt, qt};
-  TX_CUDA(ctx, cudaFuncSetAttribute(k_diff_bwd<DV>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<DV>::SMEM));
+  const Grads o{stats, sums, dq, dk, dv, dlam, nk, nq, kt < qt ? kt : qt, (unsigned)(s.causal && nk && nq), kt, qt};
+  static SmemGrant granted;
+  TX_TRY(granted.take(ctx, (const void *)k_diff_bwd<DV>, Cfg<DV>::SMEM));
   k_diff_bwd<DV><<<2 * nk * kt + nq * qt, kThreads, Cfg<DV>::SMEM, ctx->stream>>>(s, x, mq, mk, mv, mg, o);
   TX_LAUNCHED(ctx, "k_diff_bwd");
   return TX_OK;
@@ -490,8 +494,10 @@ int launch(tx_ctx *ctx, const Shape &s, const Split &x, const float *stats, floa
 
 }  // namespace
 
-int tc_backward(tx_ctx *ctx, const Shape &s, const Split &x, const float *stats, float *dq, float *dk, float *dv) {
-  return x.vw == 64 ? launch<64>(ctx, s, x, stats, dq, dk, dv) : launch<128>(ctx, s, x, stats, dq, dk, dv);
+int tc_backward(tx_ctx *ctx, const Shape &s, const Split &x, const float *stats, const float *sums, float *dq,
+                float *dk, float *dv, float *dlam) {
+  return x.vw == 64 ? launch<64>(ctx, s, x, stats, sums, dq, dk, dv, dlam)
+                    : launch<128>(ctx, s, x, stats, sums, dq, dk, dv, dlam);
 }
 
 }  // namespace tx_diff

@@ -386,7 +386,8 @@ int launch(tx_ctx *ctx, const Shape &s, const Split &x, const Out &o) {
   if (!split_map(&mq, x.q, 64, s.T, s.B * 2 * s.H) || !split_map(&mk, x.k, 64, s.S, s.B * 2 * s.Hk) ||
       !split_map(&mv, x.v, DV, s.S, s.B * s.Hk))
     return tx_fail(ctx, TX_ERR_UNSUPPORTED, "differential attention: tensor map");
-  TX_CUDA(ctx, cudaFuncSetAttribute(k_diff_fwd<DV>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<DV>::SMEM));
+  static SmemGrant granted;
+  TX_TRY(granted.take(ctx, (const void *)k_diff_fwd<DV>, Cfg<DV>::SMEM));
   const int64_t blocks = x.qt * s.B * s.H;
   k_diff_fwd<DV><<<dim3((unsigned)blocks, (unsigned)o.parts.splits), kThreads, Cfg<DV>::SMEM, ctx->stream>>>(s, x, mq, mk,
                                                                                                         mv, o);

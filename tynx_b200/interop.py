@@ -63,12 +63,13 @@ def export(tensor: Tensor, stream=None):
         own = C.c_void_p()
         ctx.check(lib.tx_stream(ctx.handle, C.byref(own)))
         stream = own.value
-    storage = tensor._storage
-    out = C.c_void_p()
-    ctx.check(lib.tx_dlpack_export(ctx.handle, storage.ptr if storage.owned else None, tensor.ptr,
-                                   N.DL_TYPES[tensor.dtype], N.i64_array(tensor.shape), tensor.ndim, stream or 1,
-                                   C.byref(out)), "dlpack")
-    return _new(out.value, _NAME, _drop_pointer)
+    storage, shape = tensor._storage, tensor.shape
+    code = lib.tx_dlpack_export(ctx.handle, storage.ptr if storage.owned else None, storage.ptr + tensor._offset,
+                                N.DL_TYPES[tensor.dtype], (C.c_int64 * len(shape))(*shape), len(shape), stream or 1,
+                                ctx._out_ref)
+    if code:
+        ctx.check(code, "dlpack")
+    return _new(ctx._out.value, _NAME, _drop_pointer)
 
 
 class _Borrowed(Storage):
