@@ -185,6 +185,7 @@ pub struct tx_diff_attention {
     pub out: *mut f32,
     pub out2: *mut f32,
     pub lse: *mut f32,
+    pub saved: *mut c_void,
     pub dout: *const f32,
     pub dq: *mut f32,
     pub dk: *mut f32,
@@ -332,6 +333,7 @@ extern "C" {
     pub fn tx_rotary_apply(ctx: *mut tx_ctx, d_x: *const f32, d_y: *mut f32, batch: i64, seq: i64, heads: i64, head_dim: i64, d_pos: *const i64, pos_stride: i64, rotary: *const tx_rotary, inverse: c_int) -> c_int;
     pub fn tx_qk_norm_rotary_fwd(ctx: *mut tx_ctx, d_q: *const f32, d_k: *const f32, d_q_weight: *const f32, d_k_weight: *const f32, d_q_out: *mut f32, d_k_out: *mut f32, batch: i64, seq: i64, heads: i64, kv_heads: i64, head_dim: i64, d_pos: *const i64, pos_stride: i64, rotary: *const tx_rotary, eps: f32) -> c_int;
     pub fn tx_qk_norm_rotary_bwd(ctx: *mut tx_ctx, d_q: *const f32, d_k: *const f32, d_q_weight: *const f32, d_k_weight: *const f32, d_dq_out: *const f32, d_dk_out: *const f32, d_dq: *mut f32, d_dk: *mut f32, d_dq_weight: *mut f32, d_dk_weight: *mut f32, batch: i64, seq: i64, heads: i64, kv_heads: i64, head_dim: i64, d_pos: *const i64, pos_stride: i64, rotary: *const tx_rotary, eps: f32) -> c_int;
+    pub fn tx_diff_attention_saved_bytes(ctx: *mut tx_ctx, desc: *const tx_diff_attention, bytes: *mut i64) -> c_int;
     pub fn tx_diff_attention_fwd(ctx: *mut tx_ctx, desc: *const tx_diff_attention) -> c_int;
     pub fn tx_diff_attention_bwd(ctx: *mut tx_ctx, desc: *const tx_diff_attention) -> c_int;
     pub fn tx_ppo_loss_fwd(ctx: *mut tx_ctx, d_logits: *const f32, rows: i64, cols: i64, d_values: *const f32, d_actions: *const i64, d_old_log_prob: *const f32, d_advantages: *const f32, d_returns: *const f32, clip: f32, value_coef: f32, entropy_coef: f32, d_loss: *mut f32) -> c_int;

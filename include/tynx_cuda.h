@@ -431,7 +431,10 @@ int tx_qk_norm_rotary_bwd(tx_ctx *ctx, const float *d_q, const float *d_k, const
  * The forward writes out [batch, queries, heads, vdim] and, for a backward,
  * out2 (the second map's own output, same shape) and lse [batch, 2 * heads,
  * queries] (log2 of each row's sum of exponentials; +inf where no key is
- * seen); both NULL without one.  The backward reads out, out2, lse and dout
+ * seen); both NULL without one.  `saved`, tx_diff_attention_saved_bytes long
+ * and 16-byte aligned, may carry the operands as the tensor cores read them
+ * from the forward to the backward (as large as q, k and v); NULL, or 0 bytes:
+ * the backward makes them again.  The backward reads out, out2, lse and dout
  * and writes dq (unless NULL), dk and dv (unless both NULL) and dlam (unless
  * NULL), sums in a fixed order.  fp32-class results in every math mode.
  * The reference has softmax attention as composed nodes only
@@ -444,9 +447,11 @@ typedef struct tx_diff_attention {
   int32_t causal;
   int64_t query_start;
   float *out, *out2, *lse;
+  void *saved;
   const float *dout;
   float *dq, *dk, *dv, *dlam;
 } tx_diff_attention;
+int tx_diff_attention_saved_bytes(tx_ctx *ctx, const tx_diff_attention *desc, int64_t *bytes);
 int tx_diff_attention_fwd(tx_ctx *ctx, const tx_diff_attention *desc);
 int tx_diff_attention_bwd(tx_ctx *ctx, const tx_diff_attention *desc);
 

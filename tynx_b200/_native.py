@@ -115,7 +115,8 @@ class DiffAttentionDesc(C.Structure):
         ("q", C.c_void_p), ("k", C.c_void_p), ("v", C.c_void_p), ("lam", C.c_void_p),
         ("key_lengths", C.c_void_p), ("scale", C.c_float), ("causal", C.c_int32),
         ("query_start", C.c_int64),
-        ("out", C.c_void_p), ("out2", C.c_void_p), ("lse", C.c_void_p), ("dout", C.c_void_p),
+        ("out", C.c_void_p), ("out2", C.c_void_p), ("lse", C.c_void_p), ("saved", C.c_void_p),
+        ("dout", C.c_void_p),
         ("dq", C.c_void_p), ("dk", C.c_void_p), ("dv", C.c_void_p), ("dlam", C.c_void_p),
     ]
 
@@ -194,6 +195,7 @@ SIGNATURES = {
                               C.POINTER(RotaryDesc), _f],
     "tx_qk_norm_rotary_bwd": [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64,
                               _i64, _vp, _i64, C.POINTER(RotaryDesc), _f],
+    "tx_diff_attention_saved_bytes": [_vp, C.POINTER(DiffAttentionDesc), _p64],
     "tx_diff_attention_fwd": [_vp, C.POINTER(DiffAttentionDesc)],
     "tx_diff_attention_bwd": [_vp, C.POINTER(DiffAttentionDesc)],
     "tx_ppo_loss_fwd": [_vp, _vp, _i64, _i64, _vp, _vp, _vp, _vp, _vp, _f, _f, _f, _vp],

@@ -32,6 +32,7 @@ struct SplitJobs {
   // stats, beside lse, and each tile's sum of D2 to sums
   const float *out, *out2, *lse;
   float *stats, *sums;
+  int first;  // the first job to do
 };
 constexpr int kSplitThreads = 512, kSplitWarps = kSplitThreads / 32;
 template <int W, bool STATS>
@@ -171,11 +172,12 @@ template <int W>
 __global__ void __launch_bounds__(kSplitThreads, 2)
     k_diff_split(const __grid_constant__ Shape s, const __grid_constant__ SplitJobs jobs) {
   __shared__ uint32_t red[3 * kSplitWarps];
-  const SplitJob &J = jobs.j[blockIdx.z];
+  const int job = jobs.first + blockIdx.z;
+  const SplitJob &J = jobs.j[job];
   if ((int64_t)blockIdx.x >= s.B * J.heads * J.tiles) return;
-  if (blockIdx.z == 3)
+  if (job == 3)
     split_tile<W, true>(s, jobs, J, red);
-  else if (blockIdx.z < 2)
+  else if (job < 2)
     split_tile<64, false>(s, jobs, J, red);
   else
     split_tile<W, false>(s, jobs, J, red);
@@ -446,51 +448,58 @@ __global__ void __launch_bounds__(32) k_diff_dlam(const __grid_constant__ Shape 
 }
 
 // ---- host ----------------------------------------------------------------------------------
-// The split operands of one call and their memory.
+// The split operands of one call: q, k and v in `saved` or in memory of the call, the output's gradient
+// in memory of the call.
 struct Operands {
-  Split x;
-  Scratch data;
-  int64_t tq = 0, tk = 0, tv = 0, tg = 0;  // tiles
-  static int width(const Shape &s) { return s.dv <= 64 ? 64 : 128; }
-  static size_t total(const Shape &s, bool gradient) {
-    const int64_t w = width(s), qt = (s.T + kRows - 1) / kRows, kt = (s.S + kRows - 1) / kRows;
-    const int64_t halves = 2 * (s.B * 2 * s.H * s.T * 64 + s.B * 2 * s.Hk * s.S * 64 + s.B * s.Hk * s.S * w +
-                                (gradient ? s.B * s.H * s.T * w : 0));
-    return (size_t)halves * 2 + (size_t)(s.B * (2 * s.H * qt + 2 * s.Hk * kt + 2 * s.Hk * kt + 2 * s.H * qt)) * 4;
+  Split x{};
+  Scratch own, grad;
+  int64_t tq, tk, tv, tg;  // tiles
+  bool ok;
+  static int64_t width(const Shape &s) { return s.dv <= 64 ? 64 : 128; }
+  static int64_t tiles(int64_t rows) { return (rows + kRows - 1) / kRows; }
+  static size_t bytes(const Shape &s) {
+    const int64_t halves = 2 * (s.B * 2 * s.H * s.T * 64 + s.B * 2 * s.Hk * s.S * 64 + s.B * s.Hk * s.S * width(s));
+    return (size_t)halves * 2 + (size_t)(s.B * (2 * s.H * tiles(s.T) + 4 * s.Hk * tiles(s.S))) * 4;
   }
-  Operands(tx_ctx *ctx, const Shape &s, bool gradient) : data(ctx, total(s, gradient)) {
-    if (!data.ptr) return;
-    const int64_t w = width(s), qt = (s.T + kRows - 1) / kRows, kt = (s.S + kRows - 1) / kRows;
+  static size_t grad_bytes(const Shape &s) {
+    return (size_t)(s.B * s.H * s.T * 2 * width(s)) * 2 + (size_t)(2 * s.B * s.H * tiles(s.T)) * 4;
+  }
+  Operands(tx_ctx *ctx, const Shape &s, void *saved, bool gradient)
+      : own(ctx, saved ? 0 : bytes(s)), grad(ctx, gradient ? grad_bytes(s) : 0) {
+    const int64_t w = width(s);
     x.vw = (int)w;
-    x.qt = qt;
-    x.kt = kt;
-    tq = s.B * 2 * s.H * qt, tk = s.B * 2 * s.Hk * kt, tv = s.B * s.Hk * kt, tg = s.B * s.H * qt;
-    __half *p = data.as<__half>();
+    x.qt = tiles(s.T);
+    x.kt = tiles(s.S);
+    tq = s.B * 2 * s.H * x.qt, tk = s.B * 2 * s.Hk * x.kt, tv = s.B * s.Hk * x.kt, tg = s.B * s.H * x.qt;
+    ok = (saved || own.ptr) && (!gradient || grad.ptr);
+    if (!ok) return;
+    __half *p = reinterpret_cast<__half *>(saved ? saved : own.ptr);
     x.q = p, p += s.B * 2 * s.H * s.T * 128;
     x.k = p, p += s.B * 2 * s.Hk * s.S * 128;
     x.v = p, p += s.B * s.Hk * s.S * 2 * w;
-    x.g = p, p += gradient ? s.B * s.H * s.T * 2 * w : 0;
     float *f = reinterpret_cast<float *>(p);
     x.fq = f, f += tq;
     x.fk = f, f += tk;
     x.fv = f, f += tv;
-    x.nv = f, f += tv;
-    x.fg = f, f += tg;
-    x.ng = f;
+    x.nv = f;
+    if (!gradient) return;
+    x.g = grad.as<__half>();
+    x.fg = reinterpret_cast<float *>(x.g + s.B * s.H * s.T * 2 * w);
+    x.ng = x.fg + tg;
   }
-  // p: the backward's description, or null
-  int fill(tx_ctx *ctx, const Shape &s, const tx_diff_attention *p, float *stats, float *sums) {
-    if (!data.ptr) return TX_ERR_OOM;
-    const float *dout = p ? p->dout : nullptr;
-    auto w = [](const float *p) { return const_cast<float *>(p); };
+  // made: q, k and v are there.  p: the backward's description, or null
+  int fill(tx_ctx *ctx, const Shape &s, bool made, const tx_diff_attention *p, float *stats, float *sums) {
+    if (!ok) return TX_ERR_OOM;
+    
     SplitJobs jobs{};
-    jobs.j[0] = SplitJob{s.q, x.q, w(x.fq), nullptr, s.T, x.qt, 2 * s.H, s.d, s.scale * kLog2e, 0};
-    jobs.j[1] = SplitJob{s.k, x.k, w(x.fk), nullptr, s.S, x.kt, 2 * s.Hk, s.d, 1.0f, 1};
-    jobs.j[2] = SplitJob{s.v, x.v, w(x.fv), w(x.nv), s.S, x.kt, s.Hk, s.dv, 1.0f, 1};
-    jobs.j[3] = SplitJob{dout, x.g, w(x.fg), w(x.ng), s.T, x.qt, s.H, s.dv, 1.0f, 0};
+    jobs.j[0] = SplitJob{s.q, x.q, x.fq, nullptr, s.T, x.qt, 2 * s.H, s.d, s.scale * kLog2e, 0};
+    jobs.j[1] = SplitJob{s.k, x.k, x.fk, nullptr, s.S, x.kt, 2 * s.Hk, s.d, 1.0f, 1};
+    jobs.j[2] = SplitJob{s.v, x.v, x.fv, x.nv, s.S, x.kt, s.Hk, s.dv, 1.0f, 1};
+    jobs.j[3] = SplitJob{p ? p->dout : nullptr, x.g, x.fg, x.ng, s.T, x.qt, s.H, s.dv, 1.0f, 0};
+    jobs.first = made ? 3 : 0;
     if (p) jobs.out = p->out, jobs.out2 = p->out2, jobs.lse = p->lse, jobs.stats = stats, jobs.sums = sums;
-    const int64_t blocks = tq > tk ? tq : tk;
-    const dim3 grid((unsigned)blocks, 1, p ? 4 : 3);
+    const int64_t blocks = made ? tg : tq > tk ? tq : tk;
+    const dim3 grid((unsigned)blocks, 1, made ? 1 : p ? 4 : 3);
     if (x.vw == 64)
       k_diff_split<64><<<grid, kSplitThreads, 0, ctx->stream>>>(s, jobs);
     else
@@ -499,6 +508,9 @@ struct Operands {
     return TX_OK;
   }
 };
+
+// Calls of so few queries take k_diff_rows.
+bool few_queries(const Shape &s) { return s.T * s.G <= 8; }
 
 int check_desc(tx_ctx *ctx, const tx_diff_attention *p, Shape &s) {
   if (!p) return tx_fail(ctx, TX_ERR_INVALID, "differential attention: no description");
@@ -583,10 +595,19 @@ bool split_map(CUtensorMap *m, const __half *base, int w, int64_t rows, int64_t 
 
 using namespace tx_diff;
 
+extern "C" int tx_diff_attention_saved_bytes(tx_ctx *ctx, const tx_diff_attention *p, int64_t *bytes) {
+  if (!ctx || !bytes) return TX_ERR_INVALID;
+  Shape s;
+  TX_TRY(check_desc(ctx, p, s));
+  *bytes = few_queries(s) || s.B * s.T * s.S == 0 ? 0 : (int64_t)Operands::bytes(s);
+  return TX_OK;
+}
+
 extern "C" int tx_diff_attention_fwd(tx_ctx *ctx, const tx_diff_attention *p) {
   if (!ctx) return TX_ERR_INVALID;
   Shape s;
   TX_TRY(check_desc(ctx, p, s));
+  if ((uintptr_t)p->saved & 15) return tx_fail(ctx, TX_ERR_INVALID, "differential attention: saved is not aligned");
   if ((p->out2 == nullptr) != (p->lse == nullptr))
     return tx_fail(ctx, TX_ERR_INVALID, "differential attention: out2 and lse come together");
   if (s.B * s.T == 0) return TX_OK;
@@ -603,9 +624,9 @@ extern "C" int tx_diff_attention_fwd(tx_ctx *ctx, const tx_diff_attention *p) {
   if (s.T * s.G <= 1) return launch_rows<1>(ctx, s, p->out, p->out2, p->lse);
   if (s.T * s.G <= 2) return launch_rows<2>(ctx, s, p->out, p->out2, p->lse);
   if (s.T * s.G <= 4) return launch_rows<4>(ctx, s, p->out, p->out2, p->lse);
-  if (s.T * s.G <= 8) return launch_rows<8>(ctx, s, p->out, p->out2, p->lse);
-  Operands x(ctx, s, false);
-  TX_TRY(x.fill(ctx, s, nullptr, nullptr, nullptr));
+  if (few_queries(s)) return launch_rows<8>(ctx, s, p->out, p->out2, p->lse);
+  Operands x(ctx, s, p->saved, false);
+  TX_TRY(x.fill(ctx, s, false, nullptr, nullptr, nullptr));
   const int splits = tc_forward_splits(ctx, s);
   if (splits == 1) return tc_forward(ctx, s, x.x, p->out, p->out2, p->lse, Parts{nullptr, nullptr, 1});
   PartMemory mem(ctx, s, splits);
@@ -618,6 +639,7 @@ extern "C" int tx_diff_attention_bwd(tx_ctx *ctx, const tx_diff_attention *p) {
   if (!ctx) return TX_ERR_INVALID;
   Shape s;
   TX_TRY(check_desc(ctx, p, s));
+  if ((uintptr_t)p->saved & 15) return tx_fail(ctx, TX_ERR_INVALID, "differential attention: saved is not aligned");
   if ((p->dk == nullptr) != (p->dv == nullptr))
     return tx_fail(ctx, TX_ERR_INVALID, "differential attention: dk and dv come together");
   const int64_t rows = s.B * s.T * s.H;
@@ -635,10 +657,11 @@ extern "C" int tx_diff_attention_bwd(tx_ctx *ctx, const tx_diff_attention *p) {
     return TX_OK;
   }
   Scratch stats(ctx, (size_t)(s.B * s.H * ((s.T + 63) / 64)) * 256 * 4);
-  Operands x(ctx, s, true);
+  const bool made = p->saved && !few_queries(s);
+  Operands x(ctx, s, made ? p->saved : nullptr, true);
   Scratch sums(ctx, (size_t)x.tg * 4);
   if (!stats.ptr || !sums.ptr) return TX_ERR_OOM;
-  TX_TRY(x.fill(ctx, s, p, stats.as<float>(), sums.as<float>()));
+  TX_TRY(x.fill(ctx, s, made, p, stats.as<float>(), sums.as<float>()));
   if (p->dq || p->dk) return tc_backward(ctx, s, x.x, stats.as<float>(), sums.as<float>(), p->dq, p->dk, p->dv, p->dlam);
   if (p->dlam) {
     k_diff_dlam<<<(unsigned)s.H, 32, 0, ctx->stream>>>(s, sums.as<float>(), x.x.qt, p->dlam);

@@ -96,8 +96,8 @@ __device__ __forceinline__ void report_length(const Shape &s, int64_t b) {
 constexpr int kRows = 128;  // rows of a tile
 struct Split {
   __half *q, *k, *v, *g;         // [b][map or head][row][2 W]; g: the output's gradient
-  const float *fq, *fk, *fv, *fg;  // f of each [b][map or head][tile]
-  const float *nv, *ng;          // the largest 2-norm of a tile's rows
+  float *fq, *fk, *fv, *fg;      // f of each [b][map or head][tile]
+  float *nv, *ng;                // the largest 2-norm of a tile's rows
   int vw;                        // W of v and g
   int64_t qt, kt;                // tiles of a head's queries and keys
 };

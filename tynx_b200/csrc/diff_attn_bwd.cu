@@ -50,6 +50,7 @@ struct Grads {
   float *dq, *dk, *dv, *dlam;
   // blocks of one tile level: K, Q and V; in turn level by level, or kind after kind
   unsigned nk, nq, levels, by_level, kt, qt;
+  int each_head;  // K and V blocks of one query head each, dk and dv for every query head
 };
 // the block's kind and its index within it
 __device__ __forceinline__ int block_kind(const Grads &o, unsigned i, unsigned &block) {
@@ -92,11 +93,12 @@ __device__ __forceinline__ void body(const Shape &s, const Split &x, const CUten
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
 
   // keys: the first tiles are seen by most queries; queries: the last tiles see most keys
-  const int heads = KEYS ? s.Hk : s.H;
+  const bool each = KEYS && o.each_head;
+  const int heads = KEYS && !each ? s.Hk : s.H;
   const int64_t rheads = s.B * heads, rtiles = KEYS ? x.kt : x.qt;
   const int64_t rt = KEYS ? block / rheads : rtiles - 1 - block / rheads;
   const int64_t bh = block % rheads, b = bh / heads;
-  const int rh = (int)(bh - b * heads), hk = KEYS ? rh : rh / s.G;
+  const int rh = (int)(bh - b * heads), hk = KEYS && !each ? rh : rh / s.G;
   const int64_t r0 = rt * 128, n = s.length(b);
   const int64_t q_steps = (s.T + kStep - 1) / kStep;
   int first = 0, per_head;  // steps of each head, keys: from step `first` on
@@ -109,7 +111,7 @@ __device__ __forceinline__ void body(const Shape &s, const Split &x, const CUten
     const int64_t last = r0 + 127 < s.T ? r0 + 127 : s.T - 1;
     per_head = (int)((s.seen(last, n) + kStep - 1) / kStep);
   }
-  const int steps = __shfl_sync(0xffffffffu, KEYS ? per_head * s.G : per_head, 0);
+  const int steps = __shfl_sync(0xffffffffu, KEYS && !each ? per_head * s.G : per_head, 0);
 
   if (threadIdx.x == 0) {
     bar_init(r_full, 1);
@@ -144,7 +146,7 @@ __device__ __forceinline__ void body(const Shape &s, const Split &x, const CUten
   }
 
   // step i: head, first streamed row
-  auto head_of = [&](int i) { return KEYS ? hk * s.G + i / per_head : rh; };
+  auto head_of = [&](int i) { return KEYS && !each ? hk * s.G + i / per_head : rh; };
   auto step_of = [&](int i) { return KEYS ? first + i % per_head : i; };
 
   if (warp < 4) {
@@ -472,6 +474,40 @@ __global__ void __launch_bounds__(kThreads, 1)
     body<DV, kModeV>(s, x, mq, mk, mv, mg, o, sm, block);
 }
 
+// dst[row][hk][w] = sum over the heads g of a group of src[row][hk G + g][w], for dk and dv in turn
+struct GroupSum {
+  const float *src[2];
+  float *dst[2];
+  int w[2];
+};
+__global__ void __launch_bounds__(256) k_diff_group_sum(const __grid_constant__ GroupSum j, int64_t heads, int G) {
+  const int which = blockIdx.y, w = j.w[which];
+  const int64_t n = heads * w;
+  const bool four = (w & 3) == 0 && ((uintptr_t)j.dst[which] & 15) == 0;
+  const int64_t step = (int64_t)gridDim.x * 256, first = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (four) {
+    const int w4 = w >> 2;
+    for (int64_t i = first; i < n >> 2; i += step) {
+      const int64_t head = i / w4;
+      const float4 *p = reinterpret_cast<const float4 *>(j.src[which]) + head * G * w4 + (i - head * w4);
+      float4 v = __ldg(p);
+      for (int g = 1; g < G; ++g) {
+        const float4 y = __ldg(p + (int64_t)g * w4);
+        v = make_float4(v.x + y.x, v.y + y.y, v.z + y.z, v.w + y.w);
+      }
+      reinterpret_cast<float4 *>(j.dst[which])[i] = v;
+    }
+  } else {
+    for (int64_t i = first; i < n; i += step) {
+      const int64_t head = i / w;
+      const float *p = j.src[which] + head * G * w + (i - head * w);
+      float v = __ldg(p);
+      for (int g = 1; g < G; ++g) v += __ldg(p + (int64_t)g * w);
+      j.dst[which][i] = v;
+    }
+  }
+}
+
 template <int DV>
 int launch(tx_ctx *ctx, const Shape &s, const Split &x, const float *stats, const float *sums, float *dq, float *dk,
            float *dv, float *dlam) {
@@ -479,16 +515,37 @@ int launch(tx_ctx *ctx, const Shape &s, const Split &x, const float *stats, cons
   if (!split_map(&mq, x.q, 64, s.T, s.B * 2 * s.H) || !split_map(&mk, x.k, 64, s.S, s.B * 2 * s.Hk) ||
       !split_map(&mv, x.v, DV, s.S, s.B * s.Hk) || !split_map(&mg, x.g, DV, s.T, s.B * s.H))
     return tx_fail(ctx, TX_ERR_UNSUPPORTED, "differential attention: tensor map");
-  const unsigned nk = dk ? (unsigned)(s.B * s.Hk) : 0, nq = dq ? (unsigned)(s.B * s.H) : 0;
+  // A key block that runs over all heads of a group may outlast everything else: then each head has
+  // blocks and sums of its own, added up afterwards (5 x 413, 3 heads over 1: 27 + 2.5 us for 64).  Where
+  // the whole fills the SMs longer anyway it would cost: 2 x 2048 causal, 8 heads over 4: 276 + 10 us for
+  // 263.  Lengths in steps; a V block's step counts half.
+  const double q_steps = (double)((s.T + kStep - 1) / kStep), k_steps = (double)((s.S + kStep - 1) / kStep);
+  const double work = (s.causal ? 0.5 : 1.0) * (double)(s.B * s.H) *
+                      ((dk ? 1.5 * (double)x.kt * q_steps : 0.0) + (dq ? (double)x.qt * k_steps : 0.0));
+  const bool each = dk && s.G > 1 && (double)s.G * q_steps > work / ctx->num_sms;
+  const size_t rows = (size_t)(s.B * s.S * s.H);
+  Scratch part(ctx, each ? rows * (size_t)(2 * s.d + s.dv) * 4 : 0);
+  if (each && !part.ptr) return TX_ERR_OOM;
+  // dv's part first, whole 16-byte groups either way
+  float *pv = part.as<float>(), *pk = each ? pv + rows * s.dv : nullptr;
+  if (each && ((rows * s.dv) & 3)) pk = pv, pv = pk + rows * 2 * s.d;
+  const unsigned nk = dk ? (unsigned)(s.B * (each ? s.H : s.Hk)) : 0, nq = dq ? (unsigned)(s.B * s.H) : 0;
   // Blocks start in order, so the longest come first.  Causal tiles get shorter from level to level:
   // the kinds take turns, and the last blocks are the shortest of each.  Otherwise K and Q blocks are
   // alike and V blocks half as long, so V comes last.
   const unsigned kt = (unsigned)x.kt, qt = (unsigned)x.qt;
-  const Grads o{stats, sums, dq, dk, dv, dlam, nk, nq, kt < qt ? kt : qt, (unsigned)(s.causal && nk && nq), kt, qt};
+  const Grads o{stats, sums, dq, each ? pk : dk, each ? pv : dv, dlam, nk, nq, kt < qt ? kt : qt,
+                (unsigned)(s.causal && nk && nq), kt, qt, each};
   static SmemGrant granted;
   TX_TRY(granted.take(ctx, (const void *)k_diff_bwd<DV>, Cfg<DV>::SMEM));
   k_diff_bwd<DV><<<2 * nk * kt + nq * qt, kThreads, Cfg<DV>::SMEM, ctx->stream>>>(s, x, mq, mk, mv, mg, o);
   TX_LAUNCHED(ctx, "k_diff_bwd");
+  if (each) {
+    const GroupSum j{{pk, pv}, {dk, dv}, {2 * s.d, s.dv}};
+    const int64_t n = s.B * s.S * s.Hk * (2 * s.d > s.dv ? 2 * s.d : s.dv);
+    k_diff_group_sum<<<dim3(grid_for(n / 4, 256), 2), 256, 0, ctx->stream>>>(j, s.B * s.S * s.Hk, s.G);
+    TX_LAUNCHED(ctx, "k_diff_group_sum");
+  }
   return TX_OK;
 }
 

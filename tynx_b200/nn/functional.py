@@ -230,7 +230,11 @@ def differential_attention(q: Tensor, k: Tensor, v: Tensor, lam: Tensor, *, scal
     query among the keys; None: ``keys - queries``, so that the last query sees
     every key).  Keys and values behind a sequence's length are never read, within
     it they must be finite; a query that sees no key returns zeros.  A length
-    outside [0, keys] raises IndexError at the next synchronisation."""
+    outside [0, keys] raises IndexError at the next synchronisation.
+
+    When a gradient is wanted, the output's second term, a number a query and map,
+    and the operands in the form the tensor cores read (as large as q, k and v)
+    are kept until the backward."""
     name = "differential_attention"
     batch, queries, maps, d = _heads(name, "q", q, q, "2 * heads")
     _, keys, kv_maps, _ = _heads(name, "k", k, q, "2 * kv_heads")
@@ -270,10 +274,14 @@ def differential_attention(q: Tensor, k: Tensor, v: Tensor, lam: Tensor, *, scal
         out2 = Tensor._empty(out.shape, "float32", ctx)
         lse = Tensor._empty((batch, maps, queries), "float32", ctx)
         desc.out2, desc.lse = out2.ptr, lse.ptr
+        size = C.c_int64()
+        ctx.check(lib.tx_diff_attention_saved_bytes(ctx.handle, desc, C.byref(size)), name)
+        saved = Tensor._empty((size.value // 8 + 1,), "int64", ctx) if size.value else None
+        desc.saved = saved.ptr if saved is not None else None
     ctx.check(lib.tx_diff_attention_fwd(ctx.handle, desc), name)
     if grad:
         # detached views keep what the description points to alive until this node is freed
-        held = [t.detach() for t in (q, k, v, lam, out)] + [out2, lse, key_lengths]
+        held = [t.detach() for t in (q, k, v, lam, out)] + [out2, lse, saved, key_lengths]
         want = [t.requires_grad for t in (q, k, v, lam)]
 
         def backward(g):
