@@ -15,6 +15,7 @@ that created them, like Tynx tensors (``crates/tynx-python/src/tensor.rs:54-92``
 from __future__ import annotations
 
 import ctypes as C
+import math
 import os
 import threading
 from contextlib import contextmanager
@@ -226,10 +227,7 @@ def _shape_tuple(shape) -> tuple:
 
 
 def _numel(shape) -> int:
-    n = 1
-    for s in shape:
-        n *= s
-    return n
+    return math.prod(shape)
 
 
 def _contig_strides(shape) -> list[int]:
@@ -295,7 +293,11 @@ class Fn:
 
 
 def _needs_grad(*tensors) -> bool:
-    return is_grad_enabled() and any(isinstance(t, Tensor) and t.requires_grad for t in tensors)
+    if is_grad_enabled():
+        for t in tensors:
+            if isinstance(t, Tensor) and t.requires_grad:
+                return True
+    return False
 
 
 _export = None  # interop.export, once it is needed
@@ -351,7 +353,10 @@ class Tensor:
         ctx = ctx or context()
         shape = _shape_tuple(shape)
         t = object.__new__(cls)
-        t._init(Storage(ctx, _numel(shape) * _DTYPES[dtype][1]), 0, shape, dtype)
+        t._storage, t._offset, t.shape, t.dtype = Storage(ctx, _numel(shape) * _DTYPES[dtype][1]), 0, shape, dtype
+        t.requires_grad = False
+        t._grad = t._fn = None
+        t._out_index = 0
         return t
 
     def detach(self) -> "Tensor":
