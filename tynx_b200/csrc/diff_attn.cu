@@ -234,7 +234,7 @@ __global__ void __launch_bounds__(kRowThreads, 2)
   constexpr int COPY = 16 / NV;                  // lanes that hold the same one
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, m = lane >> 4, l16 = lane & 15;
   const int b = blockIdx.y / s.Hk, hk = blockIdx.y - b * s.Hk;
-  const int n_items = (int)(s.T * s.G), item0 = blockIdx.z * RP;  // at most eight: launch_rows
+  const int n_items = (int)(s.T * s.G), item0 = blockIdx.z * RP;  // few_queries()
   const int64_t n = s.length(b);
   if (threadIdx.x == 0 && hk == 0 && blockIdx.x == 0 && blockIdx.z == 0) report_length(s, b);
   const int last = item0 + RP <= n_items ? item0 + RP - 1 : n_items - 1;
@@ -509,8 +509,10 @@ struct Operands {
   }
 };
 
-// Calls of so few queries take k_diff_rows.
-bool few_queries(const Shape &s) { return s.T * s.G <= 8; }
+// Calls of so few queries take k_diff_rows, which reads keys and values once for every eight of them
+// and needs no split operands (8 x 8192 keys of 4 heads: 24 queries 276 us, on the tensor cores 298; 32
+// queries 409 and 312; 4096 keys of 2 heads: 26 and 31).
+bool few_queries(const Shape &s) { return s.T * s.G <= 24; }
 
 int check_desc(tx_ctx *ctx, const tx_diff_attention *p, Shape &s) {
   if (!p) return tx_fail(ctx, TX_ERR_INVALID, "differential attention: no description");

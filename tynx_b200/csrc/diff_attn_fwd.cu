@@ -18,6 +18,9 @@
 // the 24 products of one tile 1e-7.  Shared memory: Q of both maps (64 KB), one
 // key tile of both (64 KB, each map's half refilled as soon as its S is done),
 // and a ring of three half value tiles (96 KB).
+// One CTA an SM takes (query tile, head) after (query tile, head): while its
+// warps store one's rows (through the value ring, so that whole lines go out),
+// the next one's Q and K arrive and its first scores are multiplied.
 #include "diff_attn.cuh"
 
 namespace tx_diff {
@@ -34,8 +37,9 @@ struct Cfg {
   static constexpr int RING = 3;
   static constexpr int SMEM = 4 * QK + RING * VSLOT + 512 /*barriers*/ + 2048 /*row exchange*/;
   static_assert(SMEM <= 232448, "shared memory of an SM");
-  // at the end both maps' outputs pass through Q's and K's memory
-  static_assert(2 * 128 * DV * 4 <= 4 * QK, "output staging");
+  // output rows pass through the value ring: 32 rows x CW columns a warp at a time
+  static constexpr int CW = DV == 128 ? 32 : 16;
+  static_assert(16 * 32 * CW * 4 <= RING * VSLOT, "output staging");
 };
 
 struct Out {
@@ -44,11 +48,6 @@ struct Out {
   int per;  // tiles of a range of keys
 };
 
-// 16-byte chunk c of a staged output row: rows a warp writes together spread over the banks
-template <int DV>
-__device__ __forceinline__ float4 *staged(uint8_t *sm, int m, int r, int c) {
-  return reinterpret_cast<float4 *>(sm) + m * (128 * DV / 4) + r * (DV / 4) + (c ^ (r & 7));
-}
 __device__ __forceinline__ void store4(float *dst, int c, float4 v, int dv, bool four) {
   if (four) {
     if (c < dv) *reinterpret_cast<float4 *>(dst + c) = v;
@@ -58,6 +57,37 @@ __device__ __forceinline__ void store4(float *dst, int c, float4 v, int dv, bool
     if (c + 2 < dv) dst[c + 2] = v.z;
     if (c + 3 < dv) dst[c + 3] = v.w;
   }
+}
+
+// One unit of work: a query tile of a head, and a range of its keys.
+struct Item {
+  int b, t0, n;  // sequence, first query, valid keys
+  int h, hk, qt, split, tile0, tiles;
+};
+// Item `at` in the order of work: causal, the queries with most keys first.
+__device__ __forceinline__ Item item_at(const Shape &s, const Split &x, const Out &o, unsigned at) {
+  const unsigned heads = (unsigned)(s.B * s.H), blocks = (unsigned)x.qt * heads;
+  Item w;
+  w.split = at / blocks;
+  at -= w.split * blocks;
+  const unsigned level = at / heads, bh = at - level * heads;
+  w.qt = (int)x.qt - 1 - (int)level;
+  w.b = bh / s.H;
+  w.h = bh - w.b * s.H;
+  w.hk = w.h / s.G;
+  w.t0 = w.qt * 128;
+  const int tl = w.t0 + 127 < (int)s.T ? w.t0 + 127 : (int)s.T - 1;
+  w.n = (int)s.length(w.b);
+  w.tile0 = w.split * o.per;
+  const int all = ((int)s.seen(tl, w.n) + 127) / 128;
+  w.tiles = all <= w.tile0 ? 0 : all - w.tile0 < o.per ? all - w.tile0 : o.per;
+  return w;
+}
+// The item of this CTA's round r: rounds run forth and back, so that a CTA's share of a falling order is
+// even.  False: none, in the last round.
+__device__ __forceinline__ bool item_of_round(unsigned items, int r, unsigned &at) {
+  at = r * gridDim.x + (r & 1 ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
+  return at < items;
 }
 
 template <int DV>
@@ -73,26 +103,18 @@ __global__ void __launch_bounds__(kThreads, 1)
   const uint32_t sq = su32(sm), sk = sq + 2 * C::QK, sv = sk + 2 * C::QK;
   uint64_t *bars = reinterpret_cast<uint64_t *>(sm + 4 * C::QK + C::RING * C::VSLOT);
   uint64_t *q_full = bars, *k_full = bars + 1, *k_empty = bars + 3, *v_full = bars + 5, *v_empty = bars + 8,
-           *s_full = bars + 11, *p_full = bars + 13, *o_full = bars + 15;  // o_full: of each map's tile
-  uint64_t *all_done = bars + 17;
-  uint32_t *tmem_holder = reinterpret_cast<uint32_t *>(bars + 18);
+           *s_full = bars + 11, *p_full = bars + 13, *o_full = bars + 15, *q_empty = bars + 17, *staged = bars + 18,
+           *all_done = bars + 19;
+  uint32_t *tmem_holder = reinterpret_cast<uint32_t *>(bars + 20);
   volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_holder + 1);
   float *swap = reinterpret_cast<float *>(bars + 64);  // [map][half][row]
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
-
-  // causal: the queries with most keys first
-  const int64_t heads = s.B * s.H;
-  const int split = blockIdx.y;
-  const int64_t qt = x.qt - 1 - (int64_t)blockIdx.x / heads, bh = (int64_t)blockIdx.x % heads;
-  const int64_t b = bh / s.H;
-  const int h = (int)(bh - b * s.H), hk = h / s.G;
-  const int64_t t0 = qt * 128, tl = t0 + 127 < s.T ? t0 + 127 : s.T - 1;
-  const int64_t n = s.length(b);
-  const int tile0 = split * o.per, all = (int)((s.seen(tl, n) + 127) / 128);  // this range's tiles
-  const int tiles = __shfl_sync(0xffffffffu, all <= tile0 ? 0 : all - tile0 < o.per ? all - tile0 : o.per, 0);
+  const unsigned items = (unsigned)(x.qt * s.B * s.H * o.parts.splits);
+  const int rounds = (int)((items + gridDim.x - 1) / gridDim.x);
 
   if (threadIdx.x == 0) {
     bar_init(q_full, 1);
+    bar_init(q_empty, 1);
     for (int m = 0; m < 2; ++m) {
       bar_init(k_full + m, 1);
       bar_init(k_empty + m, 1);
@@ -104,10 +126,10 @@ __global__ void __launch_bounds__(kThreads, 1)
       bar_init(v_full + i, 1);
       bar_init(v_empty + i, 1);
     }
+    bar_init(staged, 512);
     bar_init(all_done, 1);
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-    if (h == 0 && qt == 0 && split == 0) report_length(s, b);
   }
   if (warp == 1) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(su32(tmem_holder)),
@@ -121,90 +143,118 @@ __global__ void __launch_bounds__(kThreads, 1)
 
   if (warp < 4) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
-    if (warp == 0 && lane == 0 && tiles) {
-      bar_expect(q_full, 2 * C::QK);
-      for (int m = 0; m < 2; ++m)
-        for (int p = 0; p < 4; ++p)  // (head or tail, 64-row half)
-          tma_3d(sq + m * C::QK + p * C::VBLK, &mq, q_full, (p >> 1) * 64, (int)t0 + (p & 1) * 64,
-                 (int)(b * 2 * s.H + 2 * h + m));
+    if (warp == 0 && lane == 0) {
       bool ok = true;
-      int loaded_k = 0, loaded_v = 0;
-      for (int i = 0; i < tiles && ok; ++i) {
-        for (int m = 0; m < 2 && ok; ++m) {
-          if (i) ok = bar_wait(k_empty + m, (i - 1) & 1, abort_flag, s.err, 1);
+      int nq = 0, ni = 0;                // items with keys so far, items so far
+      int nk = 0, loaded_k = 0, nv = 0;  // tiles of a map so far, loads of both maps, half value tiles
+      for (int r = 0; r < rounds && ok; ++r) {
+        unsigned at;
+        if (!item_of_round(items, r, at)) continue;
+        const Item w = item_at(s, x, o, at);
+        if (w.tiles) {
+          if (nq) ok = bar_wait(q_empty, (nq - 1) & 1, abort_flag, s.err, 1);
           if (!ok) break;
-          bar_expect(k_full + m, C::QK);
-          for (int p = 0; p < 4; ++p)
-            tma_3d(sk + m * C::QK + p * C::VBLK, &mk, k_full + m, (p >> 1) * 64, (tile0 + i) * 128 + (p & 1) * 64,
-                   (int)(b * 2 * s.Hk + 2 * hk + m));
-          ++loaded_k;
+          bar_expect(q_full, 2 * C::QK);
+          for (int p = 0; p < 8; ++p)  // (map, head or tail, 64-row half)
+            tma_3d(sq + p * C::VBLK, &mq, q_full, (p >> 1 & 1) * 64, w.t0 + (p & 1) * 64,
+                   w.b * 2 * s.H + 2 * w.h + (p >> 2));
+          ++nq;
+        } else if (ni) {  // no phase is passed over: parities would repeat
+          ok = bar_wait(staged, (ni - 1) & 1, abort_flag, s.err, 3);
         }
-        for (int hf = 0; hf < 2 && ok; ++hf) {
-          const int u = 2 * i + hf, slot = u % C::RING, use = u / C::RING;
-          if (use) ok = bar_wait(v_empty + slot, (use - 1) & 1, abort_flag, s.err, 2);
-          if (!ok) break;
-          bar_expect(v_full + slot, C::VSLOT);
-          for (int p = 0; p < 2 * (DV / 64); ++p)
-            tma_3d(sv + slot * C::VSLOT + p * C::VBLK, &mv, v_full + slot, p * 64, (tile0 + i) * 128 + hf * 64,
-                   (int)(b * s.Hk + hk));
-          ++loaded_v;
+        for (int i = 0; i < w.tiles && ok; ++i, ++nk) {
+          for (int m = 0; m < 2 && ok; ++m) {
+            if (nk) ok = bar_wait(k_empty + m, (nk - 1) & 1, abort_flag, s.err, 2);
+            if (!ok) break;
+            bar_expect(k_full + m, C::QK);
+            for (int p = 0; p < 4; ++p)
+              tma_3d(sk + m * C::QK + p * C::VBLK, &mk, k_full + m, (p >> 1) * 64, (w.tile0 + i) * 128 + (p & 1) * 64,
+                     w.b * 2 * s.Hk + 2 * w.hk + m);
+            ++loaded_k;
+          }
+          // the ring carried the last item's output rows until its warps say so
+          if (ok && i == 0 && ni) ok = bar_wait(staged, (ni - 1) & 1, abort_flag, s.err, 3);
+          for (int hf = 0; hf < 2 && ok; ++hf, ++nv) {
+            const int slot = nv % C::RING, use = nv / C::RING;
+            if (use) ok = bar_wait(v_empty + slot, (use - 1) & 1, abort_flag, s.err, 4);
+            if (!ok) break;
+            bar_expect(v_full + slot, C::VSLOT);
+            for (int p = 0; p < 2 * (DV / 64); ++p)
+              tma_3d(sv + slot * C::VSLOT + p * C::VBLK, &mv, v_full + slot, p * 64, (w.tile0 + i) * 128 + hf * 64,
+                     w.b * s.Hk + w.hk);
+          }
         }
+        ++ni;
       }
       // every copy has landed before the CTA's memory is released
-      bar_drain(q_full, 0);
+      if (nq) bar_drain(q_full, (nq - 1) & 1);
       for (int m = 0; m < 2; ++m) {
         const int c = (loaded_k + 1 - m) / 2;  // loads of this map
         if (c) bar_drain(k_full + m, (c - 1) & 1);
       }
-      for (int u = loaded_v - 1; u >= 0 && u > loaded_v - 1 - C::RING; --u)
-        bar_drain(v_full + u % C::RING, (u / C::RING) & 1);
-    } else if (warp == 1 && tiles) {
+      for (int u = nv - 1; u >= 0 && u > nv - 1 - C::RING; --u) bar_drain(v_full + u % C::RING, (u / C::RING) & 1);
+    } else if (warp == 1) {
       const uint32_t one = elect_one();
       constexpr uint32_t id_s = idesc(128, false), id_o = idesc(DV, true);
-      bool ok = mma_wait(q_full, 0, abort_flag, s.err, 3);
-      for (int i = 0; i <= tiles && ok; ++i) {
-        for (int m = 0; m < 2 && ok; ++m) {
-          const uint32_t ts = tmem + m * 128, to = tmem + 256 + m * DV;
-          if (i) {  // O = P V of the tile before
-            ok = mma_wait(p_full + m, (i - 1) & 1, abort_flag, s.err, 4);
-            for (int hf = 0; hf < 2 && ok; ++hf) {
-              const int u = 2 * (i - 1) + hf, slot = u % C::RING;
-              ok = mma_wait(v_full + slot, (u / C::RING) & 1, abort_flag, s.err, 5);
+      bool ok = true, any = false;
+      int nq = 0, nt = 0, nv = 0;  // items with keys, tiles and half value tiles so far
+      for (int r = 0; r < rounds && ok; ++r) {
+        unsigned at;
+        if (!item_of_round(items, r, at)) continue;
+        const int tiles = __shfl_sync(0xffffffffu, item_at(s, x, o, at).tiles, 0);
+        if (!tiles) continue;
+        any = true;
+        ok = mma_wait(q_full, nq & 1, abort_flag, s.err, 5);
+        ++nq;
+        for (int i = 0; i <= tiles && ok; ++i) {
+          for (int m = 0; m < 2 && ok; ++m) {
+            const uint32_t ts = tmem + m * 128, to = tmem + 256 + m * DV;
+            if (i) {  // O = P V of the tile before
+              ok = mma_wait(p_full + m, (nt + i - 1) & 1, abort_flag, s.err, 6);
+              for (int hf = 0; hf < 2 && ok; ++hf) {
+                const int u = nv + 2 * (i - 1) + hf, slot = u % C::RING;
+                ok = mma_wait(v_full + slot, (u / C::RING) & 1, abort_flag, s.err, 7);
+                if (!ok) break;
+                fence_after();
+                const uint32_t vh = sv + slot * C::VSLOT, vl = vh + (DV / 64) * C::VBLK;
+                // the small products first: truncation then takes from small sums
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                  const uint32_t ph = ts + (hf * 4 + k) * 16;
+                  mma_ts(to, ph, ndesc(vl, k, C::VBLK), id_o, (hf || k) ? 1u : 0u, one);
+                  mma_ts(to, ph + 8, ndesc(vh, k, C::VBLK), id_o, 1u, one);
+                }
+#pragma unroll
+                for (int k = 0; k < 4; ++k) mma_ts(to, ts + (hf * 4 + k) * 16, ndesc(vh, k, C::VBLK), id_o, 1u, one);
+                if (m) mma_commit(v_empty + slot, one);
+              }
+              mma_commit(o_full + m, one);
+            }
+            if (i < tiles && ok) {
+              ok = mma_wait(k_full + m, (nt + i) & 1, abort_flag, s.err, 8);
               if (!ok) break;
               fence_after();
-              const uint32_t vh = sv + slot * C::VSLOT, vl = vh + (DV / 64) * C::VBLK;
-              // the small products first: truncation then takes from small sums
+              const uint32_t qh = sq + m * C::QK, ql = qh + C::HALF, kh = sk + m * C::QK, kl = kh + C::HALF;
 #pragma unroll
               for (int k = 0; k < 4; ++k) {
-                const uint32_t ph = ts + (hf * 4 + k) * 16;
-                mma_ts(to, ph, ndesc(vl, k, C::VBLK), id_o, (hf || k) ? 1u : 0u, one);
-                mma_ts(to, ph + 8, ndesc(vh, k, C::VBLK), id_o, 1u, one);
+                mma_ss(ts, kdesc(qh, k), kdesc(kl, k), id_s, k ? 1u : 0u, one);
+                mma_ss(ts, kdesc(ql, k), kdesc(kh, k), id_s, 1u, one);
               }
 #pragma unroll
-              for (int k = 0; k < 4; ++k) mma_ts(to, ts + (hf * 4 + k) * 16, ndesc(vh, k, C::VBLK), id_o, 1u, one);
-              if (m) mma_commit(v_empty + slot, one);
+              for (int k = 0; k < 4; ++k) mma_ss(ts, kdesc(qh, k), kdesc(kh, k), id_s, 1u, one);
+              mma_commit(k_empty + m, one);
+              mma_commit(s_full + m, one);
+              if (m && i == tiles - 1) mma_commit(q_empty, one);
             }
-            mma_commit(o_full + m, one);
-          }
-          if (i < tiles && ok) {
-            ok = mma_wait(k_full + m, i & 1, abort_flag, s.err, 6);
-            if (!ok) break;
-            fence_after();
-            const uint32_t qh = sq + m * C::QK, ql = qh + C::HALF, kh = sk + m * C::QK, kl = kh + C::HALF;
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              mma_ss(ts, kdesc(qh, k), kdesc(kl, k), id_s, k ? 1u : 0u, one);
-              mma_ss(ts, kdesc(ql, k), kdesc(kh, k), id_s, 1u, one);
-            }
-#pragma unroll
-            for (int k = 0; k < 4; ++k) mma_ss(ts, kdesc(qh, k), kdesc(kh, k), id_s, 1u, one);
-            mma_commit(k_empty + m, one);
-            mma_commit(s_full + m, one);
           }
         }
+        nt += tiles;
+        nv += 2 * tiles;
       }
-      mma_commit(all_done, one);  // all products of this CTA
-      bar_drain(all_done, 0);
+      if (any) {
+        mma_commit(all_done, one);  // all products of this CTA
+        bar_drain(all_done, 0);
+      }
     }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 104;");
@@ -212,21 +262,15 @@ __global__ void __launch_bounds__(kThreads, 1)
     constexpr int DH = DV / 2;  // output columns of this thread
     const uint32_t lane_row = (uint32_t)(quad * 32) << 16;
     const uint32_t ts = tmem + m * 128 + 64 * half + lane_row, to = tmem + 256 + m * DV + half * DH + lane_row;
-    const int64_t t = t0 + r;
-    const int64_t seen = (t < s.T ? s.seen(t, n) : s.seen(tl, n)) - (int64_t)tile0 * 128 - 64 * half;
-    const float fq = __ldg(x.fq + (b * 2 * s.H + 2 * h + m) * x.qt + qt);
-    const float *fk = x.fk + (b * 2 * s.Hk + 2 * hk + m) * x.kt + tile0, *fv = x.fv + (b * s.Hk + hk) * x.kt + tile0;
     float *mine = swap + (2 * m + half) * 128 + r, *other = swap + (2 * m + (half ^ 1)) * 128 + r;
+    // the two warps of a map's rows; the four warps of both maps' rows
     auto pair_sync = [&]() { asm volatile("bar.sync %0, 64;" ::"r"(1 + 4 * m + quad) : "memory"); };
+    auto quad_sync = [&]() { asm volatile("bar.sync %0, 128;" ::"r"(9 + quad) : "memory"); };
     // P = 2^(S - ref): the reference is kCarry below the row's maximum when it is set, so that fp16
     // tails hold, and follows only when the maximum has outgrown it by kSlack more (fp16 ends at 2^16)
     constexpr float kCarry = 8.f, kSlack = 6.f;
     constexpr uint32_t kGone = 0x7fc0dead;  // in a maximum's place: this warp gave up (no product has these bits)
-    float ref = -INFINITY, top = -INFINITY;  // top: the maximum that ref was set by
-    uint64_t sum2[2] = {two(0.f, 0.f), two(0.f, 0.f)};
     uint64_t acc[DH / 2];
-#pragma unroll
-    for (int j = 0; j < DH / 2; ++j) acc[j] = two(0.f, 0.f);
     auto add_tile = [&](float g) {  // acc += g O
       const uint64_t g2 = two(g, g);
 #pragma unroll
@@ -246,130 +290,187 @@ __global__ void __launch_bounds__(kThreads, 1)
       for (int j = 0; j < 16; ++j)
         if (j >= left) y[j] = 0xff800000u;  // -inf
     };
-    bool ok = true;
-    float gv = 0.f;
-    for (int i = 0; i < tiles; ++i) {
-      const float f = factor2(fq, __ldg(fk + i)), next_gv = __ldg(fv + i);
-      if (i) {  // the last tile's product, while the tensor core works on this tile's scores
-        ok = __all_sync(0xffffffffu, bar_wait(o_full + m, (i - 1) & 1, abort_flag, s.err, 8));
+    int nt = 0;  // tiles so far
+    // Named barriers have no limit: every warp passes the same ones for every item, whatever its waits
+    // said (after a wait has run out they all return at once).
+    for (int round = 0; round < rounds; ++round) {
+      unsigned index;
+      if (!item_of_round(items, round, index)) continue;
+      const Item w = item_at(s, x, o, index);
+      const int tiles = w.tiles, h = w.h;
+      if (threadIdx.x == 128 && h == 0 && w.qt == 0 && w.split == 0) report_length(s, w.b);
+      const int t = w.t0 + r;
+      const int seen = (int)s.seen(t < s.T ? t : s.T - 1, w.n) - w.tile0 * 128 - 64 * half;
+      const float fq = __ldg(x.fq + (int64_t)(w.b * 2 * s.H + 2 * h + m) * x.qt + w.qt);
+      const float *fk = x.fk + (int64_t)(w.b * 2 * s.Hk + 2 * w.hk + m) * x.kt + w.tile0, *fv = x.fv + (int64_t)(w.b * s.Hk + w.hk) * x.kt + w.tile0;
+      float ref = -INFINITY, top = -INFINITY;  // top: the maximum that ref was set by
+      uint64_t sum2[2] = {two(0.f, 0.f), two(0.f, 0.f)};
+#pragma unroll
+      for (int j = 0; j < DH / 2; ++j) acc[j] = two(0.f, 0.f);
+      bool ok = true;
+      float gv = 0.f;
+      for (int i = 0; i < tiles; ++i) {
+        const float f = factor2(fq, __ldg(fk + i)), next_gv = __ldg(fv + i);
+        if (i) {  // the last tile's product, while the tensor core works on this tile's scores
+          ok = __all_sync(0xffffffffu, bar_wait(o_full + m, (nt + i - 1) & 1, abort_flag, s.err, 9));
+          fence_after();
+          if (ok) add_tile(gv);
+        }
+        ok = ok && __all_sync(0xffffffffu, bar_wait(s_full + m, (nt + i) & 1, abort_flag, s.err, 10));
+        const int left = seen - i * 128;
+        const int lim = left < 0 ? 0 : left > 64 ? 64 : left;
+        const bool whole = __all_sync(0xffffffffu, lim == 64);
+        float mx = -INFINITY;
         fence_after();
-        if (ok) add_tile(gv);
-      }
-      ok = ok && __all_sync(0xffffffffu, bar_wait(s_full + m, i & 1, abort_flag, s.err, 7));
-      const int64_t left = seen - (int64_t)i * 128;
-      const int lim = left < 0 ? 0 : left > 64 ? 64 : (int)left;
-      const bool whole = __all_sync(0xffffffffu, lim == 64);
-      float mx = -INFINITY;
-      fence_after();
-      if (ok) {
-        float mx2[2] = {-INFINITY, -INFINITY};
+        if (ok) {
+          float mx2[2] = {-INFINITY, -INFINITY};
+#pragma unroll 1
+          for (int c = 0; c < 4; ++c) {
+            uint32_t y[16];
+            tld16_issue(ts + 16 * c, y);
+            tld_wait();
+            after_wait(y);
+            if (!whole) mask(y, lim - 16 * c);
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+              mx2[j & 1] = max3(mx2[j & 1], __uint_as_float(y[2 * j]), __uint_as_float(y[2 * j + 1]));
+          }
+          mx = fmaxf(mx2[0], mx2[1]) * f;
+        }
+        // a pair leaves the loop together, or one of them would wait for the other without a limit
+        *mine = ok ? mx : __uint_as_float(kGone);
+        pair_sync();
+        const float theirs = *other;
+        ok = ok && !__any_sync(0xffffffffu, __float_as_uint(theirs) == kGone);
+        if (!ok) break;
+        mx = fmaxf(mx, theirs);
+        gv = next_gv;
+        if (__any_sync(0xffffffffu, mx > top + kSlack || (top == -INFINITY && mx > top))) {
+          const float now = fmaxf(top, mx);
+          const float shrink = top == -INFINITY ? 0.f : ex2(top - now);
+          const uint64_t s2 = two(shrink, shrink);
+          top = now;
+          ref = now - kCarry;
+          sum2[0] = mul2(sum2[0], s2);
+          sum2[1] = mul2(sum2[1], s2);
+#pragma unroll
+          for (int j = 0; j < DH / 2; ++j) acc[j] = mul2(acc[j], s2);
+        }
+        const float at = top == -INFINITY ? 0.f : ref;  // no key yet: all weights are 2^-inf
+        const uint64_t f2 = two(f, f), at2 = two(-at, -at);
 #pragma unroll 1
         for (int c = 0; c < 4; ++c) {
-          uint32_t y[16];
+          uint32_t y[16], hi[8], lo[8];
           tld16_issue(ts + 16 * c, y);
           tld_wait();
           after_wait(y);
           if (!whole) mask(y, lim - 16 * c);
 #pragma unroll
-          for (int j = 0; j < 8; ++j)
-            mx2[j & 1] = max3(mx2[j & 1], __uint_as_float(y[2 * j]), __uint_as_float(y[2 * j + 1]));
+          for (int j = 0; j < 8; ++j) {
+            float a, d;
+            untwo(fma2(two(y[2 * j], y[2 * j + 1]), f2, at2), a, d);
+            const uint64_t p = two(ex2(a), ex2(d));
+            sum2[j & 1] = add2(sum2[j & 1], p);
+            cut2(p, hi[j], lo[j]);
+          }
+          tst_pairs(ts + 16 * c, hi, lo);
         }
-        mx = fmaxf(mx2[0], mx2[1]) * f;
+        tst_wait();
+        fence_before();
+        bar_arrive(p_full + m);
       }
-      // a pair leaves the loop together, or one of them would wait for the other without a limit
-      *mine = ok ? mx : __uint_as_float(kGone);
+      nt += tiles;
+      if (tiles) ok = __all_sync(0xffffffffu, ok && bar_wait(o_full + m, (nt - 1) & 1, abort_flag, s.err, 11));
+      fence_after();
+      if (tiles && ok) add_tile(gv);
+      float s0, s1, s2, s3;
+      untwo(sum2[0], s0, s1);
+      untwo(sum2[1], s2, s3);
+      const float part = (s0 + s1) + (s2 + s3);
+      pair_sync();  // both have read the last maxima
+      *mine = part;
       pair_sync();
-      const float theirs = *other;
-      ok = ok && !__any_sync(0xffffffffu, __float_as_uint(theirs) == kGone);
-      if (!ok) break;
-      mx = fmaxf(mx, theirs);
-      gv = next_gv;
-      if (__any_sync(0xffffffffu, mx > top + kSlack || (top == -INFINITY && mx > top))) {
-        const float now = fmaxf(top, mx);
-        const float shrink = top == -INFINITY ? 0.f : ex2(top - now);
-        const uint64_t s2 = two(shrink, shrink);
-        top = now;
-        ref = now - kCarry;
-        sum2[0] = mul2(sum2[0], s2);
-        sum2[1] = mul2(sum2[1], s2);
+      const float sum = half ? *other + part : part + *other;
+      const bool none = top == -INFINITY, live = t < s.T && ok;
+      const bool parts = o.parts.splits > 1;
+      const float inv = parts ? 1.f : none ? 0.f : 1.0f / sum;
+      const int64_t at0 = (int64_t)(w.b * s.Hk + w.hk) * s.T * s.G + (h - w.hk * s.G);  // + t * G
+      if (live && parts && half == 0)
+        o.parts.ml[((at0 + t * s.G) * 2 + m) * o.parts.splits + w.split] = make_float2(none ? -INFINITY : ref, sum);
+      if (live && !parts && o.lse && half == 0)
+        o.lse[(int64_t)(w.b * 2 * s.H + 2 * h + m) * s.T + t] = none ? INFINITY : ref + log2f(sum);
+      const uint64_t inv2 = two(inv, inv);
 #pragma unroll
-        for (int j = 0; j < DH / 2; ++j) acc[j] = mul2(acc[j], s2);
-      }
-      const float at = top == -INFINITY ? 0.f : ref;  // no key yet: all weights are 2^-inf
-      const uint64_t f2 = two(f, f), at2 = two(-at, -at);
-#pragma unroll 1
-      for (int c = 0; c < 4; ++c) {
-        uint32_t y[16], hi[8], lo[8];
-        tld16_issue(ts + 16 * c, y);
-        tld_wait();
-        after_wait(y);
-        if (!whole) mask(y, lim - 16 * c);
+      for (int j = 0; j < DH / 2; ++j) acc[j] = mul2(acc[j], inv2);
+      // map 2's rows to map 1's warps, over its own products in TMEM
+      if (m && !parts) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          float a, d;
-          untwo(fma2(two(y[2 * j], y[2 * j + 1]), f2, at2), a, d);
-          const uint64_t p = two(ex2(a), ex2(d));
-          sum2[j & 1] = add2(sum2[j & 1], p);
-          cut2(p, hi[j], lo[j]);
+        for (int c = 0; c < DH / 16; ++c) {
+          uint32_t y[2][8];
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            float a, d;
+            untwo(acc[8 * c + j], a, d);
+            y[j >> 2][2 * (j & 3)] = __float_as_uint(a);
+            y[j >> 2][2 * (j & 3) + 1] = __float_as_uint(d);
+          }
+          tst_pairs(to + 16 * c, y[0], y[1]);
         }
-        tst_pairs(ts + 16 * c, hi, lo);
+        tst_wait();
+        fence_before();
       }
-      tst_wait();
+      quad_sync();
+      if (!m && !parts) {
+        const float lam = __ldg(s.lam + h);
+        const uint64_t nl2 = two(-lam, -lam);
+        fence_after();
+#pragma unroll
+        for (int c = 0; c < DH / 16; ++c) {
+          uint32_t y[16];
+          tld16_issue(to + DV + 16 * c, y);
+          tld_wait();
+          after_wait(y);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) acc[8 * c + j] = fma2(two(y[2 * j], y[2 * j + 1]), nl2, acc[8 * c + j]);
+        }
+      }
+      // the value ring is free once the other map's last product is done too
+      if (tiles) ok = __all_sync(0xffffffffu, ok && bar_wait(o_full + (m ^ 1), (nt - 1) & 1, abort_flag, s.err, 12));
+      float *dst = parts ? o.parts.o : m ? o.out2 : o.out;
+      if (ok && dst) {
+        constexpr int CW = C::CW, CH = CW / 4;  // columns and 16-byte chunks of a staged row
+        float4 *box = reinterpret_cast<float4 *>(sm + 4 * C::QK + (warp - 4) * (32 * CW * 4));
+        auto place = [&](int row, int c) { return box + row * CH + (c ^ (CH == 8 ? row & 7 : row >> 1 & 3)); };
+        const bool four = (s.dv & 3) == 0 && ((uintptr_t)dst & 15) == 0;
+        const int64_t stride = parts ? (int64_t)2 * s.G * o.parts.splits * s.dv : (int64_t)s.H * s.dv;
+        float *base = parts ? dst + ((at0 * 2 + m) * o.parts.splits + w.split) * s.dv
+                            
+                            : dst + ((int64_t)w.b * s.T * s.H + h) * s.dv;
+        base += (w.t0 + quad * 32) * stride;
+        const int rows = (int)s.T - w.t0 - quad * 32;
+#pragma unroll
+        for (int c0 = 0; c0 < DH / CW; ++c0) {
+#pragma unroll
+          for (int c = 0; c < CH; ++c) {
+            float4 v;
+            untwo(acc[c0 * (CW / 2) + 2 * c], v.x, v.y);
+            untwo(acc[c0 * (CW / 2) + 2 * c + 1], v.z, v.w);
+            *place(lane, c) = v;
+          }
+          __syncwarp();
+          const int c = lane % CH;
+#pragma unroll
+          for (int k = 0; k < CH; ++k) {
+            const int row = k * (32 / CH) + lane / CH;
+            if (row < rows) store4(base + row * stride, half * DH + c0 * CW + 4 * c, *place(row, c), s.dv, four);
+          }
+          __syncwarp();
+        }
+      }
+      // copies write the ring next, and behind them products what was read of TMEM
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       fence_before();
-      bar_arrive(p_full + m);
-    }
-    if (tiles) ok = __all_sync(0xffffffffu, ok && bar_wait(o_full + m, (tiles - 1) & 1, abort_flag, s.err, 9));
-    fence_after();
-    if (tiles && ok) add_tile(gv);
-    // the staging below takes Q's and K's memory: no product reads it any more
-    if (tiles) ok = __all_sync(0xffffffffu, ok && bar_wait(all_done, 0, abort_flag, s.err, 10));
-    float s0, s1, s2, s3;
-    untwo(sum2[0], s0, s1);
-    untwo(sum2[1], s2, s3);
-    const float part = (s0 + s1) + (s2 + s3);
-    pair_sync();  // both have read the last maxima
-    *mine = part;
-    pair_sync();
-    const float sum = half ? *other + part : part + *other;
-    const bool none = top == -INFINITY, live = t < s.T && ok;
-    const bool parts = o.parts.splits > 1;
-    const float inv = parts ? 1.f : none ? 0.f : 1.0f / sum;
-    const int64_t n_items = s.T * s.G;
-    const int64_t at0 = (b * s.Hk + hk) * n_items + (h - hk * s.G);  // + t * G
-    if (live && parts && half == 0)
-      o.parts.ml[((at0 + t * s.G) * 2 + m) * o.parts.splits + split] = make_float2(none ? -INFINITY : ref, sum);
-    if (live && !parts && o.lse && half == 0)
-      o.lse[(b * 2 * s.H + 2 * h + m) * s.T + t] = none ? INFINITY : ref + log2f(sum);
-#pragma unroll
-    for (int c = 0; c < DH / 4; ++c) {
-      float4 v;
-      untwo(acc[2 * c], v.x, v.y);
-      untwo(acc[2 * c + 1], v.z, v.w);
-      *staged<DV>(sm, m, r, half * (DH / 4) + c) = make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv);
-    }
-    asm volatile("bar.sync 9, 512;" ::: "memory");
-    // rows of the tile, whole lines at a time
-    if (ok) {
-      constexpr int LINES = 128 / DV;  // rows a warp stores at once
-      const float lam = __ldg(s.lam + h);
-      const int c = lane % (DV / 4), sub = lane / (DV / 4);
-      for (int k = (warp - 4) * LINES + sub; k < 128; k += 16 * LINES) {
-        const int64_t tt = t0 + k;
-        if (tt >= s.T) break;
-        float4 a = *staged<DV>(sm, 0, k, c), d = *staged<DV>(sm, 1, k, c);
-        if (parts) {
-          float *dst = o.parts.o + ((at0 + tt * s.G) * 2 * o.parts.splits + split) * s.dv;
-          const bool four = (s.dv & 3) == 0;
-          store4(dst, 4 * c, a, s.dv, four);
-          store4(dst + (int64_t)o.parts.splits * s.dv, 4 * c, d, s.dv, four);
-        } else {
-          const int64_t at = ((b * s.T + tt) * s.H + h) * s.dv;
-          const bool four = (s.dv & 3) == 0 && ((uintptr_t)o.out & 15) == 0 && ((uintptr_t)o.out2 & 15) == 0;
-          a = make_float4(a.x - lam * d.x, a.y - lam * d.y, a.z - lam * d.z, a.w - lam * d.w);
-          store4(o.out + at, 4 * c, a, s.dv, four);
-          if (o.out2) store4(o.out2 + at, 4 * c, d, s.dv, four);
-        }
-      }
+      bar_arrive(staged);
     }
   }
   fence_before();
@@ -388,9 +489,9 @@ int launch(tx_ctx *ctx, const Shape &s, const Split &x, const Out &o) {
     return tx_fail(ctx, TX_ERR_UNSUPPORTED, "differential attention: tensor map");
   static SmemGrant granted;
   TX_TRY(granted.take(ctx, (const void *)k_diff_fwd<DV>, Cfg<DV>::SMEM));
-  const int64_t blocks = x.qt * s.B * s.H;
-  k_diff_fwd<DV><<<dim3((unsigned)blocks, (unsigned)o.parts.splits), kThreads, Cfg<DV>::SMEM, ctx->stream>>>(s, x, mq, mk,
-                                                                                                        mv, o);
+  const int64_t items = x.qt * s.B * s.H * o.parts.splits;
+  const unsigned blocks = (unsigned)(items < ctx->num_sms ? items : ctx->num_sms);
+  k_diff_fwd<DV><<<blocks, kThreads, Cfg<DV>::SMEM, ctx->stream>>>(s, x, mq, mk, mv, o);
   TX_LAUNCHED(ctx, "k_diff_fwd");
   return TX_OK;
 }
