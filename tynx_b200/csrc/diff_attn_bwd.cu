@@ -95,21 +95,19 @@ __device__ __forceinline__ void body(const Shape &s, const Split &x, const CUten
   // keys: the first tiles are seen by most queries; queries: the last tiles see most keys
   const bool each = KEYS && o.each_head;
   const int heads = KEYS && !each ? s.Hk : s.H;
-  const int64_t rheads = s.B * heads, rtiles = KEYS ? x.kt : x.qt;
-  const int64_t rt = KEYS ? block / rheads : rtiles - 1 - block / rheads;
-  const int64_t bh = block % rheads, b = bh / heads;
-  const int rh = (int)(bh - b * heads), hk = KEYS && !each ? rh : rh / s.G;
-  const int64_t r0 = rt * 128, n = s.length(b);
-  const int64_t q_steps = (s.T + kStep - 1) / kStep;
+  const int rheads = (int)s.B * heads, rtiles = (int)(KEYS ? x.kt : x.qt), T = (int)s.T;
+  const int level = block / rheads, bh = block - level * rheads, b = bh / heads;
+  const int rt = KEYS ? level : rtiles - 1 - level, rh = bh - b * heads, hk = KEYS && !each ? rh : rh / s.G;
+  const int r0 = rt * 128, n = (int)s.length(b), q_steps = (T + kStep - 1) / kStep;
   int first = 0, per_head;  // steps of each head, keys: from step `first` on
   if (KEYS) {
     int64_t q_first = s.causal ? r0 - s.start : 0;  // the first query that sees the first key
     if (q_first < 0) q_first = 0;
     first = (int)(q_first / kStep);
-    per_head = first < q_steps && r0 < n ? (int)q_steps - first : 0;
+    per_head = first < q_steps && r0 < n ? q_steps - first : 0;
   } else {
-    const int64_t last = r0 + 127 < s.T ? r0 + 127 : s.T - 1;
-    per_head = (int)((s.seen(last, n) + kStep - 1) / kStep);
+    const int last = r0 + 127 < T ? r0 + 127 : T - 1;
+    per_head = ((int)s.seen(last, n) + kStep - 1) / kStep;
   }
   const int steps = __shfl_sync(0xffffffffu, KEYS && !each ? per_head * s.G : per_head, 0);
 
@@ -141,7 +139,7 @@ __device__ __forceinline__ void body(const Shape &s, const Split &x, const CUten
   if (MODE != kModeV) {
     // the largest row norm of this head's values (all tiles: D runs over all keys)
     for (int64_t i = threadIdx.x; i < x.kt; i += kThreads)
-      atomicMax(vmax, __float_as_uint(__ldg(x.nv + (b * s.Hk + hk) * x.kt + i)));
+      atomicMax(vmax, __float_as_uint(__ldg(x.nv + (int64_t)(b * s.Hk + hk) * x.kt + i)));
     __syncthreads();
   }
 
@@ -154,12 +152,12 @@ __device__ __forceinline__ void body(const Shape &s, const Split &x, const CUten
     if (warp == 0 && lane == 0 && steps) {
       bar_expect(r_full, 2 * C::RQ + (MODE == kModeV ? 0 : C::RV));
       for (int p = 0; p < 8; ++p)  // (map, head or tail, 64-row half)
-        tma_3d(srq + p * C::XBLK, KEYS ? &mk : &mq, r_full, (p >> 1 & 1) * 64, (int)r0 + (p & 1) * 64,
-               (int)(KEYS ? b * 2 * s.Hk + 2 * hk : b * 2 * s.H + 2 * rh) + (p >> 2));
+        tma_3d(srq + p * C::XBLK, KEYS ? &mk : &mq, r_full, (p >> 1 & 1) * 64, r0 + (p & 1) * 64,
+               (KEYS ? b * 2 * s.Hk + 2 * hk : b * 2 * s.H + 2 * rh) + (p >> 2));
       if (MODE != kModeV)
         for (int p = 0; p < 4 * (DV / 64); ++p)
-          tma_3d(srv + p * C::XBLK, KEYS ? &mv : &mg, r_full, (p >> 1) * 64, (int)r0 + (p & 1) * 64,
-                 (int)(KEYS ? b * s.Hk + hk : b * s.H + rh));
+          tma_3d(srv + p * C::XBLK, KEYS ? &mv : &mg, r_full, (p >> 1) * 64, r0 + (p & 1) * 64,
+                 KEYS ? b * s.Hk + hk : b * s.H + rh);
       bool ok = true;
       int lx = 0, lv = 0;
       for (int i = 0; i < steps && ok; ++i) {
@@ -169,13 +167,13 @@ __device__ __forceinline__ void body(const Shape &s, const Split &x, const CUten
         bar_expect(x_full + st, 2 * C::XQ + (KEYS ? C::STAT : 0) + (MODE == kModeV ? C::XV : 0));
         for (int p = 0; p < 4; ++p)
           tma_3d(sxq + st * 2 * C::XQ + p * C::XBLK, KEYS ? &mq : &mk, x_full + st, (p & 1) * 64, step * kStep,
-                 (int)(KEYS ? b * 2 * s.H + 2 * h : b * 2 * s.Hk + 2 * hk) + (p >> 1));
+                 (KEYS ? b * 2 * s.H + 2 * h : b * 2 * s.Hk + 2 * hk) + (p >> 1));
         if (KEYS)
-          bulk_load(su32(stat) + st * C::STAT, o.stats + ((b * s.H + h) * q_steps + step) * (4 * kStep), C::STAT,
+          bulk_load(su32(stat) + st * C::STAT, o.stats + ((int64_t)(b * s.H + h) * q_steps + step) * (4 * kStep), C::STAT,
                     x_full + st);
         if (MODE == kModeV)
           for (int p = 0; p < 2 * (DV / 64); ++p)
-            tma_3d(xv_at(i) + p * C::XBLK, &mg, x_full + st, p * 64, step * kStep, (int)(b * s.H + h));
+            tma_3d(xv_at(i) + p * C::XBLK, &mg, x_full + st, p * 64, step * kStep, b * s.H + h);
         ++lx;
         if (MODE != kModeV) {
           if (i) ok = bar_wait(v_empty, (i - 1) & 1, abort_flag, s.err, 12);
@@ -183,7 +181,7 @@ __device__ __forceinline__ void body(const Shape &s, const Split &x, const CUten
           bar_expect(v_full, C::XV);
           for (int p = 0; p < 2 * (DV / 64); ++p)
             tma_3d(sxv + p * C::XBLK, KEYS ? &mg : &mv, v_full, p * 64, step * kStep,
-                   (int)(KEYS ? b * s.H + h : b * s.Hk + hk));
+                   KEYS ? b * s.H + h : b * s.Hk + hk);
           ++lv;
         }
       }
@@ -277,23 +275,25 @@ __device__ __forceinline__ void body(const Shape &s, const Split &x, const CUten
     // part / 2's columns (K, Q) or a quarter of the columns (V)
     const int part = (warp - 4) >> 2, half = part >> 1, quad = warp & 3, r = quad * 32 + lane;
     const uint32_t lane_row = (uint32_t)(quad * 32) << 16;
-    const int64_t row = r0 + r;
+    const int row = r0 + r;
     constexpr int AC = MODE == kModeV ? DV / 4 : 32;  // columns of the result a thread sums
     uint64_t acc[AC / 2];
 #pragma unroll
     for (int j = 0; j < AC / 2; ++j) acc[j] = two(0.f, 0.f);
     const float vn = __uint_as_float(*vmax);
     // resident factors: of both maps, and of V (keys) or dO (queries)
-    const int64_t rq = KEYS ? (b * 2 * s.Hk + 2 * hk) * x.kt + rt : (b * 2 * s.H + 2 * rh) * x.qt + rt;
+    const int64_t rq = (int64_t)(KEYS ? b * 2 * s.Hk + 2 * hk : b * 2 * s.H + 2 * rh) * rtiles + rt;
     const float fr0 = __ldg((KEYS ? x.fk : x.fq) + rq), fr1 = __ldg((KEYS ? x.fk : x.fq) + rq + rtiles);
-    const float frv = __ldg((KEYS ? x.fv : x.fg) + (KEYS ? b * s.Hk + hk : b * s.H + rh) * rtiles + rt);
+    const float frv = __ldg((KEYS ? x.fv : x.fg) + (int64_t)(KEYS ? b * s.Hk + hk : b * s.H + rh) * rtiles + rt);
     float mine[4] = {INFINITY, INFINITY, 0.f, 0.f};  // Q: this row's statistics
-    if (!KEYS && row < s.T) {
+    if (!KEYS && row < T) {
 #pragma unroll
       for (int k = 0; k < 4; ++k)
-        mine[k] = __ldg(o.stats + ((b * s.H + rh) * q_steps + row / kStep) * (4 * kStep) + k * kStep + row % kStep);
+        mine[k] = __ldg(o.stats + ((int64_t)(b * s.H + rh) * q_steps + row / kStep) * (4 * kStep) + k * kStep + row % kStep);
     }
-    const int64_t seen = KEYS ? 0 : row < s.T ? s.seen(row, n) : 0;
+    const int seen = KEYS ? 0 : row < T ? (int)s.seen(row, n) : 0;
+    const int64_t from64 = s.causal ? row - s.start : 0;  // keys: the first query that sees this one
+    const int from0 = from64 < 0 ? 0 : from64 > 1 << 30 ? 1 << 30 : (int)from64;
     bool ok = true;
     float ga = 0.f;  // factor of the last step's products
     auto add_products = [&]() {
@@ -310,10 +310,10 @@ __device__ __forceinline__ void body(const Shape &s, const Split &x, const CUten
     };
     for (int i = 0; i < steps; ++i) {
       const int h = head_of(i), st = i & 1;
-      const int64_t x0 = (int64_t)step_of(i) * kStep, xt = x0 >> 7;
-      const int64_t xq = KEYS ? (b * 2 * s.H + 2 * h) * x.qt + xt : (b * 2 * s.Hk + 2 * hk) * x.kt + xt;
-      const float fx0 = __ldg((KEYS ? x.fq : x.fk) + xq), fx1 = __ldg((KEYS ? x.fq : x.fk) + xq + (KEYS ? x.qt : x.kt));
-      const float fxv = __ldg((KEYS ? x.fg : x.fv) + (KEYS ? (b * s.H + h) * x.qt : (b * s.Hk + hk) * x.kt) + xt);
+      const int x0 = step_of(i) * kStep, xt = x0 >> 7, xtiles = (int)(KEYS ? x.qt : x.kt);
+      const int64_t xq = (int64_t)(KEYS ? b * 2 * s.H + 2 * h : b * 2 * s.Hk + 2 * hk) * xtiles + xt;
+      const float fx0 = __ldg((KEYS ? x.fq : x.fk) + xq), fx1 = __ldg((KEYS ? x.fq : x.fk) + xq + xtiles);
+      const float fxv = __ldg((KEYS ? x.fg : x.fv) + (int64_t)(KEYS ? b * s.H + h : b * s.Hk + hk) * xtiles + xt);
       const float lam = __ldg(s.lam + h);
       const float f0 = factor2(fr0, fx0), f1 = factor2(fr1, fx1);
       float next_ga, beta = 0.f, fp = 0.f, sw = 0.f;
@@ -323,7 +323,7 @@ __device__ __forceinline__ void body(const Shape &s, const Split &x, const CUten
         sw = __uint_as_float((uint32_t)(140 - e) << 23);
         next_ga = fxv * __uint_as_float((uint32_t)(114 + e) << 23);
       } else {  // ds scale: 2 |dO| |V| -> [2^13, 2^14)
-        const float gn = __ldg(x.ng + (b * s.H + h) * x.qt + (KEYS ? xt : rt));
+        const float gn = __ldg(x.ng + (int64_t)(b * s.H + h) * x.qt + (KEYS ? xt : rt));
         int e = (int)(__float_as_uint(2.f * gn * vn) >> 23) - 127;
         e = e < -113 ? -113 : e > 113 ? 113 : e;
         beta = __uint_as_float((uint32_t)(140 - e) << 23);
@@ -340,14 +340,12 @@ __device__ __forceinline__ void body(const Shape &s, const Split &x, const CUten
       // columns of these 16 that are seen: [lo_c, hi_c); queries behind the last have lse = +inf
       int lo_c = 0, hi_c = 16;
       if (KEYS) {
-        if (s.causal) {
-          const int64_t from = row - s.start - x0 - 16 * part;  // the first query that sees this key
-          lo_c = from < 0 ? 0 : from > 16 ? 16 : (int)from;
-        }
+        const int from = from0 - x0 - 16 * part;
+        lo_c = from < 0 ? 0 : from > 16 ? 16 : from;
         if (row >= n) hi_c = 0;
       } else {
-        const int64_t end = seen - x0 - 16 * part;
-        hi_c = end < 0 ? 0 : end > 16 ? 16 : (int)end;
+        const int end = seen - x0 - 16 * part;
+        hi_c = end < 0 ? 0 : end > 16 ? 16 : end;
       }
       const bool whole = __all_sync(0xffffffffu, lo_c == 0 && hi_c == 16);
       const uint32_t ts = tmem + lane_row + st * 192 + 16 * part;
@@ -424,7 +422,7 @@ __device__ __forceinline__ void body(const Shape &s, const Split &x, const CUten
       stage[r * CH + ((part * (AC / 4) + c) ^ (r & 7))] = v;
     }
     asm volatile("bar.sync 1, 512;" ::: "memory");
-    const int64_t rows = KEYS ? s.S : s.T;
+    const int rows = (int)(KEYS ? s.S : s.T);
     if (ok) {
       const int w = MODE == kModeV ? s.dv : s.d;  // a result row: one of w, or two maps' of w
       float *dst = MODE == kModeV ? o.dv : MODE == kModeK ? o.dk : o.dq;
@@ -434,7 +432,7 @@ __device__ __forceinline__ void body(const Shape &s, const Split &x, const CUten
       for (int k = (warp - 4) * (32 / CH) + sub; k < 128; k += 16 * (32 / CH)) {
         if (r0 + k >= rows) break;
         const float4 v = stage[k * CH + (c ^ (k & 7))];
-        float *p = dst + ((b * rows + r0 + k) * heads + rh) * (MODE == kModeV ? w : 2 * w) + m * w + e;
+        float *p = dst + (((int64_t)b * rows + r0 + k) * heads + rh) * (MODE == kModeV ? w : 2 * w) + m * w + e;
         if (four) {
           if (e < w) *reinterpret_cast<float4 *>(p) = v;
         } else {
