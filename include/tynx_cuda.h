@@ -94,8 +94,8 @@ int tx_stream(tx_ctx *ctx, void **out);
  * legacy default one) waits for the compute work issued so far.  The block is
  * freed once tx_free was called and every loan has ended (the structure's
  * deleter, callable from any thread); work issued after that waits for the
- * borrower's stream before it reuses the memory.  Not allowed during a
- * capture.  tx_dlpack_release calls the deleter of any such structure. */
+ * borrower's stream before it reuses the memory.  Every loan has to end
+ * before tx_ctx_destroy.  Not allowed during a capture.  tx_dlpack_release calls the deleter of any such structure. */
 enum { TX_DL_F32 = 0, TX_DL_I64 = 1, TX_DL_BOOL = 2 };
 int tx_dlpack_export(tx_ctx *ctx, void *d_block, void *d_data, int dtype, const int64_t *shape, int ndim,
                      void *stream, void **out);

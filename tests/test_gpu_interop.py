@@ -76,6 +76,29 @@ def test_the_owner_may_go_first():
     del others
 
 
+def test_operators_on_tensors_of_a_side_stream():
+    """A tensor still being written on another stream is waited for, and the result handed back to that
+    stream."""
+    import torch
+
+    import tynx_b200 as tx
+
+    side = torch.cuda.Stream()
+    rotary = tx.nn.Rotary(64)
+    want = None
+    for _ in range(5):
+        with torch.cuda.stream(side):
+            x = torch.ones(2, 300, 4, 64, device="cuda")
+            torch.cuda._sleep(1_000_000)
+            x *= 2.0
+            y = torch.from_dlpack(tx.nn.functional.rotary_embedding(tx.from_dlpack(x), rotary))
+            total = y.square().sum()
+        side.synchronize()
+        want = want or total.item()
+        # a rotation keeps the sum of squares: 4 a value
+        assert total.item() == want and abs(want - 4.0 * 2 * 300 * 4 * 64) < 1.0
+
+
 def test_refusals():
     import torch
 

@@ -166,6 +166,33 @@ def test_one_output_used_alone_and_empty_batches():
     np.testing.assert_array_equal(leaves[2].grad.numpy(), 0.0)
 
 
+def test_offsets_past_32_bits():
+    import torch
+
+    import tynx_b200 as tx
+
+    rotary = tx.nn.Rotary(128)
+    x = torch.ones(1, 600000, 32, 128, device="cuda")
+    assert x.numel() > 2**31
+    x[0, -1] = torch.arange(32 * 128, device="cuda").reshape(32, 128) / 4096.0
+    y = torch.from_dlpack(tx.nn.functional.rotary_embedding(tx.from_dlpack(x), rotary))
+    close(tx.from_dlpack(y[:, -2:].contiguous()), turned(x[:, -2:].cpu().numpy(), rotary, [[599998, 599999]]), 1e-6)
+
+
+def test_unaligned_rows():
+    """A view that starts off a 16-byte boundary takes the single-element path to the same values."""
+    import torch
+
+    import tynx_b200 as tx
+
+    rotary = tx.nn.Rotary(64, interleaved=True)
+    base = torch.randn(2 * 7 * 3 * 64 + 1, device="cuda")
+    x = tx.from_dlpack(base[1:].reshape(2, 7, 3, 64))
+    assert x.ptr % 16 == 4
+    y = tx.nn.functional.rotary_embedding(x, rotary)
+    close(y, turned(x.numpy(), rotary, np.broadcast_to(np.arange(7), (2, 7))), 1e-6)
+
+
 def test_gradient_agrees_with_differences():
     import tynx_b200 as tx
 

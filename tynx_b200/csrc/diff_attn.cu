@@ -111,50 +111,52 @@ __device__ __forceinline__ void split_tile(const Shape &s, const SplitJobs &jobs
     total = warp_sum(total);
     if ((threadIdx.x & 31) == 0) red[2 * kSplitWarps + (threadIdx.x >> 5)] = __float_as_uint(total);
   }
-  // the tile's largest finite magnitude (and row norm)
+  // the tile's largest finite magnitude
   uint32_t top = 0;
-  float norm = 0.f;
 #pragma unroll
-  for (int u = 0; u < UNITS; ++u) {
-    float ss = 0.f;
+  for (int u = 0; u < UNITS; ++u)
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       x[u][i] *= J.factor;
       const uint32_t a = __float_as_uint(x[u][i]) & 0x7fffffffu;
       if (a < 0x7f800000u && a > top) top = a;
-      ss += x[u][i] * x[u][i];
     }
-    if (J.norm) {
-#pragma unroll
-      for (int o = PARTS / 2; o; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-      norm = fmaxf(norm, ss);
-    }
-  }
   top = __reduce_max_sync(0xffffffffu, top);
-  const uint32_t nb = __reduce_max_sync(0xffffffffu, __float_as_uint(norm));
-  if ((threadIdx.x & 31) == 0) {
-    red[threadIdx.x >> 5] = top;
-    red[kSplitWarps + (threadIdx.x >> 5)] = nb;
-  }
+  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = top;
   __syncthreads();
-  uint32_t most = 0;
 #pragma unroll
-  for (int i = 0; i < kSplitWarps; ++i) {
-    top = red[i] > top ? red[i] : top;
-    most = red[kSplitWarps + i] > most ? red[kSplitWarps + i] : most;
-  }
+  for (int i = 0; i < kSplitWarps; ++i) top = red[i] > top ? red[i] : top;
   int e = (int)(top >> 23) - 127 - 13;
   e = e < -113 ? -113 : e > 114 ? 114 : e;
+  const float f = __uint_as_float((uint32_t)(127 + e) << 23), inv = __uint_as_float((uint32_t)(127 - e) << 23);
   if (threadIdx.x == 0) {
-    J.f[blockIdx.x] = __uint_as_float((uint32_t)(127 + e) << 23);
-    if (J.norm) J.norm[blockIdx.x] = fminf(sqrtf(__uint_as_float(most)), 1e16f);
+    J.f[blockIdx.x] = f;
     if (STATS) {
       float total = 0.f;
       for (int i = 0; i < kSplitWarps; ++i) total += __uint_as_float(red[2 * kSplitWarps + i]);
       jobs.sums[blockIdx.x] = total;
     }
   }
-  const float inv = __uint_as_float((uint32_t)(127 - e) << 23);
+  if (J.norm) {  // the largest row norm, from the scaled elements: their squares neither overflow nor vanish
+    float norm = 0.f;
+#pragma unroll
+    for (int u = 0; u < UNITS; ++u) {
+      float ss = 0.f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) ss += (x[u][i] * inv) * (x[u][i] * inv);
+#pragma unroll
+      for (int o = PARTS / 2; o; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+      norm = fmaxf(norm, ss);
+    }
+    const uint32_t nb = __reduce_max_sync(0xffffffffu, __float_as_uint(norm));
+    if ((threadIdx.x & 31) == 0) red[kSplitWarps + (threadIdx.x >> 5)] = nb;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+      uint32_t most = 0;
+      for (int i = 0; i < kSplitWarps; ++i) most = red[kSplitWarps + i] > most ? red[kSplitWarps + i] : most;
+      J.norm[blockIdx.x] = fminf(sqrtf(__uint_as_float(most)) * f, 3e38f);
+    }
+  }
 #pragma unroll
   for (int u = 0; u < UNITS; ++u) {
     const int64_t n = n0 + r0 + u * ROWS;
@@ -233,12 +235,12 @@ __global__ void __launch_bounds__(kRowThreads, 2)
   static_assert(NV <= 16, "one score a lane at the end");
   constexpr int COPY = 16 / NV;                  // lanes that hold the same one
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, m = lane >> 4, l16 = lane & 15;
-  const int b = blockIdx.y / s.Hk, hk = blockIdx.y - b * s.Hk;
-  const int n_items = (int)(s.T * s.G), item0 = blockIdx.z * RP;  // few_queries()
+  const int bh = blockIdx.x / parts.splits, split = blockIdx.x - bh * parts.splits, b = bh / s.Hk, hk = bh - b * s.Hk;
+  const int n_items = (int)(s.T * s.G), item0 = blockIdx.y * RP;  // few_queries()
   const int64_t n = s.length(b);
-  if (threadIdx.x == 0 && hk == 0 && blockIdx.x == 0 && blockIdx.z == 0) report_length(s, b);
+  if (threadIdx.x == 0 && hk == 0 && split == 0 && blockIdx.y == 0) report_length(s, b);
   const int last = item0 + RP <= n_items ? item0 + RP - 1 : n_items - 1;
-  const int64_t k0 = (int64_t)blockIdx.x * keys_per_split;
+  const int64_t k0 = (int64_t)split * keys_per_split;
   const int64_t end = s.seen(last / s.G, n) - k0;
   const int keys = end < 0 ? 0 : end > keys_per_split ? (int)keys_per_split : (int)end;  // of this block
 
@@ -358,7 +360,7 @@ __global__ void __launch_bounds__(kRowThreads, 2)
       l += ml.y * f;
       x += sh.acc[w][row][c] * f;
     }
-    const int64_t to = (((int64_t)blockIdx.y * n_items + item) * 2 + mm) * parts.splits + blockIdx.x;
+    const int64_t to = (((int64_t)bh * n_items + item) * 2 + mm) * parts.splits + split;
     if (c == 0) parts.ml[to] = make_float2(top, l);
     if (c < s.dv) parts.o[to * s.dv + c] = x;
   }
@@ -522,9 +524,12 @@ int check_desc(tx_ctx *ctx, const tx_diff_attention *p, Shape &s) {
     return tx_fail(ctx, TX_ERR_SHAPE, "differential attention: the query heads must be a multiple of the key heads");
   const int64_t most = (int64_t)1 << 30;
   if (p->batch < 0 || p->queries < 0 || p->keys < 0 || p->batch > most || p->queries > most || p->keys > most ||
-      p->query_start > most || p->query_start < -most || (p->batch && p->heads > 65535 / p->batch) ||
+      p->query_start > most || p->query_start < -most || (p->batch && p->heads > (1 << 22) / p->batch) ||
       (p->batch && (p->queries > most / p->batch || p->keys > most / p->batch)))
-    return tx_fail(ctx, TX_ERR_SHAPE, "differential attention: batch * heads up to 65535, lengths below 2^30 in all");
+    return tx_fail(ctx, TX_ERR_SHAPE, "differential attention: batch * heads up to 2^22, batch * length up to 2^30");
+  // blocks of a launch: queries of a head, and key tiles twice
+  if (p->batch * p->heads * ((p->queries + 127) / 128 + 2 * ((p->keys + 127) / 128)) >= ((int64_t)1 << 31))
+    return tx_fail(ctx, TX_ERR_SHAPE, "differential attention: too many heads and tiles for one call");
   if (!std::isfinite(p->scale)) return tx_fail(ctx, TX_ERR_INVALID, "differential attention: scale");
   s = Shape{p->batch, p->queries, p->keys, (int)p->heads, (int)p->kv_heads, (int)(p->heads / p->kv_heads), (int)p->dim,
             (int)p->vdim, p->q, p->k, p->v, p->lam, p->key_lengths, p->causal ? 1 : 0, p->query_start, p->scale,
@@ -567,7 +572,7 @@ int launch_rows(tx_ctx *ctx, const Shape &s, float *out, float *out2, float *lse
   auto kernel = vec ? k_diff_rows<RP, true> : k_diff_rows<RP, false>;
   static SmemGrant granted[2];
   TX_TRY(granted[vec].take(ctx, (const void *)kernel, smem));
-  kernel<<<dim3((unsigned)splits, (unsigned)(s.B * s.Hk), (unsigned)chunks), kRowThreads, smem, ctx->stream>>>(
+  kernel<<<dim3((unsigned)(splits * s.B * s.Hk), (unsigned)chunks), kRowThreads, smem, ctx->stream>>>(
       s, mem.parts, per);
   TX_LAUNCHED(ctx, "k_diff_rows");
   return join(ctx, s, mem.parts, out, out2, lse);

@@ -322,13 +322,15 @@ __device__ __forceinline__ void body(const Shape &s, const Split &x, const CUten
         e = e > 113 ? 113 : e;
         sw = __uint_as_float((uint32_t)(140 - e) << 23);
         next_ga = fxv * __uint_as_float((uint32_t)(114 + e) << 23);
-      } else {  // ds scale: 2 |dO| |V| -> [2^13, 2^14)
+      } else {  // ds scale: 2 |dO| |V| below 2^14
         const float gn = __ldg(x.ng + (int64_t)(b * s.H + h) * x.qt + (KEYS ? xt : rt));
-        int e = (int)(__float_as_uint(2.f * gn * vn) >> 23) - 127;
+        // (the exponents' sum: the product itself may leave fp32's range)
+        int e = (int)(__float_as_uint(gn) >> 23) + (int)(__float_as_uint(vn) >> 23) - 2 * 127 + 2;
         e = e < -113 ? -113 : e > 113 ? 113 : e;
         beta = __uint_as_float((uint32_t)(140 - e) << 23);
-        fp = factor2(frv, fxv) * beta;
+        fp = (float)((double)frv * fxv * beta);
         next_ga = (half ? -lam * fx1 : fx0) * (KEYS ? kLn2 : s.scale) * __uint_as_float((uint32_t)(114 + e) << 23);
+        next_ga = fminf(fmaxf(next_ga, -1.7014118e38f), 1.7014118e38f);
       }
       const uint64_t f02 = two(f0, f0), f12 = two(f1, f1), fp2 = two(fp, fp), nb2 = two(-beta, -beta),
                      sw2 = two(sw, sw), lw2 = two(-lam * sw, -lam * sw);

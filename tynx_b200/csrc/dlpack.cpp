@@ -44,9 +44,10 @@ struct Loan {
 
 void end_loan(DlManaged *m) {
   Loan *loan = static_cast<Loan *>(m->owner);
-  {
+  try {
     std::lock_guard<std::mutex> hold(loan->ctx->alloc.lock);
     loan->ctx->alloc.ended.push_back({loan->block, loan->borrower});
+  } catch (...) {  // no host memory for the note: the block stays lent
   }
   delete loan;
 }
