@@ -16,12 +16,18 @@
 // truncates); they carry the step's factors: f of X's tile, the scale of ds or w,
 // -lam of the head for map 2.
 // Scores are computed three times over.  In return there are no atomic additions
-// and no partial results, so sums have one order; TMEM holds two steps' scores,
-// so that a step's products run under the elementwise part of the one before
-// (a block that summed dK and dV together would have room for one); and the
-// three kinds' blocks, longest first, fill the SMs together.
-// Tensor time a step: K and Q 2 x 576 + 1152 + 768 = 3072 cycles (128 x 64 tiles
-// read shared memory for 48 cycles where the product takes 32), V 2 x 576 + 768.
+// and no partial results, so sums have one order; TMEM holds two steps' S, so that
+// a step's S and sums run under the elementwise part (a block that summed dK and
+// dV together would have room for one); and the three kinds' blocks, longest
+// first, fill the SMs together.
+// An instruction of 128 rows takes 64 cycles whether it makes 64 or 128 columns.
+// So dP multiplies R_hi with X_hi and X_lo side by side (their halves are added
+// elementwise): a step takes 24 instructions for S, 16 for dP and 24 for the sums
+// in K and Q blocks, 4096 cycles, and 24 + 12 in V blocks, 2304.  What bounds the
+// kernel is the tensor core, at the power limit's clock for large problems: 2 x
+// 2048 causal tokens of 8 heads over 4 take 253 us (with dP as three products 260;
+// with a step's S alone in TMEM 421), 256 sequences of 128 tokens of 2 heads, where
+// a block has two steps and its start and stores count as much, 144 us.
 #include "diff_attn.cuh"
 
 namespace tx_diff {
@@ -79,9 +85,12 @@ __device__ __forceinline__ void body(const Shape &s, const Split &x, const CUten
                                      unsigned block) {
   using C = Cfg<DV>;
   constexpr bool KEYS = MODE != kModeQ;  // the rows are keys
-  constexpr uint32_t ACC = 384;          // acc_1, acc_2 (64 columns each) or acc
+  // TMEM: two steps' S_1 and S_2 (64 columns each), dP in two halves, acc_1 and acc_2 (64 each) or acc
+  constexpr uint32_t kDp = 256, ACC = 384;
   const uint32_t srq = su32(sm), sx = srq + 2 * C::RQ;
   const uint32_t srv = sx, sxq = sx + C::RV, sxv = sxq + 4 * C::XQ;
+  // where block p of [heads | tails] goes
+  auto xv_block = [](int p) { return DV == 64 ? p : (p & 1) * 2 + (p >> 1); };
   auto xv_at = [&](int i) { return MODE == kModeV && (i & 1) ? srv : sxv; };
   const float *stat = reinterpret_cast<const float *>(sm + C::TILES);
   uint64_t *bars = reinterpret_cast<uint64_t *>(sm + C::TILES + 2 * C::STAT);
@@ -173,14 +182,14 @@ __device__ __forceinline__ void body(const Shape &s, const Split &x, const CUten
                     x_full + st);
         if (MODE == kModeV)
           for (int p = 0; p < 2 * (DV / 64); ++p)
-            tma_3d(xv_at(i) + p * C::XBLK, &mg, x_full + st, p * 64, step * kStep, b * s.H + h);
+            tma_3d(xv_at(i) + xv_block(p) * C::XBLK, &mg, x_full + st, p * 64, step * kStep, b * s.H + h);
         ++lx;
         if (MODE != kModeV) {
           if (i) ok = bar_wait(v_empty, (i - 1) & 1, abort_flag, s.err, 12);
           if (!ok) break;
           bar_expect(v_full, C::XV);
-          for (int p = 0; p < 2 * (DV / 64); ++p)
-            tma_3d(sxv + p * C::XBLK, KEYS ? &mg : &mv, v_full, p * 64, step * kStep,
+          for (int p = 0; p < 2 * (DV / 64); ++p)  // heads and tails of a column block side by side
+            tma_3d(sxv + xv_block(p) * C::XBLK, KEYS ? &mg : &mv, v_full, p * 64, step * kStep,
                    KEYS ? b * s.H + h : b * s.Hk + hk);
           ++lv;
         }
@@ -191,11 +200,11 @@ __device__ __forceinline__ void body(const Shape &s, const Split &x, const CUten
       if (lv) bar_drain(v_full, (lv - 1) & 1);
     } else if (warp == 1 && steps) {
       const uint32_t one = elect_one();
-      constexpr uint32_t id_s = idesc(kStep, false), id_a = idesc(64, true), id_v = idesc(DV, true);
+      constexpr uint32_t id_s = idesc(kStep, false), id_p = idesc(2 * kStep, false), id_a = idesc(64, true), id_v = idesc(DV, true);
       bool ok = mma_wait(r_full, 0, abort_flag, s.err, 13);
-      auto scores = [&](int i) {  // S_1, S_2 and dP of step i
-        const uint32_t ts = tmem + (i & 1) * 192;
+      auto scores = [&](int i) {  // S_1 and S_2 of step i
         const int st = i & 1;
+        const uint32_t ts = tmem + st * 128;
         ok = ok && mma_wait(x_full + st, (i >> 1) & 1, abort_flag, s.err, 14);
         if (!ok) return;
         fence_after();
@@ -209,46 +218,46 @@ __device__ __forceinline__ void body(const Shape &s, const Split &x, const CUten
 #pragma unroll
           for (int k = 0; k < 4; ++k) mma_ss(ts + m * 64, kdesc(rh_, k), kdesc(xh, k), id_s, 1u, one);
         }
-        if (MODE != kModeV) {
+      };
+      auto values = [&](int i) {  // dP of step i, in two halves: R_hi X_hi + R_lo X_hi and R_hi X_lo
+        if (MODE != kModeV && ok) {
           ok = mma_wait(v_full, i & 1, abort_flag, s.err, 15);
           if (!ok) return;
           fence_after();
 #pragma unroll
           for (int c = 0; c < DV / 64; ++c) {
-            const uint32_t rh_ = srv + c * 16384, rl = rh_ + (DV / 64) * 16384, xh = sxv + c * C::XBLK,
-                           xl = xh + (DV / 64) * C::XBLK;
+            const uint32_t rh_ = srv + c * 16384, rl = rh_ + (DV / 64) * 16384, xh = sxv + c * 2 * C::XBLK;
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
-              mma_ss(ts + 128, kdesc(rh_, k), kdesc(xl, k), id_s, (c || k) ? 1u : 0u, one);
-              mma_ss(ts + 128, kdesc(rl, k), kdesc(xh, k), id_s, 1u, one);
+              mma_ss(tmem + kDp, kdesc(rh_, k), kdesc(xh, k), id_p, (c || k) ? 1u : 0u, one);
+              mma_ss(tmem + kDp, kdesc(rl, k), kdesc(xh, k), id_s, 1u, one);
             }
           }
-#pragma unroll
-          for (int c = 0; c < DV / 64; ++c)
-#pragma unroll
-            for (int k = 0; k < 4; ++k)
-              mma_ss(ts + 128, kdesc(srv + c * 16384, k), kdesc(sxv + c * C::XBLK, k), id_s, 1u, one);
           mma_commit(v_empty, one);
         }
-        mma_commit(s_full + st, one);
+        if (ok) mma_commit(s_full + (i & 1), one);
       };
       scores(0);
+      values(0);
+      if (steps > 1) scores(1);
       for (int i = 0; i < steps && ok; ++i) {
-        if (i + 1 < steps) scores(i + 1);
-        const uint32_t ts = tmem + (i & 1) * 192;
         const int st = i & 1;
+        const uint32_t ts = tmem + st * 128;
         ok = ok && mma_wait(p_full + st, (i >> 1) & 1, abort_flag, s.err, 16);
         if (!ok) break;
         fence_after();
+        if (i + 1 < steps) values(i + 1);  // its dP's place is free: the elementwise part has read the last one
+        if (!ok) break;
         if (MODE == kModeV) {
-          const uint32_t xh = xv_at(i), xl = xh + (DV / 64) * C::XBLK, ta = tmem + ACC;
+          const uint32_t xh = xv_at(i), xl = xh + C::XBLK, ta = tmem + ACC;
+          constexpr uint32_t next = 2 * C::XBLK;
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
-            mma_ts(ta, ts + k * 16, ndesc(xl, k, C::XBLK), id_v, k ? 1u : 0u, one);
-            mma_ts(ta, ts + k * 16 + 8, ndesc(xh, k, C::XBLK), id_v, 1u, one);
+            mma_ts(ta, ts + k * 16, ndesc(xl, k, next), id_v, k ? 1u : 0u, one);
+            mma_ts(ta, ts + k * 16 + 8, ndesc(xh, k, next), id_v, 1u, one);
           }
 #pragma unroll
-          for (int k = 0; k < 4; ++k) mma_ts(ta, ts + k * 16, ndesc(xh, k, C::XBLK), id_v, 1u, one);
+          for (int k = 0; k < 4; ++k) mma_ts(ta, ts + k * 16, ndesc(xh, k, next), id_v, 1u, one);
         } else {
           for (int m = 0; m < 2; ++m) {
             const uint32_t xh = sxq + st * 2 * C::XQ + m * C::XQ, xl = xh + C::XBLK, ta = tmem + ACC + m * 64;
@@ -263,6 +272,7 @@ __device__ __forceinline__ void body(const Shape &s, const Split &x, const CUten
         }
         mma_commit(x_empty + st, one);
         mma_commit(a_full, one);
+        if (i + 2 < steps) scores(i + 2);
       }
       mma_commit(all_done, one);
       bar_drain(all_done, 0);
@@ -296,6 +306,26 @@ __device__ __forceinline__ void body(const Shape &s, const Split &x, const CUten
     const int from0 = from64 < 0 ? 0 : from64 > 1 << 30 ? 1 << 30 : (int)from64;
     bool ok = true;
     float ga = 0.f;  // factor of the last step's products
+    // What a step needs besides its scores; read a step ahead, or its latency adds to every step's chain
+    // (1700 cycles of 4700).
+    struct StepData {
+      float fx0, fx1, fxv, lam, gn;
+      int x0;
+    } next;
+    int step_head = KEYS && !each ? hk * s.G : rh, step = first;  // of the step to be read next
+    const int xtiles = (int)(KEYS ? x.qt : x.kt);
+    auto read_step = [&]() {
+      const int xt = step >> 1;  // tiles have two steps
+      const int64_t xq = (int64_t)(KEYS ? b * 2 * s.H + 2 * step_head : b * 2 * s.Hk + 2 * hk) * xtiles + xt;
+      next.fx0 = __ldg((KEYS ? x.fq : x.fk) + xq);
+      next.fx1 = __ldg((KEYS ? x.fq : x.fk) + xq + xtiles);
+      next.lam = __ldg(s.lam + step_head);
+      next.fxv = __ldg((KEYS ? x.fg : x.fv) + (int64_t)(KEYS ? b * s.H + step_head : b * s.Hk + hk) * xtiles + xt);
+      if (MODE != kModeV) next.gn = __ldg(x.ng + (int64_t)(b * s.H + step_head) * x.qt + (KEYS ? xt : rt));
+      next.x0 = step * kStep;
+      if (++step == first + per_head) step = first, ++step_head;
+    };
+    if (steps) read_step();
     auto add_products = [&]() {
       const uint64_t g2 = two(ga, ga);
 #pragma unroll
@@ -309,27 +339,22 @@ __device__ __forceinline__ void body(const Shape &s, const Split &x, const CUten
       }
     };
     for (int i = 0; i < steps; ++i) {
-      const int h = head_of(i), st = i & 1;
-      const int x0 = step_of(i) * kStep, xt = x0 >> 7, xtiles = (int)(KEYS ? x.qt : x.kt);
-      const int64_t xq = (int64_t)(KEYS ? b * 2 * s.H + 2 * h : b * 2 * s.Hk + 2 * hk) * xtiles + xt;
-      const float fx0 = __ldg((KEYS ? x.fq : x.fk) + xq), fx1 = __ldg((KEYS ? x.fq : x.fk) + xq + xtiles);
-      const float fxv = __ldg((KEYS ? x.fg : x.fv) + (int64_t)(KEYS ? b * s.H + h : b * s.Hk + hk) * xtiles + xt);
-      const float lam = __ldg(s.lam + h);
-      const float f0 = factor2(fr0, fx0), f1 = factor2(fr1, fx1);
+      const int st = i & 1, x0 = next.x0;
+      const float f0 = factor2(fr0, next.fx0), f1 = factor2(fr1, next.fx1), lam = next.lam;
       float next_ga, beta = 0.f, fp = 0.f, sw = 0.f;
       if (MODE == kModeV) {  // w scale: 1 + |lam| -> [2^13, 2^14)
         int e = (int)(__float_as_uint(1.f + fabsf(lam)) >> 23) - 127;
         e = e > 113 ? 113 : e;
         sw = __uint_as_float((uint32_t)(140 - e) << 23);
-        next_ga = fxv * __uint_as_float((uint32_t)(114 + e) << 23);
+        next_ga = next.fxv * __uint_as_float((uint32_t)(114 + e) << 23);
       } else {  // ds scale: 2 |dO| |V| below 2^14
-        const float gn = __ldg(x.ng + (int64_t)(b * s.H + h) * x.qt + (KEYS ? xt : rt));
-        // (the exponents' sum: the product itself may leave fp32's range)
-        int e = (int)(__float_as_uint(gn) >> 23) + (int)(__float_as_uint(vn) >> 23) - 2 * 127 + 2;
+        // (sums of exponents: the products themselves may leave fp32's range)
+        int e = (int)(__float_as_uint(next.gn) >> 23) + (int)(__float_as_uint(vn) >> 23) - 2 * 127 + 2;
         e = e < -113 ? -113 : e > 113 ? 113 : e;
         beta = __uint_as_float((uint32_t)(140 - e) << 23);
-        fp = (float)((double)frv * fxv * beta);
-        next_ga = (half ? -lam * fx1 : fx0) * (KEYS ? kLn2 : s.scale) * __uint_as_float((uint32_t)(114 + e) << 23);
+        const int ep = (int)(__float_as_uint(frv) >> 23) + (int)(__float_as_uint(next.fxv) >> 23) - 127 + 13 - e;
+        fp = ep < 1 ? 0.f : __uint_as_float((uint32_t)(ep > 254 ? 254 : ep) << 23);
+        next_ga = (half ? -lam * next.fx1 : next.fx0) * (KEYS ? kLn2 : s.scale) * __uint_as_float((uint32_t)(114 + e) << 23);
         next_ga = fminf(fmaxf(next_ga, -1.7014118e38f), 1.7014118e38f);
       }
       const uint64_t f02 = two(f0, f0), f12 = two(f1, f1), fp2 = two(fp, fp), nb2 = two(-beta, -beta),
@@ -339,6 +364,7 @@ __device__ __forceinline__ void body(const Shape &s, const Split &x, const CUten
       if (KEYS) ok = ok && __all_sync(0xffffffffu, bar_wait(x_full + st, (i >> 1) & 1, abort_flag, s.err, 18));
       if (!ok) break;
       fence_after();
+      if (i + 1 < steps) read_step();
       // columns of these 16 that are seen: [lo_c, hi_c); queries behind the last have lse = +inf
       int lo_c = 0, hi_c = 16;
       if (KEYS) {
@@ -350,17 +376,23 @@ __device__ __forceinline__ void body(const Shape &s, const Split &x, const CUten
         hi_c = end < 0 ? 0 : end > 16 ? 16 : end;
       }
       const bool whole = __all_sync(0xffffffffu, lo_c == 0 && hi_c == 16);
-      const uint32_t ts = tmem + lane_row + st * 192 + 16 * part;
+      const uint32_t ts = tmem + lane_row + st * 128 + 16 * part, tp = tmem + lane_row + kDp + 16 * part;
       const float *col = stat + st * (4 * kStep) + 16 * part;
       {
-        uint32_t y0[16], y1[16], yp[16];
+        uint32_t y0[16], y1[16], yp[16], yq[16];
         tld16_issue(ts, y0);
         tld16_issue(ts + 64, y1);
-        if (MODE != kModeV) tld16_issue(ts + 128, yp);
+        if (MODE != kModeV) {
+          tld16_issue(tp, yp);
+          tld16_issue(tp + 64, yq);
+        }
         tld_wait();
         after_wait(y0);
         after_wait(y1);
-        if (MODE != kModeV) after_wait(yp);
+        if (MODE != kModeV) {
+          after_wait(yp);
+          after_wait(yq);
+        }
         uint32_t h0[8], l0[8], h1[8], l1[8];
 #pragma unroll
         for (int j4 = 0; j4 < 4; ++j4) {  // four columns
@@ -388,7 +420,7 @@ __device__ __forceinline__ void body(const Shape &s, const Split &x, const CUten
             if (MODE == kModeV) {
               cut2(fma2(p1, lw2, mul2(p0, sw2)), h0[j], l0[j]);
             } else {
-              const uint64_t dp = two(yp[e0], yp[e1]);
+              const uint64_t dp = add2(two(yp[e0], yp[e1]), two(yq[e0], yq[e1]));
               cut2(mul2(p0, fma2(dp, fp2, mul2(st2(2), nb2))), h0[j], l0[j]);
               cut2(mul2(p1, fma2(dp, fp2, mul2(st2(3), nb2))), h1[j], l1[j]);
             }
