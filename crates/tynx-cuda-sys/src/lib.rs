@@ -280,6 +280,7 @@ extern "C" {
     pub fn tx_stream(ctx: *mut tx_ctx, out: *mut *mut c_void) -> c_int;
     pub fn tx_dlpack_export(ctx: *mut tx_ctx, d_block: *mut c_void, d_data: *mut c_void, dtype: c_int, shape: *const i64, ndim: c_int, stream: *mut c_void, out: *mut *mut c_void) -> c_int;
     pub fn tx_dlpack_release(managed: *mut c_void) -> c_int;
+    pub fn tx_dlpack_give_back(ctx: *mut tx_ctx, managed: *mut c_void) -> c_int;
     pub fn tx_alloc(ctx: *mut tx_ctx, bytes: usize, d_out: *mut *mut c_void) -> c_int;
     pub fn tx_free(ctx: *mut tx_ctx, d_ptr: *mut c_void) -> c_int;
     pub fn tx_h2d(ctx: *mut tx_ctx, d_dst: *mut c_void, h_src: *const c_void, bytes: usize) -> c_int;

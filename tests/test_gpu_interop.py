@@ -116,3 +116,33 @@ def test_refusals():
         tx.from_dlpack(torch.zeros(4, device="cuda")).__dlpack__()
     tx.ones(3).__dlpack__()  # a capsule that nobody takes ends its loan
     tx.synchronize()
+
+
+def test_giving_memory_back_keeps_the_error():
+    """A kernel's error is raised by the next synchronisation, also when borrowed memory went before it."""
+    import torch
+
+    import tynx_b200 as tx
+
+    q, k, v = (tx.ones(1, 2, 2, 16), tx.ones(1, 4, 2, 16), tx.ones(1, 4, 1, 16))
+    lengths = tx.from_dlpack(torch.tensor([9], device="cuda"))
+    out = tx.nn.functional.differential_attention(q, k, v, tx.ones(1), key_lengths=lengths)
+    del lengths
+    gc.collect()
+    with pytest.raises(IndexError):
+        tx.synchronize()
+    assert out.shape == (1, 2, 1, 16)
+    tx.synchronize()
+
+
+def test_backward_from_an_output_twice_and_from_its_input():
+    """Roots may repeat, and one may lead to another: their gradients add."""
+    import tynx_b200 as tx
+
+    x = tx.ones(3).requires_grad_()
+    y = x * 2.0
+    z = y * 3.0
+    one = tx.ones(3)
+    tx.backward([y, z, y], [one, one, one])
+    np.testing.assert_array_equal(x.grad.numpy(), 2.0 * (1 + 3 + 1))
+    np.testing.assert_array_equal(one.numpy(), 1.0)

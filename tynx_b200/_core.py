@@ -1138,6 +1138,8 @@ def backward(tensors: Sequence[Tensor], gradients: Sequence[Tensor], retain_grap
             raise ValueError("backward() called on a tensor that does not require gradients")
         if g.shape != t.shape or g.dtype != "float32":
             raise ValueError(f"backward() needs a float32 gradient of shape {t.shape}, got {g.dtype} {g.shape}")
+        if g.ctx is not t.ctx:
+            raise ValueError(f"backward() got a gradient on {g.device} for a tensor on {t.device}")
     run_backward(list(zip(tensors, gradients)), retain_graph=retain_graph)
 
 

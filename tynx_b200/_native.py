@@ -141,6 +141,7 @@ SIGNATURES = {
     "tx_stream": [_vp, C.POINTER(_vp)],
     "tx_dlpack_export": [_vp, _vp, _vp, _i32, _p64, _i32, _vp, C.POINTER(_vp)],
     "tx_dlpack_release": [_vp],
+    "tx_dlpack_give_back": [_vp, _vp],
     "tx_alloc": [_vp, C.c_size_t, C.POINTER(_vp)],
     "tx_free": [_vp, _vp],
     "tx_h2d": [_vp, _vp, _vp, C.c_size_t],

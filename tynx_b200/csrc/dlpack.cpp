@@ -112,3 +112,12 @@ extern "C" int tx_dlpack_release(void *managed) {
   if (m && m->deleter) m->deleter(m);
   return TX_OK;
 }
+
+extern "C" int tx_dlpack_give_back(tx_ctx *ctx, void *managed) {
+  if (!ctx) return TX_ERR_INVALID;
+  if (ctx->capturing) return tx_fail(ctx, TX_ERR_CAPTURE, "borrowed memory cannot be given back during a capture");
+  // a stream that failed no longer uses the memory either
+  cudaStreamSynchronize(ctx->stream);
+  cudaStreamSynchronize(ctx->comm);
+  return tx_dlpack_release(managed);
+}

@@ -98,8 +98,7 @@ def _give_back(ctx: Context, managed: int) -> None:
     if ctx.capturing or threading.get_ident() != ctx.owner:
         _held.append((ctx, managed))
         return
-    lib.tx_sync(ctx.handle, 0)
-    lib.tx_dlpack_release(managed)
+    lib.tx_dlpack_give_back(ctx.handle, managed)
 
 
 def from_dlpack(source, device: Device | None = None) -> Tensor:
