@@ -130,3 +130,16 @@ def test_backward_refusals():
     for tensors, grads in [([y], []), ([t(2, 3)], [t(2, 3)]), ([y], [t(3, 2)]), ([y], [t(2, 3, dtype="int64")])]:
         with pytest.raises(ValueError):
             backward(tensors, grads)
+
+
+def test_values_that_do_not_fit_the_call_are_refused():
+    from tynx_b200 import backward
+
+    args = t(2, 3, 8, 16), t(2, 5, 4, 16), t(2, 5, 2, 32), t(4)
+    for start in (1 << 64, -(1 << 31)):
+        with pytest.raises(ValueError, match="query_start"):
+            F().differential_attention(*args, causal=True, query_start=start)
+    y = t(2, 3)
+    y.requires_grad = True
+    with pytest.raises(ValueError, match="gradient on"):
+        backward([y], [t(2, 3, ctx=SimpleNamespace(index=1))])

@@ -492,7 +492,6 @@ struct Operands {
   // made: q, k and v are there.  p: the backward's description, or null
   int fill(tx_ctx *ctx, const Shape &s, bool made, const tx_diff_attention *p, float *stats, float *sums) {
     if (!ok) return TX_ERR_OOM;
-    
     SplitJobs jobs{};
     jobs.j[0] = SplitJob{s.q, x.q, x.fq, nullptr, s.T, x.qt, 2 * s.H, s.d, s.scale * kLog2e, 0};
     jobs.j[1] = SplitJob{s.k, x.k, x.fk, nullptr, s.S, x.kt, 2 * s.Hk, s.d, 1.0f, 1};

@@ -6,6 +6,8 @@
 #include <cuda_fp16.h>
 #include <cudaTypedefs.h>
 
+#include <atomic>
+
 #include "common.h"
 
 namespace tx_diff {
@@ -61,7 +63,7 @@ __device__ __forceinline__ void sum_dlam(const Shape &s, const float *sums, int6
 
 // Grants a kernel its dynamic shared memory once a device.
 struct SmemGrant {
-  uint64_t devices = 0;
+  std::atomic<uint64_t> devices{0};  // contexts may live on threads of their own
   int take(tx_ctx *ctx, const void *kernel, int bytes) {
     const uint64_t bit = ctx->device < 64 ? uint64_t(1) << ctx->device : 0;
     if (devices & bit) return TX_OK;

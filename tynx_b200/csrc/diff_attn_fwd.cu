@@ -302,7 +302,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int t = w.t0 + r;
       const int seen = (int)s.seen(t < s.T ? t : s.T - 1, w.n) - w.tile0 * 128 - 64 * half;
       const float fq = __ldg(x.fq + (int64_t)(w.b * 2 * s.H + 2 * h + m) * x.qt + w.qt);
-      const float *fk = x.fk + (int64_t)(w.b * 2 * s.Hk + 2 * w.hk + m) * x.kt + w.tile0, *fv = x.fv + (int64_t)(w.b * s.Hk + w.hk) * x.kt + w.tile0;
+      const float *fk = x.fk + (int64_t)(w.b * 2 * s.Hk + 2 * w.hk + m) * x.kt + w.tile0;
+      const float *fv = x.fv + (int64_t)(w.b * s.Hk + w.hk) * x.kt + w.tile0;
       float ref = -INFINITY, top = -INFINITY;  // top: the maximum that ref was set by
       uint64_t sum2[2] = {two(0.f, 0.f), two(0.f, 0.f)};
 #pragma unroll
@@ -444,7 +445,6 @@ __global__ void __launch_bounds__(kThreads, 1)
         const bool four = (s.dv & 3) == 0 && ((uintptr_t)dst & 15) == 0;
         const int64_t stride = parts ? (int64_t)2 * s.G * o.parts.splits * s.dv : (int64_t)s.H * s.dv;
         float *base = parts ? dst + ((at0 * 2 + m) * o.parts.splits + w.split) * s.dv
-                            
                             : dst + ((int64_t)w.b * s.T * s.H + h) * s.dv;
         base += (w.t0 + quad * 32) * stride;
         const int rows = (int)s.T - w.t0 - quad * 32;

@@ -11,7 +11,8 @@
 //
 // Angles: w_i arrives as turns a position in 64 bits; p * turns is reduced to
 // its fraction there, so cosine and sine of far positions are as exact as
-// those of near ones (2^-25 of a turn), and nothing has to be tabulated.
+// those of near ones (2^-25 of a turn, up to 2^27 turns; then 2^-52 of the
+// angle), and nothing has to be tabulated.
 //
 // All of it is bound by memory: one pass reads x (and dy) and writes y (or dx)
 // once.  A block takes a few tokens with all their heads, works out the
@@ -241,7 +242,7 @@ __global__ void __launch_bounds__(kThreads, kBackBlocks)
     k_qk_norm_bwd(const __grid_constant__ Args A, const __grid_constant__ tx_rotary rot) {
   using L = Lane<VEC, INTER>;
   __shared__ float2 cs[kAngles];
-  __shared__ float sums[kThreads / 32][256];
+  __shared__ __align__(16) float sums[kThreads / 32][256];
   constexpr int SLOTS = kThreads / LANES, UN = 2;
   const int lane = threadIdx.x % LANES, slot = threadIdx.x / LANES;
   const RowShape s{A.dim, rot.dim >> 1};

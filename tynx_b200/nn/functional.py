@@ -263,6 +263,8 @@ def differential_attention(q: Tensor, k: Tensor, v: Tensor, lam: Tensor, *, scal
     if not math.isfinite(scale):
         raise ValueError(f"{name} scale must be finite, got {scale}")
     start = keys - queries if query_start is None else int(query_start)
+    if abs(start) > 1 << 30:
+        raise ValueError(f"{name} query_start must be within +-2^30, got {start}")
     ctx = q.ctx
     out = Tensor._empty((batch, queries, heads, dv), "float32", ctx)
     desc = N.DiffAttentionDesc(batch=batch, queries=queries, keys=keys, heads=heads, kv_heads=kv_heads, dim=d, vdim=dv,

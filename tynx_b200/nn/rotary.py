@@ -28,8 +28,9 @@ class Rotary:
       turn less than ``beta_slow`` (1) times and blends linearly between, and
       multiplies the rotated elements by ``attention_factor`` (0.1 ln f + 1).
 
-    Frequencies are 64-bit and angles are reduced in 64 bits on the device, so
-    positions may be any int64 value; nothing is stored on the device.
+    Frequencies are 64-bit and angles are reduced in 64 bits on the device (an
+    angle is off by 2^-52 of itself at most), so positions may be any int64 value;
+    nothing is stored on the device.
     """
 
     __slots__ = ("dim", "interleaved", "frequencies", "factor", "_desc")
