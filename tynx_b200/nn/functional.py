@@ -14,7 +14,7 @@ import math
 from typing import Optional
 
 from .. import _native as N
-from .._core import Fn, Tensor, _needs_grad, full, maximum
+from .._core import Fn, Storage, Tensor, _needs_grad, full, maximum
 from .._native import lib
 from .rotary import Rotary
 
@@ -267,23 +267,23 @@ def differential_attention(q: Tensor, k: Tensor, v: Tensor, lam: Tensor, *, scal
         raise ValueError(f"{name} query_start must be within +-2^30, got {start}")
     ctx = q.ctx
     out = Tensor._empty((batch, queries, heads, dv), "float32", ctx)
-    desc = N.DiffAttentionDesc(batch=batch, queries=queries, keys=keys, heads=heads, kv_heads=kv_heads, dim=d, vdim=dv,
-                               q=q.ptr, k=k.ptr, v=v.ptr, lam=lam.ptr,
-                               key_lengths=key_lengths.ptr if key_lengths is not None else None, scale=scale,
-                               causal=int(bool(causal)), query_start=start, out=out.ptr)
+    desc = N.DiffAttentionDesc(batch, queries, keys, heads, kv_heads, d, dv, q.ptr, k.ptr, v.ptr, lam.ptr,
+                               key_lengths.ptr if key_lengths is not None else None, scale, int(bool(causal)), start,
+                               out.ptr)
     grad = _needs_grad(q, k, v, lam)
     if grad:
-        out2 = Tensor._empty(out.shape, "float32", ctx)
-        lse = Tensor._empty((batch, maps, queries), "float32", ctx)
-        desc.out2, desc.lse = out2.ptr, lse.ptr
         size = C.c_int64()
         ctx.check(lib.tx_diff_attention_saved_bytes(ctx.handle, desc, C.byref(size)), name)
-        saved = Tensor._empty((size.value // 8 + 1,), "int64", ctx) if size.value else None
-        desc.saved = saved.ptr if saved is not None else None
+        # one block: the operands, out2 and lse, each from a 16-byte boundary
+        at = -(-size.value // 16) * 16
+        end = at + -(-out.nbytes // 16) * 16
+        kept = Storage(ctx, end + batch * maps * queries * 4)
+        desc.saved = kept.ptr if size.value else None
+        desc.out2, desc.lse = kept.ptr + at, kept.ptr + end
     ctx.check(lib.tx_diff_attention_fwd(ctx.handle, desc), name)
     if grad:
         # detached views keep what the description points to alive until this node is freed
-        held = [t.detach() for t in (q, k, v, lam, out)] + [out2, lse, saved, key_lengths]
+        held = [t.detach() for t in (q, k, v, lam, out)] + [kept, key_lengths]
         want = [t.requires_grad for t in (q, k, v, lam)]
 
         def backward(g):
