@@ -146,6 +146,29 @@ def test_few_queries_against_many_keys(queries, keys):
     check([out], val[:1], tol[:1])
 
 
+@pytest.mark.parametrize("case", [
+    (2, 64, 200, 4, 2, 64, 128, True, 136, None),
+    (1, 43, 43, 3, 1, 64, 128, True, 0, None),              # 129 rows: the last token's heads in two tiles
+    (3, 5, 333, 32, 1, 16, 33, True, 328, [333, 0, 7]),
+    (1, 129, 129, 4, 2, 40, 64, True, -1, [128]),           # the first query sees nothing
+    (2, 64, 4100, 4, 2, 64, 128, False, 0, [4100, 515]),    # keys in ranges, some of them empty
+    (1, 20, 1500, 6, 2, 64, 72, True, 1480, None),
+    (1, 300, 300, 10, 2, 64, 64, True, 0, None),
+], ids=lambda c: "x".join(map(str, c[:7])))
+def test_heads_that_share_keys_without_a_gradient(case):
+    """Queries of a group's heads share tiles where nothing is kept for a backward."""
+    import tynx_b200 as tx
+
+    B, T, S, H, Hk, d, dv, causal, start, lengths = case
+    q, k, v, lam, dout = arrays(B, T, S, H, Hk, d, dv, T + S + 1)
+    val, tol = reference(q, k, v, lam, dout, d ** -0.5, causal, start, lengths)
+    with tx.no_grad():
+        out = tx.nn.functional.differential_attention(
+            *(tx.Tensor(a) for a in (q, k, v, lam)), causal=causal, query_start=start,
+            key_lengths=None if lengths is None else tx.Tensor(np.asarray(lengths, np.int64)))
+    check([out], val[:1], tol[:1])
+
+
 def test_what_lies_behind_a_length_is_not_read():
     q, k, v, lam, dout = arrays(2, 70, 150, 2, 1, 64, 128, 5)
     lengths = [149, 70]

@@ -35,8 +35,10 @@ struct SplitJobs {
   int first;  // the first job to do
 };
 constexpr int kSplitThreads = 512, kSplitWarps = kSplitThreads / 32;
+// P: Shape::P heads' queries are the rows of one
 template <int W, bool STATS>
-__device__ __forceinline__ void split_tile(const Shape &s, const SplitJobs &jobs, const SplitJob &J, uint32_t *red) {
+__device__ __forceinline__ void split_tile(const Shape &s, const SplitJobs &jobs, const SplitJob &J, uint32_t *red,
+                                           int P = 1) {
   constexpr int PARTS = W / 8, ROWS = kSplitThreads / PARTS, UNITS = kRows / ROWS;  // 8 elements a thread and unit
   const int64_t head = (int64_t)blockIdx.x / J.tiles, tile = (int64_t)blockIdx.x - head * J.tiles;
   const int64_t b = head / J.heads, n0 = tile * kRows;
@@ -51,6 +53,10 @@ __device__ __forceinline__ void split_tile(const Shape &s, const SplitJobs &jobs
     for (int i = 0; i < 8; ++i) x[u][i] = 0.f;
     if (n < n_end) {
       const float *src = J.src + ((b * J.N + n) * J.heads + hh) * J.w + c;
+      if (P > 1) {
+        const int t = (int)n / P, g = (int)n - t * P;
+        src = J.src + ((b * J.N + (int64_t)t * P) * J.heads + (hh & ~1) * P + 2 * g + (hh & 1)) * J.w + c;
+      }
       if (four) {
 #pragma unroll
         for (int i = 0; i < 2; ++i)
@@ -179,6 +185,8 @@ __global__ void __launch_bounds__(kSplitThreads, 2)
   if ((int64_t)blockIdx.x >= s.B * J.heads * J.tiles) return;
   if (job == 3)
     split_tile<W, true>(s, jobs, J, red);
+  else if (job == 0 && s.P > 1)
+    split_tile<64, false>(s, jobs, J, red, s.P);
   else if (job < 2)
     split_tile<64, false>(s, jobs, J, red);
   else
@@ -366,16 +374,19 @@ __global__ void __launch_bounds__(kRowThreads, 2)
   }
 }
 
-// out, out2 and lse from the ranges' partial rows: a warp per query, head and map, four columns a
-// lane.  Latency alone: 32 ranges' references at a time, one a lane, then loads that do not depend on
-// one another.
-constexpr int kJoinRows = 4;  // a block at most
-__global__ void __launch_bounds__(64 * kJoinRows)
+// out, out2 and lse from the ranges' partial rows: W warps per query, head and map, each a share of the
+// ranges, four columns a lane.  Latency alone: 32 ranges' references at a time, one a lane, then U loads that
+// do not depend on one another.
+constexpr int kJoinRows = 4;  // a block at most, with W = 1
+template <int U, int W>
+__global__ void __launch_bounds__(64 * (W > 1 ? W : kJoinRows))
     k_diff_join(const __grid_constant__ Shape s, const Parts parts, float *out, float *out2, float *lse) {
-  __shared__ float4 second[kJoinRows][32];
-  const int lane = threadIdx.x & 31, m = (threadIdx.x >> 5) & 1, row = threadIdx.x >> 6, splits = parts.splits;
+  __shared__ float4 second[W > 1 ? 1 : kJoinRows][32], shares[W][2][32];
+  __shared__ float sums[W][2];
+  const int lane = threadIdx.x & 31, m = (threadIdx.x >> 5) & 1, splits = parts.splits;
+  const int row = W > 1 ? 0 : threadIdx.x >> 6, share = W > 1 ? threadIdx.x >> 6 : 0;
   const int64_t n_items = s.T * s.G, rows = s.B * s.Hk * n_items;
-  const int64_t at = (int64_t)blockIdx.x * (blockDim.x >> 6) + row;  // (b, hk, item)
+  const int64_t at = W > 1 ? blockIdx.x : (int64_t)blockIdx.x * (blockDim.x >> 6) + row;  // (b, hk, item)
   const bool live = at < rows;
   const float2 *ml = parts.ml + (live ? at * 2 + m : 0) * splits;
   // the first 32 ranges' references stay in registers
@@ -390,15 +401,16 @@ __global__ void __launch_bounds__(64 * kJoinRows)
   const float *p = parts.o + (live ? at * 2 + m : 0) * splits * s.dv + c;
   float sum = 0.f;
   float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (int i0 = 0; i0 < splits; i0 += 32) {
+  const int each = (splits + W - 1) / W, first = share * each, end = first + each < splits ? first + each : splits;
+  for (int i0 = first; i0 < end; i0 += 32) {
     const float2 v = i0 == 0 ? mine : i0 + lane < splits ? __ldg(ml + i0 + lane) : make_float2(-INFINITY, 0.f);
-    const float w = ex2(v.x - ref);
+    const int n = end - i0 < 32 ? end - i0 : 32;
+    const float w = lane < n ? ex2(v.x - ref) : 0.f;
     sum += v.y * w;
-    const int n = splits - i0 < 32 ? splits - i0 : 32;
-    for (int j = 0; j < n; j += 12) {  // loads of twelve ranges in flight
-      float4 y[12];
+    for (int j = 0; j < n; j += U) {
+      float4 y[U];
 #pragma unroll
-      for (int i = 0; i < 12; ++i) {
+      for (int i = 0; i < U; ++i) {
         y[i] = make_float4(0.f, 0.f, 0.f, 0.f);
         if (j + i < n) {
           const float *q = p + (int64_t)(i0 + j + i) * s.dv;
@@ -413,17 +425,32 @@ __global__ void __launch_bounds__(64 * kJoinRows)
         }
       }
 #pragma unroll
-      for (int i = 0; i < 12; ++i) {
+      for (int i = 0; i < U; ++i) {
         const float f = __shfl_sync(0xffffffffu, w, (j + i) & 31);
         if (j + i < n) x = make_float4(x.x + y[i].x * f, x.y + y[i].y * f, x.z + y[i].z * f, x.w + y[i].w * f);
       }
     }
   }
   sum = warp_sum(sum);
+  if (W > 1) {  // the warps' shares, in their order
+    shares[share][m][lane] = x;
+    if (lane == 0) sums[share][m] = sum;
+    __syncthreads();
+    if (share) return;
+#pragma unroll
+    for (int i = 1; i < W; ++i) {
+      const float4 y = shares[i][m][lane];
+      x = make_float4(x.x + y.x, x.y + y.y, x.z + y.z, x.w + y.w);
+      sum += sums[i][m];
+    }
+  }
   const float inv = none ? 0.f : 1.f / sum;
   x = make_float4(x.x * inv, x.y * inv, x.z * inv, x.w * inv);
   if (m) second[row][lane] = x;
-  __syncthreads();
+  if (W > 1)
+    asm volatile("bar.sync 1, 64;" ::: "memory");  // the two warps that are left
+  else
+    __syncthreads();
   if (!live) return;
   const int64_t bh = at / n_items, item = at - bh * n_items;
   const int64_t b = bh / s.Hk, t = item / s.G;
@@ -461,7 +488,7 @@ struct Operands {
   static int64_t tiles(int64_t rows) { return (rows + kRows - 1) / kRows; }
   static size_t bytes(const Shape &s) {
     const int64_t halves = 2 * (s.B * 2 * s.H * s.T * 64 + s.B * 2 * s.Hk * s.S * 64 + s.B * s.Hk * s.S * width(s));
-    return (size_t)halves * 2 + (size_t)(s.B * (2 * s.H * tiles(s.T) + 4 * s.Hk * tiles(s.S))) * 4;
+    return (size_t)halves * 2 + (size_t)(s.B * (2 * s.row_heads() * tiles(s.rows()) + 4 * s.Hk * tiles(s.S))) * 4;
   }
   static size_t grad_bytes(const Shape &s) {
     return (size_t)(s.B * s.H * s.T * 2 * width(s)) * 2 + (size_t)(2 * s.B * s.H * tiles(s.T)) * 4;
@@ -470,9 +497,9 @@ struct Operands {
       : own(ctx, saved ? 0 : bytes(s)), grad(ctx, gradient ? grad_bytes(s) : 0) {
     const int64_t w = width(s);
     x.vw = (int)w;
-    x.qt = tiles(s.T);
+    x.qt = tiles(s.rows());
     x.kt = tiles(s.S);
-    tq = s.B * 2 * s.H * x.qt, tk = s.B * 2 * s.Hk * x.kt, tv = s.B * s.Hk * x.kt, tg = s.B * s.H * x.qt;
+    tq = s.B * 2 * s.row_heads() * x.qt, tk = s.B * 2 * s.Hk * x.kt, tv = s.B * s.Hk * x.kt, tg = s.B * s.H * x.qt;
     ok = (saved || own.ptr) && (!gradient || grad.ptr);
     if (!ok) return;
     __half *p = reinterpret_cast<__half *>(saved ? saved : own.ptr);
@@ -493,7 +520,7 @@ struct Operands {
   int fill(tx_ctx *ctx, const Shape &s, bool made, const tx_diff_attention *p, float *stats, float *sums) {
     if (!ok) return TX_ERR_OOM;
     SplitJobs jobs{};
-    jobs.j[0] = SplitJob{s.q, x.q, x.fq, nullptr, s.T, x.qt, 2 * s.H, s.d, s.scale * kLog2e, 0};
+    jobs.j[0] = SplitJob{s.q, x.q, x.fq, nullptr, s.rows(), x.qt, 2 * s.row_heads(), s.d, s.scale * kLog2e, 0};
     jobs.j[1] = SplitJob{s.k, x.k, x.fk, nullptr, s.S, x.kt, 2 * s.Hk, s.d, 1.0f, 1};
     jobs.j[2] = SplitJob{s.v, x.v, x.fv, x.nv, s.S, x.kt, s.Hk, s.dv, 1.0f, 1};
     jobs.j[3] = SplitJob{p ? p->dout : nullptr, x.g, x.fg, x.ng, s.T, x.qt, s.H, s.dv, 1.0f, 0};
@@ -510,10 +537,14 @@ struct Operands {
   }
 };
 
-// Calls of so few queries take k_diff_rows, which reads keys and values once for every eight of them
-// and needs no split operands (8 x 8192 keys of 4 heads: 24 queries 276 us, on the tensor cores 298; 32
-// queries 409 and 312; 4096 keys of 2 heads: 26 and 31).
-bool few_queries(const Shape &s) { return s.T * s.G <= 24; }
+// Few queries take k_diff_rows, which reads keys and values once for every eight of them and needs no split
+// operands: eight (token, head of a group), or up to 24 against so few keys that the tensor cores' longer
+// way counts.  8 x 8192 keys of 4 heads: 8 queries 110 us, on the tensor cores 173; 16 queries 210 and 174.
+// 1 x 8192: 16 queries 36 and 37, 24 queries 47 and 38; 4 x 512: 24 queries 20 and 23.
+bool few_queries(const Shape &s) {
+  const int64_t rows = s.T * s.G, reads = (rows + 7) / 8;
+  return rows <= 8 || (rows <= 24 && reads * s.B * s.Hk * s.S <= 1 << 16);
+}
 
 int check_desc(tx_ctx *ctx, const tx_diff_attention *p, Shape &s) {
   if (!p) return tx_fail(ctx, TX_ERR_INVALID, "differential attention: no description");
@@ -532,14 +563,23 @@ int check_desc(tx_ctx *ctx, const tx_diff_attention *p, Shape &s) {
   if (!std::isfinite(p->scale)) return tx_fail(ctx, TX_ERR_INVALID, "differential attention: scale");
   s = Shape{p->batch, p->queries, p->keys, (int)p->heads, (int)p->kv_heads, (int)(p->heads / p->kv_heads), (int)p->dim,
             (int)p->vdim, p->q, p->k, p->v, p->lam, p->key_lengths, p->causal ? 1 : 0, p->query_start, p->scale,
-            ctx->d_err};
+            ctx->d_err, 1};
   return TX_OK;
 }
 
 int join(tx_ctx *ctx, const Shape &s, const Parts &parts, float *out, float *out2, float *lse) {
   const int64_t rows = s.B * s.T * s.H;
+  if (parts.splits > 12 && rows < 8 * ctx->num_sms) {  // many ranges of few rows (74 of 32 rows: 5.1 us for 9.2)
+    k_diff_join<12, 4><<<(unsigned)rows, 256, 0, ctx->stream>>>(s, parts, out, out2, lse);
+    TX_LAUNCHED(ctx, "k_diff_join");
+    return TX_OK;
+  }
   const int each = rows < 8 * ctx->num_sms ? 1 : kJoinRows;  // few rows: an SM each
-  k_diff_join<<<(unsigned)((rows + each - 1) / each), 64 * each, 0, ctx->stream>>>(s, parts, out, out2, lse);
+  const unsigned blocks = (unsigned)((rows + each - 1) / each);
+  if (parts.splits <= 4)  // (3 ranges of 8192 rows: 8.9 us, with twelve loads in flight 13.7)
+    k_diff_join<4, 1><<<blocks, 64 * each, 0, ctx->stream>>>(s, parts, out, out2, lse);
+  else
+    k_diff_join<12, 1><<<blocks, 64 * each, 0, ctx->stream>>>(s, parts, out, out2, lse);
   TX_LAUNCHED(ctx, "k_diff_join");
   return TX_OK;
 }
@@ -631,6 +671,11 @@ extern "C" int tx_diff_attention_fwd(tx_ctx *ctx, const tx_diff_attention *p) {
   if (s.T * s.G <= 2) return launch_rows<2>(ctx, s, p->out, p->out2, p->lse);
   if (s.T * s.G <= 4) return launch_rows<4>(ctx, s, p->out, p->out2, p->lse);
   if (few_queries(s)) return launch_rows<8>(ctx, s, p->out, p->out2, p->lse);
+  // fewer tiles when a group's heads share them (4 x 64 queries of 8 heads over 4 against 4096 keys: 27 us for
+  // 38; as many tiles cost more than one head's: 4 x 256 queries against 512 keys 25 us for 23)
+  if (!p->saved && s.T * s.G <= (int64_t)1 << 30 &&
+      Operands::tiles(s.T * s.G) < s.G * Operands::tiles(s.T))
+    s.P = s.G;
   Operands x(ctx, s, p->saved, false);
   TX_TRY(x.fill(ctx, s, false, nullptr, nullptr, nullptr));
   const int splits = tc_forward_splits(ctx, s);

@@ -24,7 +24,12 @@ struct Shape {
   int64_t start;
   float scale;
   int *err;
+  // Query rows of the tensor-core forward: P heads' queries in turn, row i is token i / P of the head i % P
+  // of its P.  G where nothing is kept for a backward, else 1.
+  int P;
 
+  __host__ __device__ __forceinline__ int64_t rows() const { return T * P; }
+  __host__ __device__ __forceinline__ int row_heads() const { return H / P; }
   __device__ __forceinline__ int64_t length(int64_t b) const {
     if (!len) return S;
     const int64_t n = __ldg(len + b);
@@ -97,7 +102,7 @@ __device__ __forceinline__ void report_length(const Shape &s, int64_t b) {
 // log2 e, so scores come out in powers of two) and 64 or 128 for values.
 constexpr int kRows = 128;  // rows of a tile
 struct Split {
-  __half *q, *k, *v, *g;         // [b][map or head][row][2 W]; g: the output's gradient
+  __half *q, *k, *v, *g;         // [b][map or head][row][2 W] (q: Shape::rows()); g: the output's gradient
   float *fq, *fk, *fv, *fg;      // f of each [b][map or head][tile]
   float *nv, *ng;                // the largest 2-norm of a tile's rows
   int vw;                        // W of v and g

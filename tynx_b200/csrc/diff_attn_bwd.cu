@@ -219,7 +219,7 @@ __device__ __forceinline__ void body(const Shape &s, const Split &x, const CUten
           for (int k = 0; k < 4; ++k) mma_ss(ts + m * 64, kdesc(rh_, k), kdesc(xh, k), id_s, 1u, one);
         }
       };
-      auto values = [&](int i) {  // dP of step i, in two halves: R_hi X_hi + R_lo X_hi and R_hi X_lo
+      auto values = [&](int i) {  // dP of step i, in two halves: R_hi X_hi, and the small products (their truncations cost nothing there)
         if (MODE != kModeV && ok) {
           ok = mma_wait(v_full, i & 1, abort_flag, s.err, 15);
           if (!ok) return;
@@ -230,7 +230,7 @@ __device__ __forceinline__ void body(const Shape &s, const Split &x, const CUten
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
               mma_ss(tmem + kDp, kdesc(rh_, k), kdesc(xh, k), id_p, (c || k) ? 1u : 0u, one);
-              mma_ss(tmem + kDp, kdesc(rl, k), kdesc(xh, k), id_s, 1u, one);
+              mma_ss(tmem + kDp + 64, kdesc(rl, k), kdesc(xh, k), id_s, 1u, one);
             }
           }
           mma_commit(v_empty, one);

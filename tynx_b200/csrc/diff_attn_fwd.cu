@@ -59,24 +59,26 @@ __device__ __forceinline__ void store4(float *dst, int c, float4 v, int dv, bool
   }
 }
 
-// One unit of work: a query tile of a head, and a range of its keys.
+// One unit of work: a query tile of a head (of a group's heads, Shape::P), and a range of its keys.
 struct Item {
-  int b, t0, n;  // sequence, first query, valid keys
+  int b, r0, n;  // sequence, first row, valid keys
   int h, hk, qt, split, tile0, tiles;
 };
 // Item `at` in the order of work: causal, the queries with most keys first.
+template <bool PACK>
 __device__ __forceinline__ Item item_at(const Shape &s, const Split &x, const Out &o, unsigned at) {
-  const unsigned heads = (unsigned)(s.B * s.H), blocks = (unsigned)x.qt * heads;
+  const int P = PACK ? s.P : 1, row_heads = PACK ? s.row_heads() : s.H;
+  const unsigned heads = (unsigned)s.B * row_heads, blocks = (unsigned)x.qt * heads;
   Item w;
   w.split = at / blocks;
   at -= w.split * blocks;
   const unsigned level = at / heads, bh = at - level * heads;
   w.qt = (int)x.qt - 1 - (int)level;
-  w.b = bh / s.H;
-  w.h = bh - w.b * s.H;
-  w.hk = w.h / s.G;
-  w.t0 = w.qt * 128;
-  const int tl = w.t0 + 127 < (int)s.T ? w.t0 + 127 : (int)s.T - 1;
+  w.b = bh / row_heads;
+  w.h = bh - w.b * row_heads;
+  w.hk = PACK ? w.h : w.h / s.G;
+  w.r0 = w.qt * 128;
+  const int rows = (int)s.T * P, last = w.r0 + 127 < rows ? w.r0 + 127 : rows - 1, tl = PACK ? last / P : last;
   w.n = (int)s.length(w.b);
   w.tile0 = w.split * o.per;
   const int all = ((int)s.seen(tl, w.n) + 127) / 128;
@@ -90,7 +92,8 @@ __device__ __forceinline__ bool item_of_round(unsigned items, int r, unsigned &a
   return at < items;
 }
 
-template <int DV>
+// PACK: rows are queries of a group's heads (Shape::P = G), otherwise one head's
+template <int DV, bool PACK>
 __global__ void __launch_bounds__(kThreads, 1)
     k_diff_fwd(const __grid_constant__ Shape s, const __grid_constant__ Split x, const __grid_constant__ CUtensorMap mq,
                const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtensorMap mv, Out o) {
@@ -109,7 +112,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_holder + 1);
   float *swap = reinterpret_cast<float *>(bars + 64);  // [map][half][row]
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
-  const unsigned items = (unsigned)(x.qt * s.B * s.H * o.parts.splits);
+  const int P = PACK ? s.P : 1, row_heads = PACK ? s.row_heads() : s.H;
+  const unsigned items = (unsigned)(x.qt * s.B * row_heads * o.parts.splits);
   const int rounds = (int)((items + gridDim.x - 1) / gridDim.x);
 
   if (threadIdx.x == 0) {
@@ -150,14 +154,14 @@ __global__ void __launch_bounds__(kThreads, 1)
       for (int r = 0; r < rounds && ok; ++r) {
         unsigned at;
         if (!item_of_round(items, r, at)) continue;
-        const Item w = item_at(s, x, o, at);
+        const Item w = item_at<PACK>(s, x, o, at);
         if (w.tiles) {
           if (nq) ok = bar_wait(q_empty, (nq - 1) & 1, abort_flag, s.err, 1);
           if (!ok) break;
           bar_expect(q_full, 2 * C::QK);
           for (int p = 0; p < 8; ++p)  // (map, head or tail, 64-row half)
-            tma_3d(sq + p * C::VBLK, &mq, q_full, (p >> 1 & 1) * 64, w.t0 + (p & 1) * 64,
-                   w.b * 2 * s.H + 2 * w.h + (p >> 2));
+            tma_3d(sq + p * C::VBLK, &mq, q_full, (p >> 1 & 1) * 64, w.r0 + (p & 1) * 64,
+                   w.b * 2 * row_heads + 2 * w.h + (p >> 2));
           ++nq;
         } else if (ni) {  // no phase is passed over: parities would repeat
           ok = bar_wait(staged, (ni - 1) & 1, abort_flag, s.err, 3);
@@ -201,7 +205,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       for (int r = 0; r < rounds && ok; ++r) {
         unsigned at;
         if (!item_of_round(items, r, at)) continue;
-        const int tiles = __shfl_sync(0xffffffffu, item_at(s, x, o, at).tiles, 0);
+        const int tiles = __shfl_sync(0xffffffffu, item_at<PACK>(s, x, o, at).tiles, 0);
         if (!tiles) continue;
         any = true;
         ok = mma_wait(q_full, nq & 1, abort_flag, s.err, 5);
@@ -296,12 +300,14 @@ __global__ void __launch_bounds__(kThreads, 1)
     for (int round = 0; round < rounds; ++round) {
       unsigned index;
       if (!item_of_round(items, round, index)) continue;
-      const Item w = item_at(s, x, o, index);
-      const int tiles = w.tiles, h = w.h;
-      if (threadIdx.x == 128 && h == 0 && w.qt == 0 && w.split == 0) report_length(s, w.b);
-      const int t = w.t0 + r;
-      const int seen = (int)s.seen(t < s.T ? t : s.T - 1, w.n) - w.tile0 * 128 - 64 * half;
-      const float fq = __ldg(x.fq + (int64_t)(w.b * 2 * s.H + 2 * h + m) * x.qt + w.qt);
+      const Item w = item_at<PACK>(s, x, o, index);
+      const int tiles = w.tiles;
+      if (threadIdx.x == 128 && w.h == 0 && w.qt == 0 && w.split == 0) report_length(s, w.b);
+      // this thread's row is query row / P of the head w.h * P + row % P
+      const int rows = (int)s.T * P, row = w.r0 + r;
+      const int at_row = row < rows ? row : rows - 1;
+      const int seen = (int)s.seen(PACK ? at_row / P : at_row, w.n) - w.tile0 * 128 - 64 * half;
+      const float fq = __ldg(x.fq + (int64_t)(w.b * 2 * row_heads + 2 * w.h + m) * x.qt + w.qt);
       const float *fk = x.fk + (int64_t)(w.b * 2 * s.Hk + 2 * w.hk + m) * x.kt + w.tile0;
       const float *fv = x.fv + (int64_t)(w.b * s.Hk + w.hk) * x.kt + w.tile0;
       float ref = -INFINITY, top = -INFINITY;  // top: the maximum that ref was set by
@@ -388,16 +394,18 @@ __global__ void __launch_bounds__(kThreads, 1)
       untwo(sum2[0], s0, s1);
       untwo(sum2[1], s2, s3);
       const float part = (s0 + s1) + (s2 + s3);
+      const int t = PACK ? row / P : row, h = PACK ? w.h * P + (row - t * P) : w.h;
       pair_sync();  // both have read the last maxima
       *mine = part;
       pair_sync();
       const float sum = half ? *other + part : part + *other;
-      const bool none = top == -INFINITY, live = t < s.T && ok;
+      const bool none = top == -INFINITY, live = row < rows && ok;
       const bool parts = o.parts.splits > 1;
       const float inv = parts ? 1.f : none ? 0.f : 1.0f / sum;
-      const int64_t at0 = (int64_t)(w.b * s.Hk + w.hk) * s.T * s.G + (h - w.hk * s.G);  // + t * G
+      const int64_t at0 = (int64_t)(w.b * s.Hk + w.hk) * s.T * s.G + (PACK ? 0 : h - w.hk * s.G);  // row 0
+      const int next = PACK ? 1 : s.G;
       if (live && parts && half == 0)
-        o.parts.ml[((at0 + t * s.G) * 2 + m) * o.parts.splits + w.split] = make_float2(none ? -INFINITY : ref, sum);
+        o.parts.ml[((at0 + (int64_t)row * next) * 2 + m) * o.parts.splits + w.split] = make_float2(none ? -INFINITY : ref, sum);
       if (live && !parts && o.lse && half == 0)
         o.lse[(int64_t)(w.b * 2 * s.H + 2 * h + m) * s.T + t] = none ? INFINITY : ref + log2f(sum);
       const uint64_t inv2 = two(inv, inv);
@@ -441,13 +449,18 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (ok && dst) {
         constexpr int CW = C::CW, CH = CW / 4;  // columns and 16-byte chunks of a staged row
         float4 *box = reinterpret_cast<float4 *>(sm + 4 * C::QK + (warp - 4) * (32 * CW * 4));
-        auto place = [&](int row, int c) { return box + row * CH + (c ^ (CH == 8 ? row & 7 : row >> 1 & 3)); };
+        auto place = [&](int i, int c) { return box + i * CH + (c ^ (CH == 8 ? i & 7 : i >> 1 & 3)); };
         const bool four = (s.dv & 3) == 0 && ((uintptr_t)dst & 15) == 0;
-        const int64_t stride = parts ? (int64_t)2 * s.G * o.parts.splits * s.dv : (int64_t)s.H * s.dv;
+        // partial rows follow one another, a packed tile's output rows go P heads a token
+        const int64_t stride = parts ? (int64_t)2 * next * o.parts.splits * s.dv : (int64_t)s.H * s.dv;
+        const bool turns = PACK && !parts;
         float *base = parts ? dst + ((at0 * 2 + m) * o.parts.splits + w.split) * s.dv
-                            : dst + ((int64_t)w.b * s.T * s.H + h) * s.dv;
-        base += (w.t0 + quad * 32) * stride;
-        const int rows = (int)s.T - w.t0 - quad * 32;
+                            : dst + ((int64_t)w.b * s.T * s.H + w.h * P) * s.dv;
+        const int row0 = w.r0 + quad * 32;
+        if (!turns) base += row0 * stride;
+        auto row_at = [&](int i) {
+          return turns ? base + (row0 + i) / P * stride + (row0 + i) % P * s.dv : base + i * stride;
+        };
 #pragma unroll
         for (int c0 = 0; c0 < DH / CW; ++c0) {
 #pragma unroll
@@ -461,8 +474,8 @@ __global__ void __launch_bounds__(kThreads, 1)
           const int c = lane % CH;
 #pragma unroll
           for (int k = 0; k < CH; ++k) {
-            const int row = k * (32 / CH) + lane / CH;
-            if (row < rows) store4(base + row * stride, half * DH + c0 * CW + 4 * c, *place(row, c), s.dv, four);
+            const int i = k * (32 / CH) + lane / CH;
+            if (row0 + i < rows) store4(row_at(i), half * DH + c0 * CW + 4 * c, *place(i, c), s.dv, four);
           }
           __syncwarp();
         }
@@ -481,17 +494,17 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
 }
 
-template <int DV>
+template <int DV, bool PACK>
 int launch(tx_ctx *ctx, const Shape &s, const Split &x, const Out &o) {
   CUtensorMap mq, mk, mv;
-  if (!split_map(&mq, x.q, 64, s.T, s.B * 2 * s.H) || !split_map(&mk, x.k, 64, s.S, s.B * 2 * s.Hk) ||
+  if (!split_map(&mq, x.q, 64, s.rows(), s.B * 2 * s.row_heads()) || !split_map(&mk, x.k, 64, s.S, s.B * 2 * s.Hk) ||
       !split_map(&mv, x.v, DV, s.S, s.B * s.Hk))
     return tx_fail(ctx, TX_ERR_UNSUPPORTED, "differential attention: tensor map");
   static SmemGrant granted;
-  TX_TRY(granted.take(ctx, (const void *)k_diff_fwd<DV>, Cfg<DV>::SMEM));
-  const int64_t items = x.qt * s.B * s.H * o.parts.splits;
+  TX_TRY(granted.take(ctx, (const void *)k_diff_fwd<DV, PACK>, Cfg<DV>::SMEM));
+  const int64_t items = x.qt * s.B * s.row_heads() * o.parts.splits;
   const unsigned blocks = (unsigned)(items < ctx->num_sms ? items : ctx->num_sms);
-  k_diff_fwd<DV><<<blocks, kThreads, Cfg<DV>::SMEM, ctx->stream>>>(s, x, mq, mk, mv, o);
+  k_diff_fwd<DV, PACK><<<blocks, kThreads, Cfg<DV>::SMEM, ctx->stream>>>(s, x, mq, mk, mv, o);
   TX_LAUNCHED(ctx, "k_diff_fwd");
   return TX_OK;
 }
@@ -499,17 +512,22 @@ int launch(tx_ctx *ctx, const Shape &s, const Split &x, const Out &o) {
 }  // namespace
 
 int tc_forward_splits(tx_ctx *ctx, const Shape &s) {
-  // too few blocks of queries for the SMs: the keys are shared out too, two tiles at least a block
-  const int64_t blocks = (s.T + kRows - 1) / kRows * s.B * s.H, tiles = (s.S + kRows - 1) / kRows;
-  int64_t splits = ctx->num_sms / (blocks ? blocks : 1);
-  if (splits > (tiles + 1) / 2) splits = (tiles + 1) / 2;
-  return splits < 3 ? 1 : (int)splits;  // two ranges do not earn their join (60 blocks of 1 to 4 tiles: 17 + 8 us for 20)
+  // Too few query tiles for the SMs: the keys are shared out too, one range a block, where the tiles of keys
+  // that a block is spared (3.4 us each) are worth the join (4 us and 1 us for 1600 rows and heads).
+  const int64_t blocks = (s.rows() + kRows - 1) / kRows * s.B * s.row_heads(), tiles = (s.S + kRows - 1) / kRows;
+  int64_t splits = blocks ? ctx->num_sms / blocks : 1;
+  if (splits < 2) return 1;
+  const int64_t per = (tiles + splits - 1) / splits;
+  splits = (tiles + per - 1) / per;
+  const double spared = 3.4 * (double)(tiles - per), join = 4.0 + (double)(s.B * s.T * s.H) / 1600.0;
+  return spared > join ? (int)splits : 1;
 }
 
 int tc_forward(tx_ctx *ctx, const Shape &s, const Split &x, float *out, float *out2, float *lse, const Parts &parts) {
   const int64_t tiles = (s.S + kRows - 1) / kRows;
   const Out o{out, out2, lse, parts, (int)((tiles + parts.splits - 1) / parts.splits)};
-  return x.vw == 64 ? launch<64>(ctx, s, x, o) : launch<128>(ctx, s, x, o);
+  if (s.P > 1) return x.vw == 64 ? launch<64, true>(ctx, s, x, o) : launch<128, true>(ctx, s, x, o);
+  return x.vw == 64 ? launch<64, false>(ctx, s, x, o) : launch<128, false>(ctx, s, x, o);
 }
 
 }  // namespace tx_diff
