@@ -215,22 +215,28 @@ __global__ void __launch_bounds__(kThreads, 1)
             const uint32_t ts = tmem + m * 128, to = tmem + 256 + m * DV;
             if (i) {  // O = P V of the tile before
               ok = mma_wait(p_full + m, (nt + i - 1) & 1, abort_flag, s.err, 6);
-              for (int hf = 0; hf < 2 && ok; ++hf) {
-                const int u = nv + 2 * (i - 1) + hf, slot = u % C::RING;
-                ok = mma_wait(v_full + slot, (u / C::RING) & 1, abort_flag, s.err, 7);
+              // the small products of both halves first: truncation then takes from small sums
+              const int u = nv + 2 * (i - 1), slots[2] = {u % C::RING, (u + 1) % C::RING};
+#pragma unroll
+              for (int hf = 0; hf < 2; ++hf) {
+                ok = ok && mma_wait(v_full + slots[hf], ((u + hf) / C::RING) & 1, abort_flag, s.err, 7);
                 if (!ok) break;
                 fence_after();
-                const uint32_t vh = sv + slot * C::VSLOT, vl = vh + (DV / 64) * C::VBLK;
-                // the small products first: truncation then takes from small sums
+                const uint32_t vh = sv + slots[hf] * C::VSLOT, vl = vh + (DV / 64) * C::VBLK;
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
                   const uint32_t ph = ts + (hf * 4 + k) * 16;
                   mma_ts(to, ph, ndesc(vl, k, C::VBLK), id_o, (hf || k) ? 1u : 0u, one);
                   mma_ts(to, ph + 8, ndesc(vh, k, C::VBLK), id_o, 1u, one);
                 }
+              }
+              if (!ok) break;
+#pragma unroll
+              for (int hf = 0; hf < 2; ++hf) {
+                const uint32_t vh = sv + slots[hf] * C::VSLOT;
 #pragma unroll
                 for (int k = 0; k < 4; ++k) mma_ts(to, ts + (hf * 4 + k) * 16, ndesc(vh, k, C::VBLK), id_o, 1u, one);
-                if (m) mma_commit(v_empty + slot, one);
+                if (m) mma_commit(v_empty + slots[hf], one);
               }
               mma_commit(o_full + m, one);
             }
