@@ -23,11 +23,13 @@
 // An instruction of 128 rows takes 64 cycles whether it makes 64 or 128 columns.
 // So dP multiplies R_hi with X_hi and X_lo side by side (their halves are added
 // elementwise): a step takes 24 instructions for S, 16 for dP and 24 for the sums
-// in K and Q blocks, 4096 cycles, and 24 + 12 in V blocks, 2304.  What bounds the
-// kernel is the tensor core, at the power limit's clock for large problems: 2 x
-// 2048 causal tokens of 8 heads over 4 take 253 us (with dP as three products 260;
-// with a step's S alone in TMEM 421), 256 sequences of 128 tokens of 2 heads, where
-// a block has two steps and its start and stores count as much, 144 us.
+// in K and Q blocks, 4096 cycles, and 24 + 12 in V blocks, 2304.  2 x 2048 causal
+// tokens of 8 heads over 4 take 253 us (with dP as three products 260; with a
+// step's S alone in TMEM 421): these instructions are 309 of the 427 thousand
+// cycles an SM is busy, and where a step's elementwise chain (about 500
+// instructions a warp, four warps a scheduler) is behind, the tensor core waits.
+// 256 sequences of 128 tokens of 2 heads, where a block has two steps and its
+// start and stores count as much, take 144 us.
 #include "diff_attn.cuh"
 
 namespace tx_diff {

@@ -20,7 +20,12 @@
 // and a ring of three half value tiles (96 KB).
 // One CTA an SM takes (query tile, head) after (query tile, head): while its
 // warps store one's rows (through the value ring, so that whole lines go out),
-// the next one's Q and K arrive and its first scores are multiplied.
+// the next one's Q and K arrive and its first scores are multiplied.  Where few
+// queries would leave tiles half empty, a tile holds the queries of all heads
+// that share a key head (PACK).
+// 8192 causal tokens of 8 heads: 428 to 446 us, 628 GFLOP of fp16 products, the
+// tensor cores' sustained rate under the power limit; 4 x 64 queries of 8 heads
+// over 4 against 4096 keys: 27 us, four tiles a block.
 #include "diff_attn.cuh"
 
 namespace tx_diff {
