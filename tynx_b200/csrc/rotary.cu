@@ -20,9 +20,10 @@
 // of one a pair and head), and walks the (token, head) rows with 8 elements a
 // lane, so a row of 128 takes half a warp and both elements of every pair sit
 // in one lane: the rotation needs no exchange, the norm a shuffle sum over the
-// row's lanes.  Rows whose elements cannot be taken four at a time
-// (head_dim, or in halves also dim, no multiple of 8, unaligned) run the same code with a warp a row
-// and single-element accesses.
+// row's lanes.  Rows whose elements cannot be taken four at a time (head_dim, or
+// in halves also dim, no multiple of 8, unaligned) run the same code with single
+// elements: 6 x 3770 tokens of 24 heads of 40 with norms take 52 us forward and 99
+// backward, twice the floor (with a warp a row 197 and 348).
 #include "common.h"
 
 namespace {
@@ -43,11 +44,11 @@ struct RowShape {
 // VEC: the lane holds two float4 of unit u: pairs 4 u .. 4 u + 3 as elements 4 u
 // and half + 4 u (behind the rotating part 8 consecutive elements); interleaved,
 // elements 4 u and dim / 2 + 4 u, two pairs each, so that a warp's accesses are
-// whole lines either way.  Otherwise pairs lane + 32 i one by one.
-template <bool VEC, bool INTER>
+// whole lines either way.  Otherwise pairs lane + LANES i one by one.
+template <bool VEC, bool INTER, int LANES>
 struct Lane {
   static __device__ __forceinline__ int pair(const RowShape s, int lane, int i) {
-    if (!VEC) return lane + 32 * i;
+    if (!VEC) return lane + LANES * i;
     if (INTER) return (i < 2 ? 0 : s.dim >> 2) + 2 * lane + (i & 1);
     return 4 * lane + i;
   }
@@ -140,11 +141,11 @@ __device__ __forceinline__ void fill_angles(float2 *cs, const tx_rotary &rot, co
   }
 }
 
-template <bool VEC, bool INTER, bool BACK>
+template <bool VEC, bool INTER, int LANES, bool BACK>
 __device__ __forceinline__ void turn(Eight &e, const float2 *cs, const RowShape s, int lane) {
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const int p = Lane<VEC, INTER>::pair(s, lane, i);
+    const int p = Lane<VEC, INTER, LANES>::pair(s, lane, i);
     if (p < s.half) {
       const float2 a = cs[p];
       const float s = BACK ? -a.y : a.y, lo = e.lo[i], hi = e.hi[i];
@@ -176,7 +177,7 @@ struct Args {
 template <bool VEC, bool INTER, int LANES, bool NORM, bool BACK>
 __global__ void __launch_bounds__(kThreads, VEC ? (NORM ? 3 : 4) : 2)
     k_rotary(const __grid_constant__ Args A, const __grid_constant__ tx_rotary rot) {
-  using L = Lane<VEC, INTER>;
+  using L = Lane<VEC, INTER, LANES>;
   __shared__ float2 cs[kAngles];
   constexpr int SLOTS = kThreads / LANES, UN = 2;
   const int lane = threadIdx.x % LANES, slot = threadIdx.x / LANES;
@@ -227,7 +228,7 @@ __global__ void __launch_bounds__(kThreads, VEC ? (NORM ? 3 : 4) : 2)
       }
       if (r < rows) {
         const int token = second ? (r - rows0) / A.heads[1] : r / A.heads[0];
-        turn<VEC, INTER, BACK>(e[u], cs + token * s.half, s, lane);
+        turn<VEC, INTER, LANES, BACK>(e[u], cs + token * s.half, s, lane);
         L::store(row_of(A.y, r), s, lane, e[u]);
       }
     }
@@ -240,7 +241,7 @@ constexpr int kBackBlocks = 3;  // resident blocks an SM
 template <bool VEC, bool INTER, int LANES>
 __global__ void __launch_bounds__(kThreads, kBackBlocks)
     k_qk_norm_bwd(const __grid_constant__ Args A, const __grid_constant__ tx_rotary rot) {
-  using L = Lane<VEC, INTER>;
+  using L = Lane<VEC, INTER, LANES>;
   __shared__ float2 cs[kAngles];
   __shared__ __align__(16) float sums[kThreads / 32][256];
   constexpr int SLOTS = kThreads / LANES, UN = 2;
@@ -277,7 +278,7 @@ __global__ void __launch_bounds__(kThreads, kBackBlocks)
 #pragma unroll
         for (int u = 0; u < UN; ++u) {
           const int r = r0 + u * SLOTS;
-          if (r < rows) turn<VEC, INTER, true>(g[u], cs + (r / H) * s.half, s, lane);
+          if (r < rows) turn<VEC, INTER, LANES, true>(g[u], cs + (r / H) * s.half, s, lane);
           float ss = 0.f, dot = 0.f;
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
@@ -392,12 +393,17 @@ int launch_rows(tx_ctx *ctx, Args &A, const tx_rotary &rot, int mode, float *dqw
   return TX_OK;
 }
 
+template <bool VEC, bool INTER>
+int launch_width(tx_ctx *ctx, Args &A, const tx_rotary &rot, int mode, float *dqw, float *dkw) {
+  if (A.dim <= 64) return launch_rows<VEC, INTER, 8>(ctx, A, rot, mode, dqw, dkw);
+  if (A.dim <= 128) return launch_rows<VEC, INTER, 16>(ctx, A, rot, mode, dqw, dkw);
+  return launch_rows<VEC, INTER, 32>(ctx, A, rot, mode, dqw, dkw);
+}
+
 template <bool INTER>
 int launch_layout(tx_ctx *ctx, Args &A, const tx_rotary &rot, int mode, bool vec, float *dqw, float *dkw) {
-  if (!vec) return launch_rows<false, INTER, 32>(ctx, A, rot, mode, dqw, dkw);
-  if (A.dim <= 64) return launch_rows<true, INTER, 8>(ctx, A, rot, mode, dqw, dkw);
-  if (A.dim <= 128) return launch_rows<true, INTER, 16>(ctx, A, rot, mode, dqw, dkw);
-  return launch_rows<true, INTER, 32>(ctx, A, rot, mode, dqw, dkw);
+  return vec ? launch_width<true, INTER>(ctx, A, rot, mode, dqw, dkw)
+             : launch_width<false, INTER>(ctx, A, rot, mode, dqw, dkw);
 }
 
 int launch(tx_ctx *ctx, Args &A, const tx_rotary &rot, int mode, float *dqw = nullptr, float *dkw = nullptr) {
