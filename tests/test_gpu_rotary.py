@@ -120,6 +120,33 @@ def test_norms_with_the_rotation(interleaved, batch, seq, heads, kv, dim, rot):
         close(leaves[i + 2].grad, dw, 1e-5, total)
 
 
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("dim,rot", [(8, 8), (12, 12), (16, 8), (24, 10), (24, 24), (32, 32), (30, 16), (40, 20)])
+def test_narrow_heads(interleaved, dim, rot):
+    """Several rows share a warp."""
+    import tynx_b200 as tx
+
+    rng = np.random.default_rng(dim + rot)
+    rotary = tx.nn.Rotary(rot, interleaved=interleaved)
+    q, dq = (rng.standard_normal((3, 211, 7, dim)).astype(np.float32) for _ in range(2))
+    k, dk = (rng.standard_normal((3, 211, 1, dim)).astype(np.float32) for _ in range(2))
+    qw, kw = (1 + 0.2 * rng.standard_normal(dim).astype(np.float32) for _ in range(2))
+    positions = np.broadcast_to(np.arange(211), (3, 211))
+    leaves = [tx.Tensor(a, requires_grad=True) for a in (q, k, qw, kw)]
+    outs = tx.nn.functional.qk_norm_rotary(*leaves, rotary, eps=1e-5)
+    tx.backward(outs, [tx.Tensor(dq), tx.Tensor(dk)])
+    for i, (x, w, dy) in enumerate(((q, qw, dq), (k, kw, dk))):
+        y, dx, dw, size, total = norm_reference(x, w, rotary, positions, 1e-5, dy)
+        close(outs[i], y, 2e-6)
+        close(leaves[i].grad, dx, 4e-6, size)
+        close(leaves[i + 2].grad, dw, 1e-5, total)
+    x = tx.Tensor(q, requires_grad=True)
+    y = tx.nn.functional.rotary_embedding(x, rotary)
+    y.backward(tx.Tensor(dq))
+    close(y, turned(q, rotary, positions), 1e-6)
+    close(x.grad, turned(dq, rotary, positions, back=True), 1e-6)
+
+
 def test_rows_of_zeros_and_repeated_calls():
     """A row of zeros has a finite norm through eps; the same inputs give the same bits."""
     import tynx_b200 as tx

@@ -395,6 +395,8 @@ int launch_rows(tx_ctx *ctx, Args &A, const tx_rotary &rot, int mode, float *dqw
 
 template <bool VEC, bool INTER>
 int launch_width(tx_ctx *ctx, Args &A, const tx_rotary &rot, int mode, float *dqw, float *dkw) {
+  if (A.dim <= 16) return launch_rows<VEC, INTER, 2>(ctx, A, rot, mode, dqw, dkw);
+  if (A.dim <= 32) return launch_rows<VEC, INTER, 4>(ctx, A, rot, mode, dqw, dkw);
   if (A.dim <= 64) return launch_rows<VEC, INTER, 8>(ctx, A, rot, mode, dqw, dkw);
   if (A.dim <= 128) return launch_rows<VEC, INTER, 16>(ctx, A, rot, mode, dqw, dkw);
   return launch_rows<VEC, INTER, 32>(ctx, A, rot, mode, dqw, dkw);
