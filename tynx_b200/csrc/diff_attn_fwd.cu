@@ -205,6 +205,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     } else if (warp == 1) {
       const uint32_t one = elect_one();
       constexpr uint32_t id_s = idesc(128, false), id_o = idesc(DV, true);
+      const int slices = (s.d + 15) / 16;  // of queries and keys; zeros behind them
       bool ok = true, any = false;
       int nq = 0, nt = 0, nv = 0;  // items with keys, tiles and half value tiles so far
       for (int r = 0; r < rounds && ok; ++r) {
@@ -251,12 +252,14 @@ __global__ void __launch_bounds__(kThreads, 1)
               fence_after();
               const uint32_t qh = sq + m * C::QK, ql = qh + C::HALF, kh = sk + m * C::QK, kl = kh + C::HALF;
 #pragma unroll
-              for (int k = 0; k < 4; ++k) {
-                mma_ss(ts, kdesc(qh, k), kdesc(kl, k), id_s, k ? 1u : 0u, one);
-                mma_ss(ts, kdesc(ql, k), kdesc(kh, k), id_s, 1u, one);
-              }
+              for (int k = 0; k < 4; ++k)
+                if (k < slices) {
+                  mma_ss(ts, kdesc(qh, k), kdesc(kl, k), id_s, k ? 1u : 0u, one);
+                  mma_ss(ts, kdesc(ql, k), kdesc(kh, k), id_s, 1u, one);
+                }
 #pragma unroll
-              for (int k = 0; k < 4; ++k) mma_ss(ts, kdesc(qh, k), kdesc(kh, k), id_s, 1u, one);
+              for (int k = 0; k < 4; ++k)
+                if (k < slices) mma_ss(ts, kdesc(qh, k), kdesc(kh, k), id_s, 1u, one);
               mma_commit(k_empty + m, one);
               mma_commit(s_full + m, one);
               if (m && i == tiles - 1) mma_commit(q_empty, one);
