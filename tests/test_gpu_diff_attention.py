@@ -169,6 +169,44 @@ def test_heads_that_share_keys_without_a_gradient(case):
     check([out], val[:1], tol[:1])
 
 
+@pytest.mark.parametrize("weight", [1.0, -40.0, 0.0])
+@pytest.mark.parametrize("case", [
+    (25, 62, 62, 6, 2, 64, 72, True, 0, [62, 5, 0, 1, 61] * 5),
+    (13, 26, 285, 12, 4, 64, 64, False, 0, None),
+    (3, 64, 300, 64, 2, 16, 24, True, 236, [299, 300, 1]),  # 32 heads a group: 2048 rows
+    (5, 7, 50, 33, 1, 8, 16, False, 0, None),
+    (26, 50, 20, 6, 2, 40, 128, True, -30, None),           # the first queries see nothing
+    (75, 64, 64, 2, 1, 64, 128, True, 0, None),             # exactly one tile
+    (50, 43, 43, 3, 1, 64, 128, True, 0, None),             # 129 rows
+    (30, 2, 9, 6, 2, 33, 65, True, 7, None),
+    (2, 62, 62, 6, 2, 64, 72, True, 0, [62, 5]),            # too few heads: a tile each
+], ids=lambda c: "x".join(map(str, c[:7])))
+def test_short_sequences_whose_heads_share_keys(case, weight):
+    """Up to 64 tokens of many heads, forward and backward take a group's queries as rows of one tile; each row
+    and column then has its own head's weight."""
+    B, T, S, H, Hk, d, dv, causal, start, lengths = case
+    q, k, v, lam, dout = arrays(B, T, S, H, Hk, d, dv, T + S + 2)
+    lam *= np.float32(weight)
+    val, tol = reference(q, k, v, lam, dout, d ** -0.5, causal, start, lengths)
+    check(call(q, k, v, lam, dout, causal=causal, query_start=start, lengths=lengths), val, tol)
+
+
+@pytest.mark.parametrize("shape", [(50, 43, 43, 3, 1, 64, 128), (2, 43, 70, 3, 1, 40, 64)], ids=["shared", "own"])
+def test_each_gradient_alone(shape):
+    """Whichever inputs want a gradient, it is the one that all of them get together."""
+    import tynx_b200 as tx
+
+    q, k, v, lam, dout = arrays(*shape, 31)
+    kw = dict(causal=True, query_start=0)
+    together = call(q, k, v, lam, dout, lengths=None, **kw)[1:]
+    for wanted in range(4):
+        leaves = [tx.Tensor(a, requires_grad=i == wanted) for i, a in enumerate((q, k, v, lam))]
+        tx.nn.functional.differential_attention(*leaves, **kw).backward(tx.Tensor(dout))
+        for i, t in enumerate(leaves):
+            assert (t.grad is None) == (i != wanted)
+        np.testing.assert_array_equal(leaves[wanted].grad.numpy(), together[wanted].numpy())
+
+
 def test_what_lies_behind_a_length_is_not_read():
     q, k, v, lam, dout = arrays(2, 70, 150, 2, 1, 64, 128, 5)
     lengths = [149, 70]

@@ -208,8 +208,14 @@ class Storage:
     def __init__(self, ctx: Context, nbytes: int, ptr: Optional[int] = None, owned: bool = True):
         self.ctx = ctx
         self.nbytes = nbytes
-        self.owned = owned and ptr is None
-        self.ptr = ctx.alloc(nbytes) if ptr is None else ptr
+        if ptr is not None:
+            self.ptr, self.owned = ptr, False
+        else:
+            code = lib.tx_alloc(ctx.handle, nbytes or 1, ctx._out_ref)
+            if code:
+                self.owned = False
+                N.raise_for(code, ctx.handle, "alloc")
+            self.ptr, self.owned = ctx._out.value, owned
 
     def __del__(self):
         if self.owned and self.ptr:
@@ -354,6 +360,16 @@ class Tensor:
         shape = _shape_tuple(shape)
         t = object.__new__(cls)
         t._storage, t._offset, t.shape, t.dtype = Storage(ctx, _numel(shape) * _DTYPES[dtype][1]), 0, shape, dtype
+        t.requires_grad = False
+        t._grad = t._fn = None
+        t._out_index = 0
+        return t
+
+    @classmethod
+    def _new(cls, shape: tuple, ctx: Context) -> "Tensor":
+        """Uninitialised float32 memory of a shape that comes from Tensors."""
+        t = object.__new__(cls)
+        t._storage, t._offset, t.shape, t.dtype = Storage(ctx, 4 * math.prod(shape)), 0, shape, "float32"
         t.requires_grad = False
         t._grad = t._fn = None
         t._out_index = 0

@@ -31,21 +31,28 @@ struct SplitJob {
 struct SplitJobs {
   SplitJob j[4];
   // with the output's gradient (job 3) its rows' D1 = dO . (out + lam out2) and D2 = dO . out2 go to
-  // stats, beside lse, and each tile's sum of D2 to sums
+  // stats, beside lse, and each tile's sum of D2 (P > 1: each head's in the tile) to sums
   const float *out, *out2, *lse;
   float *stats, *sums;
   int first;  // the first job to do
 };
 constexpr int kSplitThreads = 512, kSplitWarps = kSplitThreads / 32;
-// P: Shape::P heads' queries are the rows of one
-template <int W, bool STATS>
+// PACK: Shape::P heads' queries are the rows of one
+template <int W, bool STATS, bool PACK>
 __device__ __forceinline__ void split_tile(const Shape &s, const SplitJobs &jobs, const SplitJob &J, uint32_t *red,
-                                           int P = 1) {
+                                           float *d2_of) {
+  const int P = PACK ? s.P : 1;
   constexpr int PARTS = W / 8, ROWS = kSplitThreads / PARTS, UNITS = kRows / ROWS;  // 8 elements a thread and unit
   const int64_t head = (int64_t)blockIdx.x / J.tiles, tile = (int64_t)blockIdx.x - head * J.tiles;
   const int64_t b = head / J.heads, n0 = tile * kRows;
   const int hh = (int)(head - b * J.heads), c = threadIdx.x % PARTS * 8, r0 = threadIdx.x / PARTS;
   const int64_t n_end = J.masked ? s.length(b) : J.N;
+  // the row of src (for P > 1: token, head of the P heads' maps or of the P heads)
+  auto row_of = [&](int64_t n) {
+    if (P == 1) return (b * J.N + n) * J.heads + hh;
+    const int t = (int)n / P, g = (int)n - t * P;
+    return (b * J.N + (int64_t)t * P) * J.heads + (STATS ? hh * P + g : (hh & ~1) * P + 2 * g + (hh & 1));
+  };
   const bool four = (J.w & 3) == 0 && ((uintptr_t)J.src & 15) == 0;
   float x[UNITS][8];
 #pragma unroll
@@ -54,11 +61,7 @@ __device__ __forceinline__ void split_tile(const Shape &s, const SplitJobs &jobs
 #pragma unroll
     for (int i = 0; i < 8; ++i) x[u][i] = 0.f;
     if (n < n_end) {
-      const float *src = J.src + ((b * J.N + n) * J.heads + hh) * J.w + c;
-      if (P > 1) {
-        const int t = (int)n / P, g = (int)n - t * P;
-        src = J.src + ((b * J.N + (int64_t)t * P) * J.heads + (hh & ~1) * P + 2 * g + (hh & 1)) * J.w + c;
-      }
+      const float *src = J.src + row_of(n) * J.w + c;
       if (four) {
 #pragma unroll
         for (int i = 0; i < 2; ++i)
@@ -74,14 +77,19 @@ __device__ __forceinline__ void split_tile(const Shape &s, const SplitJobs &jobs
     }
   }
   if (STATS) {
-    const float lam = __ldg(s.lam + hh);
+    const float lam_one = P == 1 ? __ldg(s.lam + hh) : 0.f;
+    float most;
+    const int shrink = P == 1 ? 0 : lam_exponent(s, hh * P, most);
     const int64_t steps = (J.N + 63) / 64;
     float total = 0.f;
 #pragma unroll
     for (int u = 0; u < UNITS; ++u) {
-      const int64_t n = n0 + r0 + u * ROWS, at = ((b * J.N + n) * J.heads + hh) * J.w + c;
+      const int64_t n = n0 + r0 + u * ROWS;
+      const int t = P == 1 ? (int)n : (int)n / P, h = P == 1 ? hh : hh * P + (int)n - t * P;
+      const float lam = P == 1 ? lam_one : n < J.N ? __ldg(s.lam + h) : 0.f;
       float d1 = 0.f, d2 = 0.f;
       if (n < J.N) {
+        const int64_t at = row_of(n) * J.w + c;
         auto add = [&](float g, float y, float y2) {
           d1 += g * (y + lam * y2);
           d2 += g * y2;
@@ -107,14 +115,16 @@ __device__ __forceinline__ void split_tile(const Shape &s, const SplitJobs &jobs
         d2 += __shfl_xor_sync(0xffffffffu, d2, o);
       }
       if (c == 0 && n / 64 < steps) {  // rows behind the last up to a step's end too
-        float *to = jobs.stats + (head * steps + n / 64) * 256 + n % 64;
+        float *to = jobs.stats + (head * steps + n / 64) * (P == 1 ? 256 : 320) + n % 64;
         const bool live = n < J.N;
-        to[0] = live ? __ldg(jobs.lse + (b * 2 * s.H + 2 * hh) * J.N + n) : INFINITY;
-        to[64] = live ? __ldg(jobs.lse + (b * 2 * s.H + 2 * hh + 1) * J.N + n) : INFINITY;
+        to[0] = live ? __ldg(jobs.lse + (b * 2 * s.H + 2 * h) * s.T + t) : INFINITY;
+        to[64] = live ? __ldg(jobs.lse + (b * 2 * s.H + 2 * h + 1) * s.T + t) : INFINITY;
         to[128] = d1;
         to[192] = d2;
+        if (P > 1) to[256] = lam * __uint_as_float((uint32_t)(127 - shrink) << 23);
         total += d2;
       }
+      if (P > 1 && c == 0) d2_of[r0 + u * ROWS] = d2;
     }
     total = warp_sum(total);
     if ((threadIdx.x & 31) == 0) red[2 * kSplitWarps + (threadIdx.x >> 5)] = __float_as_uint(total);
@@ -139,11 +149,16 @@ __device__ __forceinline__ void split_tile(const Shape &s, const SplitJobs &jobs
   const float f = __uint_as_float((uint32_t)(127 + e) << 23), inv = __uint_as_float((uint32_t)(127 - e) << 23);
   if (threadIdx.x == 0) {
     J.f[blockIdx.x] = f;
-    if (STATS) {
+    if (STATS && P == 1) {
       float total = 0.f;
       for (int i = 0; i < kSplitWarps; ++i) total += __uint_as_float(red[2 * kSplitWarps + i]);
       jobs.sums[blockIdx.x] = total;
     }
+  }
+  if (STATS && P > 1 && threadIdx.x < P) {  // rows of head threadIdx.x, in their order
+    float total = 0.f;
+    for (int i = (int)((threadIdx.x + P - n0 % P) % P); i < kRows && n0 + i < J.N; i += P) total += d2_of[i];
+    jobs.sums[(int64_t)blockIdx.x * P + threadIdx.x] = total;
   }
   if (J.norm) {  // the largest row norm, from the scaled elements: their squares neither overflow nor vanish
     float norm = 0.f;
@@ -178,21 +193,22 @@ __device__ __forceinline__ void split_tile(const Shape &s, const SplitJobs &jobs
   }
 }
 // W: the values' width (queries and keys have 64)
-template <int W>
+template <int W, bool PACK>
 __global__ void __launch_bounds__(kSplitThreads, 2)
     k_diff_split(const __grid_constant__ Shape s, const __grid_constant__ SplitJobs jobs) {
   __shared__ uint32_t red[3 * kSplitWarps];
+  __shared__ float d2_of[PACK ? kRows : 1];
   const int job = jobs.first + blockIdx.z;
   const SplitJob &J = jobs.j[job];
   if ((int64_t)blockIdx.x >= s.B * J.heads * J.tiles) return;
   if (job == 3)
-    split_tile<W, true>(s, jobs, J, red);
-  else if (job == 0 && s.P > 1)
-    split_tile<64, false>(s, jobs, J, red, s.P);
+    split_tile<W, true, PACK>(s, jobs, J, red, d2_of);
+  else if (PACK && job == 0)
+    split_tile<64, false, PACK>(s, jobs, J, red, d2_of);
   else if (job < 2)
-    split_tile<64, false>(s, jobs, J, red);
+    split_tile<64, false, false>(s, jobs, J, red, d2_of);
   else
-    split_tile<W, false>(s, jobs, J, red);
+    split_tile<W, false, false>(s, jobs, J, red, d2_of);
 }
 
 // ---- few query rows against many keys ----------------------------------------------------
@@ -493,7 +509,7 @@ struct Operands {
     return (size_t)halves * 2 + (size_t)(s.B * (2 * s.row_heads() * tiles(s.rows()) + 4 * s.Hk * tiles(s.S))) * 4;
   }
   static size_t grad_bytes(const Shape &s) {
-    return (size_t)(s.B * s.H * s.T * 2 * width(s)) * 2 + (size_t)(2 * s.B * s.H * tiles(s.T)) * 4;
+    return (size_t)(s.B * s.H * s.T * 2 * width(s)) * 2 + (size_t)(2 * s.B * s.row_heads() * tiles(s.rows())) * 4;
   }
   Operands(tx_ctx *ctx, const Shape &s, void *saved, bool gradient)
       : own(ctx, saved ? 0 : bytes(s)), grad(ctx, gradient ? grad_bytes(s) : 0) {
@@ -501,7 +517,7 @@ struct Operands {
     x.vw = (int)w;
     x.qt = tiles(s.rows());
     x.kt = tiles(s.S);
-    tq = s.B * 2 * s.row_heads() * x.qt, tk = s.B * 2 * s.Hk * x.kt, tv = s.B * s.Hk * x.kt, tg = s.B * s.H * x.qt;
+    tq = s.B * 2 * s.row_heads() * x.qt, tk = s.B * 2 * s.Hk * x.kt, tv = s.B * s.Hk * x.kt, tg = s.B * s.row_heads() * x.qt;
     ok = (saved || own.ptr) && (!gradient || grad.ptr);
     if (!ok) return;
     __half *p = reinterpret_cast<__half *>(saved ? saved : own.ptr);
@@ -525,15 +541,14 @@ struct Operands {
     jobs.j[0] = SplitJob{s.q, x.q, x.fq, nullptr, s.rows(), x.qt, 2 * s.row_heads(), s.d, s.scale * kLog2e, 0};
     jobs.j[1] = SplitJob{s.k, x.k, x.fk, nullptr, s.S, x.kt, 2 * s.Hk, s.d, 1.0f, 1};
     jobs.j[2] = SplitJob{s.v, x.v, x.fv, x.nv, s.S, x.kt, s.Hk, s.dv, 1.0f, 1};
-    jobs.j[3] = SplitJob{p ? p->dout : nullptr, x.g, x.fg, x.ng, s.T, x.qt, s.H, s.dv, 1.0f, 0};
+    jobs.j[3] = SplitJob{p ? p->dout : nullptr, x.g, x.fg, x.ng, s.rows(), x.qt, s.row_heads(), s.dv, 1.0f, 0};
     jobs.first = made ? 3 : 0;
     if (p) jobs.out = p->out, jobs.out2 = p->out2, jobs.lse = p->lse, jobs.stats = stats, jobs.sums = sums;
     const int64_t blocks = made ? tg : tq > tk ? tq : tk;
     const dim3 grid((unsigned)blocks, 1, made ? 1 : p ? 4 : 3);
-    if (x.vw == 64)
-      k_diff_split<64><<<grid, kSplitThreads, 0, ctx->stream>>>(s, jobs);
-    else
-      k_diff_split<128><<<grid, kSplitThreads, 0, ctx->stream>>>(s, jobs);
+    auto kernel = s.P > 1 ? (x.vw == 64 ? k_diff_split<64, true> : k_diff_split<128, true>)
+                          : (x.vw == 64 ? k_diff_split<64, false> : k_diff_split<128, false>);
+    kernel<<<grid, kSplitThreads, 0, ctx->stream>>>(s, jobs);
     TX_LAUNCHED(ctx, "k_diff_split");
     return TX_OK;
   }
@@ -546,6 +561,17 @@ struct Operands {
 bool few_queries(const Shape &s) {
   const int64_t rows = s.T * s.G, reads = (rows + 7) / 8;
   return rows <= 8 || (rows <= 24 && reads * s.B * s.Hk * s.S <= 1 << 16);
+}
+
+// Shape::P: a group's heads share query tiles where that makes fewer tiles (4 x 64 queries of 8 heads over 4
+// against 4096 keys: forward 27 us for 38; as many tiles cost more than one head's: 4 x 256 queries against
+// 512 keys 25 us for 23).  keep: for a backward, whose blocks of keys then have one run over all of a group's
+// queries: up to half a tile of tokens, if a head's blocks alone would fill the SMs (63 x 26 queries of 24 heads
+// over 8 against 285 keys: 61 and 276 us for 135 and 431; 8 x 64 queries of 4 heads over 2: 15 and 12 for 13 and 10).
+int pack_of(const tx_ctx *ctx, const Shape &s, bool keep) {
+  if (s.G == 1) return 1;
+  if (keep) return s.T <= kRows / 2 && s.G <= 32 && s.B * s.H > ctx->num_sms ? s.G : 1;
+  return s.T * s.G <= (int64_t)1 << 30 && Operands::tiles(s.T * s.G) < s.G * Operands::tiles(s.T) ? s.G : 1;
 }
 
 int check_desc(tx_ctx *ctx, const tx_diff_attention *p, Shape &s) {
@@ -647,6 +673,7 @@ extern "C" int tx_diff_attention_saved_bytes(tx_ctx *ctx, const tx_diff_attentio
   if (!ctx || !bytes) return TX_ERR_INVALID;
   Shape s;
   TX_TRY(check_desc(ctx, p, s));
+  s.P = pack_of(ctx, s, true);
   *bytes = few_queries(s) || s.B * s.T * s.S == 0 ? 0 : (int64_t)Operands::bytes(s);
   return TX_OK;
 }
@@ -673,11 +700,7 @@ extern "C" int tx_diff_attention_fwd(tx_ctx *ctx, const tx_diff_attention *p) {
   if (s.T * s.G <= 2) return launch_rows<2>(ctx, s, p->out, p->out2, p->lse);
   if (s.T * s.G <= 4) return launch_rows<4>(ctx, s, p->out, p->out2, p->lse);
   if (few_queries(s)) return launch_rows<8>(ctx, s, p->out, p->out2, p->lse);
-  // fewer tiles when a group's heads share them (4 x 64 queries of 8 heads over 4 against 4096 keys: 27 us for
-  // 38; as many tiles cost more than one head's: 4 x 256 queries against 512 keys 25 us for 23)
-  if (!p->saved && s.T * s.G <= (int64_t)1 << 30 &&
-      Operands::tiles(s.T * s.G) < s.G * Operands::tiles(s.T))
-    s.P = s.G;
+  s.P = pack_of(ctx, s, p->saved);
   Operands x(ctx, s, p->saved, false);
   TX_TRY(x.fill(ctx, s, false, nullptr, nullptr, nullptr));
   const int splits = tc_forward_splits(ctx, s);
@@ -709,10 +732,11 @@ extern "C" int tx_diff_attention_bwd(tx_ctx *ctx, const tx_diff_attention *p) {
     if (p->dlam) TX_CUDA(ctx, cudaMemsetAsync(p->dlam, 0, (size_t)s.H * 4, ctx->stream));
     return TX_OK;
   }
-  Scratch stats(ctx, (size_t)(s.B * s.H * ((s.T + 63) / 64)) * 256 * 4);
+  s.P = pack_of(ctx, s, true);
+  Scratch stats(ctx, (size_t)(s.B * s.row_heads() * ((s.rows() + 63) / 64)) * (s.P > 1 ? 320 : 256) * 4);
   const bool made = p->saved && !few_queries(s);
   Operands x(ctx, s, made ? p->saved : nullptr, true);
-  Scratch sums(ctx, (size_t)x.tg * 4);
+  Scratch sums(ctx, (size_t)(x.tg * s.P) * 4);
   if (!stats.ptr || !sums.ptr) return TX_ERR_OOM;
   TX_TRY(x.fill(ctx, s, made, p, stats.as<float>(), sums.as<float>()));
   if (p->dq || p->dk) return tc_backward(ctx, s, x.x, stats.as<float>(), sums.as<float>(), p->dq, p->dk, p->dv, p->dlam);

@@ -24,8 +24,8 @@ struct Shape {
   int64_t start;
   float scale;
   int *err;
-  // Query rows of the tensor-core forward: P heads' queries in turn, row i is token i / P of the head i % P
-  // of its P.  G where nothing is kept for a backward, else 1.
+  // Query rows of the tensor-core kernels: P heads' queries in turn, row i is token i / P of the head i % P
+  // of its P; G or 1 (pack_of)
   int P;
 
   __host__ __device__ __forceinline__ int64_t rows() const { return T * P; }
@@ -54,16 +54,25 @@ __device__ __forceinline__ float warp_sum(float v) {
   return v;
 }
 
-// dlam[h] = -sum of D2 over the tiles' sums [b][h][tiles], in a fixed order, by one warp
+// dlam[h] = -sum of D2 over the tiles' sums [b][h / P][tiles][P], in a fixed order, by one warp
 __device__ __forceinline__ void sum_dlam(const Shape &s, const float *sums, int64_t tiles, float *dlam, int h) {
-  const int lane = threadIdx.x & 31;
+  const int lane = threadIdx.x & 31, hq = h / s.P;
   float v = 0.f;
   for (int64_t i = lane; i < s.B * tiles; i += 32) {
     const int64_t b = i / tiles;
-    v += __ldg(sums + (b * s.H + h) * tiles + (i - b * tiles));
+    v += __ldg(sums + ((b * s.row_heads() + hq) * tiles + (i - b * tiles)) * s.P + (h - hq * s.P));
   }
   v = warp_sum(v);
   if (lane == 0) dlam[h] = -v;
+}
+
+// With P > 1 the backward's columns belong to several heads: their lam / 2^E, below 2, is a column's factor
+// and 2^E the tile's.
+__device__ __forceinline__ int lam_exponent(const Shape &s, int head0, float &most) {
+  most = 0.f;
+  for (int i = 0; i < s.P; ++i) most = fmaxf(most, fabsf(__ldg(s.lam + head0 + i)));
+  const int e = (int)(__float_as_uint(most) >> 23) - 127;
+  return e < -100 ? -100 : e > 113 ? 113 : e;
 }
 
 // Grants a kernel its dynamic shared memory once a device.
@@ -102,7 +111,7 @@ __device__ __forceinline__ void report_length(const Shape &s, int64_t b) {
 // log2 e, so scores come out in powers of two) and 64 or 128 for values.
 constexpr int kRows = 128;  // rows of a tile
 struct Split {
-  __half *q, *k, *v, *g;         // [b][map or head][row][2 W] (q: Shape::rows()); g: the output's gradient
+  __half *q, *k, *v, *g;         // [b][map or head][row][2 W] (q, g: Shape::rows()); g: the output's gradient
   float *fq, *fk, *fv, *fg;      // f of each [b][map or head][tile]
   float *nv, *ng;                // the largest 2-norm of a tile's rows
   int vw;                        // W of v and g
@@ -124,8 +133,9 @@ struct Parts {
 int tc_forward_splits(tx_ctx *ctx, const Shape &s);
 // out, out2 and lse, or with parts.splits > 1 the partial results
 int tc_forward(tx_ctx *ctx, const Shape &s, const Split &x, float *out, float *out2, float *lse, const Parts &parts);
-// stats [b][h][ceil(T / 64)][4][64]: the log-sum-exp of both maps (+inf behind the last query), D1, D2
-// sums [b][h][tiles of queries]: the tiles' sums of D2; dq, dk and dv, dlam are optional
+// stats [b][h / P][ceil(rows / 64)][4][64]: the log-sum-exp of both maps (+inf behind the last query), D1, D2;
+// with P > 1 [5]: lam / 2^E too (lam_exponent)
+// sums [b][h / P][tiles of queries][P]: the tiles' sums of D2; dq, dk and dv, dlam are optional
 int tc_backward(tx_ctx *ctx, const Shape &s, const Split &x, const float *stats, const float *sums, float *dq,
                 float *dk, float *dv, float *dlam);
 

@@ -38,14 +38,16 @@ namespace {
 constexpr int kThreads = 640, kStep = 64;  // producer, MMA, two spare warps, 16 elementwise warps
 enum { kModeK = 0, kModeQ = 1, kModeV = 2 };
 
-template <int DV>
+// PACK: rows of queries are those of a group's heads in turn (Shape::P = G)
+template <int DV, bool PACK>
 struct Cfg {
   static constexpr int RQ = 2 * 128 * 64 * 2;  // one map's resident tile, heads and tails
   static constexpr int RV = 2 * 128 * DV * 2;
   static constexpr int XBLK = kStep * 64 * 2;  // [64 rows x 64] fp16
   static constexpr int XQ = 2 * XBLK;          // one map's step
   static constexpr int XV = 2 * (DV / 64) * XBLK;
-  static constexpr int STAT = kStep * 16;      // lse1, lse2, D1, D2 of 64 queries
+  static constexpr int STATS = PACK ? 5 : 4;   // lse1, lse2, D1, D2 of 64 queries, and lam / 2^E
+  static constexpr int STAT = STATS * kStep * 4;
   // resident | two steps of both maps | V's or dO's step (V blocks: two, no resident value tile)
   static constexpr int TILES = 2 * RQ + RV + 2 * (2 * XQ) + XV;
   static constexpr int SMEM = TILES + 2 * STAT + 512;
@@ -54,7 +56,7 @@ struct Cfg {
 };
 
 struct Grads {
-  const float *stats, *sums;  // [b][h][ceil(T / 64)][4][64], [b][h][qt]
+  const float *stats, *sums;  // [b][h][steps of queries][4 or 5][64], [b][h][qt][P]
   float *dq, *dk, *dv, *dlam;
   // blocks of one tile level: K, Q and V; in turn level by level, or kind after kind
   unsigned nk, nq, levels, by_level, kt, qt;
@@ -81,12 +83,13 @@ __device__ __forceinline__ int block_kind(const Grads &o, unsigned i, unsigned &
   return i < k ? kModeK : i < k + q ? kModeQ : kModeV;
 }
 
-template <int DV, int MODE>
+template <int DV, int MODE, bool PACK>
 __device__ __forceinline__ void body(const Shape &s, const Split &x, const CUtensorMap &mq, const CUtensorMap &mk,
                                      const CUtensorMap &mv, const CUtensorMap &mg, const Grads &o, uint8_t *sm,
                                      unsigned block) {
-  using C = Cfg<DV>;
+  using C = Cfg<DV, PACK>;
   constexpr bool KEYS = MODE != kModeQ;  // the rows are keys
+  const int P = PACK ? s.P : 1, Hq = PACK ? s.row_heads() : s.H;
   // TMEM: two steps' S_1 and S_2 (64 columns each), dP in two halves, acc_1 and acc_2 (64 each) or acc
   constexpr uint32_t kDp = 256, ACC = 384;
   const uint32_t srq = su32(sm), sx = srq + 2 * C::RQ;
@@ -104,23 +107,23 @@ __device__ __forceinline__ void body(const Shape &s, const Split &x, const CUten
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
 
   // keys: the first tiles are seen by most queries; queries: the last tiles see most keys
-  const bool each = KEYS && o.each_head;
-  const int heads = KEYS && !each ? s.Hk : s.H;
-  const int rheads = (int)s.B * heads, rtiles = (int)(KEYS ? x.kt : x.qt), T = (int)s.T;
+  const bool each = KEYS && !PACK && o.each_head;
+  const int heads = KEYS && !each ? s.Hk : Hq;
+  const int rheads = (int)s.B * heads, rtiles = (int)(KEYS ? x.kt : x.qt), T = (int)s.T * P;  // T: rows of queries
   const int level = block / rheads, bh = block - level * rheads, b = bh / heads;
-  const int rt = KEYS ? level : rtiles - 1 - level, rh = bh - b * heads, hk = KEYS && !each ? rh : rh / s.G;
+  const int rt = KEYS ? level : rtiles - 1 - level, rh = bh - b * heads, hk = PACK || (KEYS && !each) ? rh : rh / s.G;
   const int r0 = rt * 128, n = (int)s.length(b), q_steps = (T + kStep - 1) / kStep;
   int first = 0, per_head;  // steps of each head, keys: from step `first` on
   if (KEYS) {
     int64_t q_first = s.causal ? r0 - s.start : 0;  // the first query that sees the first key
     if (q_first < 0) q_first = 0;
-    first = (int)(q_first / kStep);
+    first = q_first < s.T ? (int)q_first * P / kStep : q_steps;
     per_head = first < q_steps && r0 < n ? q_steps - first : 0;
   } else {
     const int last = r0 + 127 < T ? r0 + 127 : T - 1;
-    per_head = ((int)s.seen(last, n) + kStep - 1) / kStep;
+    per_head = ((int)s.seen(PACK ? last / P : last, n) + kStep - 1) / kStep;
   }
-  const int steps = __shfl_sync(0xffffffffu, KEYS && !each ? per_head * s.G : per_head, 0);
+  const int steps = __shfl_sync(0xffffffffu, KEYS && !each && !PACK ? per_head * s.G : per_head, 0);
 
   if (threadIdx.x == 0) {
     bar_init(r_full, 1);
@@ -155,7 +158,7 @@ __device__ __forceinline__ void body(const Shape &s, const Split &x, const CUten
   }
 
   // step i: head, first streamed row
-  auto head_of = [&](int i) { return KEYS && !each ? hk * s.G + i / per_head : rh; };
+  auto head_of = [&](int i) { return KEYS && !each && !PACK ? hk * s.G + i / per_head : rh; };
   auto step_of = [&](int i) { return KEYS ? first + i % per_head : i; };
 
   if (warp < 4) {
@@ -164,11 +167,11 @@ __device__ __forceinline__ void body(const Shape &s, const Split &x, const CUten
       bar_expect(r_full, 2 * C::RQ + (MODE == kModeV ? 0 : C::RV));
       for (int p = 0; p < 8; ++p)  // (map, head or tail, 64-row half)
         tma_3d(srq + p * C::XBLK, KEYS ? &mk : &mq, r_full, (p >> 1 & 1) * 64, r0 + (p & 1) * 64,
-               (KEYS ? b * 2 * s.Hk + 2 * hk : b * 2 * s.H + 2 * rh) + (p >> 2));
+               (KEYS ? b * 2 * s.Hk + 2 * hk : b * 2 * Hq + 2 * rh) + (p >> 2));
       if (MODE != kModeV)
         for (int p = 0; p < 4 * (DV / 64); ++p)
           tma_3d(srv + p * C::XBLK, KEYS ? &mv : &mg, r_full, (p >> 1) * 64, r0 + (p & 1) * 64,
-                 KEYS ? b * s.Hk + hk : b * s.H + rh);
+                 KEYS ? b * s.Hk + hk : b * Hq + rh);
       bool ok = true;
       int lx = 0, lv = 0;
       for (int i = 0; i < steps && ok; ++i) {
@@ -178,13 +181,13 @@ __device__ __forceinline__ void body(const Shape &s, const Split &x, const CUten
         bar_expect(x_full + st, 2 * C::XQ + (KEYS ? C::STAT : 0) + (MODE == kModeV ? C::XV : 0));
         for (int p = 0; p < 4; ++p)
           tma_3d(sxq + st * 2 * C::XQ + p * C::XBLK, KEYS ? &mq : &mk, x_full + st, (p & 1) * 64, step * kStep,
-                 (KEYS ? b * 2 * s.H + 2 * h : b * 2 * s.Hk + 2 * hk) + (p >> 1));
+                 (KEYS ? b * 2 * Hq + 2 * h : b * 2 * s.Hk + 2 * hk) + (p >> 1));
         if (KEYS)
-          bulk_load(su32(stat) + st * C::STAT, o.stats + ((int64_t)(b * s.H + h) * q_steps + step) * (4 * kStep), C::STAT,
+          bulk_load(su32(stat) + st * C::STAT, o.stats + ((int64_t)(b * Hq + h) * q_steps + step) * (C::STATS * kStep), C::STAT,
                     x_full + st);
         if (MODE == kModeV)
           for (int p = 0; p < 2 * (DV / 64); ++p)
-            tma_3d(xv_at(i) + xv_block(p) * C::XBLK, &mg, x_full + st, p * 64, step * kStep, b * s.H + h);
+            tma_3d(xv_at(i) + xv_block(p) * C::XBLK, &mg, x_full + st, p * 64, step * kStep, b * Hq + h);
         ++lx;
         if (MODE != kModeV) {
           if (i) ok = bar_wait(v_empty, (i - 1) & 1, abort_flag, s.err, 12);
@@ -192,7 +195,7 @@ __device__ __forceinline__ void body(const Shape &s, const Split &x, const CUten
           bar_expect(v_full, C::XV);
           for (int p = 0; p < 2 * (DV / 64); ++p)  // heads and tails of a column block side by side
             tma_3d(sxv + xv_block(p) * C::XBLK, KEYS ? &mg : &mv, v_full, p * 64, step * kStep,
-                   KEYS ? b * s.H + h : b * s.Hk + hk);
+                   KEYS ? b * Hq + h : b * s.Hk + hk);
           ++lv;
         }
       }
@@ -294,18 +297,25 @@ __device__ __forceinline__ void body(const Shape &s, const Split &x, const CUten
     for (int j = 0; j < AC / 2; ++j) acc[j] = two(0.f, 0.f);
     const float vn = __uint_as_float(*vmax);
     // resident factors: of both maps, and of V (keys) or dO (queries)
-    const int64_t rq = (int64_t)(KEYS ? b * 2 * s.Hk + 2 * hk : b * 2 * s.H + 2 * rh) * rtiles + rt;
+    const int64_t rq = (int64_t)(KEYS ? b * 2 * s.Hk + 2 * hk : b * 2 * Hq + 2 * rh) * rtiles + rt;
     const float fr0 = __ldg((KEYS ? x.fk : x.fq) + rq), fr1 = __ldg((KEYS ? x.fk : x.fq) + rq + rtiles);
-    const float frv = __ldg((KEYS ? x.fv : x.fg) + (int64_t)(KEYS ? b * s.Hk + hk : b * s.H + rh) * rtiles + rt);
+    const float frv = __ldg((KEYS ? x.fv : x.fg) + (int64_t)(KEYS ? b * s.Hk + hk : b * Hq + rh) * rtiles + rt);
     float mine[4] = {INFINITY, INFINITY, 0.f, 0.f};  // Q: this row's statistics
     if (!KEYS && row < T) {
 #pragma unroll
       for (int k = 0; k < 4; ++k)
-        mine[k] = __ldg(o.stats + ((int64_t)(b * s.H + rh) * q_steps + row / kStep) * (4 * kStep) + k * kStep + row % kStep);
+        mine[k] = __ldg(o.stats + ((int64_t)(b * Hq + rh) * q_steps + row / kStep) * (C::STATS * kStep) + k * kStep + row % kStep);
     }
-    const int seen = KEYS ? 0 : row < T ? (int)s.seen(row, n) : 0;
+    const int seen = KEYS ? 0 : row < T ? (int)s.seen(PACK ? row / P : row, n) : 0;
     const int64_t from64 = s.causal ? row - s.start : 0;  // keys: the first query that sees this one
-    const int from0 = from64 < 0 ? 0 : from64 > 1 << 30 ? 1 << 30 : (int)from64;
+    const int from0 = from64 < 0 ? 0 : from64 >= s.T ? T : (int)from64 * P;
+    // PACK: lam is its column's (keys: all but 2^E, which the largest in the group gives) or this row's
+    float lam_most = 0.f, lam_own = 0.f;
+    if (PACK && KEYS) {
+      const int e = lam_exponent(s, rh * P, lam_most);
+      lam_own = __uint_as_float((uint32_t)(127 + e) << 23);
+    }
+    if (PACK && !KEYS) lam_own = row < T ? __ldg(s.lam + rh * P + row % P) : 0.f;
     bool ok = true;
     float ga = 0.f;  // factor of the last step's products
     // What a step needs besides its scores; read a step ahead, or its latency adds to every step's chain
@@ -314,16 +324,16 @@ __device__ __forceinline__ void body(const Shape &s, const Split &x, const CUten
       float fx0, fx1, fxv, lam, gn;
       int x0;
     } next;
-    int step_head = KEYS && !each ? hk * s.G : rh, step = first;  // of the step to be read next
+    int step_head = KEYS && !each && !PACK ? hk * s.G : rh, step = first;  // of the step to be read next
     const int xtiles = (int)(KEYS ? x.qt : x.kt);
     auto read_step = [&]() {
       const int xt = step >> 1;  // tiles have two steps
-      const int64_t xq = (int64_t)(KEYS ? b * 2 * s.H + 2 * step_head : b * 2 * s.Hk + 2 * hk) * xtiles + xt;
+      const int64_t xq = (int64_t)(KEYS ? b * 2 * Hq + 2 * step_head : b * 2 * s.Hk + 2 * hk) * xtiles + xt;
       next.fx0 = __ldg((KEYS ? x.fq : x.fk) + xq);
       next.fx1 = __ldg((KEYS ? x.fq : x.fk) + xq + xtiles);
-      next.lam = __ldg(s.lam + step_head);
-      next.fxv = __ldg((KEYS ? x.fg : x.fv) + (int64_t)(KEYS ? b * s.H + step_head : b * s.Hk + hk) * xtiles + xt);
-      if (MODE != kModeV) next.gn = __ldg(x.ng + (int64_t)(b * s.H + step_head) * x.qt + (KEYS ? xt : rt));
+      next.lam = PACK ? lam_own : __ldg(s.lam + step_head);
+      next.fxv = __ldg((KEYS ? x.fg : x.fv) + (int64_t)(KEYS ? b * Hq + step_head : b * s.Hk + hk) * xtiles + xt);
+      if (MODE != kModeV) next.gn = __ldg(x.ng + (int64_t)(b * Hq + step_head) * x.qt + (KEYS ? xt : rt));
       next.x0 = step * kStep;
       if (++step == first + per_head) step = first, ++step_head;
     };
@@ -345,7 +355,7 @@ __device__ __forceinline__ void body(const Shape &s, const Split &x, const CUten
       const float f0 = factor2(fr0, next.fx0), f1 = factor2(fr1, next.fx1), lam = next.lam;
       float next_ga, beta = 0.f, fp = 0.f, sw = 0.f;
       if (MODE == kModeV) {  // w scale: 1 + |lam| -> [2^13, 2^14)
-        int e = (int)(__float_as_uint(1.f + fabsf(lam)) >> 23) - 127;
+        int e = (int)(__float_as_uint(1.f + (PACK ? lam_most : fabsf(lam))) >> 23) - 127;
         e = e > 113 ? 113 : e;
         sw = __uint_as_float((uint32_t)(140 - e) << 23);
         next_ga = next.fxv * __uint_as_float((uint32_t)(114 + e) << 23);
@@ -379,7 +389,7 @@ __device__ __forceinline__ void body(const Shape &s, const Split &x, const CUten
       }
       const bool whole = __all_sync(0xffffffffu, lo_c == 0 && hi_c == 16);
       const uint32_t ts = tmem + lane_row + st * 128 + 16 * part, tp = tmem + lane_row + kDp + 16 * part;
-      const float *col = stat + st * (4 * kStep) + 16 * part;
+      const float *col = stat + st * (C::STATS * kStep) + 16 * part;
       {
         uint32_t y0[16], y1[16], yp[16], yq[16];
         tld16_issue(ts, y0);
@@ -398,10 +408,11 @@ __device__ __forceinline__ void body(const Shape &s, const Split &x, const CUten
         uint32_t h0[8], l0[8], h1[8], l1[8];
 #pragma unroll
         for (int j4 = 0; j4 < 4; ++j4) {  // four columns
-          float q[4][4];
+          float q[C::STATS][4];
           if (KEYS) {
 #pragma unroll
-            for (int k = 0; k < (MODE == kModeV ? 2 : 4); ++k) {
+            for (int k = 0; k < C::STATS; ++k) {
+              if (MODE == kModeV && (k == 2 || k == 3)) continue;
               const float4 v = *reinterpret_cast<const float4 *>(col + k * kStep + 4 * j4);
               q[k][0] = v.x, q[k][1] = v.y, q[k][2] = v.z, q[k][3] = v.w;
             }
@@ -418,7 +429,9 @@ __device__ __forceinline__ void body(const Shape &s, const Split &x, const CUten
               if (e0 < lo_c || e0 >= hi_c) a = a1 = 0.f;
               if (e1 < lo_c || e1 >= hi_c) d = d1 = 0.f;
             }
-            const uint64_t p0 = two(a, d), p1 = two(a1, d1);
+            const uint64_t p0 = two(a, d);
+            uint64_t p1 = two(a1, d1);
+            if (PACK && KEYS) p1 = mul2(p1, two(q[C::STATS - 1][2 * u], q[C::STATS - 1][2 * u + 1]));
             if (MODE == kModeV) {
               cut2(fma2(p1, lw2, mul2(p0, sw2)), h0[j], l0[j]);
             } else {
@@ -458,7 +471,7 @@ __device__ __forceinline__ void body(const Shape &s, const Split &x, const CUten
       stage[r * CH + ((part * (AC / 4) + c) ^ (r & 7))] = v;
     }
     asm volatile("bar.sync 1, 512;" ::: "memory");
-    const int rows = (int)(KEYS ? s.S : s.T);
+    const int rows = KEYS ? (int)s.S : T;
     if (ok) {
       const int w = MODE == kModeV ? s.dv : s.d;  // a result row: one of w, or two maps' of w
       float *dst = MODE == kModeV ? o.dv : MODE == kModeK ? o.dk : o.dq;
@@ -468,7 +481,9 @@ __device__ __forceinline__ void body(const Shape &s, const Split &x, const CUten
       for (int k = (warp - 4) * (32 / CH) + sub; k < 128; k += 16 * (32 / CH)) {
         if (r0 + k >= rows) break;
         const float4 v = stage[k * CH + (c ^ (k & 7))];
-        float *p = dst + (((int64_t)b * rows + r0 + k) * heads + rh) * (MODE == kModeV ? w : 2 * w) + m * w + e;
+        int64_t to = ((int64_t)b * rows + r0 + k) * heads + rh;
+        if (PACK && !KEYS) to = (int64_t)b * rows * heads + (int64_t)((r0 + k) / P) * s.H + rh * P + (r0 + k) % P;
+        float *p = dst + to * (MODE == kModeV ? w : 2 * w) + m * w + e;
         if (four) {
           if (e < w) *reinterpret_cast<float4 *>(p) = v;
         } else {
@@ -488,7 +503,7 @@ __device__ __forceinline__ void body(const Shape &s, const Split &x, const CUten
   }
 }
 
-template <int DV>
+template <int DV, bool PACK>
 __global__ void __launch_bounds__(kThreads, 1)
     k_diff_bwd(const __grid_constant__ Shape s, const __grid_constant__ Split x, const __grid_constant__ CUtensorMap mq,
                const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtensorMap mv,
@@ -501,11 +516,11 @@ __global__ void __launch_bounds__(kThreads, 1)
   unsigned block;
   const int kind = block_kind(o, blockIdx.x, block);
   if (kind == kModeK)
-    body<DV, kModeK>(s, x, mq, mk, mv, mg, o, sm, block);
+    body<DV, kModeK, PACK>(s, x, mq, mk, mv, mg, o, sm, block);
   else if (kind == kModeQ)
-    body<DV, kModeQ>(s, x, mq, mk, mv, mg, o, sm, block);
+    body<DV, kModeQ, PACK>(s, x, mq, mk, mv, mg, o, sm, block);
   else
-    body<DV, kModeV>(s, x, mq, mk, mv, mg, o, sm, block);
+    body<DV, kModeV, PACK>(s, x, mq, mk, mv, mg, o, sm, block);
 }
 
 // dst[row][hk][w] = sum over the heads g of a group of src[row][hk G + g][w], for dk and dv in turn
@@ -542,12 +557,12 @@ __global__ void __launch_bounds__(256) k_diff_group_sum(const __grid_constant__ 
   }
 }
 
-template <int DV>
+template <int DV, bool PACK>
 int launch(tx_ctx *ctx, const Shape &s, const Split &x, const float *stats, const float *sums, float *dq, float *dk,
            float *dv, float *dlam) {
   CUtensorMap mq, mk, mv, mg;
-  if (!split_map(&mq, x.q, 64, s.T, s.B * 2 * s.H) || !split_map(&mk, x.k, 64, s.S, s.B * 2 * s.Hk) ||
-      !split_map(&mv, x.v, DV, s.S, s.B * s.Hk) || !split_map(&mg, x.g, DV, s.T, s.B * s.H))
+  if (!split_map(&mq, x.q, 64, s.rows(), s.B * 2 * s.row_heads()) || !split_map(&mk, x.k, 64, s.S, s.B * 2 * s.Hk) ||
+      !split_map(&mv, x.v, DV, s.S, s.B * s.Hk) || !split_map(&mg, x.g, DV, s.rows(), s.B * s.row_heads()))
     return tx_fail(ctx, TX_ERR_UNSUPPORTED, "differential attention: tensor map");
   // A key block that runs over all heads of a group may outlast everything else: then each head has
   // blocks and sums of its own, added up afterwards (5 x 413, 3 heads over 1: 27 + 2.5 us for 64).  Where
@@ -556,14 +571,14 @@ int launch(tx_ctx *ctx, const Shape &s, const Split &x, const float *stats, cons
   const double q_steps = (double)((s.T + kStep - 1) / kStep), k_steps = (double)((s.S + kStep - 1) / kStep);
   const double work = (s.causal ? 0.5 : 1.0) * (double)(s.B * s.H) *
                       ((dk ? 1.5 * (double)x.kt * q_steps : 0.0) + (dq ? (double)x.qt * k_steps : 0.0));
-  const bool each = dk && s.G > 1 && (double)s.G * q_steps > work / ctx->num_sms;
+  const bool each = !PACK && dk && s.G > 1 && (double)s.G * q_steps > work / ctx->num_sms;
   const size_t rows = (size_t)(s.B * s.S * s.H);
   Scratch part(ctx, each ? rows * (size_t)(2 * s.d + s.dv) * 4 : 0);
   if (each && !part.ptr) return TX_ERR_OOM;
   // dv's part first, whole 16-byte groups either way
   float *pv = part.as<float>(), *pk = each ? pv + rows * s.dv : nullptr;
   if (each && ((rows * s.dv) & 3)) pk = pv, pv = pk + rows * 2 * s.d;
-  const unsigned nk = dk ? (unsigned)(s.B * (each ? s.H : s.Hk)) : 0, nq = dq ? (unsigned)(s.B * s.H) : 0;
+  const unsigned nk = dk ? (unsigned)(s.B * (each ? s.H : s.Hk)) : 0, nq = dq ? (unsigned)(s.B * s.row_heads()) : 0;
   // Blocks start in order, so the longest come first.  Causal tiles get shorter from level to level:
   // the kinds take turns, and the last blocks are the shortest of each.  Otherwise K and Q blocks are
   // alike and V blocks half as long, so V comes last.
@@ -571,8 +586,8 @@ int launch(tx_ctx *ctx, const Shape &s, const Split &x, const float *stats, cons
   const Grads o{stats, sums, dq, each ? pk : dk, each ? pv : dv, dlam, nk, nq, kt < qt ? kt : qt,
                 (unsigned)(s.causal && nk && nq), kt, qt, each};
   static SmemGrant granted;
-  TX_TRY(granted.take(ctx, (const void *)k_diff_bwd<DV>, Cfg<DV>::SMEM));
-  k_diff_bwd<DV><<<2 * nk * kt + nq * qt, kThreads, Cfg<DV>::SMEM, ctx->stream>>>(s, x, mq, mk, mv, mg, o);
+  TX_TRY(granted.take(ctx, (const void *)k_diff_bwd<DV, PACK>, Cfg<DV, PACK>::SMEM));
+  k_diff_bwd<DV, PACK><<<2 * nk * kt + nq * qt, kThreads, Cfg<DV, PACK>::SMEM, ctx->stream>>>(s, x, mq, mk, mv, mg, o);
   TX_LAUNCHED(ctx, "k_diff_bwd");
   if (each) {
     const GroupSum j{{pk, pv}, {dk, dv}, {2 * s.d, s.dv}};
@@ -587,8 +602,11 @@ int launch(tx_ctx *ctx, const Shape &s, const Split &x, const float *stats, cons
 
 int tc_backward(tx_ctx *ctx, const Shape &s, const Split &x, const float *stats, const float *sums, float *dq,
                 float *dk, float *dv, float *dlam) {
-  return x.vw == 64 ? launch<64>(ctx, s, x, stats, sums, dq, dk, dv, dlam)
-                    : launch<128>(ctx, s, x, stats, sums, dq, dk, dv, dlam);
+  if (s.P > 1)
+    return x.vw == 64 ? launch<64, true>(ctx, s, x, stats, sums, dq, dk, dv, dlam)
+                      : launch<128, true>(ctx, s, x, stats, sums, dq, dk, dv, dlam);
+  return x.vw == 64 ? launch<64, false>(ctx, s, x, stats, sums, dq, dk, dv, dlam)
+                    : launch<128, false>(ctx, s, x, stats, sums, dq, dk, dv, dlam);
 }
 
 }  // namespace tx_diff

@@ -27,6 +27,7 @@ class _DLTensor(C.Structure):
 
 
 _DTYPES = {(2, 32, 1): "float32", (0, 64, 1): "int64", (6, 8, 1): "bool"}
+_SHAPES = [C.c_int64 * n for n in range(N.MAX_DIMS + 1)]
 _NAME, _USED = b"dltensor", b"used_dltensor"
 
 _api = C.pythonapi
@@ -58,15 +59,15 @@ def export(tensor: Tensor, stream=None):
         raise BufferError("a Tensor that requires gradients cannot be exported; detach() it first")
     if stream == 0:
         raise ValueError("stream 0 is ambiguous in the DLPack protocol; use 1, 2 or a stream handle")
-    ctx = tensor.ctx
+    storage, shape = tensor._storage, tensor.shape
+    ctx = storage.ctx
     if stream == -1:  # ordering with itself adds none
         own = C.c_void_p()
         ctx.check(lib.tx_stream(ctx.handle, C.byref(own)))
         stream = own.value
-    storage, shape = tensor._storage, tensor.shape
-    code = lib.tx_dlpack_export(ctx.handle, storage.ptr if storage.owned else None, storage.ptr + tensor._offset,
-                                N.DL_TYPES[tensor.dtype], (C.c_int64 * len(shape))(*shape), len(shape), stream or 1,
-                                ctx._out_ref)
+    ndim, data = len(shape), storage.ptr
+    code = lib.tx_dlpack_export(ctx.handle, data if storage.owned else None, data + tensor._offset,
+                                N.DL_TYPES[tensor.dtype], _SHAPES[ndim](*shape), ndim, stream or 1, ctx._out_ref)
     if code:
         ctx.check(code, "dlpack")
     return _new(ctx._out.value, _NAME, _drop_pointer)

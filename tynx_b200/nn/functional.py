@@ -115,22 +115,23 @@ def ppo_loss(logits: Tensor, values: Tensor, actions: Tensor, old_log_prob: Tens
     return loss
 
 
-def _heads(name: str, what: str, t: Tensor, like: Tensor, heads: str = "heads") -> tuple:
-    if t.dtype != "float32" or t.ndim != 4:
+def _heads(name: str, what: str, t: Tensor, ctx, heads: str = "heads") -> tuple:
+    shape = t.shape
+    if t.dtype != "float32" or len(shape) != 4:
         raise ValueError(f"{name} {what} must be rank-4 float32 [batch, tokens, {heads}, head_dim], got "
-                         f"{t.dtype} {t.shape}")
-    _same_device(name, what, t, like)
-    return t.shape
+                         f"{t.dtype} {shape}")
+    _same_device(name, what, t, ctx)
+    return shape
 
 
-def _same_device(name: str, what: str, t: Tensor, like: Tensor) -> None:
-    if t.ctx is not like.ctx:
-        raise ValueError(f"{name} {what} is on {t.device}, the other tensors are on {like.device}")
+def _same_device(name: str, what: str, t: Tensor, ctx) -> None:
+    if t.ctx is not ctx:
+        raise ValueError(f"{name} {what} is on cuda:{t.ctx.index}, the other tensors are on cuda:{ctx.index}")
 
 
-def _rotary_positions(name: str, rotary: Rotary, positions, like: Tensor) -> tuple:
-    """(pointer, sequence stride) of the positions of `like`'s tokens."""
-    batch, seq, _, dim = like.shape
+def _rotary_positions(name: str, rotary: Rotary, positions, shape: tuple, ctx) -> tuple:
+    """(pointer, sequence stride) of the positions of the tokens of a tensor of this shape."""
+    batch, seq, _, dim = shape
     if not isinstance(rotary, Rotary):
         raise TypeError(f"{name} rotary must be a Rotary, got {type(rotary).__qualname__}")
     if not 1 <= dim <= 2 * N.ROTARY_PAIRS:
@@ -142,8 +143,8 @@ def _rotary_positions(name: str, rotary: Rotary, positions, like: Tensor) -> tup
     if positions.dtype != "int64" or positions.shape not in ((seq,), (batch, seq)):
         raise ValueError(f"{name} positions must be int64 [{seq}] or [{batch}, {seq}], got "
                          f"{positions.dtype} {positions.shape}")
-    _same_device(name, "positions", positions, like)
-    return positions.ptr, seq if positions.ndim == 2 else 0
+    _same_device(name, "positions", positions, ctx)
+    return positions.ptr, seq if len(positions.shape) == 2 else 0
 
 
 def rotary_embedding(input: Tensor, rotary: Rotary, positions: Optional[Tensor] = None) -> Tensor:
@@ -151,23 +152,23 @@ def rotary_embedding(input: Tensor, rotary: Rotary, positions: Optional[Tensor] 
     by the tokens' positions (:class:`~tynx_b200.nn.Rotary`); elements behind
     ``rotary.dim`` pass through.  ``positions`` is int64 [tokens] or
     [batch, tokens]; None counts every sequence from 0."""
-    batch, seq, heads, dim = _heads("rotary_embedding", "input", input, input)
-    pos, stride = _rotary_positions("rotary_embedding", rotary, positions, input)
-    ctx, desc = input.ctx, rotary._desc
-    out = Tensor._empty(input.shape, "float32", ctx)
-    ctx.check(lib.tx_rotary_apply(ctx.handle, input.ptr, out.ptr, batch, seq, heads, dim, pos, stride, desc, 0),
-              "rotary_embedding")
+    name, ctx = "rotary_embedding", input.ctx
+    shape = batch, seq, heads, dim = _heads(name, "input", input, ctx)
+    pos, stride = _rotary_positions(name, rotary, positions, shape, ctx)
+    desc = rotary._desc
+    out = Tensor._new(shape, ctx)
+    ctx.check(lib.tx_rotary_apply(ctx.handle, input.ptr, out.ptr, batch, seq, heads, dim, pos, stride, desc, 0), name)
     if _needs_grad(input):
         held = positions.detach() if positions is not None else None
 
         def backward(g):
-            dx = Tensor._empty((batch, seq, heads, dim), "float32", ctx)
+            dx = Tensor._new(shape, ctx)
             ctx.check(lib.tx_rotary_apply(ctx.handle, g[0].ptr, dx.ptr, batch, seq, heads, dim,
                                           held.ptr if held is not None else None, stride, desc, 1),
                       "rotary_embedding backward")
             return [dx]
 
-        out._attach(Fn("rotary_embedding", [input], backward))
+        out._attach(Fn(name, [input], backward))
     return out
 
 
@@ -177,20 +178,20 @@ def qk_norm_rotary(q: Tensor, k: Tensor, q_weight: Tensor, k_weight: Tensor, rot
     eps) * weight``, and the rotation of :func:`rotary_embedding`, as one kernel
     over ``q [batch, tokens, heads, head_dim]`` and ``k [batch, tokens, kv_heads,
     head_dim]``; the weights are [head_dim].  Returns both rotated tensors."""
-    name = "qk_norm_rotary"
-    batch, seq, heads, dim = _heads(name, "q", q, q)
-    _heads(name, "k", k, q, "kv_heads")
-    if k.shape[:2] != (batch, seq) or k.shape[3] != dim:
+    name, ctx = "qk_norm_rotary", q.ctx
+    shape = batch, seq, heads, dim = _heads(name, "q", q, ctx)
+    kv_heads = _heads(name, "k", k, ctx, "kv_heads")[2]
+    if k.shape != (batch, seq, kv_heads, dim):
         raise ValueError(f"{name} k must be [{batch}, {seq}, kv_heads, {dim}], got {k.shape}")
     for what, w in (("q_weight", q_weight), ("k_weight", k_weight)):
         if w.dtype != "float32" or w.shape != (dim,):
             raise ValueError(f"{name} {what} must be a float32 Tensor of shape ({dim},), got {w.dtype} {w.shape}")
-        _same_device(name, what, w, q)
+        _same_device(name, what, w, ctx)
     if not eps >= 0.0:
         raise ValueError(f"{name} eps must not be negative, got {eps}")
-    pos, stride = _rotary_positions(name, rotary, positions, q)
-    kv_heads, ctx, desc = k.shape[2], q.ctx, rotary._desc
-    yq, yk = Tensor._empty(q.shape, "float32", ctx), Tensor._empty(k.shape, "float32", ctx)
+    pos, stride = _rotary_positions(name, rotary, positions, shape, ctx)
+    desc = rotary._desc
+    yq, yk = Tensor._new(shape, ctx), Tensor._new(k.shape, ctx)
     ctx.check(lib.tx_qk_norm_rotary_fwd(ctx.handle, q.ptr, k.ptr, q_weight.ptr, k_weight.ptr, yq.ptr, yk.ptr, batch,
                                         seq, heads, kv_heads, dim, pos, stride, desc, eps), name)
     if _needs_grad(q, k, q_weight, k_weight):
@@ -199,7 +200,7 @@ def qk_norm_rotary(q: Tensor, k: Tensor, q_weight: Tensor, k_weight: Tensor, rot
 
         def backward(g):
             gq, gk = (t if t is not None else full(s.shape, 0.0, ctx=ctx) for t, s in zip(g, (sq, sk)))
-            dq, dk, dwq, dwk = (Tensor._empty(t.shape, "float32", ctx) for t in (sq, sk, swq, swk))
+            dq, dk, dwq, dwk = (Tensor._new(t.shape, ctx) for t in (sq, sk, swq, swk))
             ctx.check(lib.tx_qk_norm_rotary_bwd(ctx.handle, sq.ptr, sk.ptr, swq.ptr, swk.ptr, gq.ptr, gk.ptr, dq.ptr,
                                                 dk.ptr, dwq.ptr, dwk.ptr, batch, seq, heads, kv_heads, dim,
                                                 held.ptr if held is not None else None, stride, desc, eps),
@@ -235,10 +236,10 @@ def differential_attention(q: Tensor, k: Tensor, v: Tensor, lam: Tensor, *, scal
     When a gradient is wanted, the output's second term, a number a query and map,
     and the operands in the form the tensor cores read (as large as q, k and v)
     are kept until the backward."""
-    name = "differential_attention"
-    batch, queries, maps, d = _heads(name, "q", q, q, "2 * heads")
-    _, keys, kv_maps, _ = _heads(name, "k", k, q, "2 * kv_heads")
-    _heads(name, "v", v, q, "kv_heads")
+    name, ctx = "differential_attention", q.ctx
+    batch, queries, maps, d = _heads(name, "q", q, ctx, "2 * heads")
+    _, keys, kv_maps, _ = _heads(name, "k", k, ctx, "2 * kv_heads")
+    _heads(name, "v", v, ctx, "kv_heads")
     heads, kv_heads = maps // 2, kv_maps // 2
     if maps % 2 or kv_maps % 2 or not heads or not kv_heads or heads % kv_heads:
         raise ValueError(f"{name} needs two maps a head and a number of query heads that is a multiple of the key "
@@ -253,20 +254,19 @@ def differential_attention(q: Tensor, k: Tensor, v: Tensor, lam: Tensor, *, scal
                                   f"{d} and {dv}")
     if lam.dtype != "float32" or lam.shape != (heads,):
         raise ValueError(f"{name} lam must be a float32 Tensor of shape ({heads},), got {lam.dtype} {lam.shape}")
-    _same_device(name, "lam", lam, q)
+    _same_device(name, "lam", lam, ctx)
     if key_lengths is not None:
         if key_lengths.dtype != "int64" or key_lengths.shape != (batch,):
             raise ValueError(f"{name} key_lengths must be int64 [{batch}], got {key_lengths.dtype} "
                              f"{key_lengths.shape}")
-        _same_device(name, "key_lengths", key_lengths, q)
+        _same_device(name, "key_lengths", key_lengths, ctx)
     scale = d ** -0.5 if scale is None else float(scale)
     if not math.isfinite(scale):
         raise ValueError(f"{name} scale must be finite, got {scale}")
     start = keys - queries if query_start is None else int(query_start)
     if abs(start) > 1 << 30:
         raise ValueError(f"{name} query_start must be within +-2^30, got {start}")
-    ctx = q.ctx
-    out = Tensor._empty((batch, queries, heads, dv), "float32", ctx)
+    out = Tensor._new((batch, queries, heads, dv), ctx)
     desc = N.DiffAttentionDesc(batch, queries, keys, heads, kv_heads, d, dv, q.ptr, k.ptr, v.ptr, lam.ptr,
                                key_lengths.ptr if key_lengths is not None else None, scale, int(bool(causal)), start,
                                out.ptr)
@@ -287,10 +287,10 @@ def differential_attention(q: Tensor, k: Tensor, v: Tensor, lam: Tensor, *, scal
         want = [t.requires_grad for t in (q, k, v, lam)]
 
         def backward(g):
-            dq = Tensor._empty(held[0].shape, "float32", ctx) if want[0] else None
-            dk = Tensor._empty(held[1].shape, "float32", ctx) if want[1] or want[2] else None
-            dv_ = Tensor._empty(held[2].shape, "float32", ctx) if want[1] or want[2] else None
-            dlam = Tensor._empty((heads,), "float32", ctx) if want[3] else None
+            dq = Tensor._new(held[0].shape, ctx) if want[0] else None
+            dk = Tensor._new(held[1].shape, ctx) if want[1] or want[2] else None
+            dv_ = Tensor._new(held[2].shape, ctx) if want[1] or want[2] else None
+            dlam = Tensor._new((heads,), ctx) if want[3] else None
             desc.dout = g[0].ptr
             for field, t in (("dq", dq), ("dk", dk), ("dv", dv_), ("dlam", dlam)):
                 setattr(desc, field, t.ptr if t is not None else None)
