@@ -24,12 +24,13 @@
 // So dP multiplies R_hi with X_hi and X_lo side by side (their halves are added
 // elementwise): a step takes 24 instructions for S, 16 for dP and 24 for the sums
 // in K and Q blocks, 4096 cycles, and 24 + 12 in V blocks, 2304.  2 x 2048 causal
-// tokens of 8 heads over 4 take 253 us (with dP as three products 260; with a
+// tokens of 8 heads over 4 take 252 us (with dP as three products 260; with a
 // step's S alone in TMEM 421): these instructions are 309 of the 427 thousand
 // cycles an SM is busy, and where a step's elementwise chain (about 500
 // instructions a warp, four warps a scheduler) is behind, the tensor core waits.
 // 256 sequences of 128 tokens of 2 heads, where a block has two steps and its
-// start and stores count as much, take 144 us.
+// start and stores count as much, take 142 us; so the first scores wait for what
+// they need alone (with all resident tiles 145 us).
 #include "diff_attn.cuh"
 
 namespace tx_diff {
@@ -100,7 +101,7 @@ __device__ __forceinline__ void body(const Shape &s, const Split &x, const CUten
   const float *stat = reinterpret_cast<const float *>(sm + C::TILES);
   uint64_t *bars = reinterpret_cast<uint64_t *>(sm + C::TILES + 2 * C::STAT);
   uint64_t *r_full = bars, *x_full = bars + 1, *x_empty = bars + 3, *v_full = bars + 5, *v_empty = bars + 6,
-           *s_full = bars + 7, *p_full = bars + 9, *a_full = bars + 11, *all_done = bars + 12;
+           *s_full = bars + 7, *p_full = bars + 9, *a_full = bars + 11, *all_done = bars + 12, *rv_full = bars + 13;
   uint32_t *tmem_holder = reinterpret_cast<uint32_t *>(bars + 16);
   volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_holder + 1);
   uint32_t *vmax = tmem_holder + 2;
@@ -127,6 +128,7 @@ __device__ __forceinline__ void body(const Shape &s, const Split &x, const CUten
 
   if (threadIdx.x == 0) {
     bar_init(r_full, 1);
+    bar_init(rv_full, 1);
     for (int i = 0; i < 2; ++i) {
       bar_init(x_full + i, 1);
       bar_init(x_empty + i, 1);
@@ -150,12 +152,6 @@ __device__ __forceinline__ void body(const Shape &s, const Split &x, const CUten
   __syncthreads();
   fence_after();
   const uint32_t tmem = *tmem_holder;
-  if (MODE != kModeV) {
-    // the largest row norm of this head's values (all tiles: D runs over all keys)
-    for (int64_t i = threadIdx.x; i < x.kt; i += kThreads)
-      atomicMax(vmax, __float_as_uint(__ldg(x.nv + (int64_t)(b * s.Hk + hk) * x.kt + i)));
-    __syncthreads();
-  }
 
   // step i: head, first streamed row
   auto head_of = [&](int i) { return KEYS && !each && !PACK ? hk * s.G + i / per_head : rh; };
@@ -164,14 +160,10 @@ __device__ __forceinline__ void body(const Shape &s, const Split &x, const CUten
   if (warp < 4) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
     if (warp == 0 && lane == 0 && steps) {
-      bar_expect(r_full, 2 * C::RQ + (MODE == kModeV ? 0 : C::RV));
+      bar_expect(r_full, 2 * C::RQ);
       for (int p = 0; p < 8; ++p)  // (map, head or tail, 64-row half)
         tma_3d(srq + p * C::XBLK, KEYS ? &mk : &mq, r_full, (p >> 1 & 1) * 64, r0 + (p & 1) * 64,
                (KEYS ? b * 2 * s.Hk + 2 * hk : b * 2 * Hq + 2 * rh) + (p >> 2));
-      if (MODE != kModeV)
-        for (int p = 0; p < 4 * (DV / 64); ++p)
-          tma_3d(srv + p * C::XBLK, KEYS ? &mv : &mg, r_full, (p >> 1) * 64, r0 + (p & 1) * 64,
-                 KEYS ? b * s.Hk + hk : b * Hq + rh);
       bool ok = true;
       int lx = 0, lv = 0;
       for (int i = 0; i < steps && ok; ++i) {
@@ -190,6 +182,12 @@ __device__ __forceinline__ void body(const Shape &s, const Split &x, const CUten
             tma_3d(xv_at(i) + xv_block(p) * C::XBLK, &mg, x_full + st, p * 64, step * kStep, b * Hq + h);
         ++lx;
         if (MODE != kModeV) {
+          if (i == 0) {  // behind what the first scores need
+            bar_expect(rv_full, C::RV);
+            for (int p = 0; p < 4 * (DV / 64); ++p)
+              tma_3d(srv + p * C::XBLK, KEYS ? &mv : &mg, rv_full, (p >> 1) * 64, r0 + (p & 1) * 64,
+                     KEYS ? b * s.Hk + hk : b * Hq + rh);
+          }
           if (i) ok = bar_wait(v_empty, (i - 1) & 1, abort_flag, s.err, 12);
           if (!ok) break;
           bar_expect(v_full, C::XV);
@@ -201,6 +199,7 @@ __device__ __forceinline__ void body(const Shape &s, const Split &x, const CUten
       }
       // every copy has landed before the CTA's memory is released
       bar_drain(r_full, 0);
+      if (lv) bar_drain(rv_full, 0);
       for (int i = lx - 1; i >= 0 && i > lx - 3; --i) bar_drain(x_full + (i & 1), (i >> 1) & 1);
       if (lv) bar_drain(v_full, (lv - 1) & 1);
     } else if (warp == 1 && steps) {
@@ -226,7 +225,8 @@ __device__ __forceinline__ void body(const Shape &s, const Split &x, const CUten
       };
       auto values = [&](int i) {  // dP of step i, in two halves: R_hi X_hi, and the small products (their truncations cost nothing there)
         if (MODE != kModeV && ok) {
-          ok = mma_wait(v_full, i & 1, abort_flag, s.err, 15);
+          if (i == 0) ok = mma_wait(rv_full, 0, abort_flag, s.err, 13);
+          ok = ok && mma_wait(v_full, i & 1, abort_flag, s.err, 15);
           if (!ok) return;
           fence_after();
 #pragma unroll
@@ -295,6 +295,12 @@ __device__ __forceinline__ void body(const Shape &s, const Split &x, const CUten
     uint64_t acc[AC / 2];
 #pragma unroll
     for (int j = 0; j < AC / 2; ++j) acc[j] = two(0.f, 0.f);
+    if (MODE != kModeV) {
+      // the largest row norm of this head's values (all tiles: D runs over all keys)
+      for (int64_t i = threadIdx.x - 128; i < x.kt; i += 512)
+        atomicMax(vmax, __float_as_uint(__ldg(x.nv + (int64_t)(b * s.Hk + hk) * x.kt + i)));
+      asm volatile("bar.sync 1, 512;" ::: "memory");
+    }
     const float vn = __uint_as_float(*vmax);
     // resident factors: of both maps, and of V (keys) or dO (queries)
     const int64_t rq = (int64_t)(KEYS ? b * 2 * s.Hk + 2 * hk : b * 2 * Hq + 2 * rh) * rtiles + rt;
