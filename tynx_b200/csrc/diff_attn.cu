@@ -198,6 +198,7 @@ __global__ void __launch_bounds__(kSplitThreads, 2)
     k_diff_split(const __grid_constant__ Shape s, const __grid_constant__ SplitJobs jobs) {
   __shared__ uint32_t red[3 * kSplitWarps];
   __shared__ float d2_of[PACK ? kRows : 1];
+  next_may_start();
   const int job = jobs.first + blockIdx.z;
   const SplitJob &J = jobs.j[job];
   if ((int64_t)blockIdx.x >= s.B * J.heads * J.tiles) return;
@@ -254,6 +255,7 @@ __device__ __forceinline__ void load4(const float *p, int have, uint64_t (&x)[2]
 template <int RP, bool VEC>
 __global__ void __launch_bounds__(kRowThreads, 2)
     k_diff_rows(const __grid_constant__ Shape s, const Parts parts, int64_t keys_per_split) {
+  next_may_start();
   extern __shared__ __align__(16) uint8_t raw[];
   RowSmem<RP> &sh = *reinterpret_cast<RowSmem<RP> *>(raw);
   constexpr int kGroup = kGroupOf<RP>;
@@ -407,6 +409,7 @@ __global__ void __launch_bounds__(64 * (W > 1 ? W : kJoinRows))
   const int64_t at = W > 1 ? blockIdx.x : (int64_t)blockIdx.x * (blockDim.x >> 6) + row;  // (b, hk, item)
   const bool live = at < rows;
   const float2 *ml = parts.ml + (live ? at * 2 + m : 0) * splits;
+  wait_for_previous();
   // the first 32 ranges' references stay in registers
   const float2 mine = lane < splits ? __ldg(ml + lane) : make_float2(-INFINITY, 0.f);
   float top = mine.x;
@@ -598,18 +601,13 @@ int check_desc(tx_ctx *ctx, const tx_diff_attention *p, Shape &s) {
 int join(tx_ctx *ctx, const Shape &s, const Parts &parts, float *out, float *out2, float *lse) {
   const int64_t rows = s.B * s.T * s.H;
   if (parts.splits > 12 && rows < 8 * ctx->num_sms) {  // many ranges of few rows (74 of 32 rows: 5.1 us for 9.2)
-    k_diff_join<12, 4><<<(unsigned)rows, 256, 0, ctx->stream>>>(s, parts, out, out2, lse);
-    TX_LAUNCHED(ctx, "k_diff_join");
-    return TX_OK;
+    return launch_behind(ctx, "k_diff_join", k_diff_join<12, 4>, (unsigned)rows, 256, 0, s, parts, out, out2, lse);
   }
   const int each = rows < 8 * ctx->num_sms ? 1 : kJoinRows;  // few rows: an SM each
   const unsigned blocks = (unsigned)((rows + each - 1) / each);
   if (parts.splits <= 4)  // (3 ranges of 8192 rows: 8.9 us, with twelve loads in flight 13.7)
-    k_diff_join<4, 1><<<blocks, 64 * each, 0, ctx->stream>>>(s, parts, out, out2, lse);
-  else
-    k_diff_join<12, 1><<<blocks, 64 * each, 0, ctx->stream>>>(s, parts, out, out2, lse);
-  TX_LAUNCHED(ctx, "k_diff_join");
-  return TX_OK;
+    return launch_behind(ctx, "k_diff_join", k_diff_join<4, 1>, blocks, 64 * each, 0, s, parts, out, out2, lse);
+  return launch_behind(ctx, "k_diff_join", k_diff_join<12, 1>, blocks, 64 * each, 0, s, parts, out, out2, lse);
 }
 
 // Partial results' memory.

@@ -148,6 +148,8 @@ __device__ __forceinline__ void body(const Shape &s, const Split &x, const CUten
                  "r"(512));
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
   }
+  wait_for_previous();  // the split operands and statistics
+  next_may_start();
   fence_before();
   __syncthreads();
   fence_after();
@@ -536,6 +538,7 @@ struct GroupSum {
   int w[2];
 };
 __global__ void __launch_bounds__(256) k_diff_group_sum(const __grid_constant__ GroupSum j, int64_t heads, int G) {
+  wait_for_previous();
   const int which = blockIdx.y, w = j.w[which];
   const int64_t n = heads * w;
   const bool four = (w & 3) == 0 && ((uintptr_t)j.dst[which] & 15) == 0;
@@ -593,13 +596,13 @@ int launch(tx_ctx *ctx, const Shape &s, const Split &x, const float *stats, cons
                 (unsigned)(s.causal && nk && nq), kt, qt, each};
   static SmemGrant granted;
   TX_TRY(granted.take(ctx, (const void *)k_diff_bwd<DV, PACK>, Cfg<DV, PACK>::SMEM));
-  k_diff_bwd<DV, PACK><<<2 * nk * kt + nq * qt, kThreads, Cfg<DV, PACK>::SMEM, ctx->stream>>>(s, x, mq, mk, mv, mg, o);
-  TX_LAUNCHED(ctx, "k_diff_bwd");
+  TX_TRY(launch_behind(ctx, "k_diff_bwd", k_diff_bwd<DV, PACK>, 2 * nk * kt + nq * qt, kThreads, Cfg<DV, PACK>::SMEM, s,
+                       x, mq, mk, mv, mg, o));
   if (each) {
     const GroupSum j{{pk, pv}, {dk, dv}, {2 * s.d, s.dv}};
     const int64_t n = s.B * s.S * s.Hk * (2 * s.d > s.dv ? 2 * s.d : s.dv);
-    k_diff_group_sum<<<dim3(grid_for(n / 4, 256), 2), 256, 0, ctx->stream>>>(j, s.B * s.S * s.Hk, s.G);
-    TX_LAUNCHED(ctx, "k_diff_group_sum");
+    TX_TRY(launch_behind(ctx, "k_diff_group_sum", k_diff_group_sum, dim3(grid_for(n / 4, 256), 2), 256, 0, j,
+                         s.B * s.S * s.Hk, s.G));
   }
   return TX_OK;
 }

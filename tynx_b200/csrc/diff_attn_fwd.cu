@@ -145,6 +145,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                  "r"(512));
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
   }
+  wait_for_previous();  // the split operands
+  next_may_start();
   fence_before();
   __syncthreads();
   fence_after();
@@ -518,9 +520,7 @@ int launch(tx_ctx *ctx, const Shape &s, const Split &x, const Out &o) {
   TX_TRY(granted.take(ctx, (const void *)k_diff_fwd<DV, PACK>, Cfg<DV>::SMEM));
   const int64_t items = x.qt * s.B * s.row_heads() * o.parts.splits;
   const unsigned blocks = (unsigned)(items < ctx->num_sms ? items : ctx->num_sms);
-  k_diff_fwd<DV, PACK><<<blocks, kThreads, Cfg<DV>::SMEM, ctx->stream>>>(s, x, mq, mk, mv, o);
-  TX_LAUNCHED(ctx, "k_diff_fwd");
-  return TX_OK;
+  return launch_behind(ctx, "k_diff_fwd", k_diff_fwd<DV, PACK>, blocks, kThreads, Cfg<DV>::SMEM, s, x, mq, mk, mv, o);
 }
 
 }  // namespace
