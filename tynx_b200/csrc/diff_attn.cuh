@@ -8,7 +8,7 @@
 
 #include <atomic>
 
-#include "common.h"
+#include "launch.cuh"
 
 namespace tx_diff {
 
@@ -86,27 +86,6 @@ struct SmemGrant {
     return TX_OK;
   }
 };
-
-// The kernels of one call follow one another closely: a block of the later one may start, and set itself up,
-// while the last blocks of the earlier one end, and waits for its results before it touches them.  The earlier
-// one's blocks say so at their start: the later one's blocks then come as room falls free.
-__device__ __forceinline__ void next_may_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
-__device__ __forceinline__ void wait_for_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
-template <typename... P, typename... A>
-int launch_behind(tx_ctx *ctx, const char *name, void (*kernel)(P...), dim3 grid, unsigned threads, int smem, A... args) {
-  cudaLaunchAttribute close{};
-  close.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  close.val.programmaticStreamSerializationAllowed = 1;
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = grid;
-  cfg.blockDim = dim3(threads);
-  cfg.dynamicSmemBytes = (size_t)smem;
-  cfg.stream = ctx->stream;
-  cfg.attrs = &close;
-  cfg.numAttrs = 1;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, P(args)...);
-  return e == cudaSuccess ? TX_OK : tx_cuda_fail(ctx, e, name);
-}
 
 // A key length outside [0, S] raises the context's error flag.
 __device__ __forceinline__ void report_length(const Shape &s, int64_t b) {

@@ -24,7 +24,7 @@
 // in halves also dim, no multiple of 8, unaligned) run the same code with single
 // elements: 6 x 3770 tokens of 24 heads of 40 with norms take 52 us forward and 99
 // backward, twice the floor (with a warp a row 197 and 348).
-#include "common.h"
+#include "launch.cuh"
 
 namespace {
 
@@ -242,6 +242,7 @@ template <bool VEC, bool INTER, int LANES>
 __global__ void __launch_bounds__(kThreads, kBackBlocks)
     k_qk_norm_bwd(const __grid_constant__ Args A, const __grid_constant__ tx_rotary rot) {
   using L = Lane<VEC, INTER, LANES>;
+  next_may_start();
   __shared__ float2 cs[kAngles];
   __shared__ __align__(16) float sums[kThreads / 32][256];
   constexpr int SLOTS = kThreads / LANES, UN = 2;
@@ -328,6 +329,7 @@ __global__ void __launch_bounds__(1024) k_qk_norm_dw(const float *part, int bloc
   __shared__ float sums[32][33];
   const int which = blockIdx.y, c = blockIdx.x * 32 + (threadIdx.x & 31), row = threadIdx.x >> 5;
   float v = 0.f;
+  wait_for_previous();
   if (c < dim) {
 #pragma unroll 4
     for (int b = row; b < blocks; b += 32) v += part[((int64_t)b * 2 + which) * 256 + c];
@@ -386,8 +388,8 @@ int launch_rows(tx_ctx *ctx, Args &A, const tx_rotary &rot, int mode, float *dqw
     A.part = part.as<float>();
     k_qk_norm_bwd<VEC, INTER, LANES><<<blocks, kThreads, 0, ctx->stream>>>(A, rot);
     TX_LAUNCHED(ctx, "k_qk_norm_bwd");
-    k_qk_norm_dw<<<dim3((unsigned)((A.dim + 31) / 32), 2), 1024, 0, ctx->stream>>>(part.as<float>(), (int)blocks, A.dim,
-                                                                               dqw, dkw);
+    return launch_behind(ctx, "k_qk_norm_dw", k_qk_norm_dw, dim3((unsigned)((A.dim + 31) / 32), 2), 1024, 0,
+                         part.as<float>(), (int)blocks, A.dim, dqw, dkw);
   }
   TX_LAUNCHED(ctx, "k_rotary");
   return TX_OK;
