@@ -213,13 +213,13 @@ __global__ void __launch_bounds__(kSplitThreads, 2)
 }
 
 // ---- few query rows against many keys ----------------------------------------------------
-// Bound by reading the keys and values once: 105 MB (8 sequences of 4607 to 8190 keys of 2
-// heads) in 25.6 us, 4.1 TB/s (537 MB of 8 heads in 79, the copy rate).  A block takes RP queries (token, head of the group) of one key head,
-// both maps, and a range of keys; its warps take four keys at a time in turn and meet only at the
-// end.  A lane holds four of a key's 64 elements (half a warp a map) and four of a value's 128.  The 4 RP dot products of a map are
-// added over its 16 lanes by halving: each exchange passes on the half that the partner keeps, so
-// the sum costs about one shuffle a product and leaves one (key, query) score a lane, where its
-// exponential is taken.  The weights go through shared memory back to all lanes.
+// Bound by reading the keys and values once: 105 MB (8 sequences of 4607 to 8190 keys of 2 heads) in
+// 25.6 us, 4.1 TB/s (537 MB of 8 heads in 79, the copy rate).  A block takes RP queries (token, head of the
+// group) of one key head, both maps, and a range of keys; its warps take four keys at a time in turn and meet
+// only at the end.  A lane holds four of a key's 64 elements (half a warp a map) and four of a value's 128.
+// The 4 RP dot products of a map are added over its 16 lanes by halving: each exchange passes on the half that
+// the partner keeps, so the sum costs about one shuffle a product and leaves one (key, query) score a lane,
+// where its exponential is taken.  The weights go through shared memory back to all lanes.
 // The running maximum is followed only when it has grown by 2^16 (fp32 sums lose nothing below).
 constexpr int kRowWarps = 8, kRowThreads = 32 * kRowWarps;
 // keys of a group: a lane holds 4 RP products before they are added, 2 RP for eight queries
