@@ -417,6 +417,31 @@ def test_same_inputs_give_the_same_bits():
         np.testing.assert_array_equal(a.numpy(), b.numpy())
 
 
+@pytest.mark.parametrize("shape", [
+    (8, 1, 700, 4, 2, 64, 128),      # few queries, joined
+    (2, 40, 2000, 4, 2, 64, 128),    # ranges of keys, joined
+    (40, 50, 50, 4, 2, 64, 128),     # a group's heads in one tile
+    (2, 300, 300, 6, 1, 40, 72),     # key blocks of single heads, summed
+], ids=lambda c: "x".join(map(str, c)))
+def test_calls_close_behind_one_another(shape):
+    """Kernels of a call start under the ends of one another; results are those of calls far apart."""
+    import tynx_b200 as tx
+
+    sets, want = [arrays(*shape, 50 + i) for i in range(3)], []
+    for a in sets:
+        got = call(*a, causal=True, lengths=None)
+        tx.synchronize()
+        want.append([t.numpy() for t in got])
+    many = [call(*sets[i % 3], causal=True, lengths=None) for i in range(24)]
+    with tx.no_grad():
+        tensors = [[tx.Tensor(x) for x in a[:4]] for a in sets]
+        plain = [tx.nn.functional.differential_attention(*tensors[i % 3], causal=True) for i in range(24)]
+    for i, got in enumerate(many):
+        for g, w in zip(got, want[i % 3]):
+            np.testing.assert_array_equal(g.numpy(), w)
+        np.testing.assert_array_equal(plain[i].numpy(), plain[i % 3].numpy())
+
+
 def test_layer_of_all_three_trains_and_replays():
     """Projections, norms with rotation, differential attention and a loss, eager and as a
     captured step replayed on other inputs, against each other and the 64-bit composition."""

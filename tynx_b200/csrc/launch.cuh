@@ -20,5 +20,7 @@ int launch_behind(tx_ctx *ctx, const char *name, void (*kernel)(P...), dim3 grid
   cfg.attrs = &close;
   cfg.numAttrs = 1;
   const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, P(args)...);
-  return e == cudaSuccess ? TX_OK : tx_cuda_fail(ctx, e, name);
+  if (e == cudaSuccess) return TX_OK;
+  cudaGetLastError();  // reported here, not by the next launch too
+  return tx_cuda_fail(ctx, e, name);
 }
