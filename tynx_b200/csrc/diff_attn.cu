@@ -399,7 +399,7 @@ __global__ void __launch_bounds__(kRowThreads, 2)
 // do not depend on one another.
 constexpr int kJoinRows = 4;  // a block at most, with W = 1
 template <int U, int W>
-__global__ void __launch_bounds__(64 * (W > 1 ? W : kJoinRows))
+__global__ void __launch_bounds__(64 * (W > 1 ? W : kJoinRows), W > 1 ? 2 : 3)
     k_diff_join(const __grid_constant__ Shape s, const Parts parts, float *out, float *out2, float *lse) {
   __shared__ float4 second[W > 1 ? 1 : kJoinRows][32], shares[W][2][32];
   __shared__ float sums[W][2];
@@ -411,9 +411,9 @@ __global__ void __launch_bounds__(64 * (W > 1 ? W : kJoinRows))
   const float2 *ml = parts.ml + (live ? at * 2 + m : 0) * splits;
   wait_for_previous();
   // the first 32 ranges' references stay in registers
-  const float2 mine = lane < splits ? __ldg(ml + lane) : make_float2(-INFINITY, 0.f);
+  const float2 mine = lane < splits ? ml[lane] : make_float2(-INFINITY, 0.f);
   float top = mine.x;
-  for (int i = lane + 32; i < splits; i += 32) top = fmaxf(top, __ldg(ml + i).x);
+  for (int i = lane + 32; i < splits; i += 32) top = fmaxf(top, ml[i].x);
   top = warp_max(top);
   const bool none = top == -INFINITY;
   const float ref = none ? 0.f : top;
@@ -424,7 +424,7 @@ __global__ void __launch_bounds__(64 * (W > 1 ? W : kJoinRows))
   float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
   const int each = (splits + W - 1) / W, first = share * each, end = first + each < splits ? first + each : splits;
   for (int i0 = first; i0 < end; i0 += 32) {
-    const float2 v = i0 == 0 ? mine : i0 + lane < splits ? __ldg(ml + i0 + lane) : make_float2(-INFINITY, 0.f);
+    const float2 v = i0 == 0 ? mine : i0 + lane < splits ? ml[i0 + lane] : make_float2(-INFINITY, 0.f);
     const int n = end - i0 < 32 ? end - i0 : 32;
     const float w = lane < n ? ex2(v.x - ref) : 0.f;
     sum += v.y * w;
@@ -436,12 +436,12 @@ __global__ void __launch_bounds__(64 * (W > 1 ? W : kJoinRows))
         if (j + i < n) {
           const float *q = p + (int64_t)(i0 + j + i) * s.dv;
           if (four) {
-            if (c < s.dv) y[i] = __ldg(reinterpret_cast<const float4 *>(q));
+            if (c < s.dv) y[i] = *reinterpret_cast<const float4 *>(q);
           } else {
-            if (c < s.dv) y[i].x = __ldg(q);
-            if (c + 1 < s.dv) y[i].y = __ldg(q + 1);
-            if (c + 2 < s.dv) y[i].z = __ldg(q + 2);
-            if (c + 3 < s.dv) y[i].w = __ldg(q + 3);
+            if (c < s.dv) y[i].x = q[0];
+            if (c + 1 < s.dv) y[i].y = q[1];
+            if (c + 2 < s.dv) y[i].z = q[2];
+            if (c + 3 < s.dv) y[i].w = q[3];
           }
         }
       }

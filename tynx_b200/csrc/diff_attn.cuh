@@ -60,7 +60,7 @@ __device__ __forceinline__ void sum_dlam(const Shape &s, const float *sums, int6
   float v = 0.f;
   for (int64_t i = lane; i < s.B * tiles; i += 32) {
     const int64_t b = i / tiles;
-    v += __ldg(sums + ((b * s.row_heads() + hq) * tiles + (i - b * tiles)) * s.P + (h - hq * s.P));
+    v += sums[((b * s.row_heads() + hq) * tiles + (i - b * tiles)) * s.P + (h - hq * s.P)];
   }
   v = warp_sum(v);
   if (lane == 0) dlam[h] = -v;

@@ -300,19 +300,19 @@ __device__ __forceinline__ void body(const Shape &s, const Split &x, const CUten
     if (MODE != kModeV) {
       // the largest row norm of this head's values (all tiles: D runs over all keys)
       for (int64_t i = threadIdx.x - 128; i < x.kt; i += 512)
-        atomicMax(vmax, __float_as_uint(__ldg(x.nv + (int64_t)(b * s.Hk + hk) * x.kt + i)));
+        atomicMax(vmax, __float_as_uint(x.nv[(int64_t)(b * s.Hk + hk) * x.kt + i]));
       asm volatile("bar.sync 1, 512;" ::: "memory");
     }
     const float vn = __uint_as_float(*vmax);
     // resident factors: of both maps, and of V (keys) or dO (queries)
     const int64_t rq = (int64_t)(KEYS ? b * 2 * s.Hk + 2 * hk : b * 2 * Hq + 2 * rh) * rtiles + rt;
-    const float fr0 = __ldg((KEYS ? x.fk : x.fq) + rq), fr1 = __ldg((KEYS ? x.fk : x.fq) + rq + rtiles);
-    const float frv = __ldg((KEYS ? x.fv : x.fg) + (int64_t)(KEYS ? b * s.Hk + hk : b * Hq + rh) * rtiles + rt);
+    const float fr0 = (KEYS ? x.fk : x.fq)[rq], fr1 = (KEYS ? x.fk : x.fq)[rq + rtiles];
+    const float frv = (KEYS ? x.fv : x.fg)[(int64_t)(KEYS ? b * s.Hk + hk : b * Hq + rh) * rtiles + rt];
     float mine[4] = {INFINITY, INFINITY, 0.f, 0.f};  // Q: this row's statistics
     if (!KEYS && row < T) {
 #pragma unroll
       for (int k = 0; k < 4; ++k)
-        mine[k] = __ldg(o.stats + ((int64_t)(b * Hq + rh) * q_steps + row / kStep) * (C::STATS * kStep) + k * kStep + row % kStep);
+        mine[k] = o.stats[((int64_t)(b * Hq + rh) * q_steps + row / kStep) * (C::STATS * kStep) + k * kStep + row % kStep];
     }
     const int seen = KEYS ? 0 : row < T ? (int)s.seen(PACK ? row / P : row, n) : 0;
     const int64_t from64 = s.causal ? row - s.start : 0;  // keys: the first query that sees this one
@@ -337,11 +337,11 @@ __device__ __forceinline__ void body(const Shape &s, const Split &x, const CUten
     auto read_step = [&]() {
       const int xt = step >> 1;  // tiles have two steps
       const int64_t xq = (int64_t)(KEYS ? b * 2 * Hq + 2 * step_head : b * 2 * s.Hk + 2 * hk) * xtiles + xt;
-      next.fx0 = __ldg((KEYS ? x.fq : x.fk) + xq);
-      next.fx1 = __ldg((KEYS ? x.fq : x.fk) + xq + xtiles);
+      next.fx0 = (KEYS ? x.fq : x.fk)[xq];
+      next.fx1 = (KEYS ? x.fq : x.fk)[xq + xtiles];
       next.lam = PACK ? lam_own : __ldg(s.lam + step_head);
-      next.fxv = __ldg((KEYS ? x.fg : x.fv) + (int64_t)(KEYS ? b * Hq + step_head : b * s.Hk + hk) * xtiles + xt);
-      if (MODE != kModeV) next.gn = __ldg(x.ng + (int64_t)(b * Hq + step_head) * x.qt + (KEYS ? xt : rt));
+      next.fxv = (KEYS ? x.fg : x.fv)[(int64_t)(KEYS ? b * Hq + step_head : b * s.Hk + hk) * xtiles + xt];
+      if (MODE != kModeV) next.gn = x.ng[(int64_t)(b * Hq + step_head) * x.qt + (KEYS ? xt : rt)];
       next.x0 = step * kStep;
       if (++step == first + per_head) step = first, ++step_head;
     };
@@ -548,9 +548,9 @@ __global__ void __launch_bounds__(256) k_diff_group_sum(const __grid_constant__ 
     for (int64_t i = first; i < n >> 2; i += step) {
       const int64_t head = i / w4;
       const float4 *p = reinterpret_cast<const float4 *>(j.src[which]) + head * G * w4 + (i - head * w4);
-      float4 v = __ldg(p);
+      float4 v = *p;
       for (int g = 1; g < G; ++g) {
-        const float4 y = __ldg(p + (int64_t)g * w4);
+        const float4 y = p[(int64_t)g * w4];
         v = make_float4(v.x + y.x, v.y + y.y, v.z + y.z, v.w + y.w);
       }
       reinterpret_cast<float4 *>(j.dst[which])[i] = v;
@@ -559,8 +559,8 @@ __global__ void __launch_bounds__(256) k_diff_group_sum(const __grid_constant__ 
     for (int64_t i = first; i < n; i += step) {
       const int64_t head = i / w;
       const float *p = j.src[which] + head * G * w + (i - head * w);
-      float v = __ldg(p);
-      for (int g = 1; g < G; ++g) v += __ldg(p + (int64_t)g * w);
+      float v = *p;
+      for (int g = 1; g < G; ++g) v += p[(int64_t)g * w];
       j.dst[which][i] = v;
     }
   }

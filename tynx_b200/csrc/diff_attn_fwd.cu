@@ -323,7 +323,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int rows = (int)s.T * P, row = w.r0 + r;
       const int at_row = row < rows ? row : rows - 1;
       const int seen = (int)s.seen(PACK ? at_row / P : at_row, w.n) - w.tile0 * 128 - 64 * half;
-      const float fq = __ldg(x.fq + (int64_t)(w.b * 2 * row_heads + 2 * w.h + m) * x.qt + w.qt);
+      const float fq = x.fq[(int64_t)(w.b * 2 * row_heads + 2 * w.h + m) * x.qt + w.qt];
       const float *fk = x.fk + (int64_t)(w.b * 2 * s.Hk + 2 * w.hk + m) * x.kt + w.tile0;
       const float *fv = x.fv + (int64_t)(w.b * s.Hk + w.hk) * x.kt + w.tile0;
       float ref = -INFINITY, top = -INFINITY;  // top: the maximum that ref was set by
@@ -333,7 +333,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       bool ok = true;
       float gv = 0.f;
       for (int i = 0; i < tiles; ++i) {
-        const float f = factor2(fq, __ldg(fk + i)), next_gv = __ldg(fv + i);
+        const float f = factor2(fq, fk[i]), next_gv = fv[i];
         if (i) {  // the last tile's product, while the tensor core works on this tile's scores
           ok = __all_sync(0xffffffffu, bar_wait(o_full + m, (nt + i - 1) & 1, abort_flag, s.err, 9));
           fence_after();
