@@ -286,7 +286,8 @@ __global__ void __launch_bounds__(kThreads, kBackBlocks)
             ss += x[u].lo[i] * x[u].lo[i] + x[u].hi[i] * x[u].hi[i];
             dot += g[u].lo[i] * w.lo[i] * x[u].lo[i] + g[u].hi[i] * w.hi[i] * x[u].hi[i];
           }
-          const float n = rsqrtf(row_sum<LANES>(ss) * inv + A.eps);
+          // behind the last row 0, not rsqrt(0 + eps): infinite without eps, and NaN in the weight gradients
+          const float all = row_sum<LANES>(ss), n = r < rows ? rsqrtf(all * inv + A.eps) : 0.f;
           const float c = row_sum<LANES>(dot) * inv * n * n;
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
