@@ -1,0 +1,50 @@
+"""How long memory that crosses to another library, or from one, stays out of use."""
+
+import gc
+
+import numpy as np
+import pytest
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("borrowers", [1, 3])
+def test_lent_memory_that_a_captured_step_let_go(borrowers):
+    """A captured step reads a lent tensor and drops it: replays read it whoever lets go of it afterwards."""
+    import torch
+
+    import tynx_b200 as tx
+
+    box = [tx.ones(1 << 18)]
+    there = [torch.from_dlpack(box[0]) for _ in range(borrowers)]
+    box[0].numpy()
+
+    def step(a):
+        return a + box.pop()
+
+    compiled = tx.compile(step, fullgraph=True)
+    zero = tx.zeros(1 << 18)
+    np.testing.assert_array_equal(compiled(zero).numpy(), 1.0)
+    assert not box
+    while there:
+        there.pop()
+        gc.collect()
+        others = [tx.Tensor(np.full(1 << 18, 7.0, np.float32)) for _ in range(4)]
+        np.testing.assert_array_equal(compiled(zero).numpy(), 1.0)
+        del others
+
+
+def test_lent_memory_that_was_let_go_outside_a_capture_is_used_again():
+    import torch
+
+    import tynx_b200 as tx
+
+    before = tx.ones(5_000_001)
+    at = before.ptr
+    there = torch.from_dlpack(before)
+    del before
+    assert tx.ones(5_000_001).ptr != at
+    del there
+    gc.collect()
+    held = [tx.ones(5_000_001) for _ in range(3)]
+    assert at in [t.ptr for t in held]

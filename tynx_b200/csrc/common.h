@@ -32,11 +32,15 @@ struct tx_allocator {
   tx_arena *arena = nullptr;  // non-null while capturing
   std::unordered_map<void *, tx_arena *> arena_owner;
   std::vector<void *> quarantine;  // eager blocks freed during a capture
-  // Blocks lent to other libraries (tx_dlpack_export): borrowers of each block
-  // beside its owner, and the loans that ended, with the stream of each, since
-  // the owner's thread last called.  Other threads touch `ended` only, under
-  // the lock.
-  std::unordered_map<void *, int> lent;
+  // Blocks lent to other libraries (tx_dlpack_export): the holders of each block
+  // but one, and whether one let go during a capture, whose graph may reference
+  // the block; and the loans that ended, with the stream of each, since the
+  // owner's thread last called.  Other threads touch `ended` only, under the lock.
+  struct Lent {
+    int others = 0;
+    bool captured = false;
+  };
+  std::unordered_map<void *, Lent> lent;
   std::mutex lock;
   std::vector<std::pair<void *, cudaStream_t>> ended;
 };

@@ -219,17 +219,21 @@ void tx_free_raw(tx_ctx *ctx, void *p) {
   if (A.arena_owner.count(p)) return;  // arena memory lives as long as its exec
   auto it = A.live.find(p);
   if (it == A.live.end()) return;
+  bool captured = A.arena != nullptr;  // the graph being captured may still reference this block
   if (!A.lent.empty()) {  // the last of the owner and the borrowers frees the block
     auto b = A.lent.find(p);
     if (b != A.lent.end()) {
-      if (--b->second == 0) A.lent.erase(b);
-      return;
+      captured = b->second.captured = b->second.captured || captured;
+      const bool last = b->second.others == 0;
+      if (!last) --b->second.others;
+      if (last || (b->second.others == 0 && !captured)) A.lent.erase(b);
+      if (!last) return;
     }
   }
   size_t cls = it->second;
   A.live.erase(it);
   A.in_use -= cls;
-  if (A.arena) {  // the graph being captured may still reference this block
+  if (captured) {
     A.quarantine.push_back(p);
     return;
   }

@@ -102,7 +102,7 @@ extern "C" int tx_dlpack_export(tx_ctx *ctx, void *d_block, void *d_data, int dt
   loan->ctx = ctx;
   loan->block = d_block;
   loan->borrower = static_cast<cudaStream_t>(stream);
-  ++ctx->alloc.lent[d_block];
+  ++ctx->alloc.lent[d_block].others;
   *out = &loan->managed;
   return TX_OK;
 }
