@@ -48,3 +48,33 @@ def test_lent_memory_that_was_let_go_outside_a_capture_is_used_again():
     gc.collect()
     held = [tx.ones(5_000_001) for _ in range(3)]
     assert at in [t.ptr for t in held]
+
+
+def test_a_copy_is_a_copy():
+    import torch
+
+    import tynx_b200 as tx
+
+    mine = tx.Tensor(np.arange(6, dtype=np.float32))
+    there = torch.from_dlpack(mine, copy=True)
+    there += 1.0
+    torch.cuda.synchronize()
+    np.testing.assert_array_equal(mine.numpy(), np.arange(6))
+    np.testing.assert_array_equal(there.cpu().numpy(), 1 + np.arange(6))
+    alias = torch.from_dlpack(mine, copy=False)
+    alias += 1.0
+    torch.cuda.synchronize()
+    np.testing.assert_array_equal(mine.numpy(), 1 + np.arange(6))
+    named = torch.from_dlpack(mine, device="cuda")
+    assert named.data_ptr() == mine.ptr
+    parameter = tx.ones(3).requires_grad_()
+    with pytest.raises(BufferError, match="detach"):
+        parameter.__dlpack__(copy=True)
+    kept = torch.utils.dlpack.from_dlpack(mine.reshape(2, 3).__dlpack__(stream=1, max_version=(1, 0), copy=True,
+                                                                       dl_device=(2, 0)))
+    del mine, alias, named
+    gc.collect()
+    spoil = [tx.zeros(6) for _ in range(4)]
+    tx.synchronize()
+    np.testing.assert_array_equal(kept.cpu().numpy(), 1 + np.arange(6).reshape(2, 3))
+    del spoil

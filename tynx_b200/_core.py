@@ -449,12 +449,14 @@ class Tensor:
             self.ctx.check(lib.tx_d2h(self.ctx.handle, out.ctypes.data, self.ptr, out.nbytes), "d2h")
         return out
 
-    def __dlpack__(self, *, stream=None, **unused):
-        """Lend this tensor to another library (``torch.from_dlpack(tensor)``)."""
+    def __dlpack__(self, *, stream=None, max_version=None, dl_device=None, copy=None):
+        """Lend this tensor to another library (``torch.from_dlpack(tensor)``); with
+        ``copy=True`` a copy of it.  The memory stays on its device, and the structure
+        is the protocol's first, which a consumer of any version takes."""
         global _export
         if _export is None:
             from .interop import export as _export
-        return _export(self, stream)
+        return _export(self, stream, dl_device, copy)
 
     def __dlpack_device__(self) -> tuple:
         return (2, self.ctx.index)

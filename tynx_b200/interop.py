@@ -51,14 +51,19 @@ def _drop(capsule):
 _drop_pointer = C.cast(_drop, C.c_void_p)
 
 
-def export(tensor: Tensor, stream=None):
+def export(tensor: Tensor, stream=None, device=None, copy=None):
     """The capsule behind ``Tensor.__dlpack__``; ``stream`` as the protocol has it
     for CUDA: None or 1 the legacy default stream, 2 the thread's default one, -1
-    no ordering, otherwise a ``cudaStream_t``."""
+    no ordering, otherwise a ``cudaStream_t``.  ``device`` is the (type, index) that
+    the memory has to be on, ``copy`` True for memory of its own."""
     if tensor.requires_grad:
         raise BufferError("a Tensor that requires gradients cannot be exported; detach() it first")
     if stream == 0:
         raise ValueError("stream 0 is ambiguous in the DLPack protocol; use 1, 2 or a stream handle")
+    if device is not None and tuple(map(int, device)) != tensor.__dlpack_device__():
+        raise BufferError(f"a Tensor on {tensor.device} cannot be exported to DLPack device {tuple(map(int, device))}")
+    if copy:
+        tensor = tensor.clone()
     storage, shape = tensor._storage, tensor.shape
     ctx = storage.ctx
     if stream == -1:  # ordering with itself adds none
