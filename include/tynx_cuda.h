@@ -96,8 +96,9 @@ int tx_stream(tx_ctx *ctx, void **out);
  * deleter, callable from any thread); work issued after that waits for the
  * borrower's stream before it reuses the memory.  Every loan has to end
  * before tx_ctx_destroy.  Not allowed during a capture.  tx_dlpack_release calls the deleter of any such
- * structure; tx_dlpack_give_back does so once the context's streams have passed all work issued so far
- * (for memory that was borrowed; kernels' error flag stays up for tx_sync; not during a capture). */
+ * structure; tx_dlpack_give_back, from any thread, does so once the context's streams have passed all work
+ * issued so far (for memory that was borrowed; kernels' error flag stays up for tx_sync).  During a capture it
+ * keeps the memory as long as the captured graph, which may reference it. */
 enum { TX_DL_F32 = 0, TX_DL_I64 = 1, TX_DL_BOOL = 2 };
 int tx_dlpack_export(tx_ctx *ctx, void *d_block, void *d_data, int dtype, const int64_t *shape, int ndim,
                      void *stream, void **out);

@@ -78,3 +78,77 @@ def test_a_copy_is_a_copy():
     tx.synchronize()
     np.testing.assert_array_equal(kept.cpu().numpy(), 1 + np.arange(6).reshape(2, 3))
     del spoil
+
+
+def test_borrowed_memory_that_a_captured_step_let_go():
+    """It stays with the captured graph that reads it, and goes back with it."""
+    import torch
+
+    import tynx_b200 as tx
+
+    n = 3 << 20
+    box = [tx.from_dlpack(torch.ones(n, device="cuda"))]
+
+    def step(a):
+        return a + box.pop()
+
+    compiled = tx.compile(step, fullgraph=True)
+    zero = tx.zeros(n)
+    np.testing.assert_array_equal(compiled(zero).numpy(), 1.0)
+    assert not box
+    gc.collect()
+    tx.from_dlpack(torch.zeros(1, device="cuda"))
+    others = [torch.full((n,), 7.0, device="cuda") for _ in range(3)]
+    torch.cuda.synchronize()
+    np.testing.assert_array_equal(compiled(zero).numpy(), 1.0)
+    del others
+    gc.collect()
+    held = torch.cuda.memory_allocated()
+    compiled.clear_cache()
+    gc.collect()
+    assert torch.cuda.memory_allocated() <= held - 4 * n
+
+
+def test_borrowed_memory_let_go_in_a_step_that_was_not_captured():
+    """A body that cannot be captured runs eagerly; what it let go while it was being recorded goes back."""
+    import torch
+
+    import tynx_b200 as tx
+
+    n = 3 << 20
+    gc.collect()
+    free = torch.cuda.memory_allocated()
+    box = [tx.from_dlpack(torch.ones(n, device="cuda")) for _ in range(2)]
+
+    def step(a):
+        out = a + box.pop()
+        return out * float(out.sum().item())
+
+    compiled = tx.compile(step)
+    with pytest.warns(RuntimeWarning, match="eager"):
+        out = compiled(tx.zeros(n))
+    np.testing.assert_array_equal(out.numpy(), float(n))
+    assert not box
+    gc.collect()
+    assert torch.cuda.memory_allocated() <= free
+
+
+def test_borrowed_memory_let_go_on_another_thread():
+    import threading
+
+    import torch
+
+    import tynx_b200 as tx
+
+    n = 3 << 20
+    torch.cuda.synchronize()
+    gc.collect()
+    free = torch.cuda.memory_allocated()
+    box = [tx.from_dlpack(torch.ones(n, device="cuda"))]
+    assert torch.cuda.memory_allocated() > free
+    thread = threading.Thread(target=box.clear)
+    thread.start()
+    thread.join()
+    gc.collect()
+    assert torch.cuda.memory_allocated() <= free
+    np.testing.assert_array_equal(tx.from_dlpack(torch.ones(3, device="cuda")).numpy(), 1.0)

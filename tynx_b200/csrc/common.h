@@ -22,6 +22,7 @@ struct tx_arena {
   size_t offset = 0;  // within chunks.back()
   std::unordered_set<void *> blocks;
   std::vector<void *> pinned;  // host staging for copies recorded during capture
+  std::vector<void *> borrowed;  // other libraries' memory let go during capture (tx_dlpack_give_back)
 };
 
 struct tx_allocator {
@@ -57,6 +58,7 @@ struct tx_ctx {
   int *d_err = nullptr;  // device error flag [4]
   uint64_t *d_rng = nullptr;  // call counter of the dropout stream
   bool capturing = false;
+  std::mutex capture_lock;  // capturing changes, and is relied on by other threads, under it
   cudaEvent_t order = nullptr;  // joins the compute stream with another library's
   // data parallel
   void *nccl = nullptr;

@@ -317,6 +317,7 @@ extern "C" int tx_host_free(void *h_ptr) {
 extern "C" int tx_capture_begin(tx_ctx *ctx) {
   if (!ctx) return TX_ERR_INVALID;
   if (ctx->capturing) return tx_fail(ctx, TX_ERR_CAPTURE, "a capture is already active");
+  std::lock_guard<std::mutex> hold(ctx->capture_lock);
   TX_CUDA(ctx, cudaStreamBeginCapture(ctx->stream, cudaStreamCaptureModeRelaxed));
   ctx->alloc.arena = new tx_arena();
   ctx->capturing = true;
@@ -328,7 +329,17 @@ static void drop_arena(tx_ctx *ctx, tx_arena *arena) {
   for (void *b : arena->blocks) ctx->alloc.arena_owner.erase(b);
   for (auto &c : arena->chunks) cudaFree(c.first);
   for (void *h : arena->pinned) cudaFreeHost(h);
+  for (void *m : arena->borrowed) tx_dlpack_give_back(ctx, m);
   delete arena;
+}
+
+static cudaError_t end_capture(tx_ctx *ctx, cudaGraph_t *graph, tx_arena **arena) {
+  std::lock_guard<std::mutex> hold(ctx->capture_lock);
+  const cudaError_t e = cudaStreamEndCapture(ctx->stream, graph);
+  *arena = ctx->alloc.arena;
+  ctx->alloc.arena = nullptr;
+  ctx->capturing = false;
+  return e;
 }
 
 extern "C" int tx_capture_end(tx_ctx *ctx, tx_exec **out) {
@@ -336,10 +347,8 @@ extern "C" int tx_capture_end(tx_ctx *ctx, tx_exec **out) {
   *out = nullptr;
   if (!ctx->capturing) return tx_fail(ctx, TX_ERR_CAPTURE, "no capture is active");
   cudaGraph_t graph = nullptr;
-  cudaError_t e = cudaStreamEndCapture(ctx->stream, &graph);
-  tx_arena *arena = ctx->alloc.arena;
-  ctx->alloc.arena = nullptr;
-  ctx->capturing = false;
+  tx_arena *arena = nullptr;
+  cudaError_t e = end_capture(ctx, &graph, &arena);
   if (e != cudaSuccess || ctx->err_code) {
     if (graph) cudaGraphDestroy(graph);
     drop_arena(ctx, arena);
@@ -367,12 +376,11 @@ extern "C" int tx_capture_abort(tx_ctx *ctx) {
   if (!ctx) return TX_ERR_INVALID;
   if (!ctx->capturing) return TX_OK;
   cudaGraph_t graph = nullptr;
-  cudaStreamEndCapture(ctx->stream, &graph);
+  tx_arena *arena = nullptr;
+  end_capture(ctx, &graph, &arena);
   cudaGetLastError();
   if (graph) cudaGraphDestroy(graph);
-  drop_arena(ctx, ctx->alloc.arena);
-  ctx->alloc.arena = nullptr;
-  ctx->capturing = false;
+  drop_arena(ctx, arena);
   return TX_OK;
 }
 

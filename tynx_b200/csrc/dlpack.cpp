@@ -115,9 +115,18 @@ extern "C" int tx_dlpack_release(void *managed) {
 
 extern "C" int tx_dlpack_give_back(tx_ctx *ctx, void *managed) {
   if (!ctx) return TX_ERR_INVALID;
-  if (ctx->capturing) return tx_fail(ctx, TX_ERR_CAPTURE, "borrowed memory cannot be given back during a capture");
-  // a stream that failed no longer uses the memory either
-  cudaStreamSynchronize(ctx->stream);
-  cudaStreamSynchronize(ctx->comm);
-  return tx_dlpack_release(managed);
+  {
+    std::lock_guard<std::mutex> hold(ctx->capture_lock);
+    if (ctx->capturing) {  // the graph may reference the memory: it stays as long as the graph
+      try {
+        ctx->alloc.arena->borrowed.push_back(managed);
+      } catch (...) {  // no host memory for the note: it stays for good
+      }
+      return TX_OK;
+    }
+    // a stream that failed no longer uses the memory either
+    cudaStreamSynchronize(ctx->stream);
+    cudaStreamSynchronize(ctx->comm);
+  }
+  return tx_dlpack_release(managed);  // calls into the other library: not under the lock
 }

@@ -11,7 +11,6 @@ stream has passed the point where it let go of it.
 from __future__ import annotations
 
 import ctypes as C
-import threading
 
 from . import _native as N
 from ._core import Context, Device, Storage, Tensor, context
@@ -80,7 +79,8 @@ def export(tensor: Tensor, stream=None, device=None, copy=None):
 
 class _Borrowed(Storage):
     """Another library's memory; given back when the last Tensor on it goes, once
-    the compute stream has passed the work issued on it."""
+    the compute stream has passed the work issued on it (during a capture: with
+    the captured graph, which may read it)."""
 
     __slots__ = ("managed",)
 
@@ -92,19 +92,9 @@ class _Borrowed(Storage):
         managed, self.managed = getattr(self, "managed", None), None
         if managed:
             try:
-                _give_back(self.ctx, managed)
+                lib.tx_dlpack_give_back(self.ctx.handle, managed)  # whatever thread lets go
             except Exception:  # interpreter shutdown
                 pass
-
-
-_held: list = []  # let go during a capture or on another thread: given back later
-
-
-def _give_back(ctx: Context, managed: int) -> None:
-    if ctx.capturing or threading.get_ident() != ctx.owner:
-        _held.append((ctx, managed))
-        return
-    lib.tx_dlpack_give_back(ctx.handle, managed)
 
 
 def from_dlpack(source, device: Device | None = None) -> Tensor:
@@ -119,8 +109,6 @@ def from_dlpack(source, device: Device | None = None) -> Tensor:
     ctx = context(Device(f"cuda:{index}"))
     if ctx.capturing:
         raise CaptureError("from_dlpack is not allowed during a capture")
-    while _held:
-        _give_back(*_held.pop())
     stream = C.c_void_p()
     ctx.check(lib.tx_stream(ctx.handle, C.byref(stream)))
     capsule = source.__dlpack__(stream=stream.value)
