@@ -93,9 +93,11 @@ int tx_stream(tx_ctx *ctx, void **out);
  * returned.  The given stream (a cudaStream_t of the borrower; NULL: the
  * legacy default one) waits for the compute work issued so far.  The block is
  * freed once tx_free was called and every loan has ended (the structure's
- * deleter, callable from any thread); work issued after that waits for the
- * borrower's stream before it reuses the memory.  Every loan has to end
- * before tx_ctx_destroy.  Not allowed during a capture.  tx_dlpack_release calls the deleter of any such
+ * deleter, callable from any thread while the borrower's stream exists); work
+ * issued after that waits for what the stream had been given by then before it
+ * reuses the memory.  Every loan has to end before tx_ctx_destroy.  Not allowed
+ * during a capture, on the context's stream or on the borrower's; a loan that
+ * ends while the borrower's stream is captured keeps the block for good.  tx_dlpack_release calls the deleter of any such
  * structure; tx_dlpack_give_back, from any thread, does so once the context's streams have passed all work
  * issued so far (for memory that was borrowed; kernels' error flag stays up for tx_sync).  During a capture it
  * keeps the memory as long as the captured graph, which may reference it. */

@@ -152,3 +152,86 @@ def test_borrowed_memory_let_go_on_another_thread():
     gc.collect()
     assert torch.cuda.memory_allocated() <= free
     np.testing.assert_array_equal(tx.from_dlpack(torch.ones(3, device="cuda")).numpy(), 1.0)
+
+
+def _runtime():
+    import ctypes
+
+    import torch  # noqa: F401  (maps the runtime)
+
+    with open("/proc/self/maps") as maps:
+        path = next(line.split()[-1] for line in maps if "libcudart.so" in line)
+    return ctypes.CDLL(path)
+
+
+def test_a_borrower_whose_stream_is_gone():
+    """Its memory is used again only after the work that the stream still had, without the stream's handle."""
+    import ctypes
+
+    import torch
+
+    import tynx_b200 as tx
+
+    runtime = _runtime()
+    copy = torch.empty(1 << 20, device="cuda")
+    for i in range(5):
+        handle = ctypes.c_void_p()
+        assert runtime.cudaStreamCreateWithFlags(ctypes.byref(handle), 1) == 0
+        capsule = (tx.ones(1 << 20) * float(i)).__dlpack__(stream=handle.value)
+        there = torch.utils.dlpack.from_dlpack(capsule)
+        torch.cuda.synchronize()
+        with torch.cuda.stream(torch.cuda.ExternalStream(handle.value)):
+            torch.cuda._sleep(2_000_000)
+            copy.copy_(there)
+        del there
+        assert runtime.cudaStreamDestroy(handle) == 0
+        gc.collect()
+        spoil = [tx.zeros(1 << 20) for _ in range(3)]
+        tx.synchronize()
+        torch.cuda.synchronize()
+        assert copy.min().item() == copy.max().item() == float(i)
+        del spoil
+
+
+def test_a_borrower_that_captures():
+    """What it lets go while its stream is recorded stays out of use; it cannot borrow meanwhile.  (A graph
+    that reads what was borrowed on another stream has to keep it, as it has to keep its own memory.)"""
+    import torch
+
+    import tynx_b200 as tx
+    from tynx_b200._native import CaptureError
+
+    side = torch.cuda.Stream()
+    mine = tx.ones(1 << 20)
+    with torch.cuda.stream(side):
+        box = [torch.from_dlpack(mine)]
+    del mine
+    copy = torch.zeros(1 << 20, device="cuda")
+    other = tx.ones(5)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        with pytest.raises(CaptureError):
+            torch.from_dlpack(other)
+        copy.copy_(box.pop())
+    gc.collect()
+    spoil = [tx.Tensor(np.full(1 << 20, 7.0, np.float32)) for _ in range(3)]
+    tx.synchronize()
+    graph.replay()
+    torch.cuda.synchronize()
+    assert copy.min().item() == copy.max().item() == 1.0
+    np.testing.assert_array_equal(torch.from_dlpack(other).cpu().numpy(), 1.0)
+    del spoil
+
+
+def test_one_stream_on_both_sides():
+    """A loan on the context's own stream needs no event."""
+    import torch
+
+    import tynx_b200 as tx
+
+    for i in range(20):
+        there = torch.utils.dlpack.from_dlpack((tx.ones(4096) * float(i)).__dlpack__(stream=-1))
+        tx.synchronize()
+        assert there.sum().item() == 4096.0 * i
+        again = tx.from_dlpack(tx.ones(16))
+        np.testing.assert_array_equal((again + 1.0).numpy(), 2.0)

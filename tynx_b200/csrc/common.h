@@ -35,15 +35,17 @@ struct tx_allocator {
   std::vector<void *> quarantine;  // eager blocks freed during a capture
   // Blocks lent to other libraries (tx_dlpack_export): the holders of each block
   // but one, and whether one let go during a capture, whose graph may reference
-  // the block; and the loans that ended, with the stream of each, since the
-  // owner's thread last called.  Other threads touch `ended` only, under the lock.
+  // the block; and the loans that ended since the owner's thread last called,
+  // each with an event that its borrower's stream passes then (null: this
+  // context's own).  Other threads touch `ended` only, under the lock.
   struct Lent {
     int others = 0;
     bool captured = false;
   };
   std::unordered_map<void *, Lent> lent;
   std::mutex lock;
-  std::vector<std::pair<void *, cudaStream_t>> ended;
+  std::vector<std::pair<void *, cudaEvent_t>> ended;
+  std::vector<cudaEvent_t> spare_events;
 };
 
 struct tx_ctx {

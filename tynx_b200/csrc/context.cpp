@@ -436,6 +436,7 @@ extern "C" int tx_ctx_destroy(tx_ctx *ctx) {
   cudaFree(ctx->d_err);
   cudaFree(ctx->d_rng);
   if (ctx->order) cudaEventDestroy(ctx->order);
+  for (cudaEvent_t e : ctx->alloc.spare_events) cudaEventDestroy(e);
   cudaStreamDestroy(ctx->stream);
   cudaStreamDestroy(ctx->comm);
   delete ctx;

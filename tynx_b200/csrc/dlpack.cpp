@@ -3,9 +3,11 @@
 //
 // A lent block stays out of the allocator's free lists until its owner and
 // every borrower are done with it.  A loan may end on any thread (whichever
-// drops the borrowed tensor): that only notes it; the context's own thread
-// collects the note on its next allocation, makes the compute stream wait for
-// the borrower's stream, and frees the block in stream order.
+// drops the borrowed tensor): that records an event on the borrower's stream
+// and notes it; the context's own thread collects the note on its next
+// allocation, makes the compute stream wait for the event, and frees the block
+// in stream order.  The borrower's stream is not used after the loan has ended:
+// it may be gone by then.
 #include <new>
 
 #include "common.h"
@@ -40,14 +42,40 @@ struct Loan {
   tx_ctx *ctx;
   void *block;
   cudaStream_t borrower;
+  cudaEvent_t passed;  // null where the borrower's stream is the context's own
 };
 
+// Whether work issued to the stream runs, rather than becoming part of a graph.
+cudaError_t runs(cudaStream_t stream, bool &yes) {
+  cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+  cudaError_t e = cudaStreamIsCapturing(stream, &status);
+  if (e != cudaSuccess) cudaGetLastError();  // not the borrower's next call's
+  yes = e == cudaSuccess && status == cudaStreamCaptureStatusNone;
+  return e == cudaErrorStreamCaptureImplicit ? cudaSuccess : e;
+}
+
+// Where the event cannot be recorded the block stays lent: on a stream that is being captured it would become
+// part of the borrower's graph, which may reference the block (and a wait for it would draw the compute stream
+// into that capture).
 void end_loan(DlManaged *m) {
   Loan *loan = static_cast<Loan *>(m->owner);
-  try {
-    std::lock_guard<std::mutex> hold(loan->ctx->alloc.lock);
-    loan->ctx->alloc.ended.push_back({loan->block, loan->borrower});
-  } catch (...) {  // no host memory for the note: the block stays lent
+  tx_ctx *ctx = loan->ctx;
+  {
+    DeviceScope device(ctx);
+    bool ok = true;
+    if (loan->passed) {
+      runs(loan->borrower, ok);
+      if (ok && cudaEventRecord(loan->passed, loan->borrower) != cudaSuccess) {
+        cudaGetLastError();
+        ok = false;
+      }
+      if (!ok) cudaEventDestroy(loan->passed);
+    }
+    try {
+      std::lock_guard<std::mutex> hold(ctx->alloc.lock);
+      if (ok) ctx->alloc.ended.push_back({loan->block, loan->passed});
+    } catch (...) {  // no host memory for the note: the block stays lent
+    }
   }
   delete loan;
 }
@@ -63,18 +91,23 @@ int join(tx_ctx *ctx, cudaStream_t first, cudaStream_t then) {
 
 void tx_collect_loans(tx_ctx *ctx) {
   if (ctx->capturing) return;  // a capture cannot wait for work outside it
-  std::vector<std::pair<void *, cudaStream_t>> ended;
+  std::vector<std::pair<void *, cudaEvent_t>> ended;
   {
     std::lock_guard<std::mutex> hold(ctx->alloc.lock);
     if (ctx->alloc.ended.empty()) return;
     ended.swap(ctx->alloc.ended);
   }
   DeviceScope device(ctx);
-  for (size_t i = 0; i < ended.size(); ++i) {
-    bool joined = false;  // one wait for each borrowing stream
-    for (size_t j = 0; j < i && !joined; ++j) joined = ended[j].second == ended[i].second;
-    if (!joined) join(ctx, ended[i].second, ctx->stream);
-    tx_free_raw(ctx, ended[i].first);
+  for (const auto &loan : ended) {
+    if (loan.second) {
+      if (cudaStreamWaitEvent(ctx->stream, loan.second, 0) != cudaSuccess) {
+        cudaGetLastError();
+        cudaEventDestroy(loan.second);
+        continue;  // no order with the borrower: the block stays lent
+      }
+      ctx->alloc.spare_events.push_back(loan.second);
+    }
+    tx_free_raw(ctx, loan.first);
   }
 }
 
@@ -88,11 +121,30 @@ extern "C" int tx_dlpack_export(tx_ctx *ctx, void *d_block, void *d_data, int dt
   if (!ctx->alloc.live.count(d_block))
     return tx_fail(ctx, TX_ERR_INVALID, "only a tensor that owns its memory can be exported; clone() it first");
   DeviceScope device(ctx);
+  const cudaStream_t borrower = static_cast<cudaStream_t>(stream);
+  cudaEvent_t passed = nullptr;
+  if (borrower != ctx->stream) {
+    bool yes;
+    TX_CUDA(ctx, runs(borrower, yes));
+    if (!yes) return tx_fail(ctx, TX_ERR_CAPTURE, "a tensor cannot be exported to a stream that is being captured");
+    TX_TRY(join(ctx, ctx->stream, borrower));
+    if (ctx->alloc.spare_events.empty()) {
+      TX_CUDA(ctx, cudaEventCreateWithFlags(&passed, cudaEventDisableTiming));
+    } else {
+      passed = ctx->alloc.spare_events.back();
+      ctx->alloc.spare_events.pop_back();
+    }
+  }
   Loan *loan = new (std::nothrow) Loan();
-  if (!loan) return tx_fail(ctx, TX_ERR_OOM, "dlpack export");
-  if (int rc = join(ctx, ctx->stream, static_cast<cudaStream_t>(stream))) {
+  try {
+    if (loan) ++ctx->alloc.lent[d_block].others;
+  } catch (...) {
     delete loan;
-    return rc;
+    loan = nullptr;
+  }
+  if (!loan) {
+    if (passed) cudaEventDestroy(passed);
+    return tx_fail(ctx, TX_ERR_OOM, "dlpack export");
   }
   static const DlType types[3] = {{2, 32, 1}, {0, 64, 1}, {6, 8, 1}};
   for (int i = 0; i < ndim; ++i) loan->shape[i] = shape[i];
@@ -101,8 +153,8 @@ extern "C" int tx_dlpack_export(tx_ctx *ctx, void *d_block, void *d_data, int dt
   loan->managed.deleter = end_loan;
   loan->ctx = ctx;
   loan->block = d_block;
-  loan->borrower = static_cast<cudaStream_t>(stream);
-  ++ctx->alloc.lent[d_block].others;
+  loan->borrower = borrower;
+  loan->passed = passed;
   *out = &loan->managed;
   return TX_OK;
 }
