@@ -235,3 +235,43 @@ def test_one_stream_on_both_sides():
         assert there.sum().item() == 4096.0 * i
         again = tx.from_dlpack(tx.ones(16))
         np.testing.assert_array_equal((again + 1.0).numpy(), 2.0)
+
+
+def test_the_default_stream_while_a_stream_beside_it_is_captured():
+    """The legacy default stream takes no work then: loans wait, and the capture stays whole."""
+    import ctypes
+
+    import torch
+
+    import tynx_b200 as tx
+    from tynx_b200._native import CaptureError
+
+    runtime = _runtime()
+    warm = [tx.ones(4_000_001) for _ in range(4)]
+    mine = warm.pop()
+    at = mine.ptr
+    there = torch.from_dlpack(mine)
+    small = tx.ones(3)
+    del mine, warm
+    tx.synchronize()
+    torch.cuda.synchronize()
+    handle, graph = ctypes.c_void_p(), ctypes.c_void_p()
+    assert runtime.cudaStreamCreate(ctypes.byref(handle)) == 0
+    assert runtime.cudaStreamBeginCapture(handle, 2) == 0
+    del there
+    gc.collect()
+    others = [tx.ones(4_000_001) for _ in range(3)]
+    pointers = [t.ptr for t in others]
+    refused = False
+    try:
+        torch.from_dlpack(small)
+    except CaptureError:
+        refused = True
+    assert runtime.cudaStreamEndCapture(handle, ctypes.byref(graph)) == 0
+    assert refused and at not in pointers
+    held = tx.ones(4_000_001)
+    assert held.ptr == at
+    runtime.cudaGraphDestroy(graph)
+    assert runtime.cudaStreamDestroy(handle) == 0
+    np.testing.assert_array_equal(torch.from_dlpack(small).cpu().numpy(), 1.0)
+    del others

@@ -36,15 +36,21 @@ struct tx_allocator {
   // Blocks lent to other libraries (tx_dlpack_export): the holders of each block
   // but one, and whether one let go during a capture, whose graph may reference
   // the block; and the loans that ended since the owner's thread last called,
-  // each with an event that its borrower's stream passes then (null: this
-  // context's own).  Other threads touch `ended` only, under the lock.
+  // each with the event recorded then on its borrower's stream, or the stream
+  // itself where that cannot go away (the context's own, the legacy default).
+  // Other threads touch `ended` only, under the lock.
   struct Lent {
     int others = 0;
     bool captured = false;
   };
   std::unordered_map<void *, Lent> lent;
   std::mutex lock;
-  std::vector<std::pair<void *, cudaEvent_t>> ended;
+  struct Ended {
+    void *block;
+    cudaEvent_t passed;
+    cudaStream_t stream;
+  };
+  std::vector<Ended> ended;
   std::vector<cudaEvent_t> spare_events;
 };
 

@@ -7,7 +7,8 @@
 // and notes it; the context's own thread collects the note on its next
 // allocation, makes the compute stream wait for the event, and frees the block
 // in stream order.  The borrower's stream is not used after the loan has ended:
-// it may be gone by then.
+// it may be gone by then.  The legacy default stream never is: its loans share
+// one event, recorded when they are collected (0.3 us a loan less).
 #include <new>
 
 #include "common.h"
@@ -42,7 +43,7 @@ struct Loan {
   tx_ctx *ctx;
   void *block;
   cudaStream_t borrower;
-  cudaEvent_t passed;  // null where the borrower's stream is the context's own
+  cudaEvent_t passed;  // null where the borrower's stream cannot go away
 };
 
 // Whether work issued to the stream runs, rather than becoming part of a graph.
@@ -60,22 +61,20 @@ cudaError_t runs(cudaStream_t stream, bool &yes) {
 void end_loan(DlManaged *m) {
   Loan *loan = static_cast<Loan *>(m->owner);
   tx_ctx *ctx = loan->ctx;
-  {
+  bool ok = true;
+  if (loan->passed) {
     DeviceScope device(ctx);
-    bool ok = true;
-    if (loan->passed) {
-      runs(loan->borrower, ok);
-      if (ok && cudaEventRecord(loan->passed, loan->borrower) != cudaSuccess) {
-        cudaGetLastError();
-        ok = false;
-      }
-      if (!ok) cudaEventDestroy(loan->passed);
+    runs(loan->borrower, ok);
+    if (ok && cudaEventRecord(loan->passed, loan->borrower) != cudaSuccess) {
+      cudaGetLastError();
+      ok = false;
     }
-    try {
-      std::lock_guard<std::mutex> hold(ctx->alloc.lock);
-      if (ok) ctx->alloc.ended.push_back({loan->block, loan->passed});
-    } catch (...) {  // no host memory for the note: the block stays lent
-    }
+    if (!ok) cudaEventDestroy(loan->passed);
+  }
+  try {
+    std::lock_guard<std::mutex> hold(ctx->alloc.lock);
+    if (ok) ctx->alloc.ended.push_back({loan->block, loan->passed, loan->borrower});
+  } catch (...) {  // no host memory for the note: the block stays lent
   }
   delete loan;
 }
@@ -91,23 +90,35 @@ int join(tx_ctx *ctx, cudaStream_t first, cudaStream_t then) {
 
 void tx_collect_loans(tx_ctx *ctx) {
   if (ctx->capturing) return;  // a capture cannot wait for work outside it
-  std::vector<std::pair<void *, cudaEvent_t>> ended;
+  std::vector<tx_allocator::Ended> ended;
   {
     std::lock_guard<std::mutex> hold(ctx->alloc.lock);
     if (ctx->alloc.ended.empty()) return;
     ended.swap(ctx->alloc.ended);
   }
   DeviceScope device(ctx);
+  enum { kUnknown, kJoined, kLater } legacy = kUnknown;
   for (const auto &loan : ended) {
-    if (loan.second) {
-      if (cudaStreamWaitEvent(ctx->stream, loan.second, 0) != cudaSuccess) {
+    if (loan.passed) {
+      if (cudaStreamWaitEvent(ctx->stream, loan.passed, 0) != cudaSuccess) {
         cudaGetLastError();
-        cudaEventDestroy(loan.second);
+        cudaEventDestroy(loan.passed);
         continue;  // no order with the borrower: the block stays lent
       }
-      ctx->alloc.spare_events.push_back(loan.second);
+      ctx->alloc.spare_events.push_back(loan.passed);
+    } else if (loan.stream != ctx->stream) {
+      if (legacy == kUnknown) {  // while a stream that synchronises with it is captured, it takes no work
+        bool yes;
+        runs(cudaStreamLegacy, yes);
+        legacy = yes && join(ctx, cudaStreamLegacy, ctx->stream) == TX_OK ? kJoined : kLater;
+      }
+      if (legacy == kLater) {
+        std::lock_guard<std::mutex> hold(ctx->alloc.lock);
+        ctx->alloc.ended.push_back(loan);
+        continue;
+      }
     }
-    tx_free_raw(ctx, loan.first);
+    tx_free_raw(ctx, loan.block);
   }
 }
 
@@ -121,18 +132,19 @@ extern "C" int tx_dlpack_export(tx_ctx *ctx, void *d_block, void *d_data, int dt
   if (!ctx->alloc.live.count(d_block))
     return tx_fail(ctx, TX_ERR_INVALID, "only a tensor that owns its memory can be exported; clone() it first");
   DeviceScope device(ctx);
-  const cudaStream_t borrower = static_cast<cudaStream_t>(stream);
+  const cudaStream_t borrower = stream ? static_cast<cudaStream_t>(stream) : cudaStreamLegacy;
   cudaEvent_t passed = nullptr;
   if (borrower != ctx->stream) {
     bool yes;
     TX_CUDA(ctx, runs(borrower, yes));
     if (!yes) return tx_fail(ctx, TX_ERR_CAPTURE, "a tensor cannot be exported to a stream that is being captured");
     TX_TRY(join(ctx, ctx->stream, borrower));
-    if (ctx->alloc.spare_events.empty()) {
+    std::vector<cudaEvent_t> &spare = ctx->alloc.spare_events;
+    if (borrower != cudaStreamLegacy && spare.empty()) {
       TX_CUDA(ctx, cudaEventCreateWithFlags(&passed, cudaEventDisableTiming));
-    } else {
-      passed = ctx->alloc.spare_events.back();
-      ctx->alloc.spare_events.pop_back();
+    } else if (borrower != cudaStreamLegacy) {
+      passed = spare.back();
+      spare.pop_back();
     }
   }
   Loan *loan = new (std::nothrow) Loan();
