@@ -90,6 +90,11 @@ def _default_index() -> int:
         return 0
 
 
+def _cell() -> tuple:
+    out = C.c_void_p()
+    return out, C.byref(out)
+
+
 class Context:
     """One ``tx_ctx`` (stream, allocator, latched error) per device."""
 
@@ -109,18 +114,28 @@ class Context:
         self.index = index
         self.owner = threading.get_ident()
         self.capturing = False
-        self._out = C.c_void_p()  # result of an allocation
-        self._out_ref = C.byref(self._out)
+        self.cells: list = []
+
+    def cell(self) -> tuple:
+        """Where a call leaves a pointer, and the argument for it; put back into ``cells`` once it is read.
+        Each call has its own: another thread's, or a finaliser's, may come between call and read."""
+        try:
+            return self.cells.pop()
+        except IndexError:
+            return _cell()
 
     def check(self, code: int, what: str = "") -> None:
         if code != N.TX_OK:
             N.raise_for(code, self.handle, what)
 
     def alloc(self, nbytes: int) -> int:
-        code = lib.tx_alloc(self.handle, nbytes or 1, self._out_ref)
+        cell = self.cell()
+        code = lib.tx_alloc(self.handle, nbytes or 1, cell[1])
+        ptr = cell[0].value
+        self.cells.append(cell)
         if code:
             N.raise_for(code, self.handle, "alloc")
-        return self._out.value
+        return ptr
 
     def free(self, ptr: int) -> None:
         lib.tx_free(self.handle, ptr)
@@ -211,11 +226,18 @@ class Storage:
         if ptr is not None:
             self.ptr, self.owned = ptr, False
         else:
-            code = lib.tx_alloc(ctx.handle, nbytes or 1, ctx._out_ref)
+            cells = ctx.cells  # Context.alloc, written out
+            try:
+                cell = cells.pop()
+            except IndexError:
+                cell = _cell()
+            code = lib.tx_alloc(ctx.handle, nbytes or 1, cell[1])
+            self.ptr = cell[0].value
+            cells.append(cell)
             if code:
                 self.owned = False
                 N.raise_for(code, ctx.handle, "alloc")
-            self.ptr, self.owned = ctx._out.value, owned
+            self.owned = owned
 
     def __del__(self):
         if self.owned and self.ptr:

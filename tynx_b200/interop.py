@@ -69,12 +69,14 @@ def export(tensor: Tensor, stream=None, device=None, copy=None):
         own = C.c_void_p()
         ctx.check(lib.tx_stream(ctx.handle, C.byref(own)))
         stream = own.value
-    ndim, data = len(shape), storage.ptr
+    ndim, data, cell = len(shape), storage.ptr, ctx.cell()
     code = lib.tx_dlpack_export(ctx.handle, data if storage.owned else None, data + tensor._offset,
-                                N.DL_TYPES[tensor.dtype], _SHAPES[ndim](*shape), ndim, stream or 1, ctx._out_ref)
+                                N.DL_TYPES[tensor.dtype], _SHAPES[ndim](*shape), ndim, stream or 1, cell[1])
+    managed = cell[0].value
+    ctx.cells.append(cell)
     if code:
         ctx.check(code, "dlpack")
-    return _new(ctx._out.value, _NAME, _drop_pointer)
+    return _new(managed, _NAME, _drop_pointer)
 
 
 class _Borrowed(Storage):
