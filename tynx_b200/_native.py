@@ -239,9 +239,12 @@ SIGNATURES = {
 
 
 def _share_nccl() -> None:
-    """Load the NCCL of the Python environment, where there is one, before the
-    engine would load the system's: a process holds one ``libnccl.so.2``, and
-    PyTorch, imported later for ``from_dlpack``, does not load with an older one."""
+    """Where PyTorch is installed, load the NCCL that came with it before the engine
+    would load the system's: a process holds one ``libnccl.so.2``, and PyTorch,
+    imported later for ``from_dlpack``, does not load with an older one.  Data
+    parallelism runs on that NCCL then; without PyTorch on the system's."""
+    if importlib.util.find_spec("torch") is None:
+        return
     spec = importlib.util.find_spec("nvidia")
     for place in (spec.submodule_search_locations or ()) if spec else ():
         library = Path(place) / "nccl" / "lib" / "libnccl.so.2"
