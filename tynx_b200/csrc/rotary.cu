@@ -10,9 +10,11 @@
 //   dx = r (g w - u mean(g w u)),   dw = sum over tokens and heads of g u.
 //
 // Angles: w_i arrives as turns a position in 64 bits; p * turns is reduced to
-// its fraction there, so cosine and sine of far positions are as exact as
-// those of near ones (2^-25 of a turn, up to 2^27 turns; then 2^-52 of the
-// angle), and nothing has to be tabulated.
+// its fraction there and nothing has to be tabulated.  To what the turns
+// themselves are off by this adds 2^-53 of the angle (the product) and 2^-26
+// of a turn (the fraction in fp32): the angles of positions up to some 2^25
+// turns are as exact as those of near ones.  Positions beyond 2^53 are rounded
+// to 53 bits on their way to fp64.
 //
 // All of it is bound by memory: one pass reads x (and dy) and writes y (or dx)
 // once.  A block takes a few tokens with all their heads, works out the

@@ -28,9 +28,13 @@ class Rotary:
       turn less than ``beta_slow`` (1) times and blends linearly between, and
       multiplies the rotated elements by ``attention_factor`` (0.1 ln f + 1).
 
-    Frequencies are 64-bit and angles are reduced in 64 bits on the device (an
-    angle is off by 2^-52 of itself at most), so positions may be any int64 value;
-    nothing is stored on the device.
+    Frequencies are 64-bit and angles are reduced in 64 bits on the device; nothing
+    is stored there.  An angle ``p * w`` is off by ``(5 + ln(1 / w)) 2^-53`` of itself
+    at most: the rounding of the exponent ``-2 i / dim`` grows by ``ln(1 / w)`` in the
+    power, the power, the conversion to turns and the product with the position add
+    the rest (a scaling adds its own operations, yarn's blend up to ``factor 2^-53``).
+    Positions may be any int64 value; beyond 2^53 they are rounded to 53 bits first,
+    so that neighbours may share an angle.
     """
 
     __slots__ = ("dim", "interleaved", "frequencies", "factor", "_desc")
