@@ -20,7 +20,7 @@ enum { DEVERR_NONE = 0, DEVERR_INDEX = 1, DEVERR_TIMEOUT = 2, DEVERR_LABEL = 3, 
 struct tx_arena {
   std::vector<std::pair<char *, size_t>> chunks;
   size_t offset = 0;  // within chunks.back()
-  std::unordered_set<void *> blocks;
+  std::unordered_set<void *> blocks, held;  // all, and those that have not been freed yet
   std::vector<void *> pinned;  // host staging for copies recorded during capture
   std::vector<void *> borrowed;  // other libraries' memory let go during capture (tx_dlpack_give_back)
 };
@@ -33,6 +33,9 @@ struct tx_allocator {
   tx_arena *arena = nullptr;  // non-null while capturing
   std::unordered_map<void *, tx_arena *> arena_owner;
   std::vector<void *> quarantine;  // eager blocks freed during a capture
+  // Blocks of arenas that are gone, whose holders have still to free them (how often): no eager block may have
+  // such an address, or that call would free it.
+  std::unordered_map<void *, int> gone;
   // Blocks lent to other libraries (tx_dlpack_export): the holders of each block
   // but one, and whether one let go during a capture, whose graph may reference
   // the block; and the loans that ended since the owner's thread last called,

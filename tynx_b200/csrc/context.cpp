@@ -168,6 +168,7 @@ static void *arena_alloc(tx_ctx *ctx, tx_arena *arena, size_t bytes) {
   char *p = arena->chunks.back().first + arena->offset;
   arena->offset += need;
   arena->blocks.insert(p);
+  arena->held.insert(p);
   ctx->alloc.arena_owner[p] = arena;
   return p;
 }
@@ -178,6 +179,20 @@ static void release_cached(tx_ctx *ctx) {
     for (void *p : kv.second) cudaFree(p);
   ctx->alloc.free_blocks.clear();
   ctx->alloc.cached = 0;
+}
+
+// New device memory, or null.
+static void *fresh_block(const tx_allocator &A, size_t cls) {
+  void *p = nullptr;
+  std::vector<void *> passed_over;
+  while (cudaMalloc(&p, cls) == cudaSuccess) {
+    if (!A.gone.count(p)) break;
+    passed_over.push_back(p);
+    p = nullptr;
+  }
+  if (!p) cudaGetLastError();
+  for (void *q : passed_over) cudaFree(q);
+  return p;
 }
 
 void tx_collect_loans(tx_ctx *ctx);  // dlpack.cpp
@@ -196,12 +211,11 @@ void *tx_alloc_raw(tx_ctx *ctx, size_t bytes) {
     A.in_use += cls;
     return p;
   }
-  void *p = nullptr;
-  if (cudaMalloc(&p, cls) != cudaSuccess) {
-    cudaGetLastError();
+  void *p = fresh_block(A, cls);
+  if (!p) {
     release_cached(ctx);
-    if (cudaMalloc(&p, cls) != cudaSuccess) {
-      cudaGetLastError();
+    p = fresh_block(A, cls);
+    if (!p) {
       char buf[128];
       snprintf(buf, sizeof buf, "device allocation of %zu bytes failed", cls);
       tx_fail(ctx, TX_ERR_OOM, buf);
@@ -216,7 +230,18 @@ void *tx_alloc_raw(tx_ctx *ctx, size_t bytes) {
 void tx_free_raw(tx_ctx *ctx, void *p) {
   if (!p) return;
   tx_allocator &A = ctx->alloc;
-  if (A.arena_owner.count(p)) return;  // arena memory lives as long as its exec
+  auto in_arena = A.arena_owner.find(p);
+  if (in_arena != A.arena_owner.end()) {  // arena memory lives as long as its exec
+    in_arena->second->held.erase(p);
+    return;
+  }
+  if (!A.gone.empty()) {
+    auto g = A.gone.find(p);
+    if (g != A.gone.end()) {
+      if (--g->second == 0) A.gone.erase(g);
+      return;
+    }
+  }
   auto it = A.live.find(p);
   if (it == A.live.end()) return;
   bool captured = A.arena != nullptr;  // the graph being captured may still reference this block
@@ -327,6 +352,7 @@ extern "C" int tx_capture_begin(tx_ctx *ctx) {
 static void drop_arena(tx_ctx *ctx, tx_arena *arena) {
   if (!arena) return;
   for (void *b : arena->blocks) ctx->alloc.arena_owner.erase(b);
+  for (void *b : arena->held) ++ctx->alloc.gone[b];
   for (auto &c : arena->chunks) cudaFree(c.first);
   for (void *h : arena->pinned) cudaFreeHost(h);
   for (void *m : arena->borrowed) tx_dlpack_give_back(ctx, m);
