@@ -109,7 +109,8 @@ int tx_dlpack_give_back(tx_ctx *ctx, void *managed);
 
 /* =========================================================================
  * Device memory (replaces Burn tensor storage behind DynTensor,
- * crates/tynx/src/tensor.rs:156-185).  Stream-ordered caching allocator.
+ * crates/tynx/src/tensor.rs:156-185).  Stream-ordered caching allocator;
+ * tx_alloc and tx_free may be called from any thread (a garbage collector's).
  * ========================================================================= */
 int tx_alloc(tx_ctx *ctx, size_t bytes, void **d_out);
 int tx_free(tx_ctx *ctx, void *d_ptr);

@@ -35,3 +35,40 @@ def test_a_late_release_names_no_other_tensor():
         for t in held:
             np.testing.assert_array_equal(t.numpy(), 1.0)
         del held, again
+
+
+def test_tensors_dropped_on_other_threads():
+    """Whichever thread drops the last reference, or collects garbage, the allocator stays whole."""
+    import queue
+    import threading
+
+    import tynx_b200 as tx
+
+    dropped = queue.Queue()
+
+    def drop():
+        while dropped.get() is not None:
+            pass
+
+    threads = [threading.Thread(target=drop) for _ in range(4)]
+    for thread in threads:
+        thread.start()
+    sizes = [1 << 10, 1 << 12, 1 << 16]
+    compiled = tx.compile(lambda a: a * 2.0, fullgraph=True)
+    wrong = 0
+    for i in range(6000):
+        t = tx.ones(sizes[i % 3]) * float(i)
+        u = compiled(t)
+        v = u + 1.0
+        if i % 100 == 99:
+            wrong += int((v.numpy() != 2.0 * i + 1.0).any())
+        for x in (t, u, v):
+            dropped.put(x)
+        del t, u, v, x
+    for _ in threads:
+        dropped.put(None)
+    for thread in threads:
+        thread.join()
+    assert wrong == 0
+    held = [tx.ones(1 << 12) for _ in range(200)]
+    assert len({t.ptr for t in held}) == 200

@@ -41,13 +41,13 @@ struct tx_allocator {
   // the block; and the loans that ended since the owner's thread last called,
   // each with the event recorded then on its borrower's stream, or the stream
   // itself where that cannot go away (the context's own, the legacy default).
-  // Other threads touch `ended` only, under the lock.
+  // `ended` changes under its lock, everything else under `blocks`.
   struct Lent {
     int others = 0;
     bool captured = false;
   };
   std::unordered_map<void *, Lent> lent;
-  std::mutex lock;
+  std::mutex lock, blocks;  // whichever thread collects garbage frees blocks
   struct Ended {
     void *block;
     cudaEvent_t passed;

@@ -200,6 +200,7 @@ void tx_collect_loans(tx_ctx *ctx);  // dlpack.cpp
 void *tx_alloc_raw(tx_ctx *ctx, size_t bytes) {
   tx_allocator &A = ctx->alloc;
   tx_collect_loans(ctx);
+  std::lock_guard<std::mutex> hold(A.blocks);
   if (A.arena) return arena_alloc(ctx, A.arena, bytes);
   size_t cls = size_class(bytes);
   auto it = A.free_blocks.find(cls);
@@ -230,6 +231,7 @@ void *tx_alloc_raw(tx_ctx *ctx, size_t bytes) {
 void tx_free_raw(tx_ctx *ctx, void *p) {
   if (!p) return;
   tx_allocator &A = ctx->alloc;
+  std::lock_guard<std::mutex> hold(A.blocks);
   auto in_arena = A.arena_owner.find(p);
   if (in_arena != A.arena_owner.end()) {  // arena memory lives as long as its exec
     in_arena->second->held.erase(p);
@@ -344,6 +346,7 @@ extern "C" int tx_capture_begin(tx_ctx *ctx) {
   if (ctx->capturing) return tx_fail(ctx, TX_ERR_CAPTURE, "a capture is already active");
   std::lock_guard<std::mutex> hold(ctx->capture_lock);
   TX_CUDA(ctx, cudaStreamBeginCapture(ctx->stream, cudaStreamCaptureModeRelaxed));
+  std::lock_guard<std::mutex> blocks(ctx->alloc.blocks);
   ctx->alloc.arena = new tx_arena();
   ctx->capturing = true;
   return TX_OK;
@@ -351,8 +354,11 @@ extern "C" int tx_capture_begin(tx_ctx *ctx) {
 
 static void drop_arena(tx_ctx *ctx, tx_arena *arena) {
   if (!arena) return;
-  for (void *b : arena->blocks) ctx->alloc.arena_owner.erase(b);
-  for (void *b : arena->held) ++ctx->alloc.gone[b];
+  {
+    std::lock_guard<std::mutex> hold(ctx->alloc.blocks);
+    for (void *b : arena->blocks) ctx->alloc.arena_owner.erase(b);
+    for (void *b : arena->held) ++ctx->alloc.gone[b];
+  }
   for (auto &c : arena->chunks) cudaFree(c.first);
   for (void *h : arena->pinned) cudaFreeHost(h);
   for (void *m : arena->borrowed) tx_dlpack_give_back(ctx, m);
@@ -362,6 +368,7 @@ static void drop_arena(tx_ctx *ctx, tx_arena *arena) {
 static cudaError_t end_capture(tx_ctx *ctx, cudaGraph_t *graph, tx_arena **arena) {
   std::lock_guard<std::mutex> hold(ctx->capture_lock);
   const cudaError_t e = cudaStreamEndCapture(ctx->stream, graph);
+  std::lock_guard<std::mutex> blocks(ctx->alloc.blocks);
   *arena = ctx->alloc.arena;
   ctx->alloc.arena = nullptr;
   ctx->capturing = false;

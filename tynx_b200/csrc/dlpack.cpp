@@ -129,8 +129,11 @@ extern "C" int tx_dlpack_export(tx_ctx *ctx, void *d_block, void *d_data, int dt
   if (ctx->capturing) return tx_fail(ctx, TX_ERR_CAPTURE, "a tensor cannot be exported during a capture");
   if (dtype < TX_DL_F32 || dtype > TX_DL_BOOL || ndim < 0 || ndim > TX_MAX_DIMS || (ndim && !shape))
     return tx_fail(ctx, TX_ERR_INVALID, "dlpack export: dtype or rank");
-  if (!ctx->alloc.live.count(d_block))
-    return tx_fail(ctx, TX_ERR_INVALID, "only a tensor that owns its memory can be exported; clone() it first");
+  {
+    std::lock_guard<std::mutex> hold(ctx->alloc.blocks);
+    if (!ctx->alloc.live.count(d_block))
+      return tx_fail(ctx, TX_ERR_INVALID, "only a tensor that owns its memory can be exported; clone() it first");
+  }
   DeviceScope device(ctx);
   const cudaStream_t borrower = stream ? static_cast<cudaStream_t>(stream) : cudaStreamLegacy;
   cudaEvent_t passed = nullptr;
@@ -149,6 +152,7 @@ extern "C" int tx_dlpack_export(tx_ctx *ctx, void *d_block, void *d_data, int dt
   }
   Loan *loan = new (std::nothrow) Loan();
   try {
+    std::lock_guard<std::mutex> hold(ctx->alloc.blocks);
     if (loan) ++ctx->alloc.lent[d_block].others;
   } catch (...) {
     delete loan;
