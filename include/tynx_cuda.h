@@ -97,10 +97,12 @@ int tx_stream(tx_ctx *ctx, void **out);
  * issued after that waits for what the stream had been given by then before it
  * reuses the memory.  Every loan has to end before tx_ctx_destroy.  Not allowed
  * during a capture, on the context's stream or on the borrower's; a loan that
- * ends while the borrower's stream is captured keeps the block for good.  tx_dlpack_release calls the deleter of any such
- * structure; tx_dlpack_give_back, from any thread, does so once the context's streams have passed all work
- * issued so far (for memory that was borrowed; kernels' error flag stays up for tx_sync).  During a capture it
- * keeps the memory as long as the captured graph, which may reference it. */
+ * ends while the borrower's stream is captured keeps the block for good.
+ * tx_dlpack_release calls the deleter of any such structure;
+ * tx_dlpack_give_back, from any thread, does so once the context's streams have
+ * passed all work issued so far (for memory that was borrowed; kernels' error
+ * flag stays up for tx_sync).  During a capture it keeps the memory as long as
+ * the captured graph, which may reference it. */
 enum { TX_DL_F32 = 0, TX_DL_I64 = 1, TX_DL_BOOL = 2 };
 int tx_dlpack_export(tx_ctx *ctx, void *d_block, void *d_data, int dtype, const int64_t *shape, int ndim,
                      void *stream, void **out);
@@ -110,7 +112,7 @@ int tx_dlpack_give_back(tx_ctx *ctx, void *managed);
 /* =========================================================================
  * Device memory (replaces Burn tensor storage behind DynTensor,
  * crates/tynx/src/tensor.rs:156-185).  Stream-ordered caching allocator;
- * tx_alloc and tx_free may be called from any thread (a garbage collector's).
+ * tx_free may be called from any thread (a garbage collector runs on any).
  * ========================================================================= */
 int tx_alloc(tx_ctx *ctx, size_t bytes, void **d_out);
 int tx_free(tx_ctx *ctx, void *d_ptr);
