@@ -181,11 +181,10 @@ def test_a_borrower_whose_stream_is_gone():
         there = torch.utils.dlpack.from_dlpack(capsule)
         torch.cuda.synchronize()
         with torch.cuda.stream(torch.cuda.ExternalStream(handle.value)):
-            torch.cuda._sleep(2_000_000)
+            torch.cuda._sleep(200_000_000)
             copy.copy_(there)
         del there
         assert runtime.cudaStreamDestroy(handle) == 0
-        gc.collect()
         spoil = [tx.zeros(1 << 20) for _ in range(3)]
         tx.synchronize()
         torch.cuda.synchronize()
@@ -275,3 +274,35 @@ def test_the_default_stream_while_a_stream_beside_it_is_captured():
     assert runtime.cudaStreamDestroy(handle) == 0
     np.testing.assert_array_equal(torch.from_dlpack(small).cpu().numpy(), 1.0)
     del others
+
+
+def test_a_threads_default_stream_let_go_on_another_thread():
+    """Its handle means another stream there: the borrower's work is waited for all the same."""
+    import ctypes
+    import threading
+
+    import torch
+
+    import tynx_b200 as tx
+
+    runtime, own = _runtime(), ctypes.c_void_p(2)
+    copy = torch.empty(1 << 20, device="cuda")
+    side = torch.cuda.Stream()
+    for i in range(5):
+        box = [torch.utils.dlpack.from_dlpack((tx.ones(1 << 20) * float(i)).__dlpack__(stream=2))]
+        torch.cuda.synchronize()
+        with torch.cuda.stream(side):
+            torch.cuda._sleep(200_000_000)
+            late = torch.cuda.Event()
+            late.record(side)
+        assert runtime.cudaStreamWaitEvent(own, ctypes.c_void_p(late.cuda_event), 0) == 0
+        assert runtime.cudaMemcpyAsync(ctypes.c_void_p(copy.data_ptr()), ctypes.c_void_p(box[0].data_ptr()),
+                                       ctypes.c_size_t(4 << 20), 3, own) == 0
+        thread = threading.Thread(target=box.clear)
+        thread.start()
+        thread.join()
+        spoil = [tx.zeros(1 << 20) - 1.0 for _ in range(3)]
+        assert runtime.cudaStreamSynchronize(own) == 0
+        tx.synchronize()
+        assert copy.min().item() == copy.max().item() == float(i)
+        del spoil

@@ -8,7 +8,9 @@
 // allocation, makes the compute stream wait for the event, and frees the block
 // in stream order.  The borrower's stream is not used after the loan has ended:
 // it may be gone by then.  The legacy default stream never is: its loans share
-// one event, recorded when they are collected (0.3 us a loan less).
+// one event, recorded when they are collected (0.3 us a loan less).  So do those
+// of threads' default streams, which the legacy one waits for: their handle
+// means another stream on another thread.
 #include <new>
 
 #include "common.h"
@@ -135,7 +137,7 @@ extern "C" int tx_dlpack_export(tx_ctx *ctx, void *d_block, void *d_data, int dt
       return tx_fail(ctx, TX_ERR_INVALID, "only a tensor that owns its memory can be exported; clone() it first");
   }
   DeviceScope device(ctx);
-  const cudaStream_t borrower = stream ? static_cast<cudaStream_t>(stream) : cudaStreamLegacy;
+  cudaStream_t borrower = stream ? static_cast<cudaStream_t>(stream) : cudaStreamLegacy;
   cudaEvent_t passed = nullptr;
   if (borrower != ctx->stream) {
     bool yes;
@@ -143,6 +145,7 @@ extern "C" int tx_dlpack_export(tx_ctx *ctx, void *d_block, void *d_data, int dt
     if (!yes) return tx_fail(ctx, TX_ERR_CAPTURE, "a tensor cannot be exported to a stream that is being captured");
     TX_TRY(join(ctx, ctx->stream, borrower));
     std::vector<cudaEvent_t> &spare = ctx->alloc.spare_events;
+    if (borrower == cudaStreamPerThread) borrower = cudaStreamLegacy;
     if (borrower != cudaStreamLegacy && spare.empty()) {
       TX_CUDA(ctx, cudaEventCreateWithFlags(&passed, cudaEventDisableTiming));
     } else if (borrower != cudaStreamLegacy) {
