@@ -5,7 +5,8 @@
 another library's CUDA tensor.  Both directions are ordered on the streams of
 both sides: work issued afterwards on the taker's stream sees the work that the
 giver had issued.  A block that was lent is reused only after the borrower's
-stream has passed the point where it let go of it.
+stream has passed the point where it let go of it.  A write through either side
+is seen by both, also by a backward that kept the values.
 """
 
 from __future__ import annotations
